@@ -31,6 +31,7 @@ EXPORTS = (
     "grb_static_scratch_bytes", "grb_bxr_gemv_static", "grb_dense_gemv_bf16", "grb_peer_control_bytes", "grb_peer_enable", "grb_peer_allreduce_bf16",
     "grb_peer_alloc", "grb_peer_free", "grb_peer_open", "grb_peer_close",
     "grb_rmsnorm_bf16", "grb_silu_mul_bf16", "grb_argmax_bf16", "grb_attn_decode_bf16",
+    "grb_kv_write", "grb_kv_read", "grb_kv_keep", "grb_attn_tree_scratch_bytes", "grb_attn_tree", "grb_verify_drafts",
 )
 
 
@@ -71,6 +72,29 @@ class AttnStep(ctypes.Structure):
                 ("q", VOIDP), ("part_acc", VOIDP), ("part_ml", VOIDP), ("out", VOIDP), ("rows", ctypes.c_uint32),
                 ("nq", ctypes.c_uint32), ("nkv", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("max_splits", ctypes.c_uint32),
                 ("scaling", ctypes.c_float)]
+
+
+class KvPages(ctypes.Structure):
+    _fields_ = [("k", VOIDP), ("v", VOIDP), ("k_exp", VOIDP), ("v_exp", VOIDP), ("layer_stride", ctypes.c_int64), ("exp_stride", ctypes.c_int64),
+                ("layers", ctypes.c_uint32), ("pages", ctypes.c_uint32), ("nkv", ctypes.c_uint32), ("format", ctypes.c_uint32)]
+
+
+class KvTable(ctypes.Structure):
+    _fields_ = [("table", VOIDP), ("ld", ctypes.c_int64), ("slots", ctypes.c_uint32), ("max_pages", ctypes.c_uint32)]
+
+
+class TreeStep(ctypes.Structure):
+    _fields_ = [("qkv", VOIDP), ("ldq", ctypes.c_int64), ("cos_table", VOIDP), ("sin_table", VOIDP), ("rope_rows", ctypes.c_uint32), ("row_seq", VOIDP),
+                ("row_pos", VOIDP), ("row_base", VOIDP), ("row_rope", VOIDP), ("row_mask", VOIDP), ("ldm", ctypes.c_int64), ("mask_words", ctypes.c_uint32),
+                ("pages", KvPages), ("table", KvTable), ("scratch", VOIDP), ("scratch_bytes", ctypes.c_uint64), ("out", VOIDP), ("ldo", ctypes.c_int64),
+                ("rows", ctypes.c_uint32), ("nq", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("scaling", ctypes.c_float)]
+
+
+class VerifyStep(ctypes.Structure):
+    _fields_ = [("logits", VOIDP), ("ldl", ctypes.c_int64), ("tokens", VOIDP), ("parent", VOIDP), ("starts", VOIDP), ("u_keep", VOIDP), ("u_draw", VOIDP),
+                ("draft_probs", VOIDP), ("ldq", ctypes.c_int64), ("stats", VOIDP), ("out_tokens", VOIDP), ("out_rows", VOIDP), ("out_count", VOIDP),
+                ("rows", ctypes.c_uint32), ("seqs", ctypes.c_uint32), ("vocab", ctypes.c_uint32), ("width", ctypes.c_uint32), ("dtype", ctypes.c_uint32),
+                ("temperature", ctypes.c_double)]
 
 
 def _declare(lib):
@@ -122,6 +146,14 @@ def _declare(lib):
     lib.grb_silu_mul_bf16.argtypes = [VOIDP, ctypes.c_int64, VOIDP, ctypes.c_int64, u32, u32, VOIDP]
     lib.grb_argmax_bf16.argtypes = [VOIDP, ctypes.c_int64, u32, u32, VOIDP, VOIDP]
     lib.grb_attn_decode_bf16.argtypes = [ctypes.POINTER(AttnStep), VOIDP]
+    rows = [ctypes.POINTER(KvPages), ctypes.POINTER(KvTable), VOIDP, VOIDP, VOIDP, ctypes.c_int64, VOIDP, ctypes.c_int64, u32, VOIDP]
+    lib.grb_kv_write.argtypes = rows
+    lib.grb_kv_read.argtypes = rows
+    lib.grb_kv_keep.argtypes = [ctypes.POINTER(KvPages), ctypes.POINTER(KvTable), VOIDP, VOIDP, VOIDP, ctypes.c_int64, VOIDP, u32, u32, VOIDP]
+    lib.grb_attn_tree_scratch_bytes.argtypes = [u32, u32, u32, u32]
+    lib.grb_attn_tree_scratch_bytes.restype = u64
+    lib.grb_attn_tree.argtypes = [ctypes.POINTER(TreeStep), VOIDP]
+    lib.grb_verify_drafts.argtypes = [ctypes.POINTER(VerifyStep), VOIDP]
     lib.grb_peer_control_bytes.argtypes = []
     lib.grb_peer_control_bytes.restype = u64
     lib.grb_peer_enable.argtypes = [ci]
@@ -132,7 +164,7 @@ def _declare(lib):
     lib.grb_peer_allreduce_bf16.argtypes = [VOIDP, ctypes.POINTER(VOIDP), ctypes.POINTER(VOIDP), u64, u32, u32, VOIDP, u64, u64, VOIDP, VOIDP]
     for name in EXPORTS:
         if name not in ("bcx_free", "bxr_free", "grb_bxr_workspace_bytes", "grb_static_scratch_bytes", "grb_peer_control_bytes",
-                        "bxr_layout_version", "bxr_partition_version"):
+                        "grb_attn_tree_scratch_bytes", "bxr_layout_version", "bxr_partition_version"):
             getattr(lib, name).restype = ci
 
 

@@ -13,16 +13,18 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT = PKG / "_build" / "libgeorefine_b200.so"
-SOURCES = [CSRC / "capi.cu", CSRC / "bcx_host.cpp", CSRC / "bcx_frame.cpp", CSRC / "bxr_build.cpp"]
+SOURCES = [CSRC / "capi.cu", CSRC / "spec_ops.cu", CSRC / "bcx_host.cpp", CSRC / "bcx_frame.cpp", CSRC / "bxr_build.cpp"]
 FASTCALL_SOURCE = CSRC / "fastcall.c"
 FASTCALL = PKG / "_build" / ("_fastcall" + sysconfig.get_config_var("EXT_SUFFIX"))     # (named for the interpreter's ABI)
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
-         "-Xcompiler", "-pthread", "-shared"]
+         "-Xcompiler", "-pthread"]
 
 
 def _inputs():
@@ -36,18 +38,25 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > stamp for p in _inputs() if p != FASTCALL_SOURCE)
 
 
+def _nvcc(cmd, verbose):
+    run = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose:
+        sys.stderr.write(run.stderr)
+    if run.returncode:
+        raise RuntimeError("nvcc failed:\n" + run.stderr[-4000:])
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     if force or needs_build():
         nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
         if not Path(nvcc).exists():
             raise RuntimeError("nvcc not found: the CUDA library cannot be built here and no prebuilt copy is up to date")
         OUT.parent.mkdir(parents=True, exist_ok=True)
-        cmd = [nvcc, *FLAGS, *(["-Xptxas", "-v"] if verbose else []), *map(str, SOURCES), "-o", str(OUT)]
-        run = subprocess.run(cmd, capture_output=True, text=True)
-        if verbose:
-            sys.stderr.write(run.stderr)
-        if run.returncode:
-            raise RuntimeError("nvcc failed:\n" + run.stderr[-4000:])
+        with tempfile.TemporaryDirectory(dir=OUT.parent) as objects, ThreadPoolExecutor() as pool:      # (a source at a time takes twice as long)
+            compiled = [Path(objects) / (p.name + ".o") for p in SOURCES]
+            flags = [*FLAGS, *(["-Xptxas", "-v"] if verbose else [])]
+            list(pool.map(lambda p, o: _nvcc([nvcc, *flags, "-c", str(p), "-o", str(o)], verbose), SOURCES, compiled))
+            _nvcc([nvcc, *FLAGS, "-shared", *map(str, compiled), "-o", str(OUT)], verbose)
     build_fastcall(force)
     return OUT
 

@@ -16,12 +16,11 @@
 #include "peer_reduce.cuh"
 #include "dense_gemv.cuh"
 #include "decode_ops.cuh"
+#include "launch_utils.h"
 
 namespace {
 
 using namespace grb;
-
-int cuda_status(cudaError_t e) { return e == cudaSuccess ? GRB_OK : GRB_ERR_CUDA + int(e); }
 
 uint32_t batch_tile(uint32_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128; }
 
@@ -252,35 +251,6 @@ int dense_launch(const DenseArgs& a, uint32_t groups, uint32_t sms, cudaStream_t
   // 256-bit loads need rows that start on 32-byte boundaries and a whole number of 32-byte pieces per row
   const bool wide = (reinterpret_cast<uintptr_t>(a.w) & 31) == 0 && (a.ldw & 15) == 0 && (a.cols & 15) == 0;
   return wide ? dense_launch_as<M, true>(a, groups, sms, stream) : dense_launch_as<M, false>(a, groups, sms, stream);
-}
-
-// Launch of a decode-step kernel with programmatic stream serialisation: the kernel calls
-// griddepcontrol.launch_dependents and griddepcontrol.wait before anything else, so the kernel after it in the stream
-// (a fused linear, mostly) is set up and already streams its first weights on the SMs this one leaves idle, and every
-// kernel still sees the complete output of the one before it.
-template <class... Params, class... Args>
-int launch_step(void (*kernel)(Params...), dim3 grid, dim3 block, uint32_t smem_bytes, cudaStream_t stream, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem_bytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, Params(args)...));
-}
-
-// SM count of a device, looked up once.
-int device_sm_count(int dev) {
-  static std::mutex mu;
-  static int sms[64] = {0};
-  if (dev < 0 || dev >= 64) return 0;
-  std::lock_guard<std::mutex> lock(mu);
-  if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms[dev] = 0;
-  return sms[dev];
 }
 
 template <int ROWS, int RESIDUAL>

@@ -1,0 +1,55 @@
+// What the kernels of a decode step share: BF16 values in 32-bit words, programmatic launch order, warp-level matrix
+// instructions and the shared-memory layouts of their operands.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "device_utils.cuh"
+
+namespace grb {
+
+__device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+__device__ __forceinline__ float round_bf(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+__device__ __forceinline__ uint32_t pack_bf(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// First thing in every kernel of a step (they are launched with programmatic stream serialisation): let the next
+// kernel of the stream begin its set-up, then wait until the kernel before this one has finished and its writes are
+// visible.
+__device__ __forceinline__ void step_kernel_entry() {
+  grid_dependents_may_launch();
+  grid_dependency_wait();
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// D (16 x 8, FP32) += A (16 x 16, BF16, row) * B (16 x 8, BF16, col)
+__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Byte offset of 16-byte piece `piece` (0..15) of tile row `row` (256 bytes per row).
+__device__ __forceinline__ uint32_t attn_tile_offset(uint32_t row, uint32_t piece) {
+  return row * 256u + ((((piece ^ row) & 7u) | (piece & 8u)) << 4);
+}
+// Float index of (MMA row m, dimension d) in a warp's 16 x 128 block of the merge buffer: the columns of a row are
+// permuted by the row's low bits, which spreads a warp's accumulator stores (eight rows, same columns) over the banks.
+__device__ __forceinline__ uint32_t attn_merge_index(uint32_t m, uint32_t d) { return m * 128u + (d ^ ((m & 7u) << 2)); }
+
+}  // namespace grb

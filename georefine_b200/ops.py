@@ -5,6 +5,9 @@ Thin wrappers over the C ABI (``grb_rmsnorm_bf16``, ``grb_silu_mul_bf16``, ``grb
 the current stream, without allocating or synchronising, so a whole step can be captured in a CUDA graph.  They take the
 place of the reference's step kernels (``glc_serve/fastdec_kernels.cu:83-110,324-488``) for a plain grouped-query
 decoder with head dimension 128.
+
+``KVPages``, ``kv_write``, ``kv_read``, ``kv_keep`` and ``TreeAttention`` are speculative serving over a cache in BF16 or in 8 bits
+(``csrc/kv_cache.cuh``, ``csrc/tree_attention.cuh``); the reference has no counterparts.
 """
 from __future__ import annotations
 
@@ -94,3 +97,240 @@ class PagedAttention:
         step.scaling = 1.0 / math.sqrt(HEAD_DIM)
         st = _native.lib().grb_attn_decode_bf16(ctypes.byref(step), _stream(qkv))
         _native.check(st, "grb_attn_decode_bf16")
+
+
+# ---- a cache in BF16 or in 8 bits, and attention of causal rows and draft trees over it ---------------------------------
+
+KV_FORMATS = ("bf16", "e4m3")
+MASK_WORDS = 4        # of 64 nodes: the largest tree a row's mask describes
+TREE_ROWS = 4096      # rows of one call
+
+
+def _on(t, device, dtype, what, shape=None):
+    """Refuses a tensor that the kernels would read wrongly."""
+    if t.device != device or t.dtype != dtype:
+        raise ValueError(f"{what}: {t.dtype} on {t.device}, not {dtype} on {device}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, not {shape}")
+
+
+def _vector(t, device, what, n=None):
+    """A contiguous int32 vector's address."""
+    import torch
+
+    if t.dim() != 1 or (n is not None and t.shape[0] != n) or (t.shape[0] > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: a contiguous vector{'' if n is None else f' of {n}'} is wanted")
+    _on(t, device, torch.int32, what)
+    return t.data_ptr()
+
+
+def _launch(device, name, *args):
+    """The call on the device's current stream; a device that is not the current one is made so meanwhile."""
+    import torch
+
+    index = device.index
+    if index == torch.cuda.current_device():
+        _native.check(getattr(_native.lib(), name)(*args, _native.raw_stream(index)), name)
+    else:
+        with torch.cuda.device(index):
+            _native.check(getattr(_native.lib(), name)(*args, _native.raw_stream(index)), name)
+
+
+class KVPages:
+    """Keys and values of one layer, [pages, kv heads, 256, 128], or of a stack of layers ([layers, pages, ...], layers may be
+    strided): BF16, or ``float8_e4m3fn`` codes with an exponent byte per entry (128 values of one head at one position) in
+    ``k_exp`` and ``v_exp``, [pages, kv heads, 256] (see ``csrc/kv_cache.cuh`` for the format).  An object holds no copies."""
+
+    def __init__(self, k, v, k_exp=None, v_exp=None):
+        import torch
+
+        if k.dim() not in (4, 5) or tuple(k.shape[-2:]) != (PAGE, HEAD_DIM):
+            raise ValueError("pages are [pages, kv heads, 256, 128], or that with the layers in front")
+        if k.device.type != "cuda":
+            raise ValueError("pages live on a CUDA device")
+        self.format = {torch.bfloat16: "bf16", torch.float8_e4m3fn: "e4m3"}.get(k.dtype)
+        if self.format is None:
+            raise ValueError(f"pages are BF16 or e4m3, not {k.dtype}")
+        _on(v, k.device, k.dtype, "values", tuple(k.shape))
+        if (k_exp is None) != (self.format == "bf16") or (v_exp is None) != (self.format == "bf16"):
+            raise ValueError("exponents go with e4m3 pages, and with those alone")
+        for t, what in ((k, "keys"), (v, "values"), (k_exp, "exponents of keys"), (v_exp, "exponents of values")):
+            if t is None:
+                continue
+            if t is not k and t is not v:
+                _on(t, k.device, torch.uint8, what, tuple(k.shape[:-1]))
+            if not (t if k.dim() == 4 else t[0]).is_contiguous():
+                raise ValueError(f"{what}: the pages of a layer have to be contiguous")
+        if k.dim() == 5 and k.shape[0] > 1 and (k.stride(0) != v.stride(0) or (k_exp is not None and k_exp.stride(0) != v_exp.stride(0))):
+            raise ValueError("keys and values: layers are equally far apart")
+        self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
+        self.device, self.stacked = k.device, k.dim() == 5
+        self.pages, self.kv_heads = k.shape[-4], k.shape[-3]
+        stride = (k.stride(0), 0 if k_exp is None else k_exp.stride(0)) if self.stacked else (0, 0)
+        self._c = _native.KvPages(k.data_ptr(), v.data_ptr(), None if k_exp is None else k_exp.data_ptr(), None if v_exp is None else v_exp.data_ptr(),
+                                  *stride, k.shape[0] if self.stacked else 1, self.pages, self.kv_heads, KV_FORMATS.index(self.format))
+
+    @classmethod
+    def alloc(cls, pages: int, kv_heads: int, device, *, kv_format="bf16", layers=None):
+        """Empty pages (zeros)."""
+        import torch
+
+        if kv_format not in KV_FORMATS:
+            raise ValueError(f"the cache's format is one of {KV_FORMATS}")
+        shape = (() if layers is None else (int(layers),)) + (int(pages), int(kv_heads), PAGE, HEAD_DIM)
+        if kv_format == "bf16":
+            return cls(*(torch.zeros(shape, device=device, dtype=torch.bfloat16) for _ in range(2)))
+        return cls(*(torch.zeros(shape, device=device, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)),
+                   *(torch.zeros(shape[:-1], device=device, dtype=torch.uint8) for _ in range(2)))
+
+    def layer(self, i: int) -> "KVPages":
+        """One layer of a stack."""
+        pick = lambda t: None if t is None else t[i]
+        return KVPages(pick(self.k), pick(self.v), pick(self.k_exp), pick(self.v_exp))
+
+    @property
+    def entry_bytes(self) -> int:
+        """Bytes of the cache per position, key or value head."""
+        return 2 * HEAD_DIM if self.format == "bf16" else HEAD_DIM + 1
+
+
+def _table(page_table, device):
+    import torch
+
+    if page_table.dim() != 2 or page_table.shape[0] == 0 or page_table.shape[1] == 0 or page_table.stride(1) != 1:
+        raise ValueError("the page table is [slots, pages], its rows contiguous")
+    _on(page_table, device, torch.int32, "page table")
+    return _native.KvTable(page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1])
+
+
+def _kv_rows(name, k, v, row_seq, row_pos, page_table, pages):
+    import torch
+
+    if pages.stacked:
+        raise ValueError("rows go to one layer: give pages.layer(i)")
+    rows = row_seq.shape[0]
+    for t, what in ((k, "keys"), (v, "values")):
+        _on(t, pages.device, torch.bfloat16, what, (rows, pages.kv_heads, HEAD_DIM))
+        if rows and (t.stride(2) != 1 or t.stride(1) != HEAD_DIM):
+            raise ValueError(f"{what}: the heads of a row have to lie side by side")
+    args = _table(page_table, pages.device), _vector(row_seq, pages.device, "row_seq"), _vector(row_pos, pages.device, "row_pos", rows)
+    if rows:
+        _launch(pages.device, name, pages._c, *args, k.data_ptr(), max(k.stride(0), pages.kv_heads * HEAD_DIM), v.data_ptr(),
+                max(v.stride(0), pages.kv_heads * HEAD_DIM), rows)
+
+
+def kv_write(k, v, row_seq, row_pos, page_table, pages):
+    """Stores rows of keys and values ([rows, kv heads, 128] BF16, as they are: rotated already) at positions ``row_pos`` of the
+    sequences in slots ``row_seq``, quantised when the pages are.  Rows of slot -1 are left out."""
+    _kv_rows("grb_kv_write", k, v, row_seq, row_pos, page_table, pages)
+
+
+def kv_read(row_seq, row_pos, page_table, pages, k_out, v_out):
+    """Reads entries back as BF16 rows (exactly what they stand for).  Rows of slot -1 leave their outputs as they were."""
+    _kv_rows("grb_kv_read", k_out, v_out, row_seq, row_pos, page_table, pages)
+
+
+def kv_keep(slots, base, path, count, page_table, pages):
+    """What verified draft trees keep, in every layer of ``pages``: of sequence i, the entries at ``base[i] + path[i, j]`` go to
+    ``base[i] + j`` for j = 1 .. ``count[i]`` - 1.  ``path`` and ``count`` are the ``rows`` and ``count`` of
+    ``sampling.DraftVerifier`` (paths ascend).  A slot of -1 is left out."""
+    import torch
+
+    n = slots.shape[0]
+    if path.dim() != 2 or path.shape[0] != n or (path.shape[1] > 1 and path.stride(1) != 1):
+        raise ValueError("path is [sequences, nodes], its rows contiguous")
+    _on(path, pages.device, torch.int32, "path")
+    args = _table(page_table, pages.device), _vector(slots, pages.device, "slots"), _vector(base, pages.device, "base", n)
+    kept = _vector(count, pages.device, "count", n)
+    if n and path.shape[1]:
+        _launch(pages.device, "grb_kv_keep", pages._c, *args, path.data_ptr(), max(path.stride(0), path.shape[1]), kept, n, path.shape[1])
+
+
+class TreeRows:
+    """What makes rows nodes of draft trees: ``base`` (int32 [rows]): positions below it are seen by the row; ``rope`` (int32
+    [rows]): the row's rotary position, base + its depth; ``mask`` (int64 [rows, words], 1 to 4 words): bit j of word w says
+    that the row sees position base + 64 w + j.  A node's entry is stored at its ``row_pos``, mostly base + its number."""
+
+    def __init__(self, base, rope, mask):
+        import torch
+
+        rows = base.shape[0]
+        if mask.dim() != 2 or mask.shape[0] != rows or not 1 <= mask.shape[1] <= MASK_WORDS or (mask.shape[1] > 1 and mask.stride(1) != 1):
+            raise ValueError(f"mask is [rows, 1 to {MASK_WORDS} words], its rows contiguous")
+        _on(mask, base.device, torch.int64, "mask")
+        _vector(base, base.device, "base", rows)
+        _vector(rope, base.device, "rope", rows)
+        self.base, self.rope, self.mask, self.rows = base, rope, mask, rows
+
+    @staticmethod
+    def masks(parents, words=None):
+        """Depths and masks (Python integers, ``words`` of 64 bits each) of a tree given by its nodes' parents (-1: a root),
+        parents before children: every node sees its ancestors and itself."""
+        depth, seen = [], []
+        for i, p in enumerate(parents):
+            if not -1 <= p < i:
+                raise ValueError("a node's parent comes before it")
+            depth.append(0 if p < 0 else depth[p] + 1)
+            seen.append((1 << i) | (0 if p < 0 else seen[p]))
+        words = words or max(1, -(-len(parents) // 64))
+        if len(parents) > 64 * words or words > MASK_WORDS:
+            raise ValueError(f"{len(parents)} nodes do not fit {min(words, MASK_WORDS)} words")
+        signed = lambda m: m - (1 << 64) if m >> 63 else m
+        return depth, [[signed(m >> (64 * w) & ((1 << 64) - 1)) for w in range(words)] for m in seen]
+
+
+class TreeAttention:
+    """Attention over a cache in BF16 or 8 bits, for causal rows and for nodes of draft trees: scratch and geometry for up to
+    ``max_rows`` rows a call and ``max_pages`` pages a sequence; ``__call__`` runs rotary embedding, append and attention for one
+    layer.  Up to 16 query heads per kv head.  Calls that may run at the same time need an object each: they share its scratch."""
+
+    def __init__(self, nq: int, nkv: int, max_rows: int, max_pages: int, device, *, kv_format="bf16"):
+        import torch
+
+        if kv_format not in KV_FORMATS:
+            raise ValueError(f"the cache's format is one of {KV_FORMATS}")
+        if nq < 1 or nkv < 1 or nq % nkv or nq // nkv > 16:
+            raise ValueError("query heads per kv head: a whole number up to 16")
+        if not 1 <= max_rows <= TREE_ROWS or max_pages < 1:
+            raise ValueError(f"1 to {TREE_ROWS} rows and at least one page")
+        self.nq, self.nkv, self.max_rows, self.max_pages, self.format = nq, nkv, int(max_rows), int(max_pages), kv_format
+        self.scratch_bytes = _native.lib().grb_attn_tree_scratch_bytes(self.max_rows, nq, self.max_pages, KV_FORMATS.index(kv_format))
+        self.scratch = torch.empty(self.scratch_bytes, device=device, dtype=torch.uint8)
+        self.device = self.scratch.device
+
+    def __call__(self, qkv, cos, sin, row_seq, row_pos, page_table, pages, out, *, tree=None):
+        """``qkv`` (BF16 [rows, (nq + 2 nkv) 128]) -> ``out`` (BF16 [rows, nq 128]).  Keys (rotated) and values are stored at
+        ``row_pos`` of the sequences in slots ``row_seq`` before any row reads.  Without ``tree`` row r sees positions up to its
+        own; with ``TreeRows`` what they say, a row that sees nothing giving zeros.  Rows of slot -1 are left out."""
+        import torch
+
+        device, rows = self.device, qkv.shape[0]
+        if rows > self.max_rows or page_table.shape[1] > self.max_pages:
+            raise ValueError("more rows or pages than the scratch was sized for")
+        if pages.format != self.format or pages.stacked or pages.kv_heads != self.nkv or pages.device != device:
+            raise ValueError("pages of one layer, in this object's format, heads and device")
+        bf = torch.bfloat16
+        _on(qkv, device, bf, "qkv", (rows, (self.nq + 2 * self.nkv) * HEAD_DIM))
+        _on(out, device, bf, "out", (rows, self.nq * HEAD_DIM))
+        _on(cos, device, bf, "cos")
+        _on(sin, device, bf, "sin", tuple(cos.shape))
+        if cos.dim() != 2 or cos.shape[1] != HEAD_DIM or not cos.is_contiguous() or not sin.is_contiguous():
+            raise ValueError("rotary tables are contiguous [positions, 128]")
+        if not rows:
+            return
+        if qkv.stride(1) != 1 or out.stride(1) != 1:
+            raise ValueError("rows of qkv and out have to be contiguous")
+        step = _native.TreeStep()
+        step.qkv, step.ldq = qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1])
+        step.cos_table, step.sin_table, step.rope_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        step.row_seq, step.row_pos = _vector(row_seq, device, "row_seq", rows), _vector(row_pos, device, "row_pos", rows)
+        if tree is not None:
+            if tree.rows != rows or tree.base.device != device:
+                raise ValueError("tree rows: one for each row, on the same device")
+            step.row_base, step.row_rope, step.row_mask = tree.base.data_ptr(), tree.rope.data_ptr(), tree.mask.data_ptr()
+            step.ldm, step.mask_words = max(tree.mask.stride(0), tree.mask.shape[1]), tree.mask.shape[1]
+        step.pages, step.table = pages._c, _table(page_table, device)
+        step.scratch, step.scratch_bytes = self.scratch.data_ptr(), self.scratch_bytes
+        step.out, step.ldo = out.data_ptr(), max(out.stride(0), out.shape[1])
+        step.rows, step.nq, step.head_dim, step.scaling = rows, self.nq, HEAD_DIM, 1.0 / math.sqrt(HEAD_DIM)
+        _launch(device, "grb_attn_tree", step)

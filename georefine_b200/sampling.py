@@ -89,6 +89,73 @@ class Sampler:
         return accept_drafts(self.probabilities(logits), drafts, self.generator)
 
 
+class DraftVerifier:
+    """Verification of drafted tokens on the GPU (``csrc/verify_ops.cuh``), for up to ``max_rows`` rows of ``max_seqs`` sequences a
+    call: chains and trees, random numbers given by the caller, nothing brought to the host.  ``width``: columns of the outputs,
+    the longest walk (a walk stops after ``width`` - 1 kept drafts).  A call's outputs are the object's own and hold until its next
+    call; calls that may run at the same time need an object each."""
+
+    def __init__(self, max_rows: int, max_seqs: int, width: int, device):
+        import torch
+
+        if max_rows < 1 or max_seqs < 1 or not 1 <= width <= 256:
+            raise ValueError("at least one row and sequence, and a width of 1 to 256")
+        self.max_rows, self.max_seqs, self.width = int(max_rows), int(max_seqs), int(width)
+        self.stats = torch.empty(self.max_rows, 2, device=device, dtype=torch.float64)
+        self.tokens, self.rows = (torch.empty(self.max_seqs, self.width, device=device, dtype=torch.int32) for _ in range(2))
+        self.count = torch.empty(self.max_seqs, device=device, dtype=torch.int32)
+        self.device = self.stats.device
+
+    def __call__(self, logits, tokens, starts, u_keep, u_draw, *, temperature=1.0, parent=None, draft_probs=None):
+        """``logits`` (BF16 or FP32 [rows, vocabulary]): the target's, row i those behind node i.  Rows ``starts[s]`` ..
+        ``starts[s + 1] - 1`` are sequence s's draft tree: its pending token, then the drafts, parents before children;
+        ``tokens`` are the nodes' tokens, ``parent`` their parents' numbers within the sequence (None: chains).  With p =
+        softmax(logits / temperature) at a node, its child c is kept when u_keep[c] (1 - S) < p[t_c], S being the mass of the children's
+        tokens tried before; where none is kept, the last token is drawn from p without the tried ones: the lowest whose
+        cumulative mass exceeds u_draw[s] times what is left.  ``draft_probs`` (FP32 [rows, vocabulary], chains): row i is the
+        distribution that token i was drawn from; it is kept when u q[t] < p[t], else the draw is from max(p - q, 0).  Both leave
+        the tokens distributed as draws from the target.
+
+        Returns int32 (tokens [seqs, width]: the kept drafts, then the drawn token; rows [seqs, width]: the walk's nodes, the
+        root first; count [seqs]: how many of each), padded with -1."""
+        import torch
+
+        from . import _native
+        from .ops import _launch, _on, _vector
+
+        device, n = self.device, starts.shape[0] - 1
+        if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.device != device or (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise ValueError("logits are BF16 or FP32 [rows, vocabulary] on the verifier's device, their rows contiguous")
+        rows, vocab = logits.shape
+        if not 0 <= n <= self.max_seqs or rows > self.max_rows:
+            raise ValueError("more rows or sequences than the verifier was made for")
+        if not temperature > 0:
+            raise ValueError("temperature must be positive; temperature 0 is the arg-max path")
+        for t, size, what in ((u_keep, rows, "u_keep"), (u_draw, n, "u_draw")):
+            _on(t, device, torch.float32, what, (size,))
+            if size > 1 and t.stride(0) != 1:
+                raise ValueError(f"{what} has to be contiguous")
+        step = _native.VerifyStep()
+        if draft_probs is not None:
+            if parent is not None:
+                raise ValueError("the drafter's probabilities go with chains")
+            _on(draft_probs, device, torch.float32, "draft_probs", (rows, vocab))
+            if vocab > 1 and draft_probs.stride(1) != 1:
+                raise ValueError("rows of draft_probs have to be contiguous")
+            step.draft_probs, step.ldq = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
+        out = self.tokens[:n], self.rows[:n], self.count[:n]
+        step.tokens, step.starts = _vector(tokens, device, "tokens", rows), _vector(starts, device, "starts")
+        step.parent = None if parent is None else _vector(parent, device, "parent", rows)
+        if not n:
+            return out
+        step.logits, step.ldl, step.dtype = logits.data_ptr(), max(logits.stride(0), vocab), int(logits.dtype == torch.float32)
+        step.u_keep, step.u_draw, step.stats = u_keep.data_ptr(), u_draw.data_ptr(), self.stats.data_ptr()
+        step.out_tokens, step.out_rows, step.out_count = self.tokens.data_ptr(), self.rows.data_ptr(), self.count.data_ptr()
+        step.rows, step.seqs, step.vocab, step.width, step.temperature = rows, n, vocab, self.width, float(temperature)
+        _launch(device, "grb_verify_drafts", step)
+        return out
+
+
 def make_generator(device, seed=None):
     """A generator on ``device``; seeded when a seed is given, else from the system's entropy."""
     import torch

@@ -386,6 +386,99 @@ typedef struct grb_attn_step {
 } grb_attn_step;
 int grb_attn_decode_bf16(const grb_attn_step* step, void* cuda_stream);
 
+/* ---------------------------------------------------------------------------------------------------
+ * 6. Speculative serving over a paged KV cache in BF16 or in 8 bits: storing and reading entries, attention of causal rows and
+ *    of draft trees, verification of drafted tokens from given random numbers, keeping an accepted path.  The reference has no
+ *    counterparts.  No allocation, no host synchronisation; rows and sequences do not depend on what shares the call.
+ *
+ *    An entry is the 128 values of one key or value head at one position.  In 8 bits it is 128 e4m3 codes and one exponent
+ *    byte: with a = max |x|, e = clamp(ceil(log2(a / 448)), -40, 7), the code is the e4m3 number nearest to x 2^-e (ties to
+ *    even, at most 448), the byte e + 127, the value code 2^e.  An entry with an infinity or a NaN has byte 255 and codes 0 and
+ *    reads as NaN throughout.
+ *
+ *    A row with slot -1, or one whose place is outside the table or the pool, is left out: nothing is stored or read for it
+ *    and its output stays as it was.
+ * ------------------------------------------------------------------------------------------------- */
+#define GRB_KV_BF16 0
+#define GRB_KV_E4M3 1
+typedef struct grb_kv_pages {
+  void* k;                    /* [layers][pages][nkv][256][128] BF16 or e4m3 codes, layers layer_stride elements apart */
+  void* v;
+  uint8_t* k_exp;             /* GRB_KV_E4M3: [layers][pages][nkv][256], layers exp_stride bytes apart; else NULL */
+  uint8_t* v_exp;
+  int64_t layer_stride, exp_stride;
+  uint32_t layers, pages, nkv, format;
+} grb_kv_pages;
+typedef struct grb_kv_table {
+  const int32_t* table;       /* [slots][ld]: page of positions 256 i .. 256 i + 255 of a slot's sequence */
+  int64_t ld;
+  uint32_t slots, max_pages;
+} grb_kv_table;
+
+/* Rows of keys and values (BF16, [rows][ld], nkv heads of 128 side by side) into the first layer's pages, or out of them. */
+int grb_kv_write(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t* row_seq, const int32_t* row_pos, const void* k, int64_t ldk,
+                 const void* v, int64_t ldv, uint32_t rows, void* cuda_stream);
+int grb_kv_read(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t* row_seq, const int32_t* row_pos, void* k, int64_t ldk, void* v,
+                int64_t ldv, uint32_t rows, void* cuda_stream);
+/* What a verified tree keeps: for each of n sequences, in every layer, the entries at base + path[i] go to base + i, for
+ * i = 1 .. count - 1 (at most width - 1).  Paths ascend (path[i] >= i), which is how grb_verify_drafts returns them. */
+int grb_kv_keep(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t* seqs, const int32_t* base, const int32_t* path, int64_t ldp,
+                const int32_t* count, uint32_t n, uint32_t width, void* cuda_stream);
+
+/* One attention step: rotary embedding of query and key heads, append of keys and values at row_pos, attention in parts
+ * merged in part order.  row_base == NULL: causal rows, row r sees positions 0 .. row_pos[r] and turns by row_pos[r].
+ * Otherwise a draft tree: row r sees positions below row_base[r] and base + j for every bit j of its mask (its ancestors and
+ * itself), and turns by row_rope[r] (base + its depth).  A row that sees nothing gives zeros. */
+typedef struct grb_attn_tree_step {
+  const void* qkv;            /* BF16 [rows][ldq]: nq query heads | nkv key heads | nkv value heads */
+  int64_t ldq;
+  const void* cos_table;      /* BF16 [rope_rows][128], rotate-half convention */
+  const void* sin_table;
+  uint32_t rope_rows;
+  const int32_t* row_seq;
+  const int32_t* row_pos;
+  const int32_t* row_base;
+  const int32_t* row_rope;
+  const uint64_t* row_mask;   /* [rows][ldm], mask_words (1 to 4) words of 64 nodes */
+  int64_t ldm;
+  uint32_t mask_words;
+  grb_kv_pages pages;         /* of one layer */
+  grb_kv_table table;
+  void* scratch;              /* grb_attn_tree_scratch_bytes(rows, nq, max_pages, format), 16-byte aligned; no two calls at once */
+  uint64_t scratch_bytes;
+  void* out;                  /* BF16 [rows][ldo]: nq * 128 */
+  int64_t ldo;
+  uint32_t rows, nq, head_dim;   /* rows <= 4096; head_dim must be 128; nq / nkv <= 16 */
+  float scaling;              /* 1 / sqrt(head_dim) */
+} grb_attn_tree_step;
+uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pages, uint32_t format);
+int grb_attn_tree(const grb_attn_tree_step* step, void* cuda_stream);
+
+/* Drafted tokens against p = softmax(logits / temperature).  Rows starts[s] .. starts[s + 1] - 1 are sequence s's draft tree,
+ * parents before children; the first is the pending token.  At a node the children are tried in order: child c is kept when
+ * u_keep[c] (1 - S) < p[t_c], S the mass of the tokens tried before it (a token tried twice is not kept).  Where none is kept, the
+ * last token is drawn from p without the tried ones: the lowest t whose cumulative mass exceeds u_draw[s] times the whole.
+ * With draft_probs (chains only): kept when u q[t] < p[t], else the draw is from max(p - q, 0).  Where no mass is left, the
+ * last tried token comes out.  Random numbers lie in [0, 1).  A walk stops after width - 1 kept drafts. */
+typedef struct grb_verify_step {
+  const void* logits;         /* [rows][ldl], dtype 0: BF16, 1: FP32 */
+  int64_t ldl;
+  const int32_t* tokens;      /* [rows] */
+  const int32_t* parent;      /* [rows], index within the sequence; NULL: chains */
+  const int32_t* starts;      /* [seqs + 1] */
+  const float* u_keep;        /* [rows] */
+  const float* u_draw;        /* [seqs] */
+  const float* draft_probs;   /* [rows][ldq]: what row i's token was drawn from; NULL: tokens are certain */
+  int64_t ldq;
+  double* stats;              /* scratch [rows][2], 16-byte aligned */
+  int32_t* out_tokens;        /* [seqs][width]: kept drafts, then the drawn token, then -1 */
+  int32_t* out_rows;          /* [seqs][width]: the walk's nodes (0 first), then -1 */
+  int32_t* out_count;         /* [seqs]: nodes of the walk = emitted tokens; 0 for a sequence without rows */
+  uint32_t rows, seqs, vocab, width, dtype;   /* vocab <= 524288, width <= 256, at most 256 rows a sequence are looked at */
+  double temperature;
+} grb_verify_step;
+int grb_verify_drafts(const grb_verify_step* step, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
