@@ -76,6 +76,7 @@ class Sampler:
         self.temperature, self.top_p = float(temperature), float(top_p)
         _check(self.temperature, self.top_p)
         self.generator = make_generator(device, seed)
+        self._verifier = None
 
     def probabilities(self, logits):
         return probabilities(logits, self.temperature, self.top_p)
@@ -87,6 +88,22 @@ class Sampler:
     def accept(self, logits, drafts):
         """``logits``: len(drafts) + 1 rows of one sequence's verify pass."""
         return accept_drafts(self.probabilities(logits), drafts, self.generator)
+
+    def verify(self, logits, tokens, parents, starts):
+        """Draft trees of several sequences on the GPU: ``logits`` [rows, vocabulary] of all their nodes, sequence s's from row
+        ``starts[s]`` on (lists of Python integers, ``starts`` one longer than there are sequences), the pending token first;
+        ``parents`` within the sequence.  Returns ``DraftVerifier``'s (tokens, rows, count); the random numbers are the generator's."""
+        import torch
+
+        rows, seqs = logits.shape[0], len(starts) - 1
+        width = max(hi - lo for lo, hi in zip(starts, starts[1:]))
+        if self._verifier is None or rows > self._verifier.max_rows or seqs > self._verifier.max_seqs or width > self._verifier.width:
+            self._verifier = DraftVerifier(max(rows, 128), max(seqs, 128), min(256, max(width, 16)), logits.device)
+        if self.top_p < 1:          # the nucleus renormalised is the soft-max over its tokens alone
+            logits = logits.float().masked_fill(self.probabilities(logits) == 0, float("-inf"))
+        i32 = lambda v: torch.tensor(list(v), dtype=torch.int32).to(logits.device)
+        u = torch.rand(rows + seqs, generator=self.generator, device=logits.device)
+        return self._verifier(logits, i32(tokens), i32(starts), u[:rows], u[rows:], temperature=self.temperature, parent=i32(parents))
 
 
 class DraftVerifier:

@@ -15,6 +15,10 @@ linears with bitwise batch-invariant rows, per-row norm / attention / arg-max ke
 tokens alone, inside any batch, and as rows of a speculative verify pass.
 
 All per-sequence state is indexed by absolute position (KV pages), so a rewind is "set the position".
+
+Beyond the reference: the KV cache may be held in 8 bits (``BatchDecoder(kv_format="e4m3")``: about half the memory and traffic
+of a long context), and drafts may form trees that one pass checks (``Batcher.verify_trees``), both through
+``georefine_b200.ops.TreeAttention``.
 """
 from __future__ import annotations
 
@@ -216,20 +220,36 @@ class DecoderWeights:
         return int(sum(getattr(w, "coded_bytes", 0) for w in self.linears()))
 
 
+def kv_buffers(shape, device, kv_format):
+    """A cache [..., 256, 128] of zeros and, in 8 bits, its exponents [..., 256] (else None)."""
+    import torch
+
+    if kv_format == "bf16":
+        return torch.zeros(*shape, PAGE, ops.HEAD_DIM, device=device, dtype=torch.bfloat16), None
+    z = lambda *s: torch.zeros(*s, device=device, dtype=torch.uint8)
+    return z(*shape, PAGE, ops.HEAD_DIM).view(torch.float8_e4m3fn), z(*shape, PAGE)
+
+
 class BatchDecoder:
     """The whole-step engine: static buffers, a paged KV cache, one CUDA graph per (kind, row count).
 
     Rows of a step: row r is position ``row_pos[r]`` of the sequence in slot ``row_seq[r]`` and carries token
     ``tokens[r]``.  ``kind`` "ar": one row per sequence, and the step ends by feeding every row its own arg-max and
     advancing its position on the device, so consecutive replays need nothing from the host.  ``kind`` "verify": any
-    rows (prompt chunks, speculative drafts), no advance."""
+    rows (prompt chunks, speculative drafts), no advance.  ``kind`` "tree": rows that are nodes of draft trees
+    (``set_tree_rows``), no advance.
 
-    def __init__(self, weights: DecoderWeights, *, max_rows=128, max_slots=128, max_context=2304, device="cuda:0"):
+    ``kv_format`` "e4m3" holds the KV cache in 8 bits (129 bytes for an entry of 256, each value off by at most 2^-4 of
+    itself; the format is in ``csrc/kv_cache.cuh``)."""
+
+    def __init__(self, weights: DecoderWeights, *, max_rows=128, max_slots=128, max_context=2304, device="cuda:0", kv_format="bf16"):
         import torch
 
         cfg = weights.config
         if cfg.head_dim != ops.HEAD_DIM:
             raise ValueError("the attention kernels are written for head dimension 128")
+        if kv_format not in ops.KV_FORMATS:
+            raise ValueError(f"the cache's format is one of {ops.KV_FORMATS}")
         self.w, self.cfg, self.dev = weights, cfg, torch.device(device)
         self.max_rows, self.max_slots = int(max_rows), int(max_slots)
         self.pages_per_seq = -(-int(max_context) // PAGE)
@@ -237,13 +257,19 @@ class BatchDecoder:
         n_pages = self.max_slots * self.pages_per_seq + 1           # the last page: where padding rows write
         self.scratch_page, self.pad_slot = n_pages - 1, self.max_slots
         bf, i32 = torch.bfloat16, torch.int32
-        self.kv = torch.zeros(cfg.layers, 2, n_pages, cfg.local_kv_heads, PAGE, cfg.head_dim, device=self.dev, dtype=bf)
+        self.kv_format = kv_format
+        self.kv, self.kv_exp = kv_buffers((cfg.layers, 2, n_pages, cfg.local_kv_heads), self.dev, kv_format)
         self.page_table = torch.full((self.max_slots + 1, self.pages_per_seq), self.scratch_page, device=self.dev, dtype=i32)
         self._table_host = np.full((self.max_slots + 1, self.pages_per_seq), -1, dtype=np.int64)
         self._free_pages = list(range(n_pages - 2, -1, -1))
         self._free_slots = list(range(self.max_slots - 1, -1, -1))
         self.cos, self.sin = ops.rope_tables(self.max_context, cfg.rope_theta, self.dev)
-        self.attn = ops.PagedAttention(cfg.local_heads, cfg.local_kv_heads, self.max_rows, self.pages_per_seq, self.dev)
+        self._tree_attn = None
+        self.attn = self._pages = None
+        if kv_format == "bf16":
+            self.attn = ops.PagedAttention(cfg.local_heads, cfg.local_kv_heads, self.max_rows, self.pages_per_seq, self.dev)
+        else:
+            self._tree_attention()
         # Prompts may be taken in wider than a step, where nothing else is sized by the rows of a step: no peer buffers, no
         # linears of a caller's own.  Attention and logits keep the step's rows.
         wide = self.max_rows >= 128 and cfg.tp_world == 1 and all(isinstance(w, ResidentWeight) for w in weights.linears())
@@ -275,6 +301,33 @@ class BatchDecoder:
         self._staging, self._staged = [(torch.zeros(3, R, dtype=i32).pin_memory(), torch.cuda.Event()) for _ in range(STAGING)], 0
         self.graphs = {}
 
+    def _tree_attention(self):
+        """The attention over an 8-bit cache, and of draft trees over either; made on first use (scratch of its own)."""
+        import torch
+
+        if self._tree_attn is None:
+            cfg, R = self.cfg, self.max_rows
+            self._tree_attn = ops.TreeAttention(cfg.local_heads, cfg.local_kv_heads, R, self.pages_per_seq, self.dev, kv_format=self.kv_format)
+            exps = (None, None) if self.kv_exp is None else (self.kv_exp[:, 0], self.kv_exp[:, 1])
+            self.pages = ops.KVPages(self.kv[:, 0], self.kv[:, 1], *exps)                   # of the whole stack
+            self._pages = [self.pages.layer(i) for i in range(cfg.layers)]
+            z = lambda *shape, dtype: torch.zeros(*shape, device=self.dev, dtype=dtype)
+            words = min(ops.MASK_WORDS, -(-R // 64))
+            self.row_base, self.row_rope, self.row_mask = z(R, dtype=torch.int32), z(R, dtype=torch.int32), z(R, words, dtype=torch.int64)
+            self._tree_staging = [(torch.zeros(2, R, dtype=torch.int32).pin_memory(), torch.zeros(R, words, dtype=torch.int64).pin_memory(), torch.cuda.Event())
+                                  for _ in range(STAGING)]
+            self._tree_staged = 0
+        return self._tree_attn
+
+    def attend(self, layer: int, rows: slice, tree: bool = False) -> None:
+        """Attention of rows ``rows`` over one layer's cache, into ``ctx``."""
+        qkv, seq, pos, out = self.qkv[rows], self.row_seq[rows], self.row_pos[rows], self.ctx[rows]
+        if self.attn is not None and not tree:
+            self.attn(qkv, self.cos, self.sin, seq, pos, self.page_table, self.kv[layer, 0], self.kv[layer, 1], out)
+        else:
+            nodes = ops.TreeRows(self.row_base[rows], self.row_rope[rows], self.row_mask[rows]) if tree else None
+            self._tree_attention()(qkv, self.cos, self.sin, seq, pos, self.page_table, self._pages[layer], out, tree=nodes)
+
     # ---- sequence slots and pages (host bookkeeping; the device sees only the page table) ---------------------
     def open_slot(self) -> int:
         if not self._free_slots:
@@ -302,7 +355,7 @@ class BatchDecoder:
                 self.page_table[slot, p] = page
 
     # ---- the step ----------------------------------------------------------------------------------------------
-    def _trunk(self, n: int, advance: bool, head: int | None = 0) -> None:
+    def _trunk(self, n: int, advance: bool, head: int | None = 0, tree: bool = False) -> None:
         """One pass of rows 0..n-1 through the stack on the current stream; no allocation, no host synchronisation.
         ``head``: the first row that gets logits and an arg-max (as row 0 of theirs; None: no row does)."""
         import torch
@@ -315,9 +368,7 @@ class BatchDecoder:
             ops.rmsnorm(h, layer.norm1, x, delta=delta, eps=cfg.eps)       # (the previous layer's MLP output joins the stream here)
             self._linear(layer.qkv, x, self.qkv[:n])
             for lo in range(0, n, self.max_rows):       # (rows see positions up to their own: those of earlier slices are appended)
-                rows = slice(lo, min(n, lo + self.max_rows))
-                self.attn(self.qkv[rows], self.cos, self.sin, self.row_seq[rows], self.row_pos[rows], self.page_table, self.kv[i, 0],
-                          self.kv[i, 1], self.ctx[rows])
+                self.attend(i, slice(lo, min(n, lo + self.max_rows)), tree)
             self._row_parallel(layer.o, "o", self.ctx[:n], self.o_out[:n])
             ops.rmsnorm(h, layer.norm2, x, delta=self.o_out[:n], eps=cfg.eps)
             self._linear(layer.gate_up, x, self.gate_up[:n])
@@ -349,22 +400,23 @@ class BatchDecoder:
             self.peer.reduce(slot, out)
 
     def run(self, kind: str, n: int, *, graph: bool = True) -> None:
-        """Runs rows 0..n-1 ("ar" or "verify"); replays the step's CUDA graph, capturing it on first use."""
+        """Runs rows 0..n-1 ("ar", "verify" or "tree"); replays the step's CUDA graph, capturing it on first use."""
         import torch
 
-        if kind not in ("ar", "verify") or not 1 <= n <= self.max_rows:
-            raise ValueError("kind must be 'ar' or 'verify' and 1 <= n <= max_rows")
+        if kind not in ("ar", "verify", "tree") or not 1 <= n <= self.max_rows:
+            raise ValueError("kind must be 'ar', 'verify' or 'tree' and 1 <= n <= max_rows")
+        advance, tree = kind == "ar", kind == "tree"
         if not graph:
-            return self._trunk(n, kind == "ar")
+            return self._trunk(n, advance, tree=tree)
         key = (kind, n)
         if key not in self.graphs:
             saved = self.tokens.clone(), self.row_pos.clone()
-            self._trunk(n, kind == "ar")                                   # warm-up outside the capture (lazy initialisation)
+            self._trunk(n, advance, tree=tree)                             # warm-up outside the capture (lazy initialisation)
             self.tokens.copy_(saved[0]); self.row_pos.copy_(saved[1])
             torch.cuda.synchronize(self.dev)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
-                self._trunk(n, kind == "ar")
+                self._trunk(n, advance, tree=tree)
             self.tokens.copy_(saved[0]); self.row_pos.copy_(saved[1])      # the capture does not run, but keep the state explicit
             self.graphs[key] = g
         self.graphs[key].replay()
@@ -416,9 +468,32 @@ class BatchDecoder:
             dst[:n].copy_(src[:n], non_blocking=True)
         copied.record(torch.cuda.current_stream(self.dev))
 
+    def set_tree_rows(self, slots, positions, tokens, base, rope, masks) -> None:
+        """Queues rows that are nodes of draft trees: besides slot, position and token, ``base`` (positions below it are seen),
+        ``rope`` (the rotary position) and ``masks`` (words of 64 bits: which of the positions from base on are seen), as in
+        ``ops.TreeRows``.  Rows of slot -1 are padding."""
+        import torch
+
+        self._tree_attention()
+        n = len(slots)
+        self._queue(slots, positions, tokens, self.max_rows)
+        places, words, copied = self._tree_staging[self._tree_staged % STAGING]
+        self._tree_staged += 1
+        copied.synchronize()
+        places[:, :n].copy_(torch.tensor([list(base), list(rope)], dtype=torch.int32))
+        given = torch.tensor(masks, dtype=torch.int64)
+        if given.dim() != 2 or given.shape[0] != n or given.shape[1] > words.shape[1]:
+            raise ValueError(f"masks of {n} rows with up to {words.shape[1]} words")
+        words[:n].zero_()[:, :given.shape[1]].copy_(given)
+        self.row_base[:n].copy_(places[0, :n], non_blocking=True)
+        self.row_rope[:n].copy_(places[1, :n], non_blocking=True)
+        self.row_mask[:n].copy_(words[:n], non_blocking=True)
+        copied.record(torch.cuda.current_stream(self.dev))
+
     def streamed_bytes(self, rows_context) -> dict:
         """Bytes one step streams: the compressed weights, and the KV cache of rows whose contexts are given."""
-        kv = sum(int(c) for c in rows_context) * self.cfg.local_kv_heads * self.cfg.head_dim * 2 * 2 * self.cfg.layers
+        entry = self.cfg.head_dim + 1 if self.kv_format == "e4m3" else 2 * self.cfg.head_dim
+        kv = sum(int(c) for c in rows_context) * self.cfg.local_kv_heads * entry * 2 * self.cfg.layers
         return {"weights": self.w.streamed_bytes(), "kv": kv}
 
 
@@ -592,6 +667,76 @@ class Batcher:
         return out
 
 
+    def verify_trees(self, trees: dict, *, sampler=None):
+        """Speculation with a tree of drafts for every sequence in ``trees``: {slot: (tokens, parents)}, node j = 1, 2, ... being
+        ``tokens[j - 1]`` below node ``parents[j - 1]`` < j, and node 0 the sequence's pending token.  One pass over all nodes; a walk
+        from the root goes, at each node, to the first child that is kept, and emits one more token where none is.  Without a
+        sampler a child is kept when it is the target's arg-max there; with a ``sampling.Sampler`` with the probability the target
+        gives it among what was not refused before, on the GPU (``sampling.DraftVerifier``), which leaves the emitted tokens
+        distributed as plain sampling.  The cache entries of the walk move to consecutive positions in every layer.  Returns {slot:
+        emitted tokens}."""
+        import torch
+
+        d = self.d
+        self.sync_tokens()
+        slots, positions, tokens, base, rope, masks, parents, starts = [], [], [], [], [], [], [], [0]
+        for slot, (ts, ps) in trees.items():
+            s = self.active[slot]
+            if len(ts) != len(ps):
+                raise ValueError("a parent for every draft")
+            up = [-1] + [int(p) for p in ps]
+            if any(p < 0 for p in up[1:]):
+                raise ValueError("a draft hangs below the pending token (0) or an earlier draft")
+            depth, seen = ops.TreeRows.masks(up, words=min(ops.MASK_WORDS, -(-d.max_rows // 64)))
+            n, at = len(up), s["pos"]
+            d.ensure_pages(slot, at + n)
+            slots += [slot] * n
+            positions += range(at, at + n)
+            tokens += [s["tokens"][-1]] + [int(t) for t in ts]
+            base += [at] * n
+            rope += [at + x for x in depth]
+            masks += seen
+            parents += up
+            starts.append(len(slots))
+        rows, out = len(slots), {}
+        if not rows:
+            return out
+        if rows > d.max_rows:
+            raise ValueError("verify pass larger than the decoder's row buffers")
+        pad = bucket_for(rows, self.buckets) - rows
+        d.set_tree_rows(slots + [-1] * pad, positions + [0] * pad, tokens + [0] * pad, base + [0] * pad, rope + [0] * pad,
+                        masks + [[0] * len(masks[0])] * pad)
+        d.run("tree", rows + pad)
+        if sampler is None:
+            best = d.next_token[:rows].tolist()
+            emitted, walks = [], []
+            for lo, hi in zip(starts, starts[1:]):
+                walk, got = [0], []
+                while True:
+                    got.append(int(best[lo + walk[-1]]))
+                    child = next((j for j in range(walk[-1] + 1, hi - lo) if parents[lo + j] == walk[-1] and tokens[lo + j] == got[-1]), None)
+                    if child is None:
+                        break
+                    walk.append(child)
+                emitted.append(got)
+                walks.append(walk)
+            width = max(map(len, walks))
+            path = torch.tensor([w + [-1] * (width - len(w)) for w in walks], dtype=torch.int32).to(d.dev)
+            count = torch.tensor([len(w) for w in walks], dtype=torch.int32).to(d.dev)
+        else:
+            got, path, count = sampler.verify(d.logits[:rows], tokens, parents, starts)
+            emitted = [g[:n] for g, n in zip(got.tolist(), count.tolist())]
+        first = torch.tensor([[slots[lo], base[lo]] for lo in starts[:-1]], dtype=torch.int32).to(d.dev)
+        ops.kv_keep(first[:, 0].contiguous(), first[:, 1].contiguous(), path, count, d.page_table, d.pages)
+        for slot, new in zip(trees, emitted):
+            s = self.active[slot]
+            s["tokens"] += new
+            s["pos"] += len(new)
+            out[slot] = new
+        self._dirty = True
+        return out
+
+
 @dataclass
 class State:
     """A live sequence of a ``FastSession``: prompt length, the tokens generated so far, and the logits the prompt's
@@ -622,11 +767,11 @@ class FastSession:
 
     @classmethod
     def load(cls, *, package=None, config: DecoderConfig | None = None, weights: DecoderWeights | None = None, device="cuda:0",
-             max_len=4096, seed=1, lin_factory=None, tune=None, max_rows=128, **kw) -> "FastSession":
+             max_len=4096, seed=1, lin_factory=None, tune=None, max_rows=128, kv_format="bf16", **kw) -> "FastSession":
         """A session over ``weights``; or over the decoder of a BCTX ``package`` directory, filled from its frames alone
         (``georefine_b200.checkpoint``; the draft head too, as ``session.mtp_head``, when the package has ``mtp.*``
         tensors; ``cache=image_cache.ImageCache(...)`` keeps the resident images on disk for the next start); or over
-        random-init weights of ``config``."""
+        random-init weights of ``config``.  ``kv_format``: see ``BatchDecoder``."""
         source = None
         if weights is None and package is not None:
             from . import checkpoint
@@ -637,7 +782,7 @@ class FastSession:
             if config is None:
                 raise ValueError("package=, weights= or config= required")
             weights = DecoderWeights.synthetic(config, device, seed=seed, lin_factory=lin_factory, tune=tune, **kw)
-        session = cls(BatchDecoder(weights, max_rows=max_rows, max_slots=4, max_context=max_len, device=device))
+        session = cls(BatchDecoder(weights, max_rows=max_rows, max_slots=4, max_context=max_len, device=device, kv_format=kv_format))
         if source is not None:
             session.meta["receipt"] = weights.notes["receipt"]
             if source.has_mtp and weights.config.tp_world == 1:
@@ -654,10 +799,11 @@ class FastSession:
         return State(slot, len(ids), self.batcher.active[slot]["tokens"], self.d.logits[last_row].clone())
 
     def generate(self, st: State, *, max_tokens: int, stop_ids=(), temperature: float = 0.0, top_p: float = 1.0, seed=None,
-                 spec_k: int = 0, drafter=None):
+                 spec_k: int = 0, drafter=None, tree_drafter=None):
         """Yields up to ``max_tokens`` new tokens (the token the prefill produced counts as the first).  ``temperature``
         > 0 samples (``top_p`` < 1: from the nucleus); ``seed`` makes the draws reproducible, and a tensor-parallel
-        decoder needs one, the same on every rank, for the ranks to stay in step."""
+        decoder needs one, the same on every rank, for the ranks to stay in step.  ``tree_drafter(state)`` proposes a tree of drafts
+        instead of a chain: (tokens, parents) as ``Batcher.verify_trees`` takes them."""
         from .sampling import Sampler
 
         sampler = None
@@ -678,7 +824,9 @@ class FastSession:
             if seq["tokens"][0] in stops:
                 return
         while emitted < max_tokens:
-            if spec_k and drafter is not None:
+            if tree_drafter is not None:
+                new = self.batcher.verify_trees({st.slot: tree_drafter(st)}, sampler=sampler)[st.slot]
+            elif spec_k and drafter is not None:
                 new = self.batcher.verify({st.slot: drafter(st, spec_k)}, sampler=sampler)[st.slot]
             else:
                 new = [self.batcher.step(sampler=sampler, only=[st.slot])[st.slot]]
@@ -738,7 +886,8 @@ class MTPHead:
         self.d, self.fc, self.norm_e, self.norm_h, self.layer, self.final_norm = d, fc, norm_e, norm_h, layer, final_norm
         bf, R, H = torch.bfloat16, d.max_rows, cfg.hidden
         z = lambda *shape, dtype=bf: torch.zeros(*shape, device=d.dev, dtype=dtype)
-        self.kv = torch.zeros(2, d.kv.shape[2], cfg.kv_heads, PAGE, cfg.head_dim, device=d.dev, dtype=bf)
+        self.kv, exps = kv_buffers((2, d.kv.shape[2], cfg.kv_heads), d.dev, d.kv_format)
+        self.pages = None if exps is None else ops.KVPages(self.kv[0], self.kv[1], exps[0], exps[1])
         self.tok, self.hid = z(R, dtype=torch.int32), z(R, H)
         self.e, self.cat, self.z, self.x = z(R, H), z(R, 2 * H), z(R, H), z(R, H)
         self.qkv, self.ctx, self.o_out = z(R, cfg.qkv_rows), z(R, cfg.heads * cfg.head_dim), z(R, H)
@@ -780,7 +929,11 @@ class MTPHead:
         z, x = self.z[:n], self.x[:n]
         ops.rmsnorm(z, L.norm1, x, eps=cfg.eps)
         L.qkv(x, self.qkv[:n])
-        d.attn(self.qkv[:n], d.cos, d.sin, d.row_seq[:n], d.row_pos[:n], d.page_table, self.kv[0], self.kv[1], self.ctx[:n])
+        rows = self.qkv[:n], d.cos, d.sin, d.row_seq[:n], d.row_pos[:n], d.page_table
+        if self.pages is None:
+            d.attn(*rows, self.kv[0], self.kv[1], self.ctx[:n])
+        else:
+            d._tree_attention()(*rows, self.pages, self.ctx[:n])
         L.o(self.ctx[:n], self.o_out[:n])
         ops.rmsnorm(z, L.norm2, x, delta=self.o_out[:n], eps=cfg.eps)
         L.gate_up(x, self.gate_up[:n])
