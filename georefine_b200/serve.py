@@ -886,7 +886,7 @@ class MTPHead:
         self.d, self.fc, self.norm_e, self.norm_h, self.layer, self.final_norm = d, fc, norm_e, norm_h, layer, final_norm
         bf, R, H = torch.bfloat16, d.max_rows, cfg.hidden
         z = lambda *shape, dtype=bf: torch.zeros(*shape, device=d.dev, dtype=dtype)
-        self.kv, exps = kv_buffers((2, d.kv.shape[2], cfg.kv_heads), d.dev, d.kv_format)
+        self.kv, exps = kv_buffers((2, d.kv.shape[2], cfg.kv_heads), d.dev, getattr(d, "kv_format", "bf16"))
         self.pages = None if exps is None else ops.KVPages(self.kv[0], self.kv[1], exps[0], exps[1])
         self.tok, self.hid = z(R, dtype=torch.int32), z(R, H)
         self.e, self.cat, self.z, self.x = z(R, H), z(R, 2 * H), z(R, H), z(R, H)
