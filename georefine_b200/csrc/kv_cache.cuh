@@ -101,50 +101,97 @@ struct KvRowsArgs {
   uint32_t rows;
 };
 
-// Rows into the cache (READ false) or out of it (READ true).  A warp per (row, key or value head).
+// Rows into the cache (READ false) or out of it (READ true).  A warp takes eight neighbouring entries of a row (keys, then
+// values), two at a time with 16 bytes of BF16 a lane; all its loads are on their way before the first is used, which is what
+// keeps enough bytes in flight: one entry a warp, 8 bytes a lane, took 106 us for 32768 rows of 8 heads where memory needs 31.
+constexpr uint32_t kKvEntriesPerWarp = 8;
+
 template <bool READ, bool F8>
 __global__ void __launch_bounds__(kKvWarps * 32)
 kv_rows_kernel(const KvRowsArgs a) {
   step_kernel_entry();
-  const uint32_t lane = threadIdx.x & 31u, heads = 2 * a.pages.nkv;
+  constexpr int N = kKvEntriesPerWarp / 2;
+  const uint32_t lane = threadIdx.x & 31u, half = lane >> 4, l = lane & 15u, heads = 2 * a.pages.nkv;
+  const uint32_t per_row = (heads + kKvEntriesPerWarp - 1) / kKvEntriesPerWarp;
   const uint64_t at = uint64_t(blockIdx.x) * kKvWarps + (threadIdx.x >> 5);
-  const uint32_t row = uint32_t(at / heads), head = uint32_t(at % heads);
+  const uint32_t row = uint32_t(at / per_row), head0 = uint32_t(at % per_row) * kKvEntriesPerWarp + half;
   if (row >= a.rows) return;
   const int64_t place = kv_place(a.table, a.row_seq[row], a.row_pos[row]);
   if (place < 0) return;
-  const bool value = head >= a.pages.nkv;
-  const uint32_t h = value ? head - a.pages.nkv : head;
-  const size_t entry = kv_entry(place, a.pages.nkv, h);
-  uint2* rows = reinterpret_cast<uint2*>((value ? a.v + row * a.ldv : a.k + row * a.ldk) + h * kKvDim) + lane;
-  void* const pages = value ? a.pages.v : a.pages.k;
+  size_t entry[N];
+  bool value[N], in[N];
+  uint4* rows[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t head = head0 + 2 * i;
+    in[i] = head < heads;
+    value[i] = head >= a.pages.nkv;
+    const uint32_t h = value[i] ? head - a.pages.nkv : head;
+    entry[i] = kv_entry(place, a.pages.nkv, in[i] ? h : 0);
+    rows[i] = reinterpret_cast<uint4*>((value[i] ? a.v + row * a.ldv : a.k + row * a.ldk) + (in[i] ? h : 0) * kKvDim) + l;
+  }
   if constexpr (!F8) {
-    uint2* held = reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(pages) + entry * kKvDim) + lane;
-    if (READ) *rows = *held;
-    else *held = *rows;
+    uint4 x[N];
+    auto held = [&](int i) { return reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(value[i] ? a.pages.v : a.pages.k) + entry[i] * kKvDim) + l; };
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (in[i]) x[i] = READ ? *held(i) : *rows[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (in[i]) *(READ ? rows[i] : held(i)) = x[i];
   } else {
-    uint32_t* held = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(pages) + entry * kKvDim) + lane;
-    uint8_t* exps = value ? a.pages.v_exp : a.pages.k_exp;
-    if (READ) {
-      const uint32_t code = *held, byte = exps[entry];
-      const float s = kv_scale(byte);
-      const uint32_t lo = e4m3_to_half2(code & 0xFFFFu), hi = e4m3_to_half2(code >> 16);
-      const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&lo)), a1 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-      *rows = make_uint2(pack_bf(__fmul_rn(a0.x, s), __fmul_rn(a0.y, s)), pack_bf(__fmul_rn(a1.x, s), __fmul_rn(a1.y, s)));   // (exact: 4 bits)
+    auto held = [&](int i) { return reinterpret_cast<uint2*>(static_cast<uint8_t*>(value[i] ? a.pages.v : a.pages.k) + entry[i] * kKvDim) + l; };
+    auto exps = [&](int i) { return (value[i] ? a.pages.v_exp : a.pages.k_exp) + entry[i]; };
+    if constexpr (READ) {
+      uint2 code[N];
+      uint32_t byte[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (in[i]) { code[i] = *held(i); byte[i] = *exps(i); }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (!in[i]) continue;
+        const float s = kv_scale(byte[i]);
+        auto two = [&](uint32_t pair) {               // (exact: four bits times a power of two)
+          const uint32_t h = e4m3_to_half2(pair);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          return pack_bf(__fmul_rn(f.x, s), __fmul_rn(f.y, s));
+        };
+        *rows[i] = make_uint4(two(code[i].x & 0xFFFFu), two(code[i].x >> 16), two(code[i].y & 0xFFFFu), two(code[i].y >> 16));
+      }
     } else {
-      const uint2 r = *rows;
-      const float x[4] = {bf_lo(r.x), bf_hi(r.x), bf_lo(r.y), bf_hi(r.y)};
-      const uint32_t byte = kv_warp_byte(x);
-      *held = kv_codes(x[0], x[1], byte) | (kv_codes(x[2], x[3], byte) << 16);
-      if (lane == 0) exps[entry] = uint8_t(byte);
+      uint4 x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = in[i] ? *rows[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        // magnitudes of BF16 values compare as integers; an infinity or a NaN is above all others
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+        m = max(m & 0xFFFFu, m >> 16);
+#pragma unroll
+        for (int off = 8; off; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+        const uint32_t byte = kv_exp_byte(__uint_as_float(m << 16), m < 0x7F80u);
+        uint32_t c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = kv_codes(bf_lo(w[j]), bf_hi(w[j]), byte);
+        if (in[i]) {
+          *held(i) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+          if (l == 0) *exps(i) = uint8_t(byte);
+        }
+      }
     }
   }
 }
 
 // What a draft tree keeps: entry base + path[i] of a sequence goes to base + i, for i = 1 .. count - 1, in every layer, keys
 // and values.  Paths ascend, so an entry never lands on one that is still to be read (base + i <= base + path[i] <
-// base + path[i + 1]) as long as each batch is read before it is written.  Grid (layers * 2, sequences).
+// base + path[i + 1]) as long as each batch is read before it is written.  Grid (layers * 2 / 8, sequences): where an entry
+// lies is looked up once for eight planes, whose pieces are then in flight together (a plane a CTA: 29 us for what takes 11).
 constexpr int kKeepThreads = 256;
-constexpr int kKeepChunks = 4;      // 16-byte pieces a thread holds between a batch's reads and its writes
+constexpr int kKeepPlanes = 8;      // planes (a layer's keys or values) of a CTA, one 16-byte piece of each a thread at a time
 
 struct KvKeepArgs {
   KvPagesArgs pages;
@@ -161,47 +208,49 @@ template <bool F8>
 __global__ void __launch_bounds__(kKeepThreads)
 kv_keep_kernel(const KvKeepArgs a) {
   step_kernel_entry();
-  const uint32_t s = blockIdx.y, layer = blockIdx.x >> 1, tid = threadIdx.x;
-  const bool value = blockIdx.x & 1u;
+  const uint32_t s = blockIdx.y, tid = threadIdx.x, plane0 = blockIdx.x * kKeepPlanes, planes = min(uint32_t(kKeepPlanes), 2 * a.pages.layers - plane0);
   const int32_t count = min(a.count[s], int32_t(a.width)), seq = a.seqs[s], base = a.base[s];
   constexpr uint32_t kPieces = (F8 ? 1 : 2) * kKvDim / 16;       // of an entry
-  uint4* pages = reinterpret_cast<uint4*>(static_cast<uint8_t*>(value ? a.pages.v : a.pages.k) + layer * a.pages.layer_stride * (F8 ? 1 : 2));
-  uint8_t* exps = F8 ? (value ? a.pages.v_exp : a.pages.k_exp) + layer * a.pages.exp_stride : nullptr;
-  const uint32_t per_node = a.pages.nkv * kPieces, nodes = max(1u, kKeepThreads * kKeepChunks / per_node);
-  auto moved = [&](uint32_t i, int64_t& from, int64_t& to) {
-    const int32_t node = a.path[s * a.ldp + i];
-    if (node < 0 || base < 0 || node > 0x7FFFFFFF - base) return false;
-    from = kv_place(a.table, seq, base + node);
-    to = kv_place(a.table, seq, base + int32_t(i));
-    return from >= 0 && to >= 0 && from != to;
+  const uint32_t per_node = a.pages.nkv * kPieces, nodes = max(1u, kKeepThreads / per_node);
+  // plane p: keys (even) or values of layer p / 2
+  auto pieces = [&](uint32_t p) {
+    return reinterpret_cast<uint4*>(static_cast<uint8_t*>(p & 1u ? a.pages.v : a.pages.k) + int64_t(p >> 1) * a.pages.layer_stride * (F8 ? 1 : 2));
   };
+  auto exps = [&](uint32_t p) { return (p & 1u ? a.pages.v_exp : a.pages.k_exp) + int64_t(p >> 1) * a.pages.exp_stride; };
   for (int32_t first = 1; first < count; first += nodes) {
     const uint32_t items = min(nodes, uint32_t(count - first)) * per_node;
-    uint4 x[kKeepChunks];
-    uint32_t byte[kKeepChunks];
-    size_t dst[kKeepChunks];
-    bool on[kKeepChunks];
-    for (uint32_t round = 0; round < items; round += kKeepThreads * kKeepChunks) {   // (one round, but for more than 64 KV heads)
-#pragma unroll
-      for (int j = 0; j < kKeepChunks; ++j) {
-        const uint32_t item = round + tid + j * kKeepThreads, i = first + item / per_node, head = item % per_node / kPieces, piece = item % kPieces;
-        int64_t from = 0, to = 0;
-        on[j] = item < items && moved(i, from, to);
-        if (on[j]) {
-          const size_t src = kv_entry(from, a.pages.nkv, head);
-          dst[j] = kv_entry(to, a.pages.nkv, head);
-          x[j] = pages[src * kPieces + piece];
-          if (F8) byte[j] = exps[src];
+    for (uint32_t round = 0; round < items; round += kKeepThreads) {   // (one round, but for more heads than a batch has threads for)
+      const uint32_t item = round + tid, i = first + item / per_node, head = item % per_node / kPieces, piece = item % kPieces;
+      size_t src = 0, dst = 0;
+      bool on = item < items;
+      if (on) {
+        const int32_t node = a.path[s * a.ldp + i];
+        on = node >= 0 && base >= 0 && node <= 0x7FFFFFFF - base;
+        const int64_t from = on ? kv_place(a.table, seq, base + node) : -1, to = on ? kv_place(a.table, seq, base + int32_t(i)) : -1;
+        on = from >= 0 && to >= 0 && from != to;
+        if (on) {
+          src = kv_entry(from, a.pages.nkv, head);
+          dst = kv_entry(to, a.pages.nkv, head);
         }
       }
-      __syncthreads();
+      uint4 x[kKeepPlanes];
+      uint8_t byte[kKeepPlanes];
+      if (on) {
 #pragma unroll
-      for (int j = 0; j < kKeepChunks; ++j) {
-        const uint32_t piece = (round + tid + j * kKeepThreads) % kPieces;
-        if (on[j]) {
-          pages[dst[j] * kPieces + piece] = x[j];
-          if (F8 && piece == 0) exps[dst[j]] = uint8_t(byte[j]);
-        }
+        for (int p = 0; p < kKeepPlanes; ++p)
+          if (uint32_t(p) < planes) {
+            x[p] = pieces(plane0 + p)[src * kPieces + piece];
+            if (F8 && piece == 0) byte[p] = exps(plane0 + p)[src];
+          }
+      }
+      __syncthreads();
+      if (on) {
+#pragma unroll
+        for (int p = 0; p < kKeepPlanes; ++p)
+          if (uint32_t(p) < planes) {
+            pieces(plane0 + p)[dst * kPieces + piece] = x[p];
+            if (F8 && piece == 0) exps(plane0 + p)[dst] = byte[p];
+          }
       }
       __syncthreads();
     }

@@ -43,8 +43,7 @@ int kv_rows(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t*
   if (int st = pages_of(pages, a.pages)) return st;
   if (int st = table_of(table, a.pages, a.table)) return st;
   const int64_t width = int64_t(a.pages.nkv) * kKvDim;
-  if (!row_seq || !row_pos || !k || !v || ldk < width || ldv < width || (ldk & 3) || (ldv & 3) || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 7))
-    return GRB_ERR_ARGUMENT;
+  if (!row_seq || !row_pos || !k || !v || ldk < width || ldv < width || (ldk & 7) || (ldv & 7) || !aligned16(k) || !aligned16(v)) return GRB_ERR_ARGUMENT;
   if (!rows) return GRB_OK;
   a.row_seq = row_seq;
   a.row_pos = row_pos;
@@ -53,7 +52,7 @@ int kv_rows(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t*
   a.ldk = ldk;
   a.ldv = ldv;
   a.rows = rows;
-  const uint64_t ctas = (uint64_t(rows) * 2 * a.pages.nkv + kKvWarps - 1) / kKvWarps;
+  const uint64_t warps = uint64_t(rows) * ((2 * a.pages.nkv + kKvEntriesPerWarp - 1) / kKvEntriesPerWarp), ctas = (warps + kKvWarps - 1) / kKvWarps;
   if (ctas > 0x7FFFFFFFull) return GRB_ERR_UNSUPPORTED;
   const auto kernel = pages->format == GRB_KV_E4M3 ? kv_rows_kernel<READ, true> : kv_rows_kernel<READ, false>;
   return launch_step(kernel, dim3(uint32_t(ctas)), dim3(kKvWarps * 32), 0, static_cast<cudaStream_t>(stream), a);
@@ -102,9 +101,11 @@ int launch_clusters(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint
 
 template <bool F32, bool VEC>
 int verify_launch(const VerifyArgs& a, cudaStream_t stream) {
-  if (int st = launch_clusters(verify_rows_kernel<F32, VEC>, dim3(kVerifyCluster, a.rows), kVerifyThreads, 0, kVerifyCluster, stream, a)) return st;
-  const uint32_t smem = (a.vocab + 255) / 256 * 4;
-  return launch_clusters(verify_draw_kernel<F32, VEC>, dim3(kVerifyCluster, a.seqs), kVerifyThreads, smem, kVerifyCluster, stream, a);
+  if (int st = launch_step(verify_rows_kernel<F32, VEC>, dim3(kVerifySlices, a.rows), dim3(kVerifyThreads), 0, stream, a)) return st;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return GRB_ERR_CUDA;
+  const uint32_t resident = 2 * uint32_t(device_sm_count(dev)), cluster = a.seqs * 8 <= resident ? 8 : a.seqs * 4 <= resident ? 4 : 2;
+  return launch_clusters(verify_draw_kernel<F32, VEC>, dim3(cluster, a.seqs), kVerifyDrawThreads, (a.vocab + 255) / 256 * 4, cluster, stream, a);
 }
 
 }  // namespace
@@ -136,7 +137,7 @@ int grb_kv_keep(const grb_kv_pages* pages, const grb_kv_table* table, const int3
   a.ldp = ldp;
   a.width = width;
   const auto kernel = pages->format == GRB_KV_E4M3 ? kv_keep_kernel<true> : kv_keep_kernel<false>;
-  return launch_step(kernel, dim3(a.pages.layers * 2, n), dim3(kKeepThreads), 0, static_cast<cudaStream_t>(cuda_stream), a);
+  return launch_step(kernel, dim3((a.pages.layers * 2 + kKeepPlanes - 1) / kKeepPlanes, n), dim3(kKeepThreads), 0, static_cast<cudaStream_t>(cuda_stream), a);
 }
 
 uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pages, uint32_t format) {

@@ -6,7 +6,7 @@
 // Where none is kept, the last token is drawn from p without the tried ones: the first t whose cumulative mass exceeds
 // u_draw times the whole.  With the drafter's own probabilities q (chains): kept when u q[t] < p[t], else drawn from max(p - q, 0).
 //
-// Two launches.  verify_rows: maximum and sum of every row in one pass over the logits - this is where the time goes, and memory
+// Two launches.  verify_rows: sums of every row's eighths in one pass over the logits - this is where the time goes, and memory
 // bounds it.  verify_draw: a cluster per sequence walks the tree and draws from the one row where the walk ends.  A draw has a
 // border at every token, so the masses there are summed in 64 bits: in 32 the borders of a flat distribution over 150000 tokens
 // move by per mille of a token's width.  Rows and sequences are computed on their own, in a fixed order.
@@ -20,11 +20,12 @@
 namespace grb {
 
 constexpr uint32_t kVerifyMaxNodes = 256;      // rows of one sequence
-constexpr uint32_t kVerifyCluster = 8;
+constexpr uint32_t kVerifyRegions = 128;       // runs of tiles that verify_draw sums: cut by the vocabulary alone
+constexpr uint32_t kVerifySlices = 8;          // CTAs of a row in verify_rows
 constexpr uint32_t kVerifyThreads = 256;
+constexpr uint32_t kVerifyDrawThreads = 512;
 constexpr uint32_t kVerifyTile = 256;          // tokens a warp takes at a time, eight consecutive ones a lane
-constexpr uint32_t kVerifyWarps = kVerifyCluster * kVerifyThreads / 32;
-constexpr uint32_t kVerifyMaxVocab = kVerifyWarps * 32 * kVerifyTile;
+constexpr uint32_t kVerifyMaxVocab = 524288;
 
 struct VerifyArgs {
   const void* logits;       // [rows][ldl] BF16 or FP32
@@ -36,7 +37,7 @@ struct VerifyArgs {
   const float* u_draw;      // [seqs]
   const float* q;           // [rows][ldq] or null: what row i's token was drawn from
   int64_t ldq;
-  double2* stats;           // scratch [rows]: maximum, sum of exp((l - maximum) / T)
+  double2* stats;           // scratch [rows][8]: (R, Z) of an eighth of the row: Z = sum of 2^(l[t] log2_scale - R) over it
   int32_t* out_tokens;      // [seqs][width]
   int32_t* out_rows;        // [seqs][width]
   int32_t* out_count;       // [seqs]
@@ -49,9 +50,9 @@ __device__ __forceinline__ float verify_logit(const void* row, uint32_t t) {
   if constexpr (F32) return static_cast<const float*>(row)[t];
   else return __bfloat162float(static_cast<const __nv_bfloat16*>(row)[t]);
 }
-// Eight consecutive logits from t (a multiple of 8); beyond the vocabulary -infinity.  VEC: rows start on 16-byte boundaries.
+// Eight consecutive values from t (a multiple of 8), `beyond` outside the vocabulary.  VEC: rows start on 16-byte boundaries.
 template <bool F32, bool VEC>
-__device__ __forceinline__ void verify_load8(const void* row, uint32_t t, uint32_t vocab, float (&x)[8]) {
+__device__ __forceinline__ void verify_load8(const void* row, uint32_t t, uint32_t vocab, float (&x)[8], float beyond = -INFINITY) {
   if (VEC && t + 8 <= vocab) {
     if constexpr (F32) {
       const float4 a = reinterpret_cast<const float4*>(static_cast<const float*>(row) + t)[0], b = reinterpret_cast<const float4*>(static_cast<const float*>(row) + t)[1];
@@ -65,7 +66,7 @@ __device__ __forceinline__ void verify_load8(const void* row, uint32_t t, uint32
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = t + i < vocab ? verify_logit<F32>(row, t + i) : -INFINITY;
+  for (int i = 0; i < 8; ++i) x[i] = t + i < vocab ? verify_logit<F32>(row, t + i) : beyond;
 }
 template <bool F32>
 __device__ __forceinline__ const void* verify_row(const VerifyArgs& a, uint32_t row) {
@@ -78,76 +79,132 @@ __device__ __forceinline__ double lds_f64_cluster(uint32_t a) {
   return v;
 }
 
-// (maximum, sum under it) of two shares
-struct VerifyShare {
-  float max;
-  double sum;
+// Eight consecutive logits as they are loaded, -infinity beyond the vocabulary.
+template <bool F32>
+struct VerifyOctet;
+template <>
+struct VerifyOctet<false> {
+  uint32_t w[4];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const void* row, uint32_t t, uint32_t vocab) {
+    const auto* p = static_cast<const __nv_bfloat16*>(row) + t;
+    if (VEC && t + 8 <= vocab) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+      return;
+    }
+    const auto* u = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (t + 2 * i < vocab ? u[2 * i] : 0xFF80u) | (t + 2 * i + 1 < vocab ? uint32_t(u[2 * i + 1]) << 16 : 0xFF800000u);
+  }
+  __device__ __forceinline__ float max(float m) const {
+    uint32_t x = w[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(x) : "r"(w[i]));
+    return fmaxf(m, fmaxf(bf_lo(x), bf_hi(x)));
+  }
+  __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf_hi(w[i >> 1]) : bf_lo(w[i >> 1]); }
 };
-// 2^(d scale) for d <= 0, the product to 2^-24 of itself.  (-infinity times the scale's low part may have either sign.)
-__device__ __forceinline__ float verify_exp(float d, float scale_hi, float scale_lo) {
-  d = fmaxf(d, -1e30f);
-  return exp2_approx(__fmaf_rn(d, scale_hi, __fmul_rn(d, scale_lo)));
-}
-__device__ __forceinline__ VerifyShare verify_join(VerifyShare x, VerifyShare y, float hi, float lo) {
-  const float m = fmaxf(x.max, y.max);
-  if (m == -INFINITY) return x;
-  return {m, x.sum * double(verify_exp(__fsub_rn(x.max, m), hi, lo)) + y.sum * double(verify_exp(__fsub_rn(y.max, m), hi, lo))};
-}
+template <>
+struct VerifyOctet<true> {
+  float x[8];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const void* row, uint32_t t, uint32_t vocab) { verify_load8<true, VEC>(row, t, vocab, x); }
+  __device__ __forceinline__ float max(float m) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, x[i]);
+    return m;
+  }
+  __device__ __forceinline__ float operator[](int i) const { return x[i]; }
+};
 
-// Grid (8, rows), clusters of 8: each CTA takes an eighth of the row.  Eight exponentials are added in 32 bits, the eights in 64:
-// a probability is then off by its exponentials' rounding alone, 2^-22 at most, which is what a comparison with u_keep can feel.
+// Grid (8, rows): each CTA takes an eighth of the row, a thread up to ten octets of it at a time (all of its share of 152064
+// BF16 logits), loaded together: the CTA's maximum of them, then one multiply-add, one exponential and one addition each.
+// Bound by memory, the exponentials (16 per SM and cycle) not far behind.  The eighths are put together by whoever needs the
+// row: doing it here, in a cluster, left the SMs waiting for chains of exponentials and remote reads (54 us for 546 rows).
+// The exponent l hi - c (hi: log2_scale rounded to 32 bits, c: that of the maximum m, rounded) is rounded once; what hi leaves
+// out, l (log2_scale - hi), is taken for m in R, which leaves (l - m) 2^-25 of a weight that falls with l - m.  Eight
+// exponentials are added in 32 bits, the eights in 64: a probability is off by the exponentials' 2^-22 at most.
 template <bool F32, bool VEC>
 __global__ void __launch_bounds__(kVerifyThreads)
 verify_rows_kernel(const VerifyArgs a) {
   step_kernel_entry();
-  __shared__ VerifyShare shares[kVerifyThreads / 32];
-  __shared__ __align__(8) double mine[2];
+  constexpr int B = F32 ? 3 : 5;
+  __shared__ float tops[kVerifyThreads / 32];
+  __shared__ double sums[kVerifyThreads / 32];
   const uint32_t row = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const void* const src = verify_row<F32>(a, row);
-  const float hi = float(a.log2_scale), lo = float(a.log2_scale - double(hi));
-  const uint32_t octets = (a.vocab + 7) / 8, per = (octets + kVerifyCluster - 1) / kVerifyCluster;
-  const uint32_t first = blockIdx.x * per, last = min(octets, first + per);
-  VerifyShare s{-INFINITY, 0.0};
-  for (uint32_t o = first + tid; o < last; o += kVerifyThreads) {
-    float x[8];
-    verify_load8<F32, VEC>(src, o * 8, a.vocab, x);
-    float m = s.max;
+  const float hi = float(a.log2_scale);
+  const uint32_t octets = (a.vocab + 7) / 8, per = (octets + kVerifySlices - 1) / kVerifySlices;
+  const uint32_t first = min(octets, blockIdx.x * per), last = min(octets, first + per);
+  float m = -INFINITY, c = -INFINITY;
+  double sum = 0.0;
+#pragma unroll 1
+  for (uint32_t o0 = first + tid; o0 < last; o0 += B * kVerifyThreads) {
+    VerifyOctet<F32> x[B];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, x[i]);
-    if (m == -INFINITY) continue;
-    if (m > s.max) {
-      s.sum *= double(verify_exp(__fsub_rn(s.max, m), hi, lo));
-      s.max = m;
+    for (int b = 0; b < B; ++b) x[b].template load<VEC>(src, (o0 + b * kVerifyThreads < last ? o0 + b * kVerifyThreads : octets) * 8, a.vocab);
+    float top = m;
+#pragma unroll
+    for (int b = 0; b < B; ++b) top = x[b].max(top);
+    if (top == -INFINITY) continue;
+    if (top > m) {
+      const float was = c;
+      m = top;
+      c = __fmul_rn(m, hi);
+      sum *= double(exp2_approx(__fsub_rn(was, c)));
     }
-    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = __fadd_rn(sum, verify_exp(__fsub_rn(x[i], m), hi, lo));
-    s.sum += double(sum);
-  }
+    for (int b = 0; b < B; ++b) {
+      float eight = 0.f;
 #pragma unroll
-  for (int off = 16; off; off >>= 1) {
-    const VerifyShare o{__shfl_xor_sync(0xFFFFFFFFu, s.max, off), __shfl_xor_sync(0xFFFFFFFFu, s.sum, off)};
-    s = verify_join(s, o, hi, lo);
+      for (int i = 0; i < 8; ++i) eight = __fadd_rn(eight, exp2_approx(__fmaf_rn(x[b][i], hi, -c)));
+      sum += double(eight);
+    }
   }
-  if (lane == 0) shares[warp] = s;
+  // all under the CTA's maximum (c belongs to m: the same m gives the same c)
+  float top = warp_max(m);
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < int(kVerifyThreads / 32); ++w) top = fmaxf(top, tops[w]);
+  const float all = __fmul_rn(top, hi);
+  if (m < top) sum *= double(exp2_approx(__fsub_rn(c, all)));
+#pragma unroll
+  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+  if (lane == 0) sums[warp] = sum;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < int(kVerifyThreads / 32); ++w) s = verify_join(s, shares[w], hi, lo);
-    mine[0] = double(s.max);
-    mine[1] = s.sum;
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < int(kVerifyThreads / 32); ++w) sum += sums[w];
+    a.stats[size_t(row) * kVerifySlices + blockIdx.x] = make_double2(top == -INFINITY ? -INFINITY : double(all) + double(top) * (a.log2_scale - double(hi)), sum);
   }
-  cluster_sync();
-  if (blockIdx.x == 0 && tid == 0) {
-    for (uint32_t r = 1; r < kVerifyCluster; ++r) {
-      const uint32_t at = cluster_map(smem_u32(mine), r);
-      s = verify_join(s, VerifyShare{float(lds_f64_cluster(at)), lds_f64_cluster(at + 8)}, hi, lo);
-    }
-    a.stats[row] = make_double2(double(s.max), s.sum);
-  }
-  cluster_sync();                                   // (a CTA may not leave while its share is read)
 }
 
-__device__ __forceinline__ double shfl_up_f64(double v, int off) { return __shfl_up_sync(0xFFFFFFFFu, v, off); }
+// 2^y for -101 < y < 1 to 2^-42: y = k / 16 + f, 2^(k / 16) from a table and a shift, 2^f by the first six terms of the
+// exponential series in f ln 2 (|f| <= 2^-5: the seventh is 1.4e-13).  Sixteen entries lie in as many pairs of banks, so a warp's
+// look-ups never collide; with 64 of them and one term less they did, and took three quarters of the kernel's time.
+constexpr uint32_t kExpTable = 16;
+__device__ __forceinline__ double exp2_f64(double y, const double* table) {
+  constexpr double kRound = 6755399441055744.0;     // 1.5 * 2^52: what is added to it rounds to a whole number in its low bits
+  const double t = __fma_rn(y, double(kExpTable), kRound);
+  const int k = __double2loint(t);                  // (whole and fraction: the bits above and below the table's)
+  const double f = __fma_rn(t - kRound, -1.0 / kExpTable, y);
+  double q = __fma_rn(f, 0.0013333558146428441, 0.009618129107628477);  // ln2^5 / 120, ln2^4 / 24
+  q = __fma_rn(f, q, 0.05550410866482158);                              // ln2^3 / 6
+  q = __fma_rn(f, q, 0.2402265069591007);                               // ln2^2 / 2
+  q = __fma_rn(f, q, 0.6931471805599453);
+  const double r = table[k & int(kExpTable - 1)] * __fma_rn(f, q, 1.0);
+  return __hiloint2double(__double2hiint(r) + ((k & -int(kExpTable)) << 16), __double2loint(r));
+}
+
+// x 2^-896 in 64 bits, for a finite x, by integer operations (conversions between the two widths run at a quarter of their rate);
+// a zero or a subnormal becomes some number below 2^-1022.
+__device__ __forceinline__ double widen(float x) {
+  const int u = __float_as_int(x);
+  return __hiloint2double((u >> 3) & int(0x8FFFFFFFu), int(uint32_t(u) << 29));
+}
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
   for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
@@ -157,37 +214,38 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 __device__ __forceinline__ double warp_scan_f64(double v, uint32_t lane) {
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const double o = shfl_up_f64(v, off);
+    const double o = __shfl_up_sync(0xFFFFFFFFu, v, off);
     if (lane >= uint32_t(off)) v += o;
   }
   return v;
 }
 
-// What verify_draw draws from: eight consecutive tokens' masses.
-template <bool F32, bool VEC>
+// What verify_draw draws from: masses of a row's tokens.  A mass below 2^-100 of the likeliest token's counts as that much, which no
+// draw can feel (a draw's target is at least 2^-75): that saves a comparison and a selection a token.
+constexpr double kLeastMass = 8.077935669463161e-28, kLeastTarget = 2.6469779601696886e-23;    // 2^-90, 2^-75
 struct VerifyMasses {
-  const void* row;
   const float* q;           // refused draft's distribution, or null
-  const uint32_t* struck;   // one bit for every eight tokens that hold a tried one
   const int32_t* tried;     // the tried tokens
+  const double* table;
   uint32_t tried_count, vocab;
-  double maximum, scale, total;   // total: of the masses without q, where q is subtracted
+  bool q_vec;               // rows of q start on 16-byte boundaries
+  float least;              // the logit of 2^-100 of the likeliest
+  double ref, scale, inverse;   // scale: times 2^896; inverse: of the sum of the masses without q, where q is subtracted
 
-  __device__ __forceinline__ void whole(uint32_t t, double (&m)[8]) const {
-    float x[8];
-    verify_load8<F32, VEC>(row, t, vocab, x);
+  // Eight consecutive tokens from t.  `plain`: without q.  `some`: of them were tried.  (No branch between the exponentials: each
+  // is a chain of a dozen dependent operations, and only side by side do they keep the unit busy.)
+  template <bool F32>
+  __device__ __forceinline__ void eight(const VerifyOctet<F32>& x, uint32_t t, bool plain, bool some, double (&m)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double y = (double(x[i]) - maximum) * scale;
-      m[i] = y > -100.0 ? exp2(y) : 0.0;           // below 2^-100 of the likeliest: none
-    }
-  }
-  __device__ __forceinline__ void operator()(uint32_t t, double (&m)[8]) const {
-    whole(t, m);
-    if (q) {
+    for (int i = 0; i < 8; ++i) m[i] = exp2_f64(__fma_rn(widen(fmaxf(x[i], least)), scale, -ref), table);
+    if (q && !plain) {
+      float o[8];
+      if (q_vec) verify_load8<true, true>(q, t, vocab, o, 0.f);
+      else verify_load8<true, false>(q, t, vocab, o, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m[i] = t + i < vocab ? fmax(m[i] / total - double(q[t + i]), 0.0) : 0.0;
-    } else if (struck[t >> 8] >> ((t >> 3) & 31u) & 1u) {
+      for (int i = 0; i < 8; ++i) m[i] = fmax(__fma_rn(m[i], inverse, -double(o[i])), 0.0);
+    } else if (some && !q) {
+#pragma unroll 1
       for (uint32_t j = 0; j < tried_count; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -196,18 +254,26 @@ struct VerifyMasses {
   }
 };
 
-// Grid (8, sequences), clusters of 8.
+// Grid (CTAs of a sequence, sequences), a cluster per sequence: every warp of the cluster sums its regions of the row in 64 bits;
+// the sums are exchanged, and the warp in whose region the draw falls goes through it again, tile by tile.  All three passes
+// (the middle one for every draw, the first where q is subtracted, the last) run the same loop: unrolled, or written out for each,
+// the kernel was bound by the fetching of its own instructions (30 us for one sequence instead of 9).
+// The cluster is as large (8, 4 or 2 CTAs) as lets all sequences be resident at once: a CTA's chain of dependent loads and
+// barriers is 9 us long, so a second wave costs more than the larger share of a CTA in the first.
 template <bool F32, bool VEC>
-__global__ void __launch_bounds__(kVerifyThreads)
+__global__ void __launch_bounds__(kVerifyDrawThreads, 2)
 verify_draw_kernel(const VerifyArgs a) {
   step_kernel_entry();
-  extern __shared__ uint32_t struck[];              // ceil(vocab / 256) words
+  extern __shared__ uint32_t struck[];              // ceil(vocab / 256) words: one bit for every eight tokens that hold a tried one
   __shared__ int32_t token[kVerifyMaxNodes], up[kVerifyMaxNodes], next[kVerifyMaxNodes], tried[kVerifyMaxNodes];
+  __shared__ double node_ref[kVerifyMaxNodes], node_sum[kVerifyMaxNodes];
   __shared__ double node_mass[kVerifyMaxNodes];     // the parent's probability of a node's token; 0 for one tried before
-  __shared__ double warp_total[kVerifyThreads / 32], region[kVerifyWarps];
+  __shared__ __align__(128) double table[kExpTable];
+  __shared__ double sums[kVerifyRegions], region[kVerifyRegions];
   __shared__ uint32_t at_end, tried_count, path_count;
-  __shared__ int32_t refused;
+  __shared__ int32_t last_tried;
   const uint32_t seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const float u_draw = a.u_draw[seq];
   const int64_t begin = a.starts[seq], end = a.starts[seq + 1];
   const bool some = begin >= 0 && end > begin && end <= int64_t(a.rows);
   const uint32_t first = some ? uint32_t(begin) : 0u, n = some ? uint32_t(min(end - begin, int64_t(kVerifyMaxNodes))) : 0u;
@@ -215,48 +281,60 @@ verify_draw_kernel(const VerifyArgs a) {
   int32_t* const out_rows = a.out_rows + size_t(seq) * a.width;
   if (!n) {                                         // (the whole cluster alike)
     if (blockIdx.x == 0) {
-      for (uint32_t i = tid; i < a.width; i += kVerifyThreads) out_tokens[i] = out_rows[i] = -1;
+      for (uint32_t i = tid; i < a.width; i += kVerifyDrawThreads) out_tokens[i] = out_rows[i] = -1;
       if (tid == 0) a.out_count[seq] = 0;
     }
     return;
   }
-  // every node's token, parent, and the parent's probability of the token
-  const uint32_t words = (a.vocab + 255) / 256;
-  for (uint32_t i = tid; i < words; i += kVerifyThreads) struck[i] = 0u;
+  // every node's token, parent, and row sum; then the parent's probability of the token
+  const uint32_t tiles = (a.vocab + kVerifyTile - 1) / kVerifyTile, per = (tiles + kVerifyRegions - 1) / kVerifyRegions;
+  float u_keep = 0.f;
   if (tid < n) {
     const int32_t t = a.tokens[first + tid];
     int32_t p = tid == 0 ? -1 : a.parent ? a.parent[first + tid] : int32_t(tid) - 1;
     if (p < 0 || p >= int32_t(tid)) p = -1;
+    u_keep = a.u_keep[first + tid];
+    double2 part[kVerifySlices];
+#pragma unroll
+    for (int i = 0; i < int(kVerifySlices); ++i) part[i] = a.stats[size_t(first + tid) * kVerifySlices + i];
+    double ref = part[0].x, sum = 0.0;
+#pragma unroll
+    for (int i = 1; i < int(kVerifySlices); ++i) ref = fmax(ref, part[i].x);
+#pragma unroll
+    for (int i = 0; i < int(kVerifySlices); ++i)
+      if (part[i].x > -INFINITY) sum += part[i].y * double(exp2_approx(float(part[i].x - ref)));
+    node_ref[tid] = ref;
+    node_sum[tid] = sum;
     token[tid] = t;
     up[tid] = p;
     next[tid] = 0x7FFFFFFF;
-    double mass = 0.0;
-    if (p >= 0 && uint32_t(t) < a.vocab) {
-      const double2 st = a.stats[first + p];
-      mass = exp2((double(verify_logit<F32>(verify_row<F32>(a, first + p), uint32_t(t))) - st.x) * a.log2_scale) / st.y;
-    }
-    node_mass[tid] = mass;
   }
+  for (uint32_t i = tid; i < tiles; i += kVerifyDrawThreads) struck[i] = 0u;
+  if (tid >= kVerifyDrawThreads - kExpTable) table[tid - (kVerifyDrawThreads - kExpTable)] = exp2(double(tid - (kVerifyDrawThreads - kExpTable)) / kExpTable);
+  if (tid == 0) tried_count = 0u, last_tried = -1;
   __syncthreads();
-  const int32_t mine_up = tid > 0 && tid < n ? up[tid] : -1;
-  bool again = false;                               // a token tried before at this node
-  if (mine_up >= 0 && a.parent)
-    for (uint32_t j = uint32_t(mine_up) + 1; j < tid; ++j) again = again || (up[j] == mine_up && token[j] == token[tid]);
-  __syncthreads();
-  if (again) node_mass[tid] = 0.0;
+  const int32_t mine_up = tid < n ? up[tid] : -1;
+  float q_mine = 0.f;
+  double mass = 0.0;
+  if (mine_up >= 0 && uint32_t(token[tid]) < a.vocab) {
+    if (a.q) q_mine = a.q[int64_t(first + tid) * a.ldq + token[tid]];
+    mass = exp2(__fma_rn(double(verify_logit<F32>(verify_row<F32>(a, first + mine_up), uint32_t(token[tid]))), a.log2_scale, -node_ref[mine_up])) / node_sum[mine_up];
+  }
+  if (a.parent && mine_up >= 0)                     // a token tried before at this node
+    for (uint32_t j = uint32_t(mine_up) + 1; j < tid; ++j)
+      if (up[j] == mine_up && token[j] == token[tid]) mass = 0.0;
+  if (tid < n) node_mass[tid] = mass;
   __syncthreads();
   if (mine_up >= 0) {
-    bool keep;
+    double left = double(u_keep);
     if (a.q) {
-      const int32_t t = token[tid];
-      keep = uint32_t(t) < a.vocab && double(a.u_keep[first + tid]) * double(a.q[int64_t(first + tid) * a.ldq + t]) < node_mass[tid];
-    } else {
+      left *= double(q_mine);
+    } else if (a.parent) {
       double before = 0.0;
-      if (a.parent)
-        for (uint32_t j = uint32_t(mine_up) + 1; j < tid; ++j) before += up[j] == mine_up ? node_mass[j] : 0.0;
-      keep = double(a.u_keep[first + tid]) * (1.0 - before) < node_mass[tid];
+      for (uint32_t j = uint32_t(mine_up) + 1; j < tid; ++j) before += up[j] == mine_up ? node_mass[j] : 0.0;
+      left *= 1.0 - before;
     }
-    if (keep) atomicMin(&next[mine_up], int32_t(tid));
+    if (left < mass) atomicMin(&next[mine_up], int32_t(tid));
   }
   __syncthreads();
   if (tid == 0) {
@@ -267,103 +345,114 @@ verify_draw_kernel(const VerifyArgs a) {
       if (blockIdx.x == 0) { out_tokens[count - 1] = token[node]; out_rows[count] = int32_t(node); }
       ++count;
     }
-    // cut short by the width of the outputs: the node's children were not tried
-    const bool cut = next[node] < int32_t(n);
-    uint32_t k = 0;
-    for (uint32_t j = node + 1; j < n && !cut; ++j)
-      if (up[j] == int32_t(node)) tried[k++] = token[j];
     at_end = node;
     path_count = count;
-    tried_count = k;
-    refused = k ? tried[k - 1] : 0;
-    if (blockIdx.x == 0) {
-      for (uint32_t i = count; i < a.width; ++i) { out_tokens[i] = -1; out_rows[i] = -1; }
-      a.out_count[seq] = int32_t(count);
-    }
+    if (blockIdx.x == 0) a.out_count[seq] = int32_t(count);
   }
-  __syncthreads();
-  if (tid < tried_count && uint32_t(tried[tid]) < a.vocab) atomicOr(&struck[tried[tid] >> 8], 1u << ((tried[tid] >> 3) & 31));
   __syncthreads();
   const uint32_t node = at_end, count = path_count;
-  VerifyMasses<F32, VEC> masses;
-  masses.row = verify_row<F32>(a, first + node);
+  if (blockIdx.x == 0)
+    for (uint32_t i = count + tid; i < a.width; i += kVerifyDrawThreads) { out_tokens[i] = -1; out_rows[i] = -1; }
+  // the children of the last node were tried and refused (where the outputs' width cut the walk short, they were not tried)
+  if (mine_up == int32_t(node) && next[node] >= int32_t(n)) {
+    tried[atomicAdd(&tried_count, 1u)] = token[tid];
+    atomicMax(&last_tried, int32_t(tid));
+    if (uint32_t(token[tid]) < a.vocab) atomicOr(&struck[token[tid] >> 8], 1u << ((token[tid] >> 3) & 31));
+  }
+  __syncthreads();
+  VerifyMasses masses;
   masses.q = a.q && tried_count ? a.q + int64_t(first + node + 1) * a.ldq : nullptr;
-  masses.struck = struck;
+  masses.q_vec = (reinterpret_cast<uintptr_t>(masses.q) & 15) == 0;
   masses.tried = tried;
+  masses.table = table;
   masses.tried_count = tried_count;
   masses.vocab = a.vocab;
-  masses.scale = a.log2_scale;
-  masses.maximum = a.stats[first + node].x;
-  masses.total = 1.0;
-  const uint32_t tiles = (a.vocab + kVerifyTile - 1) / kVerifyTile, per = (tiles + kVerifyWarps - 1) / kVerifyWarps;   // (per <= 32)
-  const uint32_t unit = blockIdx.x * (kVerifyThreads / 32) + warp, tile0 = min(tiles, unit * per), tile1 = min(tiles, tile0 + per);
-  double of_tile = 0.0;                             // lane i: of the warp's tile i
-  double r0 = 0.0, r1 = 0.0, upto_region = 0.0;     // lane i: regions 2 i and 2 i + 1, and their running sum
-  for (int pass = masses.q ? 0 : 1; pass < 2; ++pass) {
-    of_tile = 0.0;
-    for (uint32_t tile = tile0; tile < tile1; ++tile) {
-      double m[8], sum = 0.0;
-      if (pass) masses(tile * kVerifyTile + lane * 8, m);
-      else masses.whole(tile * kVerifyTile + lane * 8, m);
+  masses.scale = a.log2_scale * 5.282945311356653e+269;    // 2^896
+  masses.ref = node_ref[node];
+  masses.inverse = 1.0;
+  masses.least = float((masses.ref - 100.0) / a.log2_scale);
+  const void* const row = verify_row<F32>(a, first + node);
+  constexpr uint32_t kWarps = kVerifyDrawThreads / 32, kLane = kVerifyRegions / 32;     // regions of a lane, where one looks them over
+  const uint32_t of_cta = kVerifyRegions / gridDim.x, of_warp = of_cta / kWarps;
+  uint32_t region0 = blockIdx.x * of_cta + warp * of_warp, region1 = region0 + of_warp;
+  double target = 0.0, at = 0.0;                    // last pass: the mass to pass, and the mass before the tile
+  int32_t fallback = -1;                            // last pass: where rounding leaves no such place, the last token with any mass
+#pragma unroll 1
+  for (int pass = masses.q ? 0 : 1; pass < 3; ++pass) {
+#pragma unroll 1
+    for (uint32_t r = region0; r < region1; ++r) {
+      const uint32_t tile0 = min(tiles, r * per), tile1 = min(tiles, tile0 + per);
+      double total = 0.0;
+      VerifyOctet<F32> x;
+      x.template load<VEC>(row, tile0 < tile1 ? tile0 * kVerifyTile + lane * 8 : a.vocab, a.vocab);
+#pragma unroll 1
+      for (uint32_t tile = tile0; tile < tile1; ++tile) {
+        const VerifyOctet<F32> now = x;
+        const uint32_t t0 = tile * kVerifyTile + lane * 8;
+        x.template load<VEC>(row, tile + 1 < tile1 ? t0 + kVerifyTile : a.vocab, a.vocab);
+        const bool any = struck[tile] >> lane & 1u;
+        double m[8];
+        masses.eight(now, t0, pass == 0, any, m);
+        const double eight = ((m[0] + m[1]) + (m[2] + m[3])) + ((m[4] + m[5]) + (m[6] + m[7]));
+        if (pass < 2) {
+          total += eight;
+          continue;
+        }
+        const double upto = at + warp_scan_f64(eight, lane);
+        const uint32_t with = __ballot_sync(0xFFFFFFFFu, eight > kLeastMass), past = __ballot_sync(0xFFFFFFFFu, eight > kLeastMass && upto > target);
+        at = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        if (!with) continue;
+        const uint32_t owner = past ? uint32_t(__ffs(past)) - 1u : 31u - __clz(with);
+        double running = upto - eight;
+        int32_t t = -1;                             // of this lane: the last token that the running mass had not passed before
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += m[i];
-      sum = warp_sum_f64(sum);
-      if (lane == tile - tile0) of_tile = sum;
-    }
-    const double total = warp_sum_f64(of_tile);
-    if (lane == 0) warp_total[warp] = total;
-    cluster_sync();
-    if (tid < kVerifyWarps) region[tid] = lds_f64_cluster(cluster_map(smem_u32(&warp_total[tid & 7u]), tid >> 3));
-    cluster_sync();                                 // all shares have been read: the next pass may write its own
-    r0 = region[2 * lane];
-    r1 = region[2 * lane + 1];
-    upto_region = warp_scan_f64(r0 + r1, lane);
-    if (!pass) masses.total = __shfl_sync(0xFFFFFFFFu, upto_region, 31);
-  }
-  // the region (a warp's tiles), the tile, the lane and the token where the running mass passes the target; rounding that
-  // leaves no such place falls back to the last one with any mass
-  const double whole = __shfl_sync(0xFFFFFFFFu, upto_region, 31), target = double(a.u_draw[seq]) * whole;
-  if (!(whole > 0.0)) {                             // nothing left to draw from (a drafted token of probability 1 that was refused)
-    if (blockIdx.x == 0 && tid == 0) out_tokens[count - 1] = refused;
-    return;
-  }
-  const double from_region = upto_region - r1 - r0, half_region = upto_region - r1;
-  const uint32_t past0 = __ballot_sync(0xFFFFFFFFu, r0 > 0.0 && half_region > target), past1 = __ballot_sync(0xFFFFFFFFu, r1 > 0.0 && upto_region > target);
-  const uint32_t with0 = __ballot_sync(0xFFFFFFFFu, r0 > 0.0), with1 = __ballot_sync(0xFFFFFFFFu, r1 > 0.0);
-  uint32_t chosen;
-  if (past0 | past1) {
-    const uint32_t l = __ffs(past0 | past1) - 1;
-    chosen = 2 * l + (past0 >> l & 1u ? 0u : 1u);
-  } else {
-    const uint32_t l = 31 - __clz(with0 | with1);
-    chosen = 2 * l + (with1 >> l & 1u);
-  }
-  if (chosen != unit) return;
-  const double before = __shfl_sync(0xFFFFFFFFu, chosen & 1u ? half_region : from_region, chosen >> 1);
-  const double upto_tile = before + warp_scan_f64(of_tile, lane);
-  const uint32_t with_tile = __ballot_sync(0xFFFFFFFFu, of_tile > 0.0), past_tile = __ballot_sync(0xFFFFFFFFu, of_tile > 0.0 && upto_tile > target);
-  const uint32_t pick = past_tile ? uint32_t(__ffs(past_tile)) - 1u : 31u - __clz(with_tile);
-  const double before_tile = __shfl_sync(0xFFFFFFFFu, upto_tile - of_tile, pick);
-  const uint32_t t0 = (tile0 + pick) * kVerifyTile + lane * 8;
-  double m[8], sum = 0.0;
-  masses(t0, m);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) sum += m[i];
-  const double upto = before_tile + warp_scan_f64(sum, lane);
-  const uint32_t with = __ballot_sync(0xFFFFFFFFu, sum > 0.0), past = __ballot_sync(0xFFFFFFFFu, sum > 0.0 && upto > target);
-  const uint32_t owner = past ? uint32_t(__ffs(past)) - 1u : 31u - __clz(with);
-  if (lane == owner) {
-    double run = upto - sum;
-    uint32_t t = t0;
-    for (int i = 0; i < 8; ++i) {
-      run += m[i];
-      if (m[i] > 0.0) {
-        t = t0 + i;
-        if (run > target) break;
+        for (int i = 0; i < 8; ++i) {
+          if (m[i] > kLeastMass && (running <= target || t < 0)) t = int32_t(t0) + i;
+          running += m[i];
+        }
+        fallback = __shfl_sync(0xFFFFFFFFu, t, owner);
+        if (past) break;
+      }
+      if (pass < 2) {
+        total = warp_sum_f64(total);
+        if (lane == 0) sums[r - blockIdx.x * of_cta] = total;
       }
     }
-    out_tokens[count - 1] = int32_t(t);
+    if (pass == 2) break;
+    cluster_sync();
+    if (tid < kVerifyRegions) region[tid] = lds_f64_cluster(cluster_map(smem_u32(&sums[tid % of_cta]), tid / of_cta));
+    cluster_sync();                                 // all sums have been read: the next pass may write its own
+    double share[kLane], of_lane = 0.0;
+#pragma unroll
+    for (uint32_t r = 0; r < kLane; ++r) of_lane += share[r] = region[kLane * lane + r];
+    const double upto = warp_scan_f64(of_lane, lane), whole = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (!pass) {
+      masses.inverse = 1.0 / whole;
+      continue;
+    }
+    // the region where the running mass passes the target, or the last one with any mass
+    target = fmax(double(u_draw) * whole, kLeastTarget);
+    if (!(whole > kLeastTarget)) {                           // nothing left to draw from (a drafted token of probability 1 that was refused)
+      if (blockIdx.x == 0 && tid == 0) out_tokens[count - 1] = last_tried >= 0 ? token[last_tried] : 0;
+      return;
+    }
+    const uint32_t past = __ballot_sync(0xFFFFFFFFu, of_lane > kLeastMass && upto > target), with = __ballot_sync(0xFFFFFFFFu, of_lane > kLeastMass);
+    const uint32_t holder = past ? uint32_t(__ffs(past)) - 1u : 31u - __clz(with);
+    double run = __shfl_sync(0xFFFFFFFFu, upto - of_lane, holder);
+    uint32_t chosen = 0;
+    bool there = false;
+#pragma unroll
+    for (uint32_t r = 0; r < kLane; ++r) {
+      const double s = __shfl_sync(0xFFFFFFFFu, share[r], holder);
+      if (!there && s > kLeastMass) { chosen = kLane * holder + r; at = run; }
+      run += s;
+      there = there || (s > kLeastMass && run > target);
+    }
+    if (chosen < region0 || chosen >= region1) return;
+    region0 = chosen;
+    region1 = chosen + 1;
   }
+  if (lane == 0) out_tokens[count - 1] = fallback;
 }
 
 }  // namespace grb

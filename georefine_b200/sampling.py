@@ -118,7 +118,7 @@ class DraftVerifier:
         if max_rows < 1 or max_seqs < 1 or not 1 <= width <= 256:
             raise ValueError("at least one row and sequence, and a width of 1 to 256")
         self.max_rows, self.max_seqs, self.width = int(max_rows), int(max_seqs), int(width)
-        self.stats = torch.empty(self.max_rows, 2, device=device, dtype=torch.float64)
+        self.stats = torch.empty(self.max_rows, 16, device=device, dtype=torch.float64)
         self.tokens, self.rows = (torch.empty(self.max_seqs, self.width, device=device, dtype=torch.int32) for _ in range(2))
         self.count = torch.empty(self.max_seqs, device=device, dtype=torch.int32)
         self.device = self.stats.device

@@ -470,7 +470,7 @@ typedef struct grb_verify_step {
   const float* u_draw;        /* [seqs] */
   const float* draft_probs;   /* [rows][ldq]: what row i's token was drawn from; NULL: tokens are certain */
   int64_t ldq;
-  double* stats;              /* scratch [rows][2], 16-byte aligned */
+  double* stats;              /* scratch [rows][16], 16-byte aligned */
   int32_t* out_tokens;        /* [seqs][width]: kept drafts, then the drawn token, then -1 */
   int32_t* out_rows;          /* [seqs][width]: the walk's nodes (0 first), then -1 */
   int32_t* out_count;         /* [seqs]: nodes of the walk = emitted tokens; 0 for a sequence without rows */
