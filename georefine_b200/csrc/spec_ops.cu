@@ -9,6 +9,7 @@
 #include "kv_cache.cuh"
 #include "launch_utils.h"
 #include "tree_attention.cuh"
+#include "tree_wide.cuh"
 #include "verify_ops.cuh"
 
 namespace {
@@ -67,6 +68,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GRB_ERR_CUDA;
   std::call_once(once[dev], [&] {
     prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_part_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
+    if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem)));
   });
   if (prepared[dev]) return prepared[dev];
   const int sms = device_sm_count(dev);
@@ -75,9 +77,11 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   if (int st = launch_step(tree_prep_kernel<F8>, dim3(uint32_t((vectors + 7) / 8) + 1), dim3(kTreePrepThreads), 0, stream, a, P::kPositions)) return st;
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
   if (int st = launch_step(tree_part_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
+  if (a.wide_from && a.wide_from <= a.rows) {
+    if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem, stream, a)) return st;
+  }
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
-  return launch_step(tree_combine_kernel<8>, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a,
-                     P::kPositions);
+  return launch_step(tree_combine_kernel<8>, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a);
 }
 
 template <class... Params>
@@ -144,7 +148,7 @@ uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pa
   if (!rows || rows > kTreeMaxRows || !nq || !max_pages || format > GRB_KV_E4M3) return 0;
   const uint64_t parts = uint64_t(max_pages) * (format == GRB_KV_E4M3 ? kKvPage / TreePart<true>::kPositions : kKvPage / TreePart<false>::kPositions);
   const uint64_t pairs = uint64_t(rows) * nq;
-  return ((rows * 16 + rows * 4 + 8 + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * 2 + pairs * parts * (kKvDim * 4 + 8);
+  return ((32 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * 2 + pairs * parts * (kKvDim * 4 + 8);
 }
 
 int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
@@ -180,16 +184,23 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.rows = s->rows;
   a.max_parts = s->table.max_pages * (f8 ? kKvPage / TreePart<true>::kPositions : kKvPage / TreePart<false>::kPositions);
   a.tile_rows = 16 / a.group;
+  a.wide_rows = kWideTile / a.group;
+  // Runs for the wide kernel: trees of more rows than two tiles of the narrow one take; of causal rows prompt chunks, so that the
+  // rows of a speculative chain keep the bits of single steps.
+  a.wide_from = s->row_base ? 32 / a.group + 1 : 64;
   a.scaling = s->scaling;
   a.out = static_cast<__nv_bfloat16*>(s->out);
   a.ldo = s->ldo;
   uint8_t* at = static_cast<uint8_t*>(s->scratch);
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
-  a.tiles = reinterpret_cast<int4*>(at);
-  a.extent = reinterpret_cast<int32_t*>(at + a.rows * 16ull);
-  a.plan = reinterpret_cast<uint32_t*>(at + a.rows * 20ull);
-  a.q_scale = reinterpret_cast<float*>(at + a.rows * 20ull + 8);
-  at += (a.rows * 20ull + 8 + pairs * 4 + 255) & ~uint64_t(255);
+  a.status = reinterpret_cast<uint32_t*>(at);                // (first of the scratch: the caller reads it there)
+  a.plan = a.status + 4;
+  a.tiles = reinterpret_cast<int4*>(at + 32);
+  a.wide_tiles = a.tiles + a.rows;
+  a.extent = reinterpret_cast<int32_t*>(a.wide_tiles + a.rows);
+  a.row_parts = reinterpret_cast<uint32_t*>(a.extent + a.rows);
+  a.q_scale = reinterpret_cast<float*>(a.row_parts + a.rows);
+  at += (32 + a.rows * 40ull + pairs * 4 + 255) & ~uint64_t(255);
   a.q = reinterpret_cast<uint16_t*>(at);
   at += pairs * kKvDim * 2;
   a.part_acc = reinterpret_cast<float*>(at);

@@ -4,10 +4,11 @@
 //   out[r, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(q_rh . k_j / sqrt(128)),  j over the positions that row r sees:
 //   causal: j <= row_pos[r];  tree: j < base[r], or bit j - base[r] of the row's mask.  A row that sees nothing gives 0.
 //
-// Three launches.  tree_prep: rotates the queries (once rounded, to the type the matrix instruction takes), stores keys and
+// Three launches, four where many rows of a sequence may come together.  tree_prep: rotates the queries (once rounded, to the type the matrix instruction takes), stores keys and
 // values, and one CTA lays down the plan: tiles of rows of one sequence, and units = (tile, part of the positions, kv head).
-// tree_part: persistent CTAs take units in turn.  tree_combine: merges a row's parts.  The parts of a row depend on its own
-// positions alone, and every sum runs in a fixed order, so a row's bits do not depend on the batch it is in.
+// tree_part: persistent CTAs take units in turn.  tree_wide (tree_wide.cuh) does for runs of many rows.
+// tree_combine: merges a row's parts.  The parts of a row depend on its own sequence alone (in tree_part on its
+// own positions), and every sum runs in a fixed order, so a row's bits do not depend on the batch it is in.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -20,6 +21,8 @@ namespace grb {
 
 constexpr uint32_t kTreeMaxRows = 4096, kTreeMaskWords = 4;
 constexpr int kTreePrepThreads = 256;
+constexpr uint32_t kWideMostPart = 2048;                    // positions of a wide tile's unit: the most, and those of contexts up to
+constexpr uint32_t kWideLeastPart = 512, kWideShort = 4096;  // kWideShort, whose few units would leave SMs idle
 
 struct TreeArgs {
   const __nv_bfloat16* qkv;   // [rows][ldq]: nq query heads | nkv key heads | nkv value heads, 128 each
@@ -38,14 +41,18 @@ struct TreeArgs {
   KvPagesArgs pages;          // of one layer
   uint16_t* q;                // scratch: [rows][nq][128]: rotated queries, BF16 or (8-bit caches) FP16 times a power of two
   float* q_scale;             // scratch: [rows][nq]: what a query's scores are multiplied by, in units of log 2
+  uint32_t* status;           // scratch: kStatusTimeout where a wait ran out
   int32_t* extent;            // scratch: [rows]: positions up to the last one the row sees
-  int4* tiles;                // scratch: [rows]: first row, rows, first unit, parts
-  uint32_t* plan;             // scratch: tiles, units
+  uint32_t* row_parts;        // scratch: [rows]: parts of the row
+  int4* tiles;                // scratch: [rows]: first row, rows, first unit, positions of a unit
+  int4* wide_tiles;           // scratch: [rows]: the same of wide tiles
+  uint32_t* plan;             // scratch: tiles, units, wide tiles, wide units
   float* part_acc;            // scratch: [rows][nq][max_parts][128]
   float2* part_ml;            // scratch: [rows][nq][max_parts]: maximum and sum of a part
   __nv_bfloat16* out;         // [rows][ldo]: nq * 128
   int64_t ldo;
   uint32_t rows, nq, nkv, group, tile_rows, max_parts;
+  uint32_t wide_rows, wide_from;   // rows of a wide tile; a run of so many rows (0: none) is cut into wide tiles
   float scaling;
 };
 
@@ -88,34 +95,68 @@ __device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
   return v;
 }
 
-// A tile is up to tile_rows consecutive rows of one sequence; rows that are left out or see nothing belong to none.
+// A tile is up to tile_rows (wide_rows) consecutive rows of one sequence; rows that are left out or see nothing may be among them.
+// What it needs of the rows is read once, side by side; the rest runs in shared memory.
 __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_positions) {
-  __shared__ int32_t scratch[kTreePrepThreads / 32];
-  __shared__ int32_t carry_run, carry_tiles, carry_units;
+  __shared__ int32_t scratch[kTreePrepThreads / 32], extents[kTreeMaxRows];
+  __shared__ uint16_t run_of[kTreeMaxRows];                  // first row of the row's run (rows of one sequence in a row)
   const uint32_t tid = threadIdx.x;
-  if (tid == 0) carry_run = 0, carry_tiles = 0, carry_units = 0;
+  const auto larger = [](int32_t x, int32_t y) { return max(x, y); };
+  const auto sum = [](int32_t x, int32_t y) { return x + y; };
+  int32_t run = 0;
   for (uint32_t lo = 0; lo < a.rows; lo += kTreePrepThreads) {
     const uint32_t r = lo + tid;
     const bool in = r < a.rows;
+    const int32_t extent = in ? tree_extent(a, r) : 0;
+    const bool start = in && (r == 0 || a.row_seq[r] != a.row_seq[r - 1]);
+    const int32_t first = cta_scan(start ? int32_t(r) : run, scratch, larger);
+    if (in) {
+      extents[r] = extent;
+      run_of[r] = uint16_t(first);
+      a.extent[r] = extent;
+    }
     __syncthreads();
-    const int32_t seq = in ? a.row_seq[r] : -1, before = r && in ? a.row_seq[r - 1] : -1;
-    const int32_t run0 = carry_run, tiles0 = carry_tiles, units0 = carry_units;
-    if (in) a.extent[r] = tree_extent(a, r);
-    const int32_t start = cta_scan(in && (r == 0 || seq != before) ? int32_t(r) : run0, scratch, [](int32_t x, int32_t y) { return max(x, y); });
-    const bool first = in && (r - uint32_t(start)) % a.tile_rows == 0;
-    uint32_t n = 0, parts = 0;
-    if (first)
-      for (; n < a.tile_rows && r + n < a.rows && a.row_seq[r + n] == seq; ++n)
-        parts = max(parts, (uint32_t(tree_extent(a, r + n)) + part_positions - 1) / part_positions);
-    const bool tile = first && parts;
-    const int32_t tiles = cta_scan(int32_t(tile), scratch, [](int32_t x, int32_t y) { return x + y; });
-    const int32_t units = cta_scan(tile ? int32_t(parts * a.nkv) : 0, scratch, [](int32_t x, int32_t y) { return x + y; });
-    if (tile) a.tiles[tiles0 + tiles - 1] = make_int4(int32_t(r), int32_t(n), units0 + units - int32_t(parts * a.nkv), int32_t(parts));
-    __syncthreads();
-    if (tid == kTreePrepThreads - 1) carry_run = start, carry_tiles = tiles0 + tiles, carry_units = units0 + units;
+    run = run_of[min(lo + kTreePrepThreads, a.rows) - 1];
   }
-  __syncthreads();
-  if (tid == 0) a.plan[0] = uint32_t(carry_tiles), a.plan[1] = uint32_t(carry_units);
+  int32_t tiles = 0, units = 0, wide_tiles = 0, wide_units = 0;
+  for (uint32_t lo = 0; lo < a.rows; lo += kTreePrepThreads) {
+    const uint32_t r = lo + tid;
+    uint32_t n = 0, parts = 0, positions = part_positions;
+    bool wide = false;
+    if (r < a.rows) {
+      const uint32_t first = run_of[r], last = first + a.wide_from - 1;
+      wide = a.wide_from && last < a.rows && run_of[last] == first;
+      const uint32_t per = wide ? a.wide_rows : a.tile_rows;
+      if ((r - first) % per == 0) {
+        int32_t extent = 0;
+        for (; n < per && r + n < a.rows && run_of[r + n] == first; ++n) extent = max(extent, extents[r + n]);
+        if (wide) positions = uint32_t(extent) <= kWideShort ? kWideLeastPart : kWideMostPart;
+        parts = (uint32_t(extent) + positions - 1) / positions;
+        for (uint32_t i = 0; i < n; ++i) a.row_parts[r + i] = wide ? parts : (uint32_t(extents[r + i]) + positions - 1) / positions;
+      }
+    }
+    const int32_t mine = int32_t(parts * a.nkv);
+    const int32_t t = cta_scan(int32_t(parts && !wide), scratch, sum), u = cta_scan(wide ? 0 : mine, scratch, sum);
+    int32_t wt = 0, wu = 0;
+    if (a.wide_from) {
+      wt = cta_scan(int32_t(parts && wide), scratch, sum);
+      wu = cta_scan(wide ? mine : 0, scratch, sum);
+    }
+    if (parts) {
+      if (wide) a.wide_tiles[wide_tiles + wt - 1] = make_int4(int32_t(r), int32_t(n), wide_units + wu - mine, int32_t(positions));
+      else a.tiles[tiles + t - 1] = make_int4(int32_t(r), int32_t(n), units + u - mine, int32_t(positions));
+    }
+    // the last thread's sums go to everybody
+    __shared__ int32_t totals[4];
+    __syncthreads();
+    if (tid == kTreePrepThreads - 1) totals[0] = t, totals[1] = u, totals[2] = wt, totals[3] = wu;
+    __syncthreads();
+    tiles += totals[0];
+    units += totals[1];
+    wide_tiles += totals[2];
+    wide_units += totals[3];
+  }
+  if (tid == 0) a.plan[0] = uint32_t(tiles), a.plan[1] = uint32_t(units), a.plan[2] = uint32_t(wide_tiles), a.plan[3] = uint32_t(wide_units);
 }
 
 // Grid: ceil(rows * heads / 8) CTAs of eight warps, a warp per (row, head), and one more for the plan.  A lane owns dimensions
@@ -600,14 +641,14 @@ tree_part_kernel(const TreeArgs a) {
 constexpr int kTreeCombineWarps = 4;
 template <int UNROLL>
 __global__ void __launch_bounds__(kTreeCombineWarps * 32)
-tree_combine_kernel(const TreeArgs a, uint32_t part_positions) {
+tree_combine_kernel(const TreeArgs a) {
   step_kernel_entry();
   const uint64_t pair = uint64_t(blockIdx.x) * kTreeCombineWarps + (threadIdx.x >> 5);
   const uint32_t lane = threadIdx.x & 31u;
   if (pair >= uint64_t(a.rows) * a.nq) return;
   const uint32_t row = uint32_t(pair / a.nq), head = uint32_t(pair % a.nq);
   if (tree_place(a, row) < 0) return;
-  const uint32_t parts = (uint32_t(a.extent[row]) + part_positions - 1) / part_positions;
+  const uint32_t parts = a.row_parts[row];
   const size_t base = size_t(pair) * a.max_parts;
   float mx = -INFINITY;
   for (uint32_t s = lane; s < parts; s += 32) mx = fmaxf(mx, a.part_ml[base + s].x);

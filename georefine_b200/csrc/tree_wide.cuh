@@ -1,0 +1,482 @@
+// The attention of tree_attention.cuh for many rows of one sequence at a time: wide trees and prompt chunks, on tcgen05.
+//
+// A tile is up to 128 rows (row of the step, query head of the group) of one sequence and kv head: the M of one instruction.  A
+// unit is a tile and a chunk of the positions, taken 128 at a time:
+//   S = Q K^T (Q, K in shared memory, S in tensor memory);  weights P = exp2(S scale - reference), written over S;
+//   O += P V (P from tensor memory, V in shared memory, O in tensor memory).
+// Four warps, a thread per row, turn scores into weights (the first of them issues the products); four warps bring K and V: BF16
+// as it is, 8 bits through registers, where a code becomes FP16 (one conversion for two) times its entry's scale relative to the chunk's
+// largest.  256 columns of tensor memory and 104 KB of shared memory leave room for two CTAs on an SM, and while one waits for
+// its products the other's exponentials run: those bound the kernel (16 per SM and cycle: 1024 cycles for a tile of 128
+// positions, whose products take 512).
+//
+// FP16 weights reach down to 2^-24 and V's entries to 2^-24 times a code of 1: both are scaled up as far as FP16 goes (weights at
+// most 2^15, values at most 57344), so what falls out at the bottom is 2^-39 of the largest - beyond what the 32-bit sums keep.
+// The reference of a row's weights moves only when its maximum has passed it by 2^8 (then O, in tensor memory, is scaled down).
+#pragma once
+#include "tree_attention.cuh"
+
+namespace grb {
+
+constexpr int kWideThreads = 256;                // softmax warps 0-3, loading warps 4-7
+constexpr uint32_t kWideTile = 128;              // rows of a tile, positions of a step
+constexpr uint32_t kWideOperand = 32768;         // Q, K or V of a tile: two halves of 64 dimensions, 128 rows of 128 bytes each
+constexpr uint32_t kWideScalesAt = 3 * kWideOperand;
+constexpr uint32_t kWideSmem = 3 * kWideOperand + 2 * 2 * kWideMostPart + 1024;   // operands, FP16 scales of a chunk's K and V, alignment
+constexpr uint32_t kWideColumns = 256;           // tensor memory: S (and P over it), O
+
+// Byte offset of 16-byte piece `piece` (0..15) of row `row` of an operand: 128-byte swizzle in each half.
+__device__ __forceinline__ uint32_t wide_offset(uint32_t row, uint32_t piece) {
+  return (piece >> 3) * (kWideOperand / 2) + row * 128u + (((piece ^ row) & 7u) << 4);
+}
+// V as the B operand with its dimensions contiguous (N-major): 64 dimensions per 128-byte row, the other half 16 KB on, groups of
+// eight positions 1024 bytes apart.
+__device__ __forceinline__ uint64_t wide_desc_v(uint32_t smem_addr) {
+  return uint64_t((smem_addr >> 4) & 0x3FFFu) | (uint64_t(kWideOperand / 2 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+// 2^e in FP16, e <= 15; below its range 0.
+__device__ __forceinline__ uint32_t half_power(int e) { return e >= -14 ? uint32_t(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u; }
+
+// Two values at a time: a * b + c, a + b.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+struct WideUnit {
+  uint32_t first, rows, kvh, part;
+  int32_t seq, start, extent;      // positions start .. extent - 1 (at most a chunk): what some row sees, up to the last such
+};
+
+template <bool F8>
+__global__ void __launch_bounds__(kWideThreads, 2)
+tree_wide_kernel(const TreeArgs a) {
+  step_kernel_entry();
+  extern __shared__ unsigned char wide_smem_raw[];
+  __shared__ __align__(8) uint64_t bars[5];                  // K stored, V stored, S done, P stored, O done
+  __shared__ uint32_t tmem_at, aborted;
+  __shared__ uint32_t k_top, v_top;                          // largest exponent bytes of the chunk
+  __shared__ int32_t seen_by_all;                            // positions below it are seen by every row of the tile
+  __shared__ uint32_t bad[2][kWideTile / 32];                // positions of a step whose key or value is not a number (two steps' worth)
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+  const uint32_t smem = (smem_u32(wide_smem_raw) + 1023u) & ~1023u, qs = smem, ks = smem + kWideOperand, vs = smem + 2 * kWideOperand;
+  const uint32_t k_scales = smem + kWideScalesAt, v_scales = k_scales + 2 * kWideMostPart;
+  const uint32_t bar_k = smem_u32(&bars[0]), bar_v = smem_u32(&bars[1]), bar_s = smem_u32(&bars[2]), bar_p = smem_u32(&bars[3]), bar_o = smem_u32(&bars[4]);
+  const uint32_t tiles = a.plan[2], units = a.plan[3];
+  if (blockIdx.x >= units) return;
+  if (tid == 0) {
+    mbar_init(bar_k, 4);
+    mbar_init(bar_v, 4);
+    mbar_init(bar_s, 1);
+    mbar_init(bar_p, 4);
+    mbar_init(bar_o, 1);
+    mbar_fence_init();
+    aborted = 0u;
+  }
+  if (tid < 8) bad[tid >> 2][tid & 3u] = 0u;
+  if (warp == 4) {
+    tmem_alloc(smem_u32(&tmem_at), kWideColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t s_tmem = tmem_at, o_tmem = tmem_at + 128;
+  // A wait that runs out is everybody's: nobody waits again, every loop runs to its end, and the status says so.
+  auto wait = [&](uint32_t bar, uint32_t step) {
+    if (*reinterpret_cast<volatile uint32_t*>(&aborted)) return;
+    if (!mbar_wait(bar, step & 1u, false)) {
+      *reinterpret_cast<volatile uint32_t*>(&aborted) = 1u;
+      atomicOr(a.status, kStatusTimeout);
+    }
+  };
+  uint32_t step0 = 0, tile = 0;                              // steps this CTA has taken; the tile of its unit
+  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+    // ---- the unit (every warp finds it for itself)
+    WideUnit t;
+    for (;;) {
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, tile + 1 + lane < tiles && uint32_t(a.wide_tiles[tile + 1 + lane].z) <= u);
+      tile += __popc(past);
+      if (past != 0xFFFFFFFFu) break;
+    }
+    const int4 d = a.wide_tiles[tile];
+    const uint32_t local = u - uint32_t(d.z), part_positions = uint32_t(d.w);
+    t.first = uint32_t(d.x);
+    t.rows = uint32_t(d.y);
+    t.kvh = local % a.nkv;
+    t.part = local / a.nkv;
+    t.seq = a.row_seq[t.first];
+    t.start = int32_t(t.part * part_positions);
+    const uint32_t used = t.rows * a.group;
+    if (tid == 0) { k_top = v_top = 0u; seen_by_all = 0x7FFFFFFF; }
+    __syncthreads();
+    // the queries, by all warps; what the tile's rows see
+    for (uint32_t c = tid; c < kWideTile * 16; c += kWideThreads) {
+      const uint32_t m = c >> 4, piece = c & 15u, r = m / a.group;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (m < used) x = reinterpret_cast<const uint4*>(a.q + ((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kKvDim)[piece];
+      sts128(qs + wide_offset(m, piece), x);
+    }
+    int32_t extent = 0;
+    for (uint32_t i = lane; i < t.rows; i += 32) {
+      const int32_t e = a.extent[t.first + i];
+      extent = max(extent, e);
+      if (warp == 0) atomicMin(&seen_by_all, a.row_base ? min(max(a.row_base[t.first + i], 0), e) : e);
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) extent = max(extent, __shfl_xor_sync(0xFFFFFFFFu, extent, off));
+    t.extent = min(extent, t.start + int32_t(part_positions));
+    const uint32_t steps = t.extent > t.start ? (uint32_t(t.extent - t.start) + kWideTile - 1) / kWideTile : 0u;
+    // entry (of the layer) of the first position of a step; the step's positions lie in one page
+    auto entry_of = [&](uint32_t j) {
+      const int64_t place = kv_place(a.table, t.seq, t.start + int32_t(j * kWideTile));
+      return place < 0 ? int64_t(-1) : int64_t(kv_entry(place, a.nkv, t.kvh));
+    };
+    if constexpr (F8) {
+      // scales of the chunk: the largest exponents first (those of no entry, 135 to 254, may stand where nobody wrote)
+      for (uint32_t c = tid; c < steps * 16; c += kWideThreads) {         // 16 bytes: K then V
+        const uint32_t j = c >> 4, v = c >> 3 & 1u, at = c & 7u;
+        const int64_t entry = entry_of(j);
+        if (entry < 0) continue;
+        const uint4 x = *reinterpret_cast<const uint4*>((v ? a.pages.v_exp : a.pages.k_exp) + entry + at * 16);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t top = 0;
+        const int32_t left = t.extent - t.start - int32_t(j * kWideTile + at * 16);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t b = w[i >> 2] >> (8 * (i & 3)) & 0xFFu;
+          if (i < left && b != kKvNanByte) top = max(top, min(b, 134u));
+        }
+        atomicMax(v ? &v_top : &k_top, top);
+      }
+      __syncthreads();
+      for (uint32_t c = tid; c < steps * kWideTile * 2; c += kWideThreads) {
+        const uint32_t v = c >= steps * kWideTile, p = v ? c - steps * kWideTile : c;
+        const int64_t entry = entry_of(p / kWideTile);
+        const uint32_t b = entry < 0 ? 0u : (v ? a.pages.v_exp : a.pages.k_exp)[entry + p % kWideTile];
+        // (an entry that is no number: 0 here, and its position in `bad`)
+        sts_u16((v ? v_scales : k_scales) + 2 * p, b > 134u ? 0u : half_power(min(int(b) - int(v ? v_top : k_top) + 7, 7)));
+      }
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+    const bool edge = seen_by_all < t.extent;                // some step of the unit is not seen whole by every row
+    auto whole = [&](uint32_t j) { return !edge || seen_by_all >= t.start + int32_t((j + 1) * kWideTile); };
+    if (warp >= 4) {
+      // ---- loading ----------------------------------------------------------------------------------------------
+      const uint32_t lt = tid - 128;
+      if constexpr (F8) {
+        uint4 k[8], v[8];
+        auto ask = [&](uint4 (&x)[8], const void* pool, uint32_t j) {
+          const int64_t entry = j < steps ? entry_of(j) : -1;
+          const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t c = lt + 128 * i;
+            x[i] = int32_t(c >> 3) < npos ? reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim)[c] : make_uint4(0u, 0u, 0u, 0u);
+          }
+        };
+        auto store = [&](const uint4 (&x)[8], uint32_t dst, uint32_t scales, uint32_t j, bool clean) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t c = lt + 128 * i, row = c >> 3, piece = c & 7u;
+            const uint32_t s16 = lds_u16(scales + 2 * (j * kWideTile + row)), s = s16 | (s16 << 16);
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              h[2 * q] = e4m3_to_half2(w[q] & 0xFFFFu);
+              h[2 * q + 1] = e4m3_to_half2(w[q] >> 16);
+            }
+            if (clean) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) h[q] = half2_number(h[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[q]) : "r"(s));
+            // the lanes of a row's second half take its second piece first: eight lanes, eight groups of banks
+            const uint32_t swap = piece >> 2;
+            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+            sts128(dst + wide_offset(row, 2 * piece + swap), swap ? hi : lo);
+            sts128(dst + wide_offset(row, 2 * piece + 1 - swap), swap ? lo : hi);
+          }
+        };
+        ask(k, a.pages.k, 0);
+        ask(v, a.pages.v, 0);
+        for (uint32_t j = 0; j < steps; ++j) {
+          const uint32_t g = step0 + j;
+          if (g) wait(bar_s, g - 1);                         // the scores of the step before have been taken from K
+          store(k, ks, k_scales, j, false);
+          if (warp == 4) {                                   // positions whose entry is no number
+            const int64_t entry = entry_of(j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool in = entry >= 0 && t.start + int32_t(j * kWideTile + 32 * i + lane) < t.extent;
+              const bool b = in && (a.pages.k_exp[entry + 32 * i + lane] == kKvNanByte || a.pages.v_exp[entry + 32 * i + lane] == kKvNanByte);
+              const uint32_t m = __ballot_sync(0xFFFFFFFFu, b);
+              if (lane == 0) bad[g & 1u][i] = m;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_k);
+          ask(k, a.pages.k, j + 1);
+          if (g) wait(bar_o, g - 1);                         // the values of the step before have been used
+          store(v, vs, v_scales, j, !whole(j));
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_v);
+          ask(v, a.pages.v, j + 1);
+        }
+      } else {
+        auto ask = [&](uint32_t dst, const void* pool, uint32_t j) {
+          const int64_t entry = entry_of(j);
+          const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
+          const uint8_t* src = static_cast<const uint8_t*>(pool) + (entry < 0 ? 0 : entry) * kKvDim * 2;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t c = lt + 128 * i;
+            const bool in = int32_t(c >> 4) < npos;
+            cp_async_16(dst + wide_offset(c >> 4, c & 15u), src + (in ? c * 16 : 0u), in ? 16u : 0u);
+          }
+          cp_async_commit();
+        };
+        for (uint32_t j = 0; j < steps; ++j) {
+          const uint32_t g = step0 + j;
+          if (g) wait(bar_s, g - 1);
+          ask(ks, a.pages.k, j);
+          if (g) wait(bar_o, g - 1);
+          if (warp == 4 && lane < 4) bad[(g + 1) & 1u][lane] = 0u;   // (read last for step g - 1, which is over)
+          ask(vs, a.pages.v, j);
+          cp_async_wait<1>();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_k);
+          cp_async_wait<0>();
+          if (!whole(j)) {                                   // values that are not finite would reach, as 0 * infinity, rows that do not see them
+            uint32_t mine = 0;                               // bit i: of the thread's piece i
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t c = lt + 128 * i, at = vs + wide_offset(c >> 4, c & 15u);
+              const uint4 x = lds128(at);
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              bool b = false;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) b = b || (w[q] & 0x7F80u) == 0x7F80u || (w[q] & 0x7F800000u) == 0x7F800000u;
+              if (b) sts128(at, make_uint4(0u, 0u, 0u, 0u));
+              mine |= uint32_t(b) << i;
+            }
+            // piece i of this warp's lanes lies in positions 8 i + 2 (warp - 4) and the next
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t m = __ballot_sync(0xFFFFFFFFu, mine >> i & 1u);
+              const uint32_t p = 8 * i + 2 * (warp - 4);
+              if (lane == 0 && m) atomicOr(&bad[g & 1u][p >> 5], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_v);
+        }
+      }
+    } else {
+      // ---- weights: thread = row m of the tile, lane m of tensor memory --------------------------------------------
+      const uint32_t m = tid, r = min(m, used - 1) / a.group, row = t.first + r, lanes = (warp * 32u) << 16;
+      const size_t pair = size_t(row) * a.nq + t.kvh * a.group + (min(m, used - 1) - r * a.group);
+      const float scale = F8 ? __fmul_rn(a.q_scale[pair], __uint_as_float((k_top > 7u ? k_top - 7u : 127u) << 23)) : a.q_scale[pair];
+      const int32_t base = a.row_base ? a.row_base[row] : 0, mine = a.extent[row];
+      constexpr float kSlack = 8.f, kBias = F8 ? 7.f : 0.f;  // FP16: weights up to 2^(7 + 8)
+      constexpr uint32_t kIdesc = umma_idesc_bf16(128) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);      // FP16 or BF16 operands
+      float ref = -INFINITY;
+      float2 sum = make_float2(0.f, 0.f);
+      for (uint32_t j = 0; j < steps; ++j) {
+        const uint32_t g = step0 + j;
+        const int32_t at = t.start + int32_t(j * kWideTile);
+        if (warp == 0) {                                     // (behind the values' product of the step before, in issue order)
+          wait(bar_k, g);
+          __syncwarp();
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {                    // 16 dimensions each
+              const uint32_t half = (s >> 2) * (kWideOperand / 2) + (s & 3) * 32;
+              umma_bf16(s_tmem, umma_desc_sw128(qs + half), umma_desc_sw128(ks + half), kIdesc, s > 0);
+            }
+            umma_commit(bar_s);
+          }
+          __syncwarp();
+        }
+        wait(bar_s, g);
+        tc_fence_after();
+        // which of the step's positions the row sees
+        const bool there = entry_of(j) >= 0;                 // (a page outside the pool: as if nobody saw its positions)
+        const bool every = whole(j) && there;
+        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+        bool poisoned = false;
+        if (!every) {
+          wait(bar_v, g);                                    // (`bad` is complete)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int32_t p = at + 32 * w, most = min(max(mine - p, 0), 32);
+            const uint32_t below = most == 32 ? ~0u : (1u << most) - 1u;            // up to the last position the row sees
+            uint32_t bits = ~0u;
+            if (a.row_base) {
+              const int32_t n0 = p - base;                   // node of the word's first bit
+              if (n0 + 31 < 0) bits = ~0u;
+              else {
+                auto word = [&](int32_t n) -> uint64_t { return n >= 0 && uint32_t(n) < a.mask_words ? a.row_mask[row * a.ldm + n] : 0ull; };
+                if (n0 >= 0) {
+                  const uint32_t sh = uint32_t(n0) & 63u;
+                  bits = uint32_t(word(n0 >> 6) >> sh);
+                  if (sh > 32) bits |= uint32_t(word((n0 >> 6) + 1) << (64 - sh));
+                } else {
+                  bits = uint32_t(word(0)) << (-n0) | ((1u << (-n0)) - 1u);           // (-n0 is 1 to 31)
+                }
+              }
+            }
+            see[w] = there ? bits & below : 0u;
+          }
+        }
+        if (F8 || !every) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) poisoned = poisoned || ((F8 || !every) && (*reinterpret_cast<volatile uint32_t*>(&bad[g & 1u][w]) & see[w]));
+        }
+        auto masked = [&](uint32_t (&x)[32], int w) {
+          if (!every) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = see[w] >> i & 1u ? x[i] : 0xFF800000u;
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x[32];
+          tmem_ld32(s_tmem + lanes + 32 * w, x);
+          tmem_ld_wait();
+          masked(x, w);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+        }
+        top = __fmul_rn(top, scale);
+        const bool move = top > (ref == -INFINITY ? ref : __fadd_rn(ref, kSlack));
+        if (__any_sync(0xFFFFFFFFu, move)) {
+          const float to = move ? top : ref, f = move ? exp2_approx(__fsub_rn(ref, to)) : 1.f;        // (from -infinity: 0)
+          sum.x = __fmul_rn(sum.x, f);
+          sum.y = __fmul_rn(sum.y, f);
+          ref = to;
+          if (j > 0) {
+            wait(bar_o, g - 1);
+            tc_fence_after();
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t x[32];
+              tmem_ld32(o_tmem + lanes + 32 * w, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__fmul_rn(__uint_as_float(x[i]), f));
+              tmem_st32(o_tmem + lanes + 32 * w, x);
+            }
+          }
+        }
+        const float low = (ref == -INFINITY ? 0.f : ref) - kBias;
+        const float2 scale2 = make_float2(scale, scale), low2 = make_float2(-low, -low);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x[32], p[16];
+          tmem_ld32(s_tmem + lanes + 32 * w, x);
+          tmem_ld_wait();
+          masked(x, w);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 e = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, low2);
+            e.x = exp2_approx(e.x);
+            e.y = exp2_approx(e.y);
+            sum = add2(sum, e);
+            if constexpr (F8) {
+              const __half2 h = __floats2half2_rn(e.x, e.y);
+              p[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+              p[i] = pack_bf(e.x, e.y);
+            }
+          }
+          tmem_st16(s_tmem + lanes + 16 * w, p);             // (over scores that have been read)
+        }
+        if (poisoned) sum.x = __uint_as_float(0x7FC00000u);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p);
+        if (warp == 0) {
+          wait(bar_p, g);
+          wait(bar_v, g);
+          __syncwarp();
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < 8; ++s)                      // 16 positions each
+              umma_bf16_ts(o_tmem, s_tmem + 8 * s, wide_desc_v(vs + 2048 * s), kIdesc | (1u << 16), j > 0 || s > 0);
+            umma_commit(bar_o);
+          }
+          __syncwarp();
+        }
+      }
+      // ---- the unit's partial result
+      if (steps) {
+        wait(bar_o, step0 + steps - 1);
+        tc_fence_after();
+      }
+      const float back = F8 ? __uint_as_float((v_top > 7u ? v_top - 7u : 0u) << 23) : 1.f;
+      const size_t out = pair * a.max_parts + t.part;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t x[32];
+        if (steps) {
+          tmem_ld32(o_tmem + lanes + 32 * w, x);
+          tmem_ld_wait();
+        }
+        if (m < used) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (steps) o = make_float4(__uint_as_float(x[i]) * back, __uint_as_float(x[i + 1]) * back, __uint_as_float(x[i + 2]) * back, __uint_as_float(x[i + 3]) * back);
+            *reinterpret_cast<float4*>(a.part_acc + out * kKvDim + 32 * w + i) = o;
+          }
+        }
+      }
+      if (m < used) a.part_ml[out] = make_float2(ref == -INFINITY ? ref : ref - kBias, sum.x + sum.y);
+      tc_fence_before();
+    }
+    step0 += steps;
+    __syncthreads();                                         // operands, scales and accumulators are free
+    if (!F8 && tid < 8) bad[tid >> 2][tid & 3u] = 0u;        // (the next use lies behind another barrier)
+  }
+  // (every product has been waited for, or its wait ran out: then the tensor memory is given back after a moment for what may
+  // still be under way)
+  if (aborted) {
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < kLingerNs) {}
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 4) tmem_dealloc(tmem_at, kWideColumns);
+}
+
+}  // namespace grb

@@ -296,7 +296,16 @@ class TreeAttention:
         self.nq, self.nkv, self.max_rows, self.max_pages, self.format = nq, nkv, int(max_rows), int(max_pages), kv_format
         self.scratch_bytes = _native.lib().grb_attn_tree_scratch_bytes(self.max_rows, nq, self.max_pages, KV_FORMATS.index(kv_format))
         self.scratch = torch.empty(self.scratch_bytes, device=device, dtype=torch.uint8)
+        self.scratch[:16].zero_()
         self.device = self.scratch.device
+
+    def check_status(self) -> int:
+        """GRB_STATUS_* bits of the calls since the last check (0: their outputs can be trusted).  Synchronises."""
+        import torch
+
+        bits = int(self.scratch[:4].view(torch.int32).item())
+        self.scratch[:4].zero_()
+        return bits
 
     def __call__(self, qkv, cos, sin, row_seq, row_pos, page_table, pages, out, *, tree=None):
         """``qkv`` (BF16 [rows, (nq + 2 nkv) 128]) -> ``out`` (BF16 [rows, nq 128]).  Keys (rotated) and values are stored at

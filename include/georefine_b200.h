@@ -444,7 +444,8 @@ typedef struct grb_attn_tree_step {
   uint32_t mask_words;
   grb_kv_pages pages;         /* of one layer */
   grb_kv_table table;
-  void* scratch;              /* grb_attn_tree_scratch_bytes(rows, nq, max_pages, format), 16-byte aligned; no two calls at once */
+  void* scratch;              /* grb_attn_tree_scratch_bytes(rows, nq, max_pages, format), 16-byte aligned, its first word zeroed
+                                 once: GRB_STATUS_* bits of the calls since; no two calls at once */
   uint64_t scratch_bytes;
   void* out;                  /* BF16 [rows][ldo]: nq * 128 */
   int64_t ldo;
