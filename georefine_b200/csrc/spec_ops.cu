@@ -73,11 +73,11 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   if (prepared[dev]) return prepared[dev];
   const int sms = device_sm_count(dev);
   if (sms <= 0) return GRB_ERR_CUDA;
-  const uint64_t vectors = uint64_t(a.rows) * (a.nq + 2 * a.nkv);
-  if (int st = launch_step(tree_prep_kernel<F8>, dim3(uint32_t((vectors + 7) / 8) + 1), dim3(kTreePrepThreads), 0, stream, a, P::kPositions)) return st;
+  const uint32_t warps = a.rows * ((a.nq + 2 * a.nkv + kTreeHeadsPerWarp - 1) / kTreeHeadsPerWarp);
+  if (int st = launch_step(tree_prep_kernel<F8>, dim3((warps + 7) / 8 + 1), dim3(kTreePrepThreads), a.rows * 6, stream, a, P::kPositions)) return st;
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
   if (int st = launch_step(tree_part_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
-  if (a.wide_from && a.wide_from <= a.rows) {
+  if (a.wide_from) {
     if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem, stream, a)) return st;
   }
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
@@ -187,7 +187,9 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.wide_rows = kWideTile / a.group;
   // Runs for the wide kernel: trees of more rows than two tiles of the narrow one take; of causal rows prompt chunks, so that the
   // rows of a speculative chain keep the bits of single steps.
+  const uint32_t longest = s->longest_run ? s->longest_run : s->row_base ? s->rows : s->rows / s->table.slots;
   a.wide_from = s->row_base ? 32 / a.group + 1 : 64;
+  if (a.wide_from > s->rows || a.wide_from > longest) a.wide_from = 0;
   a.scaling = s->scaling;
   a.out = static_cast<__nv_bfloat16*>(s->out);
   a.ldo = s->ldo;

@@ -21,8 +21,10 @@ namespace grb {
 
 constexpr uint32_t kTreeMaxRows = 4096, kTreeMaskWords = 4;
 constexpr int kTreePrepThreads = 256;
-constexpr uint32_t kWideMostPart = 2048;                    // positions of a wide tile's unit: the most, and those of contexts up to
-constexpr uint32_t kWideLeastPart = 512, kWideShort = 4096;  // kWideShort, whose few units would leave SMs idle
+// Positions of a wide tile's unit: the most, for long contexts (a unit's result is as large as 256 positions of an 8-bit cache); fewer
+// for short ones, whose few units would leave SMs idle.
+constexpr uint32_t kWideMostPart = 2048;
+__device__ __forceinline__ uint32_t wide_part(uint32_t extent) { return extent <= 1024 ? 256u : extent <= 4096 ? 512u : kWideMostPart; }
 
 struct TreeArgs {
   const __nv_bfloat16* qkv;   // [rows][ldq]: nq query heads | nkv key heads | nkv value heads, 128 each
@@ -98,8 +100,9 @@ __device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
 // A tile is up to tile_rows (wide_rows) consecutive rows of one sequence; rows that are left out or see nothing may be among them.
 // What it needs of the rows is read once, side by side; the rest runs in shared memory.
 __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_positions) {
-  __shared__ int32_t scratch[kTreePrepThreads / 32], extents[kTreeMaxRows];
-  __shared__ uint16_t run_of[kTreeMaxRows];                  // first row of the row's run (rows of one sequence in a row)
+  extern __shared__ int32_t extents[];                       // [rows]
+  uint16_t* const run_of = reinterpret_cast<uint16_t*>(extents + a.rows);      // [rows]: first row of the row's run (rows of one sequence in a row)
+  __shared__ int32_t scratch[kTreePrepThreads / 32];
   const uint32_t tid = threadIdx.x;
   const auto larger = [](int32_t x, int32_t y) { return max(x, y); };
   const auto sum = [](int32_t x, int32_t y) { return x + y; };
@@ -130,7 +133,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
       if ((r - first) % per == 0) {
         int32_t extent = 0;
         for (; n < per && r + n < a.rows && run_of[r + n] == first; ++n) extent = max(extent, extents[r + n]);
-        if (wide) positions = uint32_t(extent) <= kWideShort ? kWideLeastPart : kWideMostPart;
+        if (wide) positions = wide_part(uint32_t(extent));
         parts = (uint32_t(extent) + positions - 1) / positions;
         for (uint32_t i = 0; i < n; ++i) a.row_parts[r + i] = wide ? parts : (uint32_t(extents[r + i]) + positions - 1) / positions;
       }
@@ -159,85 +162,95 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
   if (tid == 0) a.plan[0] = uint32_t(tiles), a.plan[1] = uint32_t(units), a.plan[2] = uint32_t(wide_tiles), a.plan[3] = uint32_t(wide_units);
 }
 
-// Grid: ceil(rows * heads / 8) CTAs of eight warps, a warp per (row, head), and one more for the plan.  A lane owns dimensions
-// 2 l, 2 l + 1 and the two that the rotation pairs with them.  The products of BF16 values are exact in FP32, so the rotation
-// rounds once before the result is rounded to its type.
+// The first CTA lays down the plan; in the others a warp takes up to eight neighbouring heads of a row, all their loads on their
+// way together (one head a warp: 43 us for 1024 rows of 56 heads).  A lane owns dimensions 2 l, 2 l + 1 and the two that the
+// rotation pairs with them.  The products of BF16 values are exact in FP32, so the rotation rounds once before the result is
+// rounded to its type.
+constexpr uint32_t kTreeHeadsPerWarp = 8;
 template <bool F8>
 __global__ void __launch_bounds__(kTreePrepThreads)
 tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
   step_kernel_entry();
-  if (blockIdx.x == gridDim.x - 1) return tree_plan(a, part_positions);
-  const uint32_t heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 31u;
-  const uint64_t at = uint64_t(blockIdx.x) * (kTreePrepThreads / 32) + (threadIdx.x >> 5);
-  const uint32_t row = uint32_t(at / heads), head = uint32_t(at % heads);
+  if (blockIdx.x == 0) return tree_plan(a, part_positions);
+  const uint32_t heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 31u, per_row = (heads + kTreeHeadsPerWarp - 1) / kTreeHeadsPerWarp;
+  const uint32_t at = (blockIdx.x - 1) * (kTreePrepThreads / 32) + (threadIdx.x >> 5), row = at / per_row, head0 = at % per_row * kTreeHeadsPerWarp;
   if (row >= a.rows) return;
-  const uint32_t* src = reinterpret_cast<const uint32_t*>(a.qkv + row * a.ldq + size_t(head) * kKvDim) + lane;
-  const uint32_t lo = src[0], hi = src[32];
+  const uint32_t n = min(kTreeHeadsPerWarp, heads - head0);
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(a.qkv + row * a.ldq + size_t(head0) * kKvDim) + lane;
+  uint32_t lo[kTreeHeadsPerWarp], hi[kTreeHeadsPerWarp];
+#pragma unroll
+  for (uint32_t i = 0; i < kTreeHeadsPerWarp; ++i)
+    if (i < n) { lo[i] = src[i * (kKvDim / 2)]; hi[i] = src[i * (kKvDim / 2) + 32]; }
   const int32_t rope = a.row_base ? a.row_rope[row] : a.row_pos[row];
   const int64_t place = tree_place(a, row);
   if (place < 0) return;
-  float x[4] = {bf_lo(lo), bf_hi(lo), bf_lo(hi), bf_hi(hi)};
-  const bool query = head < a.nq, value = head >= a.nq + a.nkv;
-  if (!value) {
-    const uint32_t* cs = reinterpret_cast<const uint32_t*>(a.cos_table + size_t(rope) * kKvDim) + lane;
-    const uint32_t* sn = reinterpret_cast<const uint32_t*>(a.sin_table + size_t(rope) * kKvDim) + lane;
-    const float c[4] = {bf_lo(cs[0]), bf_hi(cs[0]), bf_lo(cs[32]), bf_hi(cs[32])};
-    const float s[4] = {bf_lo(sn[0]), bf_hi(sn[0]), bf_lo(sn[32]), bf_hi(sn[32])};
-    float y[4];
-    if (!F8 && !query) {      // keys of a BF16 cache: the bits that attn_prep_kernel stores, each product and the sum rounded
+  const uint32_t* cs = reinterpret_cast<const uint32_t*>(a.cos_table + size_t(rope) * kKvDim) + lane;
+  const uint32_t* sn = reinterpret_cast<const uint32_t*>(a.sin_table + size_t(rope) * kKvDim) + lane;
+  const float c[4] = {bf_lo(cs[0]), bf_hi(cs[0]), bf_lo(cs[32]), bf_hi(cs[32])};
+  const float s[4] = {bf_lo(sn[0]), bf_hi(sn[0]), bf_lo(sn[32]), bf_hi(sn[32])};
+  const float log2_scale = __fmul_rn(a.scaling, 1.4426950408889634f);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        y[i] = round_bf(__fadd_rn(round_bf(__fmul_rn(x[i], c[i])), round_bf(__fmul_rn(-x[i + 2], s[i]))));
-        y[i + 2] = round_bf(__fadd_rn(round_bf(__fmul_rn(x[i + 2], c[i + 2])), round_bf(__fmul_rn(x[i], s[i + 2]))));
-      }
-    } else {
+  for (uint32_t i = 0; i < kTreeHeadsPerWarp; ++i) {
+    const uint32_t head = head0 + i;
+    if (i >= n) break;
+    float x[4] = {bf_lo(lo[i]), bf_hi(lo[i]), bf_lo(hi[i]), bf_hi(hi[i])};
+    const bool query = head < a.nq, value = head >= a.nq + a.nkv;
+    if (!value) {
+      float y[4];
+      if (!F8 && !query) {    // keys of a BF16 cache: the bits that attn_prep_kernel stores, each product and the sum rounded
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        y[i] = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(x[i + 2], s[i]));
-        y[i + 2] = __fadd_rn(__fmul_rn(x[i + 2], c[i + 2]), __fmul_rn(x[i], s[i + 2]));
+        for (int k = 0; k < 2; ++k) {
+          y[k] = round_bf(__fadd_rn(round_bf(__fmul_rn(x[k], c[k])), round_bf(__fmul_rn(-x[k + 2], s[k]))));
+          y[k + 2] = round_bf(__fadd_rn(round_bf(__fmul_rn(x[k + 2], c[k + 2])), round_bf(__fmul_rn(x[k], s[k + 2]))));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          y[k] = __fsub_rn(__fmul_rn(x[k], c[k]), __fmul_rn(x[k + 2], s[k]));
+          y[k + 2] = __fadd_rn(__fmul_rn(x[k + 2], c[k + 2]), __fmul_rn(x[k], s[k + 2]));
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = y[k];
     }
+    if (query) {
+      const size_t pair = size_t(row) * a.nq + head;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + pair * kKvDim) + lane;
+      if constexpr (F8) {
+        // FP16 times a power of two that brings the largest component to [2^14, 2^15): 11 bits where BF16 has 8, and what falls
+        // below FP16's normal range is 2^-28 of the largest.
+        const float m = warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+        bool fine = true;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = y[i];
-  }
-  if (query) {
-    uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + (size_t(row) * a.nq + head) * kKvDim) + lane;
-    const float log2_scale = __fmul_rn(a.scaling, 1.4426950408889634f);
+        for (int k = 0; k < 4; ++k) fine = fine && fabsf(x[k]) <= 3.4028234e38f;
+        fine = __all_sync(0xFFFFFFFFu, fine);
+        const int e = max(int(__float_as_uint(m) >> 23) - 127 - 14, -100);        // (<= 113)
+        const float down = __uint_as_float(uint32_t(127 - e) << 23);
+        const __half2 h0 = fine ? __floats2half2_rn(x[0] * down, x[1] * down) : __floats2half2_rn(0.f, 0.f);
+        const __half2 h1 = fine ? __floats2half2_rn(x[2] * down, x[3] * down) : __floats2half2_rn(0.f, 0.f);
+        dst[0] = *reinterpret_cast<const uint32_t*>(&h0);
+        dst[32] = *reinterpret_cast<const uint32_t*>(&h1);
+        if (lane == 0) a.q_scale[pair] = fine ? __fmul_rn(log2_scale, __uint_as_float(uint32_t(127 + e) << 23)) : __uint_as_float(0x7FC00000u);
+      } else {
+        dst[0] = pack_bf(x[0], x[1]);
+        dst[32] = pack_bf(x[2], x[3]);
+        if (lane == 0) a.q_scale[pair] = log2_scale;
+      }
+      continue;
+    }
+    const size_t entry = kv_entry(place, a.nkv, value ? head - a.nq - a.nkv : head - a.nq);
+    void* const pages = value ? a.pages.v : a.pages.k;
     if constexpr (F8) {
-      // FP16 times a power of two that brings the largest component to [2^14, 2^15): 11 bits where BF16 has 8, and what falls
-      // below FP16's normal range is 2^-28 of the largest.
-      const float m = warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-      bool fine = true;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fine = fine && fabsf(x[i]) <= 3.4028234e38f;
-      fine = __all_sync(0xFFFFFFFFu, fine);
-      const int e = max(int(__float_as_uint(m) >> 23) - 127 - 14, -100);        // (<= 113)
-      const float down = __uint_as_float(uint32_t(127 - e) << 23);
-      const __half2 h0 = fine ? __floats2half2_rn(x[0] * down, x[1] * down) : __floats2half2_rn(0.f, 0.f);
-      const __half2 h1 = fine ? __floats2half2_rn(x[2] * down, x[3] * down) : __floats2half2_rn(0.f, 0.f);
-      dst[0] = *reinterpret_cast<const uint32_t*>(&h0);
-      dst[32] = *reinterpret_cast<const uint32_t*>(&h1);
-      if (lane == 0) a.q_scale[size_t(row) * a.nq + head] = fine ? __fmul_rn(log2_scale, __uint_as_float(uint32_t(127 + e) << 23)) : __uint_as_float(0x7FC00000u);
+      const uint32_t byte = kv_warp_byte(x);
+      uint16_t* dst = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(pages) + entry * kKvDim) + lane;
+      dst[0] = uint16_t(kv_codes(x[0], x[1], byte));
+      dst[32] = uint16_t(kv_codes(x[2], x[3], byte));
+      if (lane == 0) (value ? a.pages.v_exp : a.pages.k_exp)[entry] = uint8_t(byte);
     } else {
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(pages) + entry * kKvDim) + lane;
       dst[0] = pack_bf(x[0], x[1]);
       dst[32] = pack_bf(x[2], x[3]);
-      if (lane == 0) a.q_scale[size_t(row) * a.nq + head] = log2_scale;
     }
-    return;
-  }
-  const uint32_t h = value ? head - a.nq - a.nkv : head - a.nq;
-  const size_t entry = kv_entry(place, a.nkv, h);
-  void* const pages = value ? a.pages.v : a.pages.k;
-  if constexpr (F8) {
-    const uint32_t byte = kv_warp_byte(x);
-    uint16_t* dst = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(pages) + entry * kKvDim) + lane;
-    dst[0] = uint16_t(kv_codes(x[0], x[1], byte));
-    dst[32] = uint16_t(kv_codes(x[2], x[3], byte));
-    if (lane == 0) (value ? a.pages.v_exp : a.pages.k_exp)[entry] = uint8_t(byte);
-  } else {
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(pages) + entry * kKvDim) + lane;
-    dst[0] = pack_bf(x[0], x[1]);
-    dst[32] = pack_bf(x[2], x[3]);
   }
 }
 

@@ -74,7 +74,8 @@ tree_wide_kernel(const TreeArgs a) {
   __shared__ uint32_t tmem_at, aborted;
   __shared__ uint32_t k_top, v_top;                          // largest exponent bytes of the chunk
   __shared__ int32_t seen_by_all;                            // positions below it are seen by every row of the tile
-  __shared__ uint32_t bad[2][kWideTile / 32];                // positions of a step whose key or value is not a number (two steps' worth)
+  __shared__ int64_t entries[kWideMostPart / kWideTile];     // entry (of the layer) of each step's first position; -1: no page
+  __shared__ uint32_t bad[kWideMostPart / 32], any_bad;      // positions of the chunk whose key or value is not a number; whether there are any
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t smem = (smem_u32(wide_smem_raw) + 1023u) & ~1023u, qs = smem, ks = smem + kWideOperand, vs = smem + 2 * kWideOperand;
   const uint32_t k_scales = smem + kWideScalesAt, v_scales = k_scales + 2 * kWideMostPart;
@@ -90,7 +91,6 @@ tree_wide_kernel(const TreeArgs a) {
     mbar_fence_init();
     aborted = 0u;
   }
-  if (tid < 8) bad[tid >> 2][tid & 3u] = 0u;
   if (warp == 4) {
     tmem_alloc(smem_u32(&tmem_at), kWideColumns);
     tmem_relinquish();
@@ -125,55 +125,74 @@ tree_wide_kernel(const TreeArgs a) {
     t.seq = a.row_seq[t.first];
     t.start = int32_t(t.part * part_positions);
     const uint32_t used = t.rows * a.group;
-    if (tid == 0) { k_top = v_top = 0u; seen_by_all = 0x7FFFFFFF; }
-    __syncthreads();
-    // the queries, by all warps; what the tile's rows see
-    for (uint32_t c = tid; c < kWideTile * 16; c += kWideThreads) {
-      const uint32_t m = c >> 4, piece = c & 15u, r = m / a.group;
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (m < used) x = reinterpret_cast<const uint4*>(a.q + ((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kKvDim)[piece];
-      sts128(qs + wide_offset(m, piece), x);
+    if (tid == 0) { k_top = v_top = any_bad = 0u; seen_by_all = 0x7FFFFFFF; }
+    if (tid < kWideMostPart / 32) bad[tid] = 0u;
+    if (tid >= 128 && tid < 128 + part_positions / kWideTile) {            // (a step's positions lie in one page)
+      const int64_t place = kv_place(a.table, t.seq, t.start + int32_t((tid - 128) * kWideTile));
+      entries[tid - 128] = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
     }
-    int32_t extent = 0;
+    int32_t extent = 0, all = 0x7FFFFFFF;
     for (uint32_t i = lane; i < t.rows; i += 32) {
       const int32_t e = a.extent[t.first + i];
       extent = max(extent, e);
-      if (warp == 0) atomicMin(&seen_by_all, a.row_base ? min(max(a.row_base[t.first + i], 0), e) : e);
+      all = min(all, a.row_base ? min(max(a.row_base[t.first + i], 0), e) : e);
     }
 #pragma unroll
     for (int off = 16; off; off >>= 1) extent = max(extent, __shfl_xor_sync(0xFFFFFFFFu, extent, off));
     t.extent = min(extent, t.start + int32_t(part_positions));
     const uint32_t steps = t.extent > t.start ? (uint32_t(t.extent - t.start) + kWideTile - 1) / kWideTile : 0u;
-    // entry (of the layer) of the first position of a step; the step's positions lie in one page
-    auto entry_of = [&](uint32_t j) {
-      const int64_t place = kv_place(a.table, t.seq, t.start + int32_t(j * kWideTile));
-      return place < 0 ? int64_t(-1) : int64_t(kv_entry(place, a.nkv, t.kvh));
-    };
-    if constexpr (F8) {
-      // scales of the chunk: the largest exponents first (those of no entry, 135 to 254, may stand where nobody wrote)
-      for (uint32_t c = tid; c < steps * 16; c += kWideThreads) {         // 16 bytes: K then V
-        const uint32_t j = c >> 4, v = c >> 3 & 1u, at = c & 7u;
-        const int64_t entry = entry_of(j);
-        if (entry < 0) continue;
-        const uint4 x = *reinterpret_cast<const uint4*>((v ? a.pages.v_exp : a.pages.k_exp) + entry + at * 16);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t top = 0;
-        const int32_t left = t.extent - t.start - int32_t(j * kWideTile + at * 16);
+    // the queries: sixteen lanes a row
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t b = w[i >> 2] >> (8 * (i & 3)) & 0xFFu;
-          if (i < left && b != kKvNanByte) top = max(top, min(b, 134u));
-        }
-        atomicMax(v ? &v_top : &k_top, top);
+    for (int half = 0; half < 2; ++half) {
+      uint4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t m = (tid >> 4) + (4 * half + i) * (kWideThreads / 16), r = m / a.group;
+        x[i] = m < used ? reinterpret_cast<const uint4*>(a.q + ((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kKvDim)[tid & 15u]
+                        : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sts128(qs + wide_offset((tid >> 4) + (4 * half + i) * (kWideThreads / 16), tid & 15u), x[i]);
+    }
+    __syncthreads();
+    if (warp == 0) atomicMin(&seen_by_all, all);
+    // exponents of the chunk: a thread takes sixteen positions' of K or of V
+    if constexpr (F8) {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      const uint32_t of_v = tid >> 7, at16 = tid & 127u;
+      const int64_t entry = at16 < steps * 8 ? entries[at16 >> 3] : -1;
+      if (entry >= 0) {
+        const uint4 x = *reinterpret_cast<const uint4*>((of_v ? a.pages.v_exp : a.pages.k_exp) + entry + (at16 & 7u) * 16);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+      }
+      // bytes of no entry (135 to 254, where nobody wrote) do not count, nor do those behind the last position
+      const int32_t left = t.extent - t.start - int32_t(at16 * 16);
+      uint32_t top = 0, none = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t b = w[i >> 2] >> (8 * (i & 3)) & 0xFFu;
+        if (i < left && b == kKvNanByte) none |= 1u << i;
+        if (i < left && b <= 134u) top = max(top, b);
+      }
+#pragma unroll
+      for (int off = 16; off; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+      if (lane == 0 && top) atomicMax(of_v ? &v_top : &k_top, top);
+      if (none) {
+        atomicOr(&bad[at16 >> 1], none << (16 * (at16 & 1u)));
+        any_bad = 1u;
       }
       __syncthreads();
-      for (uint32_t c = tid; c < steps * kWideTile * 2; c += kWideThreads) {
-        const uint32_t v = c >= steps * kWideTile, p = v ? c - steps * kWideTile : c;
-        const int64_t entry = entry_of(p / kWideTile);
-        const uint32_t b = entry < 0 ? 0u : (v ? a.pages.v_exp : a.pages.k_exp)[entry + p % kWideTile];
-        // (an entry that is no number: 0 here, and its position in `bad`)
-        sts_u16((v ? v_scales : k_scales) + 2 * p, b > 134u ? 0u : half_power(min(int(b) - int(v ? v_top : k_top) + 7, 7)));
+      top = of_v ? v_top : k_top;
+      uint32_t h[8];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t b = w[i >> 2] >> (8 * (i & 3)) & 0xFFu;
+        const uint32_t p = b > 134u ? 0u : half_power(min(int(b) - int(top) + 7, 7));
+        h[i >> 1] = i & 1 ? h[i >> 1] | p << 16 : p;
       }
+      const uint32_t dst = (of_v ? v_scales : k_scales) + at16 * 32;
+      sts128(dst, make_uint4(h[0], h[1], h[2], h[3]));
+      sts128(dst + 16, make_uint4(h[4], h[5], h[6], h[7]));
     }
     fence_proxy_async_smem();
     __syncthreads();
@@ -185,7 +204,7 @@ tree_wide_kernel(const TreeArgs a) {
       if constexpr (F8) {
         uint4 k[8], v[8];
         auto ask = [&](uint4 (&x)[8], const void* pool, uint32_t j) {
-          const int64_t entry = j < steps ? entry_of(j) : -1;
+          const int64_t entry = j < steps ? entries[j] : -1;
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -224,16 +243,6 @@ tree_wide_kernel(const TreeArgs a) {
           const uint32_t g = step0 + j;
           if (g) wait(bar_s, g - 1);                         // the scores of the step before have been taken from K
           store(k, ks, k_scales, j, false);
-          if (warp == 4) {                                   // positions whose entry is no number
-            const int64_t entry = entry_of(j);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool in = entry >= 0 && t.start + int32_t(j * kWideTile + 32 * i + lane) < t.extent;
-              const bool b = in && (a.pages.k_exp[entry + 32 * i + lane] == kKvNanByte || a.pages.v_exp[entry + 32 * i + lane] == kKvNanByte);
-              const uint32_t m = __ballot_sync(0xFFFFFFFFu, b);
-              if (lane == 0) bad[g & 1u][i] = m;
-            }
-          }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_k);
@@ -247,7 +256,7 @@ tree_wide_kernel(const TreeArgs a) {
         }
       } else {
         auto ask = [&](uint32_t dst, const void* pool, uint32_t j) {
-          const int64_t entry = entry_of(j);
+          const int64_t entry = entries[j];
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
           const uint8_t* src = static_cast<const uint8_t*>(pool) + (entry < 0 ? 0 : entry) * kKvDim * 2;
 #pragma unroll
@@ -263,7 +272,6 @@ tree_wide_kernel(const TreeArgs a) {
           if (g) wait(bar_s, g - 1);
           ask(ks, a.pages.k, j);
           if (g) wait(bar_o, g - 1);
-          if (warp == 4 && lane < 4) bad[(g + 1) & 1u][lane] = 0u;   // (read last for step g - 1, which is over)
           ask(vs, a.pages.v, j);
           cp_async_wait<1>();
           fence_proxy_async_smem();
@@ -288,7 +296,7 @@ tree_wide_kernel(const TreeArgs a) {
             for (int i = 0; i < 16; ++i) {
               const uint32_t m = __ballot_sync(0xFFFFFFFFu, mine >> i & 1u);
               const uint32_t p = 8 * i + 2 * (warp - 4);
-              if (lane == 0 && m) atomicOr(&bad[g & 1u][p >> 5], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
+              if (lane == 0 && m) atomicOr(&bad[j * (kWideTile / 32) + (p >> 5)], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
             }
           }
           fence_proxy_async_smem();
@@ -326,7 +334,7 @@ tree_wide_kernel(const TreeArgs a) {
         wait(bar_s, g);
         tc_fence_after();
         // which of the step's positions the row sees
-        const bool there = entry_of(j) >= 0;                 // (a page outside the pool: as if nobody saw its positions)
+        const bool there = entries[j] >= 0;                 // (a page outside the pool: as if nobody saw its positions)
         const bool every = whole(j) && there;
         uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
         bool poisoned = false;
@@ -354,9 +362,9 @@ tree_wide_kernel(const TreeArgs a) {
             see[w] = there ? bits & below : 0u;
           }
         }
-        if (F8 || !every) {
+        if (F8 ? any_bad != 0u : !every) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) poisoned = poisoned || ((F8 || !every) && (*reinterpret_cast<volatile uint32_t*>(&bad[g & 1u][w]) & see[w]));
+          for (int w = 0; w < 4; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&bad[j * (kWideTile / 32) + w]) & see[w]);
         }
         auto masked = [&](uint32_t (&x)[32], int w) {
           if (!every) {
@@ -366,13 +374,20 @@ tree_wide_kernel(const TreeArgs a) {
         };
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t x[32];
+        for (int w = 0; w < 4; w += 2) {
+          uint32_t x[32], y[32];
           tmem_ld32(s_tmem + lanes + 32 * w, x);
+          tmem_ld32(s_tmem + lanes + 32 * w + 32, y);
           tmem_ld_wait();
           masked(x, w);
+          masked(y, w + 1);
+          float even = -INFINITY, odd = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+          for (int i = 0; i < 32; i += 2) {
+            even = fmaxf(even, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+            odd = fmaxf(odd, fmaxf(__uint_as_float(y[i]), __uint_as_float(y[i + 1])));
+          }
+          top = fmaxf(top, fmaxf(even, odd));
         }
         top = __fmul_rn(top, scale);
         const bool move = top > (ref == -INFINITY ? ref : __fadd_rn(ref, kSlack));
@@ -397,18 +412,16 @@ tree_wide_kernel(const TreeArgs a) {
         }
         const float low = (ref == -INFINITY ? 0.f : ref) - kBias;
         const float2 scale2 = make_float2(scale, scale), low2 = make_float2(-low, -low);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t x[32], p[16];
-          tmem_ld32(s_tmem + lanes + 32 * w, x);
-          tmem_ld_wait();
+        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        auto weigh = [&](uint32_t (&x)[32], int w) {
           masked(x, w);
+          uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float2 e = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, low2);
             e.x = exp2_approx(e.x);
             e.y = exp2_approx(e.y);
-            sum = add2(sum, e);
+            sums[i & 1] = add2(sums[i & 1], e);
             if constexpr (F8) {
               const __half2 h = __floats2half2_rn(e.x, e.y);
               p[i] = *reinterpret_cast<const uint32_t*>(&h);
@@ -417,7 +430,20 @@ tree_wide_kernel(const TreeArgs a) {
             }
           }
           tmem_st16(s_tmem + lanes + 16 * w, p);             // (over scores that have been read)
-        }
+        };
+        uint32_t x[32], y[32];
+        tmem_ld32(s_tmem + lanes, x);
+        tmem_ld32(s_tmem + lanes + 32, y);
+        tmem_ld_wait();
+        weigh(x, 0);
+        tmem_ld32(s_tmem + lanes + 64, x);
+        weigh(y, 1);
+        tmem_ld_wait();
+        tmem_ld32(s_tmem + lanes + 96, y);
+        weigh(x, 2);
+        tmem_ld_wait();
+        weigh(y, 3);
+        sum = add2(sum, add2(sums[0], sums[1]));
         if (poisoned) sum.x = __uint_as_float(0x7FC00000u);
         tmem_st_wait();
         tc_fence_before();
@@ -465,7 +491,6 @@ tree_wide_kernel(const TreeArgs a) {
     }
     step0 += steps;
     __syncthreads();                                         // operands, scales and accumulators are free
-    if (!F8 && tid < 8) bad[tid >> 2][tid & 3u] = 0u;        // (the next use lies behind another barrier)
   }
   // (every product has been waited for, or its wait ran out: then the tensor memory is given back after a moment for what may
   // still be under way)

@@ -110,7 +110,7 @@ def _on(t, device, dtype, what, shape=None):
     """Refuses a tensor that the kernels would read wrongly."""
     if t.device != device or t.dtype != dtype:
         raise ValueError(f"{what}: {t.dtype} on {t.device}, not {dtype} on {device}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, not {shape}")
 
 
@@ -118,7 +118,7 @@ def _vector(t, device, what, n=None):
     """A contiguous int32 vector's address."""
     import torch
 
-    if t.dim() != 1 or (n is not None and t.shape[0] != n) or (t.shape[0] > 1 and t.stride(0) != 1):
+    if t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous vector{'' if n is None else f' of {n}'} is wanted")
     _on(t, device, torch.int32, what)
     return t.data_ptr()
@@ -129,11 +129,13 @@ def _launch(device, name, *args):
     import torch
 
     index = device.index
-    if index == torch.cuda.current_device():
-        _native.check(getattr(_native.lib(), name)(*args, _native.raw_stream(index)), name)
+    if index == torch._C._cuda_getDevice():
+        status = _native.packed(name)(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            _native.check(getattr(_native.lib(), name)(*args, _native.raw_stream(index)), name)
+            status = _native.packed(name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _native.check(status, name)
 
 
 class KVPages:
@@ -167,8 +169,10 @@ class KVPages:
         self.device, self.stacked = k.device, k.dim() == 5
         self.pages, self.kv_heads = k.shape[-4], k.shape[-3]
         stride = (k.stride(0), 0 if k_exp is None else k_exp.stride(0)) if self.stacked else (0, 0)
-        self._c = _native.KvPages(k.data_ptr(), v.data_ptr(), None if k_exp is None else k_exp.data_ptr(), None if v_exp is None else v_exp.data_ptr(),
-                                  *stride, k.shape[0] if self.stacked else 1, self.pages, self.kv_heads, KV_FORMATS.index(self.format))
+        # (fields of the C structure)
+        self._fields = (k.data_ptr(), v.data_ptr(), 0 if k_exp is None else k_exp.data_ptr(), 0 if v_exp is None else v_exp.data_ptr(), *stride,
+                        k.shape[0] if self.stacked else 1, self.pages, self.kv_heads, KV_FORMATS.index(self.format))
+        self._packed = _native.KV_PAGES.pack(*self._fields)
 
     @classmethod
     def alloc(cls, pages: int, kv_heads: int, device, *, kv_format="bf16", layers=None):
@@ -195,12 +199,14 @@ class KVPages:
 
 
 def _table(page_table, device):
+    """Fields of the C structure of a page table."""
     import torch
 
-    if page_table.dim() != 2 or page_table.shape[0] == 0 or page_table.shape[1] == 0 or page_table.stride(1) != 1:
+    slots, pages = page_table.shape if page_table.dim() == 2 else (0, 0)
+    if not slots or not pages or page_table.stride(1) != 1:
         raise ValueError("the page table is [slots, pages], its rows contiguous")
     _on(page_table, device, torch.int32, "page table")
-    return _native.KvTable(page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1])
+    return page_table.data_ptr(), page_table.stride(0), slots, pages
 
 
 def _kv_rows(name, k, v, row_seq, row_pos, page_table, pages):
@@ -208,15 +214,15 @@ def _kv_rows(name, k, v, row_seq, row_pos, page_table, pages):
 
     if pages.stacked:
         raise ValueError("rows go to one layer: give pages.layer(i)")
-    rows = row_seq.shape[0]
+    rows, device, width = row_seq.shape[0], pages.device, pages.kv_heads * HEAD_DIM
+    shape = (rows, pages.kv_heads, HEAD_DIM)
     for t, what in ((k, "keys"), (v, "values")):
-        _on(t, pages.device, torch.bfloat16, what, (rows, pages.kv_heads, HEAD_DIM))
-        if rows and (t.stride(2) != 1 or t.stride(1) != HEAD_DIM):
+        _on(t, device, torch.bfloat16, what, shape)
+        if rows and not (t.is_contiguous() or (t.stride(2) == 1 and t.stride(1) == HEAD_DIM)):
             raise ValueError(f"{what}: the heads of a row have to lie side by side")
-    args = _table(page_table, pages.device), _vector(row_seq, pages.device, "row_seq"), _vector(row_pos, pages.device, "row_pos", rows)
+    args = _native.KV_TABLE.pack(*_table(page_table, device)), _vector(row_seq, device, "row_seq"), _vector(row_pos, device, "row_pos", rows)
     if rows:
-        _launch(pages.device, name, pages._c, *args, k.data_ptr(), max(k.stride(0), pages.kv_heads * HEAD_DIM), v.data_ptr(),
-                max(v.stride(0), pages.kv_heads * HEAD_DIM), rows)
+        _launch(device, name, pages._packed, *args, k.data_ptr(), max(k.stride(0), width), v.data_ptr(), max(v.stride(0), width), rows)
 
 
 def kv_write(k, v, row_seq, row_pos, page_table, pages):
@@ -240,10 +246,11 @@ def kv_keep(slots, base, path, count, page_table, pages):
     if path.dim() != 2 or path.shape[0] != n or (path.shape[1] > 1 and path.stride(1) != 1):
         raise ValueError("path is [sequences, nodes], its rows contiguous")
     _on(path, pages.device, torch.int32, "path")
-    args = _table(page_table, pages.device), _vector(slots, pages.device, "slots"), _vector(base, pages.device, "base", n)
-    kept = _vector(count, pages.device, "count", n)
+    device = pages.device
+    args = _native.KV_TABLE.pack(*_table(page_table, device)), _vector(slots, device, "slots"), _vector(base, device, "base", n)
+    kept = _vector(count, device, "count", n)
     if n and path.shape[1]:
-        _launch(pages.device, "grb_kv_keep", pages._c, *args, path.data_ptr(), max(path.stride(0), path.shape[1]), kept, n, path.shape[1])
+        _launch(device, "grb_kv_keep", pages._packed, *args, path.data_ptr(), max(path.stride(0), path.shape[1]), kept, n, path.shape[1])
 
 
 class TreeRows:
@@ -260,7 +267,10 @@ class TreeRows:
         _on(mask, base.device, torch.int64, "mask")
         _vector(base, base.device, "base", rows)
         _vector(rope, base.device, "rope", rows)
-        self.base, self.rope, self.mask, self.rows = base, rope, mask, rows
+        self.rows, self.device = rows, base.device
+        self.base, self.rope, self.mask = base, rope, mask
+        # (fields of the C structure)
+        self._fields = base.data_ptr(), rope.data_ptr(), mask.data_ptr(), max(mask.stride(0), mask.shape[1]), mask.shape[1]
 
     @staticmethod
     def masks(parents, words=None):
@@ -298,6 +308,7 @@ class TreeAttention:
         self.scratch = torch.empty(self.scratch_bytes, device=device, dtype=torch.uint8)
         self.scratch[:16].zero_()
         self.device = self.scratch.device
+        self._bf16, self._scaling, self._width = torch.bfloat16, 1.0 / math.sqrt(HEAD_DIM), ((nq + 2 * nkv) * HEAD_DIM, nq * HEAD_DIM)
 
     def check_status(self) -> int:
         """GRB_STATUS_* bits of the calls since the last check (0: their outputs can be trusted).  Synchronises."""
@@ -307,39 +318,38 @@ class TreeAttention:
         self.scratch[:4].zero_()
         return bits
 
-    def __call__(self, qkv, cos, sin, row_seq, row_pos, page_table, pages, out, *, tree=None):
+    def __call__(self, qkv, cos, sin, row_seq, row_pos, page_table, pages, out, *, tree=None, longest_run=None):
         """``qkv`` (BF16 [rows, (nq + 2 nkv) 128]) -> ``out`` (BF16 [rows, nq 128]).  Keys (rotated) and values are stored at
         ``row_pos`` of the sequences in slots ``row_seq`` before any row reads.  Without ``tree`` row r sees positions up to its
-        own; with ``TreeRows`` what they say, a row that sees nothing giving zeros.  Rows of slot -1 are left out."""
-        import torch
-
-        device, rows = self.device, qkv.shape[0]
+        own; with ``TreeRows`` what they say, a row that sees nothing giving zeros.  Rows of slot -1 are left out.
+        ``longest_run``: how many rows of one sequence follow one another, at most, where the caller knows it; runs of 64 causal rows
+        or of more than 32 tree rows and heads are multiplied together (without it: causal rows are taken to be spread evenly
+        over the slots, tree rows to be anyhow)."""
+        device, bf, (wide, narrow) = self.device, self._bf16, self._width
+        rows = qkv.shape[0]
         if rows > self.max_rows or page_table.shape[1] > self.max_pages:
             raise ValueError("more rows or pages than the scratch was sized for")
         if pages.format != self.format or pages.stacked or pages.kv_heads != self.nkv or pages.device != device:
             raise ValueError("pages of one layer, in this object's format, heads and device")
-        bf = torch.bfloat16
-        _on(qkv, device, bf, "qkv", (rows, (self.nq + 2 * self.nkv) * HEAD_DIM))
-        _on(out, device, bf, "out", (rows, self.nq * HEAD_DIM))
+        _on(qkv, device, bf, "qkv", (rows, wide))
+        _on(out, device, bf, "out", (rows, narrow))
         _on(cos, device, bf, "cos")
-        _on(sin, device, bf, "sin", tuple(cos.shape))
+        _on(sin, device, bf, "sin", cos.shape)
         if cos.dim() != 2 or cos.shape[1] != HEAD_DIM or not cos.is_contiguous() or not sin.is_contiguous():
             raise ValueError("rotary tables are contiguous [positions, 128]")
+        if longest_run is not None and longest_run < 1:
+            raise ValueError("longest_run is at least 1")
         if not rows:
             return
         if qkv.stride(1) != 1 or out.stride(1) != 1:
             raise ValueError("rows of qkv and out have to be contiguous")
-        step = _native.TreeStep()
-        step.qkv, step.ldq = qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1])
-        step.cos_table, step.sin_table, step.rope_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-        step.row_seq, step.row_pos = _vector(row_seq, device, "row_seq", rows), _vector(row_pos, device, "row_pos", rows)
+        nodes = (0, 0, 0, 0, 0)
         if tree is not None:
-            if tree.rows != rows or tree.base.device != device:
+            if tree.rows != rows or tree.device != device:
                 raise ValueError("tree rows: one for each row, on the same device")
-            step.row_base, step.row_rope, step.row_mask = tree.base.data_ptr(), tree.rope.data_ptr(), tree.mask.data_ptr()
-            step.ldm, step.mask_words = max(tree.mask.stride(0), tree.mask.shape[1]), tree.mask.shape[1]
-        step.pages, step.table = pages._c, _table(page_table, device)
-        step.scratch, step.scratch_bytes = self.scratch.data_ptr(), self.scratch_bytes
-        step.out, step.ldo = out.data_ptr(), max(out.stride(0), out.shape[1])
-        step.rows, step.nq, step.head_dim, step.scaling = rows, self.nq, HEAD_DIM, 1.0 / math.sqrt(HEAD_DIM)
+            nodes = tree._fields
+        step = _native.TREE_STEP.pack(
+            qkv.data_ptr(), max(qkv.stride(0), wide), cos.data_ptr(), sin.data_ptr(), cos.shape[0], _vector(row_seq, device, "row_seq", rows),
+            _vector(row_pos, device, "row_pos", rows), *nodes, *pages._fields, *_table(page_table, device), self.scratch.data_ptr(), self.scratch_bytes,
+            out.data_ptr(), max(out.stride(0), narrow), rows, self.nq, HEAD_DIM, self._scaling, longest_run or 0)
         _launch(device, "grb_attn_tree", step)

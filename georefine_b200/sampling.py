@@ -122,6 +122,7 @@ class DraftVerifier:
         self.tokens, self.rows = (torch.empty(self.max_seqs, self.width, device=device, dtype=torch.int32) for _ in range(2))
         self.count = torch.empty(self.max_seqs, device=device, dtype=torch.int32)
         self.device = self.stats.device
+        self._places = tuple(t.data_ptr() for t in (self.stats, self.tokens, self.rows, self.count))
 
     def __call__(self, logits, tokens, starts, u_keep, u_draw, *, temperature=1.0, parent=None, draft_probs=None):
         """``logits`` (BF16 or FP32 [rows, vocabulary]): the target's, row i those behind node i.  Rows ``starts[s]`` ..
@@ -141,7 +142,8 @@ class DraftVerifier:
         from .ops import _launch, _on, _vector
 
         device, n = self.device, starts.shape[0] - 1
-        if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.device != device or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        kind = 0 if logits.dtype is torch.bfloat16 else 1 if logits.dtype is torch.float32 else None
+        if logits.dim() != 2 or kind is None or logits.device != device or (logits.shape[1] > 1 and logits.stride(1) != 1):
             raise ValueError("logits are BF16 or FP32 [rows, vocabulary] on the verifier's device, their rows contiguous")
         rows, vocab = logits.shape
         if not 0 <= n <= self.max_seqs or rows > self.max_rows:
@@ -150,26 +152,23 @@ class DraftVerifier:
             raise ValueError("temperature must be positive; temperature 0 is the arg-max path")
         for t, size, what in ((u_keep, rows, "u_keep"), (u_draw, n, "u_draw")):
             _on(t, device, torch.float32, what, (size,))
-            if size > 1 and t.stride(0) != 1:
+            if not t.is_contiguous():
                 raise ValueError(f"{what} has to be contiguous")
-        step = _native.VerifyStep()
+        q = ldq = 0
         if draft_probs is not None:
             if parent is not None:
                 raise ValueError("the drafter's probabilities go with chains")
             _on(draft_probs, device, torch.float32, "draft_probs", (rows, vocab))
             if vocab > 1 and draft_probs.stride(1) != 1:
                 raise ValueError("rows of draft_probs have to be contiguous")
-            step.draft_probs, step.ldq = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
-        out = self.tokens[:n], self.rows[:n], self.count[:n]
-        step.tokens, step.starts = _vector(tokens, device, "tokens", rows), _vector(starts, device, "starts")
-        step.parent = None if parent is None else _vector(parent, device, "parent", rows)
-        if not n:
-            return out
-        step.logits, step.ldl, step.dtype = logits.data_ptr(), max(logits.stride(0), vocab), int(logits.dtype == torch.float32)
-        step.u_keep, step.u_draw, step.stats = u_keep.data_ptr(), u_draw.data_ptr(), self.stats.data_ptr()
-        step.out_tokens, step.out_rows, step.out_count = self.tokens.data_ptr(), self.rows.data_ptr(), self.count.data_ptr()
-        step.rows, step.seqs, step.vocab, step.width, step.temperature = rows, n, vocab, self.width, float(temperature)
-        _launch(device, "grb_verify_drafts", step)
+            q, ldq = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
+        above = 0 if parent is None else _vector(parent, device, "parent", rows)
+        tokens_at, starts_at = _vector(tokens, device, "tokens", rows), _vector(starts, device, "starts")
+        out = (self.tokens, self.rows, self.count) if n == self.max_seqs else (self.tokens[:n], self.rows[:n], self.count[:n])
+        if n:
+            step = _native.VERIFY_STEP.pack(logits.data_ptr(), max(logits.stride(0), vocab), tokens_at, above, starts_at, u_keep.data_ptr(), u_draw.data_ptr(), q, ldq,
+                                            *self._places, rows, n, vocab, self.width, kind, float(temperature))
+            _launch(device, "grb_verify_drafts", step)
         return out
 
 

@@ -319,14 +319,14 @@ class BatchDecoder:
             self._tree_staged = 0
         return self._tree_attn
 
-    def attend(self, layer: int, rows: slice, tree: bool = False) -> None:
-        """Attention of rows ``rows`` over one layer's cache, into ``ctx``."""
+    def attend(self, layer: int, rows: slice, tree: bool = False, longest: int | None = None) -> None:
+        """Attention of rows ``rows`` over one layer's cache, into ``ctx``.  ``longest``: see ``ops.TreeAttention``."""
         qkv, seq, pos, out = self.qkv[rows], self.row_seq[rows], self.row_pos[rows], self.ctx[rows]
         if self.attn is not None and not tree:
             self.attn(qkv, self.cos, self.sin, seq, pos, self.page_table, self.kv[layer, 0], self.kv[layer, 1], out)
         else:
             nodes = ops.TreeRows(self.row_base[rows], self.row_rope[rows], self.row_mask[rows]) if tree else None
-            self._tree_attention()(qkv, self.cos, self.sin, seq, pos, self.page_table, self._pages[layer], out, tree=nodes)
+            self._tree_attention()(qkv, self.cos, self.sin, seq, pos, self.page_table, self._pages[layer], out, tree=nodes, longest_run=longest)
 
     # ---- sequence slots and pages (host bookkeeping; the device sees only the page table) ---------------------
     def open_slot(self) -> int:
@@ -368,7 +368,7 @@ class BatchDecoder:
             ops.rmsnorm(h, layer.norm1, x, delta=delta, eps=cfg.eps)       # (the previous layer's MLP output joins the stream here)
             self._linear(layer.qkv, x, self.qkv[:n])
             for lo in range(0, n, self.max_rows):       # (rows see positions up to their own: those of earlier slices are appended)
-                self.attend(i, slice(lo, min(n, lo + self.max_rows)), tree)
+                self.attend(i, slice(lo, min(n, lo + self.max_rows)), tree, 1 if advance else None if tree else self.max_rows)
             self._row_parallel(layer.o, "o", self.ctx[:n], self.o_out[:n])
             ops.rmsnorm(h, layer.norm2, x, delta=self.o_out[:n], eps=cfg.eps)
             self._linear(layer.gate_up, x, self.gate_up[:n])

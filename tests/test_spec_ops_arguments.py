@@ -152,3 +152,18 @@ def test_masks_of_a_tree():
         ops.TreeRows.masks([-1] * 65, words=1)
     with pytest.raises(ValueError, match="words"):
         ops.TreeRows.masks([-1] * 257)
+
+
+def test_structures_packed_in_one_go_are_the_c_structures():
+    import struct
+
+    for packed, c in ((_native.KV_PAGES, _native.KvPages), (_native.KV_TABLE, _native.KvTable), (_native.TREE_STEP, _native.TreeStep), (_native.VERIFY_STEP, _native.VerifyStep)):
+        assert packed.size == ctypes.sizeof(c)
+
+        def flat(s):
+            for name, kind in s._fields_:
+                value = getattr(s, name)
+                yield from flat(value) if isinstance(value, ctypes.Structure) else [value or 0]
+
+        values = [0.5 if code in "fd" else i + 1 for i, code in enumerate(packed.format.replace("4x", "")[1:])]
+        assert list(flat(c.from_buffer_copy(packed.pack(*values)))) == values
