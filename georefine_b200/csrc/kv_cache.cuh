@@ -68,6 +68,10 @@ __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t pair) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(uint16_t(pair)));
   return r;
 }
+// Four codes as two pairs.
+__device__ __forceinline__ void e4m3_to_half4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int off = 16; off; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));

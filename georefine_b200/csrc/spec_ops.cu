@@ -81,7 +81,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
     if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem, stream, a)) return st;
   }
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
-  return launch_step(tree_combine_kernel<8>, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a);
+  return launch_step(tree_combine_kernel, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a);
 }
 
 template <class... Params>

@@ -21,6 +21,7 @@ namespace grb {
 
 constexpr uint32_t kTreeMaxRows = 4096, kTreeMaskWords = 4;
 constexpr int kTreePrepThreads = 256;
+constexpr uint32_t kTreeRowAbsent = 0xFFFFFFFFu;             // row_parts of a row that is left out: its output stays as it was
 // Positions of a wide tile's unit: the most, for long contexts (a unit's result is as large as 256 positions of an 8-bit cache); fewer
 // for short ones, whose few units would leave SMs idle.
 constexpr uint32_t kWideMostPart = 2048;
@@ -46,8 +47,8 @@ struct TreeArgs {
   uint32_t* status;           // scratch: kStatusTimeout where a wait ran out
   int32_t* extent;            // scratch: [rows]: positions up to the last one the row sees
   uint32_t* row_parts;        // scratch: [rows]: parts of the row
-  int4* tiles;                // scratch: [rows]: first row, rows, first unit, positions of a unit
-  int4* wide_tiles;           // scratch: [rows]: the same of wide tiles
+  int4* tiles;                // scratch: [rows]: first row, rows, first unit, positions up to the last one its rows see
+  int4* wide_tiles;           // scratch: [rows]: first row, rows, first unit, positions of a unit
   uint32_t* plan;             // scratch: tiles, units, wide tiles, wide units
   float* part_acc;            // scratch: [rows][nq][max_parts][128]
   float2* part_ml;            // scratch: [rows][nq][max_parts]: maximum and sum of a part
@@ -64,9 +65,9 @@ __device__ __forceinline__ int64_t tree_place(const TreeArgs& a, uint32_t r) {
   const int32_t pos = a.row_pos[r], rope = a.row_base ? a.row_rope[r] : pos;
   return uint32_t(rope) < a.rope_rows ? kv_place(a.table, a.row_seq[r], pos) : -1;
 }
-// One past the last position that row r sees.
+// One past the last position that row r sees; -1: left out.
 __device__ __forceinline__ int32_t tree_extent(const TreeArgs& a, uint32_t r) {
-  if (tree_place(a, r) < 0) return 0;
+  if (tree_place(a, r) < 0) return -1;
   if (!a.row_base) return a.row_pos[r] + 1;
   const int32_t most = int32_t(a.table.max_pages * kKvPage);
   const int32_t base = min(max(a.row_base[r], 0), most);
@@ -100,66 +101,65 @@ __device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
 // A tile is up to tile_rows (wide_rows) consecutive rows of one sequence; rows that are left out or see nothing may be among them.
 // What it needs of the rows is read once, side by side; the rest runs in shared memory.
 __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_positions) {
-  extern __shared__ int32_t extents[];                       // [rows]
+  extern __shared__ int32_t extents[];                       // [rows]; -1: left out
   uint16_t* const run_of = reinterpret_cast<uint16_t*>(extents + a.rows);      // [rows]: first row of the row's run (rows of one sequence in a row)
   __shared__ int32_t scratch[kTreePrepThreads / 32];
+  __shared__ unsigned long long sums[kTreePrepThreads / 32], total;
   const uint32_t tid = threadIdx.x;
-  const auto larger = [](int32_t x, int32_t y) { return max(x, y); };
-  const auto sum = [](int32_t x, int32_t y) { return x + y; };
   int32_t run = 0;
   for (uint32_t lo = 0; lo < a.rows; lo += kTreePrepThreads) {
     const uint32_t r = lo + tid;
     const bool in = r < a.rows;
-    const int32_t extent = in ? tree_extent(a, r) : 0;
+    const int32_t extent = in ? tree_extent(a, r) : -1;
     const bool start = in && (r == 0 || a.row_seq[r] != a.row_seq[r - 1]);
-    const int32_t first = cta_scan(start ? int32_t(r) : run, scratch, larger);
+    const int32_t first = cta_scan(start ? int32_t(r) : run, scratch, [](int32_t x, int32_t y) { return max(x, y); });
     if (in) {
       extents[r] = extent;
       run_of[r] = uint16_t(first);
-      a.extent[r] = extent;
+      a.extent[r] = max(extent, 0);
     }
     __syncthreads();
     run = run_of[min(lo + kTreePrepThreads, a.rows) - 1];
   }
-  int32_t tiles = 0, units = 0, wide_tiles = 0, wide_units = 0;
+  // how many tiles and units there are before a tile, of either kind: tiles above, units (at most 2^32) below
+  unsigned long long done = 0, wide_done = 0;
   for (uint32_t lo = 0; lo < a.rows; lo += kTreePrepThreads) {
     const uint32_t r = lo + tid;
     uint32_t n = 0, parts = 0, positions = part_positions;
+    int32_t extent = 0;
     bool wide = false;
     if (r < a.rows) {
       const uint32_t first = run_of[r], last = first + a.wide_from - 1;
       wide = a.wide_from && last < a.rows && run_of[last] == first;
       const uint32_t per = wide ? a.wide_rows : a.tile_rows;
       if ((r - first) % per == 0) {
-        int32_t extent = 0;
         for (; n < per && r + n < a.rows && run_of[r + n] == first; ++n) extent = max(extent, extents[r + n]);
         if (wide) positions = wide_part(uint32_t(extent));
         parts = (uint32_t(extent) + positions - 1) / positions;
-        for (uint32_t i = 0; i < n; ++i) a.row_parts[r + i] = wide ? parts : (uint32_t(extents[r + i]) + positions - 1) / positions;
+        if (wide)
+          for (uint32_t i = 0; i < n; ++i) a.row_parts[r + i] = extents[r + i] < 0 ? kTreeRowAbsent : parts;
       }
+      if (!wide) a.row_parts[r] = extents[r] < 0 ? kTreeRowAbsent : (uint32_t(extents[r]) + part_positions - 1) / part_positions;
     }
-    const int32_t mine = int32_t(parts * a.nkv);
-    const int32_t t = cta_scan(int32_t(parts && !wide), scratch, sum), u = cta_scan(wide ? 0 : mine, scratch, sum);
-    int32_t wt = 0, wu = 0;
+    const unsigned long long mine = parts ? (1ull << 32) + parts * a.nkv : 0ull;
+    auto scan = [&](bool counts, unsigned long long before) {
+      const auto sum = [](unsigned long long x, unsigned long long y) { return x + y; };
+      const unsigned long long upto = before + cta_scan(counts ? mine : 0ull, sums, sum);
+      if (tid == kTreePrepThreads - 1) total = upto;
+      return upto;
+    };
+    const unsigned long long upto = scan(!wide, done);
+    if (parts && !wide) a.tiles[(upto >> 32) - 1] = make_int4(int32_t(r), int32_t(n), int32_t(uint32_t(upto) - parts * a.nkv), extent);
+    __syncthreads();
+    done = total;
     if (a.wide_from) {
-      wt = cta_scan(int32_t(parts && wide), scratch, sum);
-      wu = cta_scan(wide ? mine : 0, scratch, sum);
+      const unsigned long long wide_upto = scan(wide, wide_done);
+      if (parts && wide) a.wide_tiles[(wide_upto >> 32) - 1] = make_int4(int32_t(r), int32_t(n), int32_t(uint32_t(wide_upto) - parts * a.nkv), int32_t(positions));
+      __syncthreads();
+      wide_done = total;
     }
-    if (parts) {
-      if (wide) a.wide_tiles[wide_tiles + wt - 1] = make_int4(int32_t(r), int32_t(n), wide_units + wu - mine, int32_t(positions));
-      else a.tiles[tiles + t - 1] = make_int4(int32_t(r), int32_t(n), units + u - mine, int32_t(positions));
-    }
-    // the last thread's sums go to everybody
-    __shared__ int32_t totals[4];
-    __syncthreads();
-    if (tid == kTreePrepThreads - 1) totals[0] = t, totals[1] = u, totals[2] = wt, totals[3] = wu;
-    __syncthreads();
-    tiles += totals[0];
-    units += totals[1];
-    wide_tiles += totals[2];
-    wide_units += totals[3];
   }
-  if (tid == 0) a.plan[0] = uint32_t(tiles), a.plan[1] = uint32_t(units), a.plan[2] = uint32_t(wide_tiles), a.plan[3] = uint32_t(wide_units);
+  if (tid == 0) a.plan[0] = uint32_t(done >> 32), a.plan[1] = uint32_t(done), a.plan[2] = uint32_t(wide_done >> 32), a.plan[3] = uint32_t(wide_done);
 }
 
 // The first CTA lays down the plan; in the others a warp takes up to eight neighbouring heads of a row, all their loads on their
@@ -291,54 +291,86 @@ __device__ __forceinline__ uint32_t half2_number(uint32_t v) {
   return r;
 }
 
+// Units are numbered tile by tile, part by part, kv head by kv head; a CTA takes a run of them, so that it looks up a tile, and the page
+// of a part, once for all kv heads (units dealt round in turn spent longer in chains of look-ups than in arithmetic).
 struct TreeUnit {
   int64_t k;                // byte offset of the part's K and V tile in its pool
-  size_t exps;
-  uint32_t first, rows, kvh, part;
-  int32_t start;
-  uint32_t npos;            // positions of the part up to the tile's last visible one; 0: no unit
+  int64_t place;            // of the part's first position; -1: no page
+  uint32_t tile, first, rows, kvh, part, parts;
+  int32_t seq, extent, start;
+  uint32_t npos;            // positions of the part up to the tile's last visible one; 0: none
 };
-
+// First places of the part the unit is at.
 template <bool F8>
-__device__ __forceinline__ TreeUnit tree_unit(const TreeArgs& a, uint32_t u, uint32_t units, uint32_t tiles, uint32_t& tile) {
-  TreeUnit t{};
-  if (u >= units) return t;
-  // tiles are in the order of their units; this CTA's units ascend
-  const uint32_t lane = threadIdx.x & 31u;
-  for (;;) {
-    const uint32_t next = tile + 1 + lane;
-    const uint32_t past = __ballot_sync(0xFFFFFFFFu, next < tiles && uint32_t(a.tiles[next].z) <= u);
-    tile += __popc(past);
-    if (past != 0xFFFFFFFFu) break;
-  }
-  const int4 d = a.tiles[tile];
-  const uint32_t local = u - uint32_t(d.z);
+__device__ __forceinline__ void tree_look_up(const TreeArgs& a, TreeUnit& t) {
+  t.start = int32_t(t.part * TreePart<F8>::kPositions);
+  t.place = kv_place(a.table, t.seq, t.start);             // (a part starts on a page or in its middle; outside the pool: as if nobody saw it)
+  t.npos = t.place < 0 || t.extent <= t.start ? 0u : min(TreePart<F8>::kPositions, uint32_t(t.extent - t.start));
+}
+template <bool F8>
+__device__ __forceinline__ void tree_set_tile(const TreeArgs& a, TreeUnit& t, const int4& d) {
   t.first = uint32_t(d.x);
   t.rows = uint32_t(d.y);
+  t.extent = d.w;
+  t.parts = (uint32_t(t.extent) + TreePart<F8>::kPositions - 1) / TreePart<F8>::kPositions;
+  t.seq = a.row_seq[t.first];
+}
+template <bool F8>
+__device__ __forceinline__ void tree_locate(const TreeArgs& a, TreeUnit& t) {
+  t.k = t.npos ? int64_t(kv_entry(t.place, a.nkv, t.kvh)) * TreePart<F8>::kRowBytes : 0;
+}
+// The unit of number u.  Whole warp.
+template <bool F8>
+__device__ __forceinline__ TreeUnit tree_unit(const TreeArgs& a, uint32_t u, uint32_t tiles) {
+  TreeUnit t;
+  const uint32_t lane = threadIdx.x & 31u;
+  uint32_t lo = 0, n = tiles;                              // the tile is one of n from lo on
+  while (n > 1) {
+    const uint32_t step = (n + 31) / 32, at = lo + lane * step;
+    const uint32_t past = __ballot_sync(0xFFFFFFFFu, lane * step < n && uint32_t(a.tiles[at].z) <= u);      // (lane 0 always)
+    const uint32_t k = __popc(past) - 1;
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  t.tile = lo;
+  const int4 d = a.tiles[lo];
+  tree_set_tile<F8>(a, t, d);
+  const uint32_t local = u - uint32_t(d.z);
   t.kvh = local % a.nkv;
   t.part = local / a.nkv;
-  t.start = int32_t(t.part * TreePart<F8>::kPositions);
-  int32_t extent = 0;
-  for (uint32_t i = lane; i < t.rows; i += 32) extent = max(extent, a.extent[t.first + i]);
-#pragma unroll
-  for (int off = 16; off; off >>= 1) extent = max(extent, __shfl_xor_sync(0xFFFFFFFFu, extent, off));
-  const int64_t place = kv_place(a.table, a.row_seq[t.first], t.start);   // (a part starts on a page or in its middle)
-  if (place < 0 || extent <= t.start) return t;                  // (a page outside the pool: as if nobody saw the part)
-  t.npos = min(TreePart<F8>::kPositions, uint32_t(extent - t.start));
-  const size_t entry = kv_entry(place, a.nkv, t.kvh);
-  t.k = int64_t(entry) * TreePart<F8>::kRowBytes;
-  t.exps = entry;
+  tree_look_up<F8>(a, t);
+  tree_locate<F8>(a, t);
   return t;
 }
+template <bool F8>
+__device__ __forceinline__ void tree_next(const TreeArgs& a, TreeUnit& t) {
+  if (++t.kvh == a.nkv) {
+    t.kvh = 0;
+    if (++t.part == t.parts) {
+      t.part = 0;
+      tree_set_tile<F8>(a, t, a.tiles[++t.tile]);
+    }
+    tree_look_up<F8>(a, t);
+  }
+  tree_locate<F8>(a, t);
+}
 
+// A thread takes the same piece of every sixteenth (BF16: eighth) row, whose places in shared memory are equally far apart.
 template <bool F8>
 __device__ __forceinline__ void tree_request(uint32_t dst, const void* pool, const TreeUnit& t, uint32_t tid) {
-  const uint8_t* src = static_cast<const uint8_t*>(pool) + t.k;
-  constexpr uint32_t kPieces = TreePart<F8>::kRowBytes / 16;
+  constexpr uint32_t kPieces = TreePart<F8>::kRowBytes / 16, kRows = TreePart<F8>::kThreads / kPieces;
+  const uint32_t r0 = tid / kPieces;
+  const uint8_t* src = static_cast<const uint8_t*>(pool) + t.k + tid * 16;
+  dst += TreePart<F8>::offset(r0, tid % kPieces);
+  if (t.npos == TreePart<F8>::kPositions) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t c = tid + i * TreePart<F8>::kThreads, r = c / kPieces, piece = c % kPieces;
-    cp_async_16(dst + TreePart<F8>::offset(r, piece), src + (r < t.npos ? c * 16 : 0u), r < t.npos ? 16u : 0u);
+    for (int i = 0; i < 16; ++i) cp_async_16(dst + i * TreePart<F8>::kThreads * 16, src + i * TreePart<F8>::kThreads * 16, 16u);
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const bool in = r0 + i * kRows < t.npos;
+      cp_async_16(dst + i * TreePart<F8>::kThreads * 16, in ? src + i * TreePart<F8>::kThreads * 16 : src, in ? 16u : 0u);
+    }
   }
 }
 // K with both exponent runs (positions beyond the last visible one: bytes of the same page, under a mask)
@@ -347,7 +379,7 @@ __device__ __forceinline__ void tree_request_k(const TreeArgs& a, uint32_t smem,
   if (t.npos) {
     tree_request<F8>(smem, a.pages.k, t, tid);
     if constexpr (F8) {
-      if (tid < 32) cp_async_16(smem + TreePart<F8>::kExpAt + tid * 16, (tid < 16 ? a.pages.k_exp : a.pages.v_exp) + t.exps + (tid & 15u) * 16, 16u);
+      if (tid < 32) cp_async_16(smem + TreePart<F8>::kExpAt + tid * 16, (tid < 16 ? a.pages.k_exp : a.pages.v_exp) + t.k / 128 + (tid & 15u) * 16, 16u);
     }
   }
   cp_async_commit();
@@ -362,24 +394,25 @@ __device__ __forceinline__ void tree_request_v(const TreeArgs& a, uint32_t smem,
 // for the writers (eight lanes: two rows, pieces 8 apart) and the readers (a row at a time) alike.
 __device__ __forceinline__ uint32_t tree_merge_index(uint32_t m, uint32_t piece) { return m * 128u + ((piece ^ ((piece >> 3) | ((m & 1u) << 2))) << 2); }
 
-template <bool F8, bool CLEAN>
+template <bool CLEAN>
 __device__ __forceinline__ void tree_values_f8(float (&o)[16][4], const uint32_t (&pa)[4][4], uint32_t vs, uint32_t p_warp, uint32_t lane) {
   const uint32_t g = lane >> 2, c = lane & 3u;
+  const uint32_t even = vs + TreePart<true>::offset(p_warp + 2 * c, g), odd = vs + TreePart<true>::offset(p_warp + 2 * c + 1, g);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {                    // 16 positions per step
-    const uint32_t p = p_warp + 16 * t + 2 * c;
     uint4 r[4];
-    r[0] = lds128(vs + TreePart<true>::offset(p, g));
-    r[1] = lds128(vs + TreePart<true>::offset(p + 1, g));
-    r[2] = lds128(vs + TreePart<true>::offset(p + 8, g));
-    r[3] = lds128(vs + TreePart<true>::offset(p + 9, g));
+    r[0] = lds128(even + 2048 * t);
+    r[1] = lds128(odd + 2048 * t);
+    r[2] = lds128(even + 2048 * t + 1024);
+    r[3] = lds128(odd + 2048 * t + 1024);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const uint32_t x0 = (&r[0].x)[w], x1 = (&r[1].x)[w], x2 = (&r[2].x)[w], x3 = (&r[3].x)[w];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {       // dimensions 16 g + 4 w + 2 half and the next
-        const uint32_t lo = __byte_perm(x0, x1, half ? 0x7362 : 0x5140), hi = __byte_perm(x2, x3, half ? 0x7362 : 0x5140);
-        uint32_t b00 = e4m3_to_half2(lo & 0xFFFFu), b01 = e4m3_to_half2(hi & 0xFFFFu), b10 = e4m3_to_half2(lo >> 16), b11 = e4m3_to_half2(hi >> 16);
+        uint32_t b00, b01, b10, b11;
+        e4m3_to_half4(__byte_perm(x0, x1, half ? 0x7362 : 0x5140), b00, b10);
+        e4m3_to_half4(__byte_perm(x2, x3, half ? 0x7362 : 0x5140), b01, b11);
         if (CLEAN) { b00 = half2_number(b00); b01 = half2_number(b01); b10 = half2_number(b10); b11 = half2_number(b11); }
         mma_f16_16816(o[4 * w + 2 * half], pa[t], b00, b01);
         mma_f16_16816(o[4 * w + 2 * half + 1], pa[t], b10, b11);
@@ -397,45 +430,33 @@ tree_part_kernel(const TreeArgs a) {
   extern __shared__ __align__(128) unsigned char tree_smem[];
   __shared__ float ml_sm[4][16][2];
   __shared__ uint32_t bad_sm[P::kPositions / 32];     // BF16: positions of the part whose value is not finite
+  __shared__ __align__(16) float scales_sm[F8 ? 3 : 1][F8 ? P::kPositions : 4];     // 8 bits: 2^e of K, e and 2^-e of V
   const uint32_t smem = smem_u32(tree_smem), vs = smem + P::kTileBytes;
   float* const merge = reinterpret_cast<float*>(tree_smem + P::kTileBytes);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, c = lane & 3u;
   const uint32_t m0 = lane >> 2, m1 = m0 + 8;         // the two MMA rows whose scores and outputs this lane holds
   const uint32_t tiles = a.plan[0], units = a.plan[1];
-  uint32_t tile = 0;
-  TreeUnit t = tree_unit<F8>(a, blockIdx.x, units, tiles, tile);
+  const uint32_t u0 = uint32_t(uint64_t(units) * blockIdx.x / gridDim.x), u1 = uint32_t(uint64_t(units) * (blockIdx.x + 1) / gridDim.x);
+  if (u0 == u1) return;
+  TreeUnit t = tree_unit<F8>(a, u0, tiles);
   tree_request_k<F8>(a, smem, t, tid);
   tree_request_v<F8>(a, smem, t, tid);
-  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const TreeUnit next = tree_unit<F8>(a, u + gridDim.x, units, tiles, tile);
-    if (!t.npos) {            // a page outside the pool: as if no row saw the part (alike in the whole CTA)
-      for (uint32_t m = warp; m < t.rows * a.group; m += 4) {
-        const size_t at = (size_t(t.first + m / a.group) * a.nq + t.kvh * a.group + m % a.group) * a.max_parts + t.part;
-        *reinterpret_cast<float4*>(a.part_acc + at * kKvDim + lane * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (lane == 0) a.part_ml[at] = make_float2(-INFINITY, 0.f);
-      }
-      cp_async_wait<0>();
-      __syncthreads();
-      tree_request_k<F8>(a, smem, next, tid);
-      tree_request_v<F8>(a, smem, next, tid);
-      t = next;
-      continue;
-    }
-    // MMA row m = (row of the tile) * group + (query head of the group)
-    const uint32_t used = t.rows * a.group, rl0 = m0 / a.group, rl1 = m1 / a.group;
+  uint32_t qa[8][4];
+  float scale0 = 0.f, scale1 = 0.f;
+  // the queries of a unit as A fragments, MMA row m = (row of the tile) * group + (query head of the group), and their scales
+  auto ask_q = [&](const TreeUnit& n) {
+    const uint32_t used = n.rows * a.group, rl0 = m0 / a.group, rl1 = m1 / a.group;
     const bool ok0 = m0 < used, ok1 = m1 < used;
-    const uint32_t row0 = t.first + (ok0 ? rl0 : 0), row1 = t.first + (ok1 ? rl1 : 0);
-    const size_t q0 = size_t(row0) * a.nq + t.kvh * a.group + (ok0 ? m0 - rl0 * a.group : 0);
-    const size_t q1 = size_t(row1) * a.nq + t.kvh * a.group + (ok1 ? m1 - rl1 * a.group : 0);
-    uint32_t qa[8][4];
+    const size_t q0 = ok0 ? size_t(n.first + rl0) * a.nq + n.kvh * a.group + (m0 - rl0 * a.group) : 0;
+    const size_t q1 = ok1 ? size_t(n.first + rl1) * a.nq + n.kvh * a.group + (m1 - rl1 * a.group) : 0;
     if constexpr (F8) {       // step 4 h + j of the product takes dimensions 64 h + 16 c + 4 j .. + 3 of lane group c
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint4 x[2] = {}, y[2] = {};
         if (ok0) { const uint4* s = reinterpret_cast<const uint4*>(a.q + q0 * kKvDim + 64 * h + 16 * c); x[0] = s[0]; x[1] = s[1]; }
         if (ok1) { const uint4* s = reinterpret_cast<const uint4*>(a.q + q1 * kKvDim + 64 * h + 16 * c); y[0] = s[0]; y[1] = s[1]; }
-        const uint32_t* xs = &x[0].x;
-        const uint32_t* ys = &y[0].x;
+        const uint32_t xs[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+        const uint32_t ys[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           qa[4 * h + j][0] = xs[2 * j]; qa[4 * h + j][1] = ys[2 * j];
@@ -453,13 +474,38 @@ tree_part_kernel(const TreeArgs a) {
         qa[k][3] = ok1 ? *reinterpret_cast<const uint32_t*>(s1 + 16 * k + 8) : 0u;
       }
     }
-    const float scale0 = ok0 ? a.q_scale[q0] : 0.f, scale1 = ok1 ? a.q_scale[q1] : 0.f;
+    scale0 = ok0 ? a.q_scale[q0] : 0.f;
+    scale1 = ok1 ? a.q_scale[q1] : 0.f;
+  };
+  ask_q(t);
+  for (uint32_t u = u0; u < u1; ++u) {
+    TreeUnit next = t;
+    const bool more = u + 1 < u1;
+    if (more) tree_next<F8>(a, next);
+    else next.npos = 0;
+    if (!t.npos) {            // a page outside the pool: as if no row saw the part (alike in the whole CTA)
+      for (uint32_t m = warp; m < t.rows * a.group; m += 4) {
+        const size_t at = (size_t(t.first + m / a.group) * a.nq + t.kvh * a.group + m % a.group) * a.max_parts + t.part;
+        *reinterpret_cast<float4*>(a.part_acc + at * kKvDim + lane * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane == 0) a.part_ml[at] = make_float2(-INFINITY, 0.f);
+      }
+      cp_async_wait<0>();
+      __syncthreads();
+      tree_request_k<F8>(a, smem, next, tid);
+      tree_request_v<F8>(a, smem, next, tid);
+      if (more) ask_q(next);
+      t = next;
+      continue;
+    }
+    const uint32_t used = t.rows * a.group, rl0 = m0 / a.group, rl1 = m1 / a.group;
+    const bool ok0 = m0 < used, ok1 = m1 < used;
+    const uint32_t row0 = t.first + (ok0 ? rl0 : 0), row1 = t.first + (ok1 ? rl1 : 0);
     // positions of this part below which rows m0 and m1 see everything; behind them, in a tree, the mask decides
     const int32_t base0 = a.row_base ? a.row_base[row0] : 0, base1 = a.row_base ? a.row_base[row1] : 0;
     const int32_t seen0 = ok0 ? min(a.row_base ? base0 : a.extent[row0], a.extent[row0]) - t.start : 0;
     const int32_t seen1 = ok1 ? min(a.row_base ? base1 : a.extent[row1], a.extent[row1]) - t.start : 0;
-    // whether the part holds positions that some row of the tile does not see
-    const bool holes = __syncthreads_or((ok0 && seen0 < int32_t(t.npos)) || (ok1 && seen1 < int32_t(t.npos)));
+    // whether some row of the tile does not see the whole part
+    const bool holes = __syncthreads_or((ok0 && seen0 < int32_t(P::kPositions)) || (ok1 && seen1 < int32_t(P::kPositions)));
     if (!F8 && holes) {       // values that are not finite would reach, as 0 * infinity, the rows that do not see them
       if (tid < P::kPositions / 32) bad_sm[tid] = 0u;
       cp_async_wait<0>();
@@ -488,16 +534,31 @@ tree_part_kernel(const TreeArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
     if constexpr (F8) {
+      // what the positions' exponents mean, a thread two positions of K or of V: 2^e; e and 2^-e
+      {
+        const uint32_t pair = lds_u16(smem + P::kExpAt + tid * 2), b0 = pair & 0xFFu, b1 = pair >> 8;        // K: this thread's two positions
+        const uint32_t vpair = lds_u16(smem + P::kExpAt + 256 + tid * 2), v0 = vpair & 0xFFu, v1 = vpair >> 8;
+        *reinterpret_cast<float2*>(&scales_sm[0][2 * tid]) = make_float2(kv_scale(b0), kv_scale(b1));
+        *reinterpret_cast<float2*>(&scales_sm[1][2 * tid]) = make_float2(v0 == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(v0) - 127),
+                                                                         v1 == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(v1) - 127));
+        *reinterpret_cast<float2*>(&scales_sm[2][2 * tid]) = make_float2(kv_inverse(v0), kv_inverse(v1));
+      }
+      const uint32_t k0 = smem + P::offset(p_warp + (lane >> 2), c), k1 = smem + P::offset(p_warp + (lane >> 2), c + 4);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint4 k = lds128(smem + P::offset(p_warp + 8 * nt + (lane >> 2), c + 4 * h));
+          const uint4 k = lds128((h ? k1 : k0) + 1024 * nt);
           const uint32_t w[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma_f16_16816(sc[nt], qa[4 * h + j], e4m3_to_half2(w[j] & 0xFFFFu), e4m3_to_half2(w[j] >> 16));
+          for (int j = 0; j < 4; ++j) {
+            uint32_t lo, hi;
+            e4m3_to_half4(w[j], lo, hi);
+            mma_f16_16816(sc[nt], qa[4 * h + j], lo, hi);
+          }
         }
       }
+      __syncthreads();                              // scales_sm is complete
     } else {
 #pragma unroll
       for (int kq = 0; kq < 4; ++kq)
@@ -509,80 +570,98 @@ tree_part_kernel(const TreeArgs a) {
           mma_bf16_16816(sc[nt], qa[2 * kq + 1], b[2], b[3]);
         }
     }
-    // scores in units of log 2, masked; then the weights
+    // scores in units of log 2, masked where the part has holes; then the weights
     float mx0 = -INFINITY, mx1 = -INFINITY;
-    uint32_t evs[F8 ? NT : 1];      // exponent bytes of the lane's two positions of every tile: values'
+    const bool two = used > 8;      // (otherwise the MMA's upper eight rows are nobody's)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t p = p_warp + 8 * nt + 2 * c;
-      float k0 = 1.f, k1 = 1.f, v0 = 0.f, v1 = 0.f;
       if constexpr (F8) {
-        const uint32_t eks = lds_u16(smem + P::kExpAt + p);
-        evs[nt] = lds_u16(smem + P::kExpAt + 256 + p);
-        k0 = kv_scale(eks & 0xFFu); k1 = kv_scale(eks >> 8);
-        const uint32_t b0 = evs[nt] & 0xFFu, b1 = evs[nt] >> 8;
-        v0 = b0 == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(b0) - 127);
-        v1 = b1 == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(b1) - 127);
-      } else if (holes) {
-        const uint32_t bad = bad_sm[p >> 5] >> (p & 31u);
-        if (bad & 1u) v0 = __uint_as_float(0x7FC00000u);
-        if (bad & 2u) v1 = __uint_as_float(0x7FC00000u);
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int32_t pos = int32_t(p) + j;
-        bool see0 = pos < seen0, see1 = pos < seen1;
-        if (holes && a.row_base) {
-          see0 = ok0 && (see0 || tree_sees(a, row0, t.start + pos - base0));
-          see1 = ok1 && (see1 || tree_sees(a, row1, t.start + pos - base1));
+        const uint32_t p = p_warp + 8 * nt + 2 * c;
+        const float2 k = *reinterpret_cast<const float2*>(&scales_sm[0][p]), v = *reinterpret_cast<const float2*>(&scales_sm[1][p]);
+        sc[nt][0] = __fmaf_rn(__fmul_rn(sc[nt][0], scale0), k.x, v.x);
+        sc[nt][1] = __fmaf_rn(__fmul_rn(sc[nt][1], scale0), k.y, v.y);
+        if (two) {
+          sc[nt][2] = __fmaf_rn(__fmul_rn(sc[nt][2], scale1), k.x, v.x);
+          sc[nt][3] = __fmaf_rn(__fmul_rn(sc[nt][3], scale1), k.y, v.y);
         }
-        const float k = j ? k1 : k0, v = j ? v1 : v0;
-        sc[nt][j] = see0 ? __fmaf_rn(__fmul_rn(sc[nt][j], scale0), k, v) : -INFINITY;
-        sc[nt][2 + j] = see1 ? __fmaf_rn(__fmul_rn(sc[nt][2 + j], scale1), k, v) : -INFINITY;
-        mx0 = fmaxf(mx0, sc[nt][j]);
-        mx1 = fmaxf(mx1, sc[nt][2 + j]);
-      }
-    }
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xFFFFFFFFu, mx0, 1));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xFFFFFFFFu, mx0, 2));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xFFFFFFFFu, mx1, 1));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xFFFFFFFFu, mx1, 2));
-    const float low0 = mx0 == -INFINITY ? 0.f : mx0, low1 = mx1 == -INFINITY ? 0.f : mx1;
-    float l0 = 0.f, l1 = 0.f;
-    uint32_t pa[NT / 2][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float p00 = exp2_approx(__fsub_rn(sc[nt][0], low0)), p01 = exp2_approx(__fsub_rn(sc[nt][1], low0));
-      const float p10 = exp2_approx(__fsub_rn(sc[nt][2], low1)), p11 = exp2_approx(__fsub_rn(sc[nt][3], low1));
-      if constexpr (F8) {
-        const float i0 = kv_inverse(evs[nt] & 0xFFu), i1 = kv_inverse(evs[nt] >> 8);
-        l0 = __fmaf_rn(p00, i0, __fmaf_rn(p01, i1, l0));
-        l1 = __fmaf_rn(p10, i0, __fmaf_rn(p11, i1, l1));
-        const __half2 h0 = __floats2half2_rn(p00, p01), h1 = __floats2half2_rn(p10, p11);
-        pa[nt >> 1][(nt & 1) * 2] = *reinterpret_cast<const uint32_t*>(&h0);
-        pa[nt >> 1][(nt & 1) * 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
       } else {
-        l0 = __fadd_rn(l0, __fadd_rn(p00, p01));
-        l1 = __fadd_rn(l1, __fadd_rn(p10, p11));
-        pa[nt >> 1][(nt & 1) * 2] = pack_bf(p00, p01);
-        pa[nt >> 1][(nt & 1) * 2 + 1] = pack_bf(p10, p11);
+        sc[nt][0] = __fmul_rn(sc[nt][0], scale0);
+        sc[nt][1] = __fmul_rn(sc[nt][1], scale0);
+        sc[nt][2] = __fmul_rn(sc[nt][2], scale1);
+        sc[nt][3] = __fmul_rn(sc[nt][3], scale1);
       }
     }
-    l0 = __fadd_rn(l0, __shfl_xor_sync(0xFFFFFFFFu, l0, 1));
-    l0 = __fadd_rn(l0, __shfl_xor_sync(0xFFFFFFFFu, l0, 2));
-    l1 = __fadd_rn(l1, __shfl_xor_sync(0xFFFFFFFFu, l1, 1));
-    l1 = __fadd_rn(l1, __shfl_xor_sync(0xFFFFFFFFu, l1, 2));
+    if (holes) {
+#pragma unroll 1
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t p = p_warp + 8 * nt + 2 * c;
+        float x[4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          if (n == nt) { x[0] = sc[n][0]; x[1] = sc[n][1]; x[2] = sc[n][2]; x[3] = sc[n][3]; }
+        uint32_t bad = 0;
+        if constexpr (!F8) bad = bad_sm[p >> 5] >> (p & 31u);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int32_t pos = int32_t(p) + j;
+          bool see0 = pos < seen0, see1 = pos < seen1;
+          if (a.row_base) {
+            see0 = ok0 && (see0 || tree_sees(a, row0, t.start + pos - base0));
+            see1 = ok1 && (see1 || tree_sees(a, row1, t.start + pos - base1));
+          }
+          if (bad >> j & 1u) x[j] = x[2 + j] = __uint_as_float(0x7FC00000u);
+          if (!see0) x[j] = -INFINITY;
+          if (!see1) x[2 + j] = -INFINITY;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          if (n == nt) { sc[n][0] = x[0]; sc[n][1] = x[1]; sc[n][2] = x[2]; sc[n][3] = x[3]; }
+      }
+    }
+    uint32_t pa[NT / 2][4];
+    float l0 = 0.f, l1 = 0.f;
+    // one of the lane's two rows: its maximum over the warp's positions, its weights as A fragments, their sum
+    auto weigh = [&](int r, float& mx, float& l) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][2 * r], sc[nt][2 * r + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+      const float low = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float p0 = exp2_approx(__fsub_rn(sc[nt][2 * r], low)), p1 = exp2_approx(__fsub_rn(sc[nt][2 * r + 1], low));
+        if constexpr (F8) {
+          const float2 i = *reinterpret_cast<const float2*>(&scales_sm[2][p_warp + 8 * nt + 2 * c]);
+          l = __fmaf_rn(p0, i.x, __fmaf_rn(p1, i.y, l));
+          const __half2 h = __floats2half2_rn(p0, p1);
+          pa[nt >> 1][(nt & 1) * 2 + r] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          l = __fadd_rn(l, __fadd_rn(p0, p1));
+          pa[nt >> 1][(nt & 1) * 2 + r] = pack_bf(p0, p1);
+        }
+      }
+      l = __fadd_rn(l, __shfl_xor_sync(0xFFFFFFFFu, l, 1));
+      l = __fadd_rn(l, __shfl_xor_sync(0xFFFFFFFFu, l, 2));
+    };
+    weigh(0, mx0, l0);
+    if (two) {
+      weigh(1, mx1, l1);
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) pa[nt >> 1][(nt & 1) * 2 + 1] = 0u;
+    }
     cp_async_wait<0>();
     __syncthreads();                                // V is in shared memory, and every warp is done with K
     tree_request_k<F8>(a, smem, next, tid);
+    if (more) ask_q(next);                          // (this unit's scores are done)
     float o[16][4];
 #pragma unroll
     for (int nt = 0; nt < 16; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
     if constexpr (F8) {
-      if (holes && a.row_base) tree_values_f8<F8, true>(o, pa, vs, p_warp, lane);
-      else tree_values_f8<F8, false>(o, pa, vs, p_warp, lane);
+      if (holes && a.row_base) tree_values_f8<true>(o, pa, vs, p_warp, lane);
+      else tree_values_f8<false>(o, pa, vs, p_warp, lane);
     } else {
 #pragma unroll
       for (int s = 0; s < NT / 2; ++s) {
@@ -604,6 +683,7 @@ tree_part_kernel(const TreeArgs a) {
         for (int i = 0; i < 4; ++i) {
           *reinterpret_cast<float4*>(mine + tree_merge_index(m0, 8 * c + i)) = make_float4(o[4 * i][0], o[4 * i + 1][0], o[4 * i + 2][0], o[4 * i + 3][0]);
           *reinterpret_cast<float4*>(mine + tree_merge_index(m0, 8 * c + 4 + i)) = make_float4(o[4 * i][1], o[4 * i + 1][1], o[4 * i + 2][1], o[4 * i + 3][1]);
+          if (!two) continue;
           *reinterpret_cast<float4*>(mine + tree_merge_index(m1, 8 * c + i)) = make_float4(o[4 * i][2], o[4 * i + 1][2], o[4 * i + 2][2], o[4 * i + 3][2]);
           *reinterpret_cast<float4*>(mine + tree_merge_index(m1, 8 * c + 4 + i)) = make_float4(o[4 * i][3], o[4 * i + 1][3], o[4 * i + 2][3], o[4 * i + 3][3]);
         }
@@ -612,7 +692,7 @@ tree_part_kernel(const TreeArgs a) {
         for (int nt = 0; nt < 16; ++nt) {
           const uint32_t col = 8 * nt + c * 2;
           *reinterpret_cast<float2*>(mine + attn_merge_index(m0, col)) = make_float2(o[nt][0], o[nt][1]);
-          *reinterpret_cast<float2*>(mine + attn_merge_index(m1, col)) = make_float2(o[nt][2], o[nt][3]);
+          if (two) *reinterpret_cast<float2*>(mine + attn_merge_index(m1, col)) = make_float2(o[nt][2], o[nt][3]);
         }
       }
       if (c == 0) {
@@ -650,41 +730,43 @@ tree_part_kernel(const TreeArgs a) {
   cp_async_wait<0>();
 }
 
-// The parts of a (row, query head) merged under their common maximum, in part order, one division, BF16 out.  One warp each.
+// The parts of a (row, query head) merged under their common maximum, in part order, one division, BF16 out.  One warp each; what it
+// loads first depends on the number of parts alone.
 constexpr int kTreeCombineWarps = 4;
-template <int UNROLL>
 __global__ void __launch_bounds__(kTreeCombineWarps * 32)
 tree_combine_kernel(const TreeArgs a) {
   step_kernel_entry();
-  const uint64_t pair = uint64_t(blockIdx.x) * kTreeCombineWarps + (threadIdx.x >> 5);
-  const uint32_t lane = threadIdx.x & 31u;
-  if (pair >= uint64_t(a.rows) * a.nq) return;
-  const uint32_t row = uint32_t(pair / a.nq), head = uint32_t(pair % a.nq);
-  if (tree_place(a, row) < 0) return;
-  const uint32_t parts = a.row_parts[row];
+  constexpr uint32_t kAtOnce = 8;
+  const uint32_t pair = blockIdx.x * kTreeCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+  if (pair >= a.rows * a.nq) return;
+  const uint32_t row = pair / a.nq, head = pair % a.nq, parts = a.row_parts[row];
+  if (parts == kTreeRowAbsent) return;
   const size_t base = size_t(pair) * a.max_parts;
-  float mx = -INFINITY;
-  for (uint32_t s = lane; s < parts; s += 32) mx = fmaxf(mx, a.part_ml[base + s].x);
+  const float4* acc = reinterpret_cast<const float4*>(a.part_acc + base * kKvDim) + lane;
+  float4 v[kAtOnce];
+  auto load = [&](uint32_t s0) {
+#pragma unroll
+    for (uint32_t k = 0; k < kAtOnce; ++k) v[k] = s0 + k < parts ? acc[(s0 + k) * (kKvDim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  load(0);
+  float2 ml = lane < parts ? a.part_ml[base + lane] : make_float2(-INFINITY, 0.f);    // of part s0 + lane, s0 a multiple of 32
+  float mx = ml.x;
+  for (uint32_t s = lane + 32; s < parts; s += 32) mx = fmaxf(mx, a.part_ml[base + s].x);
   mx = warp_max(mx);
   float den = 0.f;
   float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t s0 = 0; s0 < parts; s0 += UNROLL) {
-    float4 v[UNROLL];
-    float2 ml[UNROLL];
+  for (uint32_t s0 = 0; s0 < parts; s0 += kAtOnce) {
+    if (s0) load(s0);
+    if (s0 && s0 % 32 == 0) ml = s0 + lane < parts ? a.part_ml[base + s0 + lane] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      const bool in = s0 + j < parts;
-      v[j] = in ? *(reinterpret_cast<const float4*>(a.part_acc + (base + s0 + j) * kKvDim) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-      ml[j] = in ? a.part_ml[base + s0 + j] : make_float2(-INFINITY, 0.f);
-    }
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      const float e = ml[j].x == -INFINITY ? 1.f : exp2f(__fsub_rn(ml[j].x, mx));
-      den = __fmaf_rn(e, ml[j].y, den);
-      num.x = __fmaf_rn(e, v[j].x, num.x);
-      num.y = __fmaf_rn(e, v[j].y, num.y);
-      num.z = __fmaf_rn(e, v[j].z, num.z);
-      num.w = __fmaf_rn(e, v[j].w, num.w);
+    for (uint32_t k = 0; k < kAtOnce; ++k) {
+      const float m = __shfl_sync(0xFFFFFFFFu, ml.x, (s0 + k) & 31u), l = __shfl_sync(0xFFFFFFFFu, ml.y, (s0 + k) & 31u);
+      const float e = m == -INFINITY ? 1.f : exp2f(__fsub_rn(m, mx));      // (a part that saw nothing adds zeros)
+      den = __fmaf_rn(e, l, den);
+      num.x = __fmaf_rn(e, v[k].x, num.x);
+      num.y = __fmaf_rn(e, v[k].y, num.y);
+      num.z = __fmaf_rn(e, v[k].z, num.z);
+      num.w = __fmaf_rn(e, v[k].w, num.w);
     }
   }
   if (den == 0.f) den = 1.f;      // nothing seen: zeros
