@@ -148,7 +148,7 @@ uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pa
   if (!rows || rows > kTreeMaxRows || !nq || !max_pages || format > GRB_KV_E4M3) return 0;
   const uint64_t parts = uint64_t(max_pages) * (format == GRB_KV_E4M3 ? kKvPage / TreePart<true>::kPositions : kKvPage / TreePart<false>::kPositions);
   const uint64_t pairs = uint64_t(rows) * nq;
-  return ((32 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * 2 + pairs * parts * (kKvDim * 4 + 8);
+  return ((48 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * 2 + pairs * parts * (kKvDim * 4 + 8);
 }
 
 int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
@@ -197,12 +197,12 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
   a.status = reinterpret_cast<uint32_t*>(at);                // (first of the scratch: the caller reads it there)
   a.plan = a.status + 4;
-  a.tiles = reinterpret_cast<int4*>(at + 32);
+  a.tiles = reinterpret_cast<int4*>(at + 48);
   a.wide_tiles = a.tiles + a.rows;
   a.extent = reinterpret_cast<int32_t*>(a.wide_tiles + a.rows);
   a.row_parts = reinterpret_cast<uint32_t*>(a.extent + a.rows);
   a.q_scale = reinterpret_cast<float*>(a.row_parts + a.rows);
-  at += (32 + a.rows * 40ull + pairs * 4 + 255) & ~uint64_t(255);
+  at += (48 + a.rows * 40ull + pairs * 4 + 255) & ~uint64_t(255);
   a.q = reinterpret_cast<uint16_t*>(at);
   at += pairs * kKvDim * 2;
   a.part_acc = reinterpret_cast<float*>(at);

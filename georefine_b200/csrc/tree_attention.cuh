@@ -49,7 +49,7 @@ struct TreeArgs {
   uint32_t* row_parts;        // scratch: [rows]: parts of the row
   int4* tiles;                // scratch: [rows]: first row, rows, first unit, positions up to the last one its rows see
   int4* wide_tiles;           // scratch: [rows]: first row, rows, first unit, positions of a unit
-  uint32_t* plan;             // scratch: tiles, units, wide tiles, wide units
+  uint32_t* plan;             // scratch: tiles, units, wide tiles, wide units, wide units taken
   float* part_acc;            // scratch: [rows][nq][max_parts][128]
   float2* part_ml;            // scratch: [rows][nq][max_parts]: maximum and sum of a part
   __nv_bfloat16* out;         // [rows][ldo]: nq * 128
@@ -159,6 +159,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
       wide_done = total;
     }
   }
+  if (tid == 0) a.plan[4] = 0u;                              // units that CTAs of the wide kernel have taken beyond their first
   if (tid == 0) a.plan[0] = uint32_t(done >> 32), a.plan[1] = uint32_t(done), a.plan[2] = uint32_t(wide_done >> 32), a.plan[3] = uint32_t(wide_done);
 }
 

@@ -73,9 +73,11 @@ tree_wide_kernel(const TreeArgs a) {
   __shared__ __align__(8) uint64_t bars[5];                  // K stored, V stored, S done, P stored, O done
   __shared__ uint32_t tmem_at, aborted;
   __shared__ uint32_t k_top, v_top;                          // largest exponent bytes of the chunk
+  __shared__ uint32_t next_unit;
   __shared__ int32_t seen_by_all;                            // positions below it are seen by every row of the tile
   __shared__ int64_t entries[kWideMostPart / kWideTile];     // entry (of the layer) of each step's first position; -1: no page
-  __shared__ uint32_t bad[kWideMostPart / 32], any_bad;      // positions of the chunk whose key or value is not a number; whether there are any
+  __shared__ uint32_t bad[kWideMostPart / 32], any_bad, any_absent;   // positions of the chunk whose key or value is not a number; whether there are
+                                                             // any; whether a step has no page
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t smem = (smem_u32(wide_smem_raw) + 1023u) & ~1023u, qs = smem, ks = smem + kWideOperand, vs = smem + 2 * kWideOperand;
   const uint32_t k_scales = smem + kWideScalesAt, v_scales = k_scales + 2 * kWideMostPart;
@@ -107,8 +109,9 @@ tree_wide_kernel(const TreeArgs a) {
       atomicOr(a.status, kStatusTimeout);
     }
   };
+  // Units differ in length, so a CTA takes the next one when it is through with its own (who computes a unit changes nothing in it).
   uint32_t step0 = 0, tile = 0;                              // steps this CTA has taken; the tile of its unit
-  for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
+  for (uint32_t u = blockIdx.x; u < units;) {
     // ---- the unit (every warp finds it for itself)
     WideUnit t;
     for (;;) {
@@ -125,11 +128,18 @@ tree_wide_kernel(const TreeArgs a) {
     t.seq = a.row_seq[t.first];
     t.start = int32_t(t.part * part_positions);
     const uint32_t used = t.rows * a.group;
-    if (tid == 0) { k_top = v_top = any_bad = 0u; seen_by_all = 0x7FFFFFFF; }
+    if (tid == 0) {
+      k_top = v_top = any_bad = any_absent = 0u;
+      seen_by_all = 0x7FFFFFFF;
+      next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
+    }
     if (tid < kWideMostPart / 32) bad[tid] = 0u;
-    if (tid >= 128 && tid < 128 + part_positions / kWideTile) {            // (a step's positions lie in one page)
+    const bool looks = tid >= 128 && tid < 128 + part_positions / kWideTile;
+    bool absent = false;
+    if (looks) {                                             // (a step's positions lie in one page)
       const int64_t place = kv_place(a.table, t.seq, t.start + int32_t((tid - 128) * kWideTile));
-      entries[tid - 128] = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
+      absent = place < 0;
+      entries[tid - 128] = absent ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
     }
     int32_t extent = 0, all = 0x7FFFFFFF;
     for (uint32_t i = lane; i < t.rows; i += 32) {
@@ -156,6 +166,7 @@ tree_wide_kernel(const TreeArgs a) {
     }
     __syncthreads();
     if (warp == 0) atomicMin(&seen_by_all, all);
+    if (absent) any_absent = 1u;
     // exponents of the chunk: a thread takes sixteen positions' of K or of V
     if constexpr (F8) {
       uint32_t w[4] = {0u, 0u, 0u, 0u};
@@ -196,45 +207,43 @@ tree_wide_kernel(const TreeArgs a) {
     }
     fence_proxy_async_smem();
     __syncthreads();
-    const bool edge = seen_by_all < t.extent;                // some step of the unit is not seen whole by every row
-    auto whole = [&](uint32_t j) { return !edge || seen_by_all >= t.start + int32_t((j + 1) * kWideTile); };
+    // steps, from the first on, whose positions every row sees
+    const uint32_t plain = any_absent ? 0u : seen_by_all >= t.extent ? steps : uint32_t(max(seen_by_all - t.start, 0)) / kWideTile;
+    auto whole = [&](uint32_t j) { return j < plain; };
     if (warp >= 4) {
       // ---- loading ----------------------------------------------------------------------------------------------
       const uint32_t lt = tid - 128;
       if constexpr (F8) {
+        // A thread's pieces: the same quarter of both halves of every 32nd row.  Eight lanes take four pieces of two neighbouring rows,
+        // which the swizzle spreads over all banks when their sixteen values each are stored.
+        const uint32_t row0 = lt >> 2;
         uint4 k[8], v[8];
         auto ask = [&](uint4 (&x)[8], const void* pool, uint32_t j) {
           const int64_t entry = j < steps ? entries[j] : -1;
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim) + row0 * 8 + (lt & 3u);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t c = lt + 128 * i;
-            x[i] = int32_t(c >> 3) < npos ? reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim)[c] : make_uint4(0u, 0u, 0u, 0u);
-          }
+          for (int i = 0; i < 8; ++i) x[i] = int32_t(row0 + 32 * (i >> 1)) < npos ? src[256 * (i >> 1) + 4 * (i & 1)] : make_uint4(0u, 0u, 0u, 0u);
         };
+        const uint32_t to_lo = wide_offset(row0, 2 * (lt & 3u)), to_hi = wide_offset(row0, 2 * (lt & 3u) + 1);     // (32 rows on: 4096 bytes)
         auto store = [&](const uint4 (&x)[8], uint32_t dst, uint32_t scales, uint32_t j, bool clean) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const uint32_t c = lt + 128 * i, row = c >> 3, piece = c & 7u;
-            const uint32_t s16 = lds_u16(scales + 2 * (j * kWideTile + row)), s = s16 | (s16 << 16);
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            const uint32_t s16 = lds_u16(scales + 2 * (j * kWideTile + row0 + 32 * (i >> 1))), s = s16 | (s16 << 16);
             uint32_t h[8];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              h[2 * q] = e4m3_to_half2(w[q] & 0xFFFFu);
-              h[2 * q + 1] = e4m3_to_half2(w[q] >> 16);
-            }
+            e4m3_to_half4(x[i].x, h[0], h[1]);
+            e4m3_to_half4(x[i].y, h[2], h[3]);
+            e4m3_to_half4(x[i].z, h[4], h[5]);
+            e4m3_to_half4(x[i].w, h[6], h[7]);
             if (clean) {
 #pragma unroll
               for (int q = 0; q < 8; ++q) h[q] = half2_number(h[q]);
             }
 #pragma unroll
             for (int q = 0; q < 8; ++q) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[q]) : "r"(s));
-            // the lanes of a row's second half take its second piece first: eight lanes, eight groups of banks
-            const uint32_t swap = piece >> 2;
-            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-            sts128(dst + wide_offset(row, 2 * piece + swap), swap ? hi : lo);
-            sts128(dst + wide_offset(row, 2 * piece + 1 - swap), swap ? lo : hi);
+            const uint32_t at = dst + 4096 * (i >> 1) + (kWideOperand / 2) * (i & 1);
+            sts128(at + to_lo, make_uint4(h[0], h[1], h[2], h[3]));
+            sts128(at + to_hi, make_uint4(h[4], h[5], h[6], h[7]));
           }
         };
         ask(k, a.pages.k, 0);
@@ -335,7 +344,7 @@ tree_wide_kernel(const TreeArgs a) {
         tc_fence_after();
         // which of the step's positions the row sees
         const bool there = entries[j] >= 0;                 // (a page outside the pool: as if nobody saw its positions)
-        const bool every = whole(j) && there;
+        const bool every = whole(j);
         uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
         bool poisoned = false;
         if (!every) {
@@ -490,6 +499,7 @@ tree_wide_kernel(const TreeArgs a) {
       tc_fence_before();
     }
     step0 += steps;
+    u = next_unit;
     __syncthreads();                                         // operands, scales and accumulators are free
   }
   // (every product has been waited for, or its wait ran out: then the tensor memory is given back after a moment for what may
