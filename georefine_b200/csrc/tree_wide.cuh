@@ -64,24 +64,31 @@ struct WideUnit {
   uint32_t first, rows, kvh, part;
   int32_t seq, start, extent;      // positions start .. extent - 1 (at most a chunk): what some row sees, up to the last such
 };
+// What the loading warps tell the others of a unit.
+struct WideInfo {
+  uint32_t valid, first, rows, kvh, part, steps;
+  uint32_t plain;                  // steps, from the first on, whose positions every row sees
+  int32_t start;
+  uint32_t k_top, v_top, any_bad;  // largest exponent bytes of the chunk; whether `bad` has bits
+};
+__device__ __forceinline__ void wide_loaders_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <bool F8>
 __global__ void __launch_bounds__(kWideThreads, 2)
 tree_wide_kernel(const TreeArgs a) {
   step_kernel_entry();
   extern __shared__ unsigned char wide_smem_raw[];
-  __shared__ __align__(8) uint64_t bars[5];                  // K stored, V stored, S done, P stored, O done
-  __shared__ uint32_t tmem_at, aborted;
-  __shared__ uint32_t k_top, v_top;                          // largest exponent bytes of the chunk
-  __shared__ uint32_t next_unit;
-  __shared__ int32_t seen_by_all;                            // positions below it are seen by every row of the tile
-  __shared__ int64_t entries[kWideMostPart / kWideTile];     // entry (of the layer) of each step's first position; -1: no page
-  __shared__ uint32_t bad[kWideMostPart / 32], any_bad, any_absent;   // positions of the chunk whose key or value is not a number; whether there are
-                                                             // any; whether a step has no page
+  __shared__ __align__(8) uint64_t bars[6];                  // K stored, V stored, S done, P stored, O done, unit set up
+  __shared__ uint32_t tmem_at, aborted, next_unit;
+  __shared__ uint32_t k_top, v_top, any_bad, any_absent;     // the loaders' own, while they set a unit up
+  __shared__ WideInfo info[2];                               // of a unit and the next
+  __shared__ int64_t entries[2][kWideMostPart / kWideTile];  // entry (of the layer) of each step's first position; -1: no page
+  __shared__ uint32_t bad[2][kWideMostPart / 32];            // positions of the chunk whose key or value is not a number
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t smem = (smem_u32(wide_smem_raw) + 1023u) & ~1023u, qs = smem, ks = smem + kWideOperand, vs = smem + 2 * kWideOperand;
   const uint32_t k_scales = smem + kWideScalesAt, v_scales = k_scales + 2 * kWideMostPart;
-  const uint32_t bar_k = smem_u32(&bars[0]), bar_v = smem_u32(&bars[1]), bar_s = smem_u32(&bars[2]), bar_p = smem_u32(&bars[3]), bar_o = smem_u32(&bars[4]);
+  const uint32_t bar_k = smem_u32(&bars[0]), bar_v = smem_u32(&bars[1]), bar_s = smem_u32(&bars[2]), bar_p = smem_u32(&bars[3]), bar_o = smem_u32(&bars[4]),
+                 bar_u = smem_u32(&bars[5]);
   const uint32_t tiles = a.plan[2], units = a.plan[3];
   if (blockIdx.x >= units) return;
   if (tid == 0) {
@@ -90,6 +97,7 @@ tree_wide_kernel(const TreeArgs a) {
     mbar_init(bar_s, 1);
     mbar_init(bar_p, 4);
     mbar_init(bar_o, 1);
+    mbar_init(bar_u, 4);
     mbar_fence_init();
     aborted = 0u;
   }
@@ -109,117 +117,94 @@ tree_wide_kernel(const TreeArgs a) {
       atomicOr(a.status, kStatusTimeout);
     }
   };
-  // Units differ in length, so a CTA takes the next one when it is through with its own (who computes a unit changes nothing in it).
-  uint32_t step0 = 0, tile = 0;                              // steps this CTA has taken; the tile of its unit
-  for (uint32_t u = blockIdx.x; u < units;) {
-    // ---- the unit (every warp finds it for itself)
+  // Units differ in length, so a CTA takes the next one when it is through with its own (who computes a unit changes nothing in it);
+  // its loaders set the next one up while the last step of this one is multiplied and its result stored.
+  uint32_t step0 = 0;                                        // steps this CTA has taken before the unit
+  if (warp >= 4) {
+    // ---- loading ------------------------------------------------------------------------------------------------
+    const uint32_t lt = tid - 128;
+    uint32_t tile = 0, slot = 0, steps_before = 0;
     WideUnit t;
-    for (;;) {
-      const uint32_t past = __ballot_sync(0xFFFFFFFFu, tile + 1 + lane < tiles && uint32_t(a.wide_tiles[tile + 1 + lane].z) <= u);
-      tile += __popc(past);
-      if (past != 0xFFFFFFFFu) break;
-    }
-    const int4 d = a.wide_tiles[tile];
-    const uint32_t local = u - uint32_t(d.z), part_positions = uint32_t(d.w);
-    t.first = uint32_t(d.x);
-    t.rows = uint32_t(d.y);
-    t.kvh = local % a.nkv;
-    t.part = local / a.nkv;
-    t.seq = a.row_seq[t.first];
-    t.start = int32_t(t.part * part_positions);
-    const uint32_t used = t.rows * a.group;
-    if (tid == 0) {
-      k_top = v_top = any_bad = any_absent = 0u;
-      seen_by_all = 0x7FFFFFFF;
-      next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
-    }
-    if (tid < kWideMostPart / 32) bad[tid] = 0u;
-    const bool looks = tid >= 128 && tid < 128 + part_positions / kWideTile;
-    bool absent = false;
-    if (looks) {                                             // (a step's positions lie in one page)
-      const int64_t place = kv_place(a.table, t.seq, t.start + int32_t((tid - 128) * kWideTile));
-      absent = place < 0;
-      entries[tid - 128] = absent ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
-    }
-    int32_t extent = 0, all = 0x7FFFFFFF;
-    for (uint32_t i = lane; i < t.rows; i += 32) {
-      const int32_t e = a.extent[t.first + i];
-      extent = max(extent, e);
-      all = min(all, a.row_base ? min(max(a.row_base[t.first + i], 0), e) : e);
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) extent = max(extent, __shfl_xor_sync(0xFFFFFFFFu, extent, off));
-    t.extent = min(extent, t.start + int32_t(part_positions));
-    const uint32_t steps = t.extent > t.start ? (uint32_t(t.extent - t.start) + kWideTile - 1) / kWideTile : 0u;
-    // the queries: sixteen lanes a row
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint4 x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t m = (tid >> 4) + (4 * half + i) * (kWideThreads / 16), r = m / a.group;
-        x[i] = m < used ? reinterpret_cast<const uint4*>(a.q + ((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kKvDim)[tid & 15u]
-                        : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t steps = 0, plain = 0;
+    for (uint32_t u = blockIdx.x; u < units; slot ^= 1u) {
+      // the unit (every warp finds it for itself), and where its steps lie
+      for (;;) {
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, tile + 1 + lane < tiles && uint32_t(a.wide_tiles[tile + 1 + lane].z) <= u);
+        tile += __popc(past);
+        if (past != 0xFFFFFFFFu) break;
+      }
+      const int4 d = a.wide_tiles[tile];
+      const uint32_t local = u - uint32_t(d.z), part_positions = uint32_t(d.w);
+      t.first = uint32_t(d.x);
+      t.rows = uint32_t(d.y);
+      t.kvh = local % a.nkv;
+      t.part = local / a.nkv;
+      t.seq = a.row_seq[t.first];
+      t.start = int32_t(t.part * part_positions);
+      const uint32_t used = t.rows * a.group;
+      if (lt < kWideMostPart / 32) bad[slot][lt] = 0u;
+      if (lt == 0) {
+        k_top = v_top = any_bad = 0u;
+        next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
+      }
+      if (warp == 4) {                                       // (a step's positions lie in one page)
+        int64_t place = 0;
+        if (lane < part_positions / kWideTile) {
+          place = kv_place(a.table, t.seq, t.start + int32_t(lane * kWideTile));
+          entries[slot][lane] = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
+        }
+        const bool absent = __any_sync(0xFFFFFFFFu, place < 0);
+        if (lane == 0) any_absent = absent;
+      }
+      int32_t extent = 0, all = 0x7FFFFFFF;
+      for (uint32_t i = lane; i < t.rows; i += 32) {
+        const int32_t e = a.extent[t.first + i];
+        extent = max(extent, e);
+        all = min(all, a.row_base ? min(max(a.row_base[t.first + i], 0), e) : e);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sts128(qs + wide_offset((tid >> 4) + (4 * half + i) * (kWideThreads / 16), tid & 15u), x[i]);
-    }
-    __syncthreads();
-    if (warp == 0) atomicMin(&seen_by_all, all);
-    if (absent) any_absent = 1u;
-    // exponents of the chunk: a thread takes sixteen positions' of K or of V
-    if constexpr (F8) {
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
-      const uint32_t of_v = tid >> 7, at16 = tid & 127u;
-      const int64_t entry = at16 < steps * 8 ? entries[at16 >> 3] : -1;
-      if (entry >= 0) {
-        const uint4 x = *reinterpret_cast<const uint4*>((of_v ? a.pages.v_exp : a.pages.k_exp) + entry + (at16 & 7u) * 16);
-        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+      for (int off = 16; off; off >>= 1) {
+        extent = max(extent, __shfl_xor_sync(0xFFFFFFFFu, extent, off));
+        all = min(all, __shfl_xor_sync(0xFFFFFFFFu, all, off));
       }
-      // bytes of no entry (135 to 254, where nobody wrote) do not count, nor do those behind the last position
-      const int32_t left = t.extent - t.start - int32_t(at16 * 16);
-      uint32_t top = 0, none = 0;
+      t.extent = min(extent, t.start + int32_t(part_positions));
+      steps = (uint32_t(t.extent - t.start) + kWideTile - 1) / kWideTile;       // (a unit has a position at least)
+      wide_loaders_meet();                                   // (the scales of the unit before have been read, too)
+      u = next_unit;
+      plain = any_absent ? 0u : all >= t.extent ? steps : uint32_t(max(all - t.start, 0)) / kWideTile;
+      const int64_t* const at = entries[slot];
+      // the queries, sixteen lanes a row, once the scores of the unit before are done
+      auto queries = [&]() {
+        if (step0) wait(bar_s, step0 - 1);
+#pragma unroll 1
+        for (int part = 0; part < 4; ++part) {
+          uint4 x[4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t b = w[i >> 2] >> (8 * (i & 3)) & 0xFFu;
-        if (i < left && b == kKvNanByte) none |= 1u << i;
-        if (i < left && b <= 134u) top = max(top, b);
-      }
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t m = (lt >> 4) + (4 * part + i) * 8, r = m / a.group;
+            x[i] = m < used ? reinterpret_cast<const uint4*>(a.q + ((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kKvDim)[lt & 15u]
+                            : make_uint4(0u, 0u, 0u, 0u);
+          }
 #pragma unroll
-      for (int off = 16; off; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-      if (lane == 0 && top) atomicMax(of_v ? &v_top : &k_top, top);
-      if (none) {
-        atomicOr(&bad[at16 >> 1], none << (16 * (at16 & 1u)));
-        any_bad = 1u;
-      }
-      __syncthreads();
-      top = of_v ? v_top : k_top;
-      uint32_t h[8];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t b = w[i >> 2] >> (8 * (i & 3)) & 0xFFu;
-        const uint32_t p = b > 134u ? 0u : half_power(min(int(b) - int(top) + 7, 7));
-        h[i >> 1] = i & 1 ? h[i >> 1] | p << 16 : p;
-      }
-      const uint32_t dst = (of_v ? v_scales : k_scales) + at16 * 32;
-      sts128(dst, make_uint4(h[0], h[1], h[2], h[3]));
-      sts128(dst + 16, make_uint4(h[4], h[5], h[6], h[7]));
-    }
-    fence_proxy_async_smem();
-    __syncthreads();
-    // steps, from the first on, whose positions every row sees
-    const uint32_t plain = any_absent ? 0u : seen_by_all >= t.extent ? steps : uint32_t(max(seen_by_all - t.start, 0)) / kWideTile;
-    auto whole = [&](uint32_t j) { return j < plain; };
-    if (warp >= 4) {
-      // ---- loading ----------------------------------------------------------------------------------------------
-      const uint32_t lt = tid - 128;
+          for (int i = 0; i < 4; ++i) sts128(qs + wide_offset((lt >> 4) + (4 * part + i) * 8, lt & 15u), x[i]);
+        }
+      };
+      // everything is there: tells the weights' warps, who have all looked at the unit before by the time its second step's values
+      // were used (of a unit of one step: its only step's)
+      auto publish = [&]() {
+        if (lt == 0) info[slot] = WideInfo{1u, t.first, t.rows, t.kvh, t.part, steps, plain, t.start, k_top, v_top, any_bad};
+        if (steps_before == 1) wait(bar_o, step0 - 1);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_u);
+      };
       if constexpr (F8) {
         // A thread's pieces: the same quarter of both halves of every 32nd row.  Eight lanes take four pieces of two neighbouring rows,
         // which the swizzle spreads over all banks when their sixteen values each are stored.
         const uint32_t row0 = lt >> 2;
         uint4 k[8], v[8];
         auto ask = [&](uint4 (&x)[8], const void* pool, uint32_t j) {
-          const int64_t entry = j < steps ? entries[j] : -1;
+          const int64_t entry = j < steps ? at[j] : -1;
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
           const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim) + row0 * 8 + (lt & 3u);
 #pragma unroll
@@ -247,7 +232,53 @@ tree_wide_kernel(const TreeArgs a) {
           }
         };
         ask(k, a.pages.k, 0);
+        // exponents of the chunk: a thread takes sixteen positions' of K and of V; bytes of no entry (135 to 254, where nobody wrote)
+        // do not count, nor do those behind the last position
+        uint32_t w[2][4];
+#pragma unroll
+        for (int of_v = 0; of_v < 2; ++of_v) {
+          const int64_t entry = lt < steps * 8 ? at[lt >> 3] : -1;
+          const uint4 x = entry >= 0 ? *reinterpret_cast<const uint4*>((of_v ? a.pages.v_exp : a.pages.k_exp) + entry + (lt & 7u) * 16) : make_uint4(0u, 0u, 0u, 0u);
+          w[of_v][0] = x.x; w[of_v][1] = x.y; w[of_v][2] = x.z; w[of_v][3] = x.w;
+        }
+        const int32_t left = t.extent - t.start - int32_t(lt * 16);
+        uint32_t none = 0;
+#pragma unroll
+        for (int of_v = 0; of_v < 2; ++of_v) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t b = w[of_v][i >> 2] >> (8 * (i & 3)) & 0xFFu;
+            if (i < left && b == kKvNanByte) none |= 1u << i;
+            if (i < left && b <= 134u) top = max(top, b);
+          }
+#pragma unroll
+          for (int off = 16; off; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+          if (lane == 0 && top) atomicMax(of_v ? &v_top : &k_top, top);
+        }
+        if (none) {
+          atomicOr(&bad[slot][lt >> 1], none << (16 * (lt & 1u)));
+          any_bad = 1u;
+        }
+        wide_loaders_meet();
+#pragma unroll
+        for (int of_v = 0; of_v < 2; ++of_v) {
+          const uint32_t top = of_v ? v_top : k_top;
+          uint32_t h[8];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t b = w[of_v][i >> 2] >> (8 * (i & 3)) & 0xFFu;
+            const uint32_t p = b > 134u ? 0u : half_power(min(int(b) - int(top) + 7, 7));
+            h[i >> 1] = i & 1 ? h[i >> 1] | p << 16 : p;
+          }
+          const uint32_t dst = (of_v ? v_scales : k_scales) + lt * 32;
+          sts128(dst, make_uint4(h[0], h[1], h[2], h[3]));
+          sts128(dst + 16, make_uint4(h[4], h[5], h[6], h[7]));
+        }
         ask(v, a.pages.v, 0);
+        queries();
+        publish();
+        wide_loaders_meet();                                 // the scales are complete
         for (uint32_t j = 0; j < steps; ++j) {
           const uint32_t g = step0 + j;
           if (g) wait(bar_s, g - 1);                         // the scores of the step before have been taken from K
@@ -257,7 +288,7 @@ tree_wide_kernel(const TreeArgs a) {
           if (lane == 0) mbar_arrive(bar_k);
           ask(k, a.pages.k, j + 1);
           if (g) wait(bar_o, g - 1);                         // the values of the step before have been used
-          store(v, vs, v_scales, j, !whole(j));
+          store(v, vs, v_scales, j, j >= plain);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_v);
@@ -265,7 +296,7 @@ tree_wide_kernel(const TreeArgs a) {
         }
       } else {
         auto ask = [&](uint32_t dst, const void* pool, uint32_t j) {
-          const int64_t entry = entries[j];
+          const int64_t entry = at[j];
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
           const uint8_t* src = static_cast<const uint8_t*>(pool) + (entry < 0 ? 0 : entry) * kKvDim * 2;
 #pragma unroll
@@ -276,6 +307,9 @@ tree_wide_kernel(const TreeArgs a) {
           }
           cp_async_commit();
         };
+        wide_loaders_meet();                                 // (the unit after this one and its pages are known to all)
+        queries();
+        publish();
         for (uint32_t j = 0; j < steps; ++j) {
           const uint32_t g = step0 + j;
           if (g) wait(bar_s, g - 1);
@@ -287,7 +321,7 @@ tree_wide_kernel(const TreeArgs a) {
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_k);
           cp_async_wait<0>();
-          if (!whole(j)) {                                   // values that are not finite would reach, as 0 * infinity, rows that do not see them
+          if (j >= plain) {                                   // values that are not finite would reach, as 0 * infinity, rows that do not see them
             uint32_t mine = 0;                               // bit i: of the thread's piece i
 #pragma unroll 1
             for (int i = 0; i < 16; ++i) {
@@ -305,7 +339,7 @@ tree_wide_kernel(const TreeArgs a) {
             for (int i = 0; i < 16; ++i) {
               const uint32_t m = __ballot_sync(0xFFFFFFFFu, mine >> i & 1u);
               const uint32_t p = 8 * i + 2 * (warp - 4);
-              if (lane == 0 && m) atomicOr(&bad[j * (kWideTile / 32) + (p >> 5)], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
+              if (lane == 0 && m) atomicOr(&bad[slot][j * (kWideTile / 32) + (p >> 5)], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
             }
           }
           fence_proxy_async_smem();
@@ -313,19 +347,35 @@ tree_wide_kernel(const TreeArgs a) {
           if (lane == 0) mbar_arrive(bar_v);
         }
       }
-    } else {
-      // ---- weights: thread = row m of the tile, lane m of tensor memory --------------------------------------------
-      const uint32_t m = tid, r = min(m, used - 1) / a.group, row = t.first + r, lanes = (warp * 32u) << 16;
-      const size_t pair = size_t(row) * a.nq + t.kvh * a.group + (min(m, used - 1) - r * a.group);
-      const float scale = F8 ? __fmul_rn(a.q_scale[pair], __uint_as_float((k_top > 7u ? k_top - 7u : 127u) << 23)) : a.q_scale[pair];
+      step0 += steps;
+      steps_before = steps;
+    }
+    // no unit is left
+    if (lt == 0) info[slot].valid = 0u;
+    if (steps_before == 1) wait(bar_o, step0 - 1);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_u);
+  } else {
+    // ---- weights: thread = row m of the tile, lane m of tensor memory ------------------------------------------------
+    constexpr float kSlack = 8.f, kBias = F8 ? 7.f : 0.f;    // FP16: weights up to 2^(7 + 8)
+    constexpr uint32_t kIdesc = umma_idesc_bf16(128) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);      // FP16 or BF16 operands
+    const uint32_t m = tid, lanes = (warp * 32u) << 16;
+    for (uint32_t n = 0;; ++n) {
+      const uint32_t slot = n & 1u;
+      wait(bar_u, n);
+      const WideInfo unit = info[slot];
+      if (!unit.valid || *reinterpret_cast<volatile uint32_t*>(&aborted)) break;
+      const uint32_t steps = unit.steps, plain = unit.plain, used = unit.rows * a.group, r = min(m, used - 1) / a.group, row = unit.first + r;
+      const int32_t start = unit.start;
+      const bool any_bad = unit.any_bad != 0u;
+      const size_t pair = size_t(row) * a.nq + unit.kvh * a.group + (min(m, used - 1) - r * a.group);
+      const float scale = F8 ? __fmul_rn(a.q_scale[pair], __uint_as_float((unit.k_top > 7u ? unit.k_top - 7u : 127u) << 23)) : a.q_scale[pair];
       const int32_t base = a.row_base ? a.row_base[row] : 0, mine = a.extent[row];
-      constexpr float kSlack = 8.f, kBias = F8 ? 7.f : 0.f;  // FP16: weights up to 2^(7 + 8)
-      constexpr uint32_t kIdesc = umma_idesc_bf16(128) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);      // FP16 or BF16 operands
       float ref = -INFINITY;
       float2 sum = make_float2(0.f, 0.f);
       for (uint32_t j = 0; j < steps; ++j) {
         const uint32_t g = step0 + j;
-        const int32_t at = t.start + int32_t(j * kWideTile);
+        const int32_t at = start + int32_t(j * kWideTile);
         if (warp == 0) {                                     // (behind the values' product of the step before, in issue order)
           wait(bar_k, g);
           __syncwarp();
@@ -343,8 +393,8 @@ tree_wide_kernel(const TreeArgs a) {
         wait(bar_s, g);
         tc_fence_after();
         // which of the step's positions the row sees
-        const bool there = entries[j] >= 0;                 // (a page outside the pool: as if nobody saw its positions)
-        const bool every = whole(j);
+        const bool there = entries[slot][j] >= 0;                 // (a page outside the pool: as if nobody saw its positions)
+        const bool every = j < plain;
         uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
         bool poisoned = false;
         if (!every) {
@@ -371,9 +421,9 @@ tree_wide_kernel(const TreeArgs a) {
             see[w] = there ? bits & below : 0u;
           }
         }
-        if (F8 ? any_bad != 0u : !every) {
+        if (F8 ? any_bad : !every) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&bad[j * (kWideTile / 32) + w]) & see[w]);
+          for (int w = 0; w < 4; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&bad[slot][j * (kWideTile / 32) + w]) & see[w]);
         }
         auto masked = [&](uint32_t (&x)[32], int w) {
           if (!every) {
@@ -473,34 +523,27 @@ tree_wide_kernel(const TreeArgs a) {
         }
       }
       // ---- the unit's partial result
-      if (steps) {
-        wait(bar_o, step0 + steps - 1);
-        tc_fence_after();
-      }
-      const float back = F8 ? __uint_as_float((v_top > 7u ? v_top - 7u : 0u) << 23) : 1.f;
-      const size_t out = pair * a.max_parts + t.part;
+      wait(bar_o, step0 + steps - 1);
+      tc_fence_after();
+      const float back = F8 ? __uint_as_float((unit.v_top > 7u ? unit.v_top - 7u : 0u) << 23) : 1.f;
+      const size_t out = pair * a.max_parts + unit.part;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t x[32];
-        if (steps) {
-          tmem_ld32(o_tmem + lanes + 32 * w, x);
-          tmem_ld_wait();
-        }
+        tmem_ld32(o_tmem + lanes + 32 * w, x);
+        tmem_ld_wait();
         if (m < used) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (steps) o = make_float4(__uint_as_float(x[i]) * back, __uint_as_float(x[i + 1]) * back, __uint_as_float(x[i + 2]) * back, __uint_as_float(x[i + 3]) * back);
+            const float4 o = make_float4(__uint_as_float(x[i]) * back, __uint_as_float(x[i + 1]) * back, __uint_as_float(x[i + 2]) * back, __uint_as_float(x[i + 3]) * back);
             *reinterpret_cast<float4*>(a.part_acc + out * kKvDim + 32 * w + i) = o;
           }
         }
       }
       if (m < used) a.part_ml[out] = make_float2(ref == -INFINITY ? ref : ref - kBias, sum.x + sum.y);
-      tc_fence_before();
+      tc_fence_before();                                     // (the next unit's first product waits for this warp's first weights)
+      step0 += steps;
     }
-    step0 += steps;
-    u = next_unit;
-    __syncthreads();                                         // operands, scales and accumulators are free
   }
   // (every product has been waited for, or its wait ran out: then the tensor memory is given back after a moment for what may
   // still be under way)
