@@ -74,7 +74,8 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   const int sms = device_sm_count(dev);
   if (sms <= 0) return GRB_ERR_CUDA;
   const uint32_t warps = a.rows * ((a.nq + 2 * a.nkv + kTreeHeadsPerWarp - 1) / kTreeHeadsPerWarp);
-  if (int st = launch_step(tree_prep_kernel<F8>, dim3((warps + 7) / 8 + 1), dim3(kTreePrepThreads), a.rows * 6, stream, a, P::kPositions)) return st;
+  const uint32_t threads = a.rows > kTreePrepThreads ? kTreePrepMost : kTreePrepThreads;
+  if (int st = launch_step(tree_prep_kernel<F8>, dim3((warps + threads / 32 - 1) / (threads / 32) + 1), dim3(threads), a.rows * 6, stream, a, P::kPositions)) return st;
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
   if (int st = launch_step(tree_part_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
   if (a.wide_from) {
@@ -148,7 +149,7 @@ uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pa
   if (!rows || rows > kTreeMaxRows || !nq || !max_pages || format > GRB_KV_E4M3) return 0;
   const uint64_t parts = uint64_t(max_pages) * (format == GRB_KV_E4M3 ? kKvPage / TreePart<true>::kPositions : kKvPage / TreePart<false>::kPositions);
   const uint64_t pairs = uint64_t(rows) * nq;
-  return ((48 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * 2 + pairs * parts * (kKvDim * 4 + 8);
+  return ((48 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * 2 + 16 + pairs * parts * (kKvDim * 4 + 8);
 }
 
 int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
@@ -205,6 +206,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   at += (48 + a.rows * 40ull + pairs * 4 + 255) & ~uint64_t(255);
   a.q = reinterpret_cast<uint16_t*>(at);
   at += pairs * kKvDim * 2;
+  at += reinterpret_cast<uintptr_t>(at) & 16;                // (the scratch starts on 16 bytes, the parts on 32)
   a.part_acc = reinterpret_cast<float*>(at);
   at += pairs * a.max_parts * kKvDim * 4;
   a.part_ml = reinterpret_cast<float2*>(at);

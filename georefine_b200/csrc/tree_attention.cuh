@@ -20,7 +20,7 @@
 namespace grb {
 
 constexpr uint32_t kTreeMaxRows = 4096, kTreeMaskWords = 4;
-constexpr int kTreePrepThreads = 256;
+constexpr uint32_t kTreePrepThreads = 256, kTreePrepMost = 1024;   // of a CTA, up to 256 rows and beyond: the plan's CTA takes as many rows at a time
 constexpr uint32_t kTreeRowAbsent = 0xFFFFFFFFu;             // row_parts of a row that is left out: its output stays as it was
 // Positions of a wide tile's unit: the most, for long contexts (a unit's result is as large as 256 positions of an 8-bit cache); fewer
 // for short ones, whose few units would leave SMs idle.
@@ -82,20 +82,25 @@ __device__ __forceinline__ bool tree_sees(const TreeArgs& a, uint32_t r, int32_t
   return uint32_t(node) < a.mask_words * 64u && (a.row_mask[r * a.ldm + (node >> 6)] >> (node & 63) & 1u);
 }
 
-// Inclusive scans over the CTA.
+// Inclusive scans over the CTA.  Op: sums and maxima of values >= 0 alone (the order is free, and 0 changes nothing).
 template <class T, class Op>
-__device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
-  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+__device__ __forceinline__ T warp_scan(T v, Op op) {
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const T o = __shfl_up_sync(0xFFFFFFFFu, v, off);
-    if (lane >= uint32_t(off)) v = op(o, v);
+    if ((threadIdx.x & 31u) >= uint32_t(off)) v = op(o, v);
   }
+  return v;
+}
+template <class T, class Op>
+__device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+  v = warp_scan(v, op);
   __syncthreads();
   if (lane == 31) scratch[warp] = v;
   __syncthreads();
-  for (uint32_t w = 0; w < warp; ++w) v = op(scratch[w], v);   // (only sums and maxima of values >= 0 run here: the order is free)
-  return v;
+  const T before = __shfl_sync(0xFFFFFFFFu, warp_scan(lane < blockDim.x / 32 ? scratch[lane] : T(0), op), int(warp + 31) & 31);
+  return warp ? op(before, v) : v;
 }
 
 // A tile is up to tile_rows (wide_rows) consecutive rows of one sequence; rows that are left out or see nothing may be among them.
@@ -103,11 +108,11 @@ __device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
 __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_positions) {
   extern __shared__ int32_t extents[];                       // [rows]; -1: left out
   uint16_t* const run_of = reinterpret_cast<uint16_t*>(extents + a.rows);      // [rows]: first row of the row's run (rows of one sequence in a row)
-  __shared__ int32_t scratch[kTreePrepThreads / 32];
-  __shared__ unsigned long long sums[kTreePrepThreads / 32], total;
+  __shared__ int32_t scratch[kTreePrepMost / 32];
+  __shared__ unsigned long long sums[kTreePrepMost / 32], total;
   const uint32_t tid = threadIdx.x;
   int32_t run = 0;
-  for (uint32_t lo = 0; lo < a.rows; lo += kTreePrepThreads) {
+  for (uint32_t lo = 0; lo < a.rows; lo += blockDim.x) {
     const uint32_t r = lo + tid;
     const bool in = r < a.rows;
     const int32_t extent = in ? tree_extent(a, r) : -1;
@@ -119,11 +124,11 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
       a.extent[r] = max(extent, 0);
     }
     __syncthreads();
-    run = run_of[min(lo + kTreePrepThreads, a.rows) - 1];
+    run = run_of[min(lo + blockDim.x, a.rows) - 1];
   }
   // how many tiles and units there are before a tile, of either kind: tiles above, units (at most 2^32) below
   unsigned long long done = 0, wide_done = 0;
-  for (uint32_t lo = 0; lo < a.rows; lo += kTreePrepThreads) {
+  for (uint32_t lo = 0; lo < a.rows; lo += blockDim.x) {
     const uint32_t r = lo + tid;
     uint32_t n = 0, parts = 0, positions = part_positions;
     int32_t extent = 0;
@@ -145,7 +150,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
     auto scan = [&](bool counts, unsigned long long before) {
       const auto sum = [](unsigned long long x, unsigned long long y) { return x + y; };
       const unsigned long long upto = before + cta_scan(counts ? mine : 0ull, sums, sum);
-      if (tid == kTreePrepThreads - 1) total = upto;
+      if (tid == blockDim.x - 1) total = upto;
       return upto;
     };
     const unsigned long long upto = scan(!wide, done);
@@ -164,17 +169,17 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
 }
 
 // The first CTA lays down the plan; in the others a warp takes up to eight neighbouring heads of a row, all their loads on their
-// way together (one head a warp: 43 us for 1024 rows of 56 heads).  A lane owns dimensions 2 l, 2 l + 1 and the two that the
+// way together (one head a warp: 43 us for 1024 rows of 56 heads, eight: 27, a plan's CTA of 1024 threads: 15).  A lane owns dimensions 2 l, 2 l + 1 and the two that the
 // rotation pairs with them.  The products of BF16 values are exact in FP32, so the rotation rounds once before the result is
 // rounded to its type.
 constexpr uint32_t kTreeHeadsPerWarp = 8;
 template <bool F8>
-__global__ void __launch_bounds__(kTreePrepThreads)
+__global__ void __launch_bounds__(kTreePrepMost)
 tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
   step_kernel_entry();
   if (blockIdx.x == 0) return tree_plan(a, part_positions);
   const uint32_t heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 31u, per_row = (heads + kTreeHeadsPerWarp - 1) / kTreeHeadsPerWarp;
-  const uint32_t at = (blockIdx.x - 1) * (kTreePrepThreads / 32) + (threadIdx.x >> 5), row = at / per_row, head0 = at % per_row * kTreeHeadsPerWarp;
+  const uint32_t at = (blockIdx.x - 1) * (blockDim.x / 32) + (threadIdx.x >> 5), row = at / per_row, head0 = at % per_row * kTreeHeadsPerWarp;
   if (row >= a.rows) return;
   const uint32_t n = min(kTreeHeadsPerWarp, heads - head0);
   const uint32_t* src = reinterpret_cast<const uint32_t*>(a.qkv + row * a.ldq + size_t(head0) * kKvDim) + lane;
