@@ -69,6 +69,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity, boo
   }
   return ok != 0;
 }
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Waits for the phase with the given parity to complete.  False after kWaitLimitNs: the caller must
 // record kStatusTimeout and unwind.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, bool suspend = true) {

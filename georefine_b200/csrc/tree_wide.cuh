@@ -1,14 +1,18 @@
 // The attention of tree_attention.cuh for many rows of one sequence at a time: wide trees and prompt chunks, on tcgen05.
 //
 // A tile is up to 128 rows (row of the step, query head of the group) of one sequence and kv head: the M of one instruction.  A
-// unit is a tile and a chunk of the positions, taken 128 at a time:
+// unit is a tile and a chunk of the positions, taken 64 at a time:
 //   S = Q K^T (Q, K in shared memory, S in tensor memory);  weights P = exp2(S scale - reference), written over S;
 //   O += P V (P from tensor memory, V in shared memory, O in tensor memory).
-// Four warps, a thread per row, turn scores into weights (the first of them issues the products); four warps bring K and V: BF16
-// as it is, 8 bits through registers, where a code becomes FP16 (one conversion for two) times its entry's scale relative to the chunk's
-// largest.  256 columns of tensor memory and 104 KB of shared memory leave room for two CTAs on an SM, and while one waits for
-// its products the other's exponentials run: those bound the kernel (16 per SM and cycle: 1024 cycles for a tile of 128
-// positions, whose products take 512).
+// Four warps, a thread per row, turn scores into weights; four bring K and V: BF16 as it is, 8 bits through registers, where a code
+// becomes FP16 (one conversion for two) times its entry's scale relative to the chunk's largest; one issues the products.  K, V and
+// S of two steps are held, so a step's scores are computed while the step before is weighed, and the loaders set the next unit up
+// while this one ends.  256 columns of tensor memory and 105 KB of shared memory leave room for two CTAs on an SM.
+//
+// 16 trees of 64 nodes behind 8192 positions, 40 query heads of 8 kv heads: 317 us in 8 bits, 291 in BF16 (all launches), 0.42 PFLOP/s
+// - one step at a time and barriers between units: 438; steps of 128 with one S, the products issued by a weights' warp: 340.
+// What bounds it now is the loaders' chain of a step, 2500 cycles in which a CTA waits for a stage, converts 64 positions of K and
+// of V and asks for the next (without the loads 266 us; without the exponentials as long as with them).
 //
 // FP16 weights reach down to 2^-24 and V's entries to 2^-24 times a code of 1: both are scaled up as far as FP16 goes (weights at
 // most 2^15, values at most 57344), so what falls out at the bottom is 2^-39 of the largest - beyond what the 32-bit sums keep.
@@ -18,30 +22,24 @@
 
 namespace grb {
 
-constexpr int kWideThreads = 256;                // softmax warps 0-3, loading warps 4-7
-constexpr uint32_t kWideTile = 128;              // rows of a tile, positions of a step
-constexpr uint32_t kWideOperand = 32768;         // Q, K or V of a tile: two halves of 64 dimensions, 128 rows of 128 bytes each
+constexpr int kWideThreads = 384;                // softmax warps 0-3, loading warps 4-7, a warp that issues the products
+constexpr uint32_t kWideTile = 128;              // rows of a tile
+constexpr uint32_t kWideStep = 64;               // positions of a step
+constexpr uint32_t kWideOperand = 32768;         // Q: two halves of 64 dimensions, 128 rows of 128 bytes each; K or V of two steps
+constexpr uint32_t kWideStage = kWideOperand / 2;        // K or V of a step: two halves of 64 dimensions, 64 rows each
 constexpr uint32_t kWideScalesAt = 3 * kWideOperand;
 constexpr uint32_t kWideSmem = 3 * kWideOperand + 2 * 2 * kWideMostPart + 1024;   // operands, FP16 scales of a chunk's K and V, alignment
-constexpr uint32_t kWideColumns = 256;           // tensor memory: S (and P over it), O
+constexpr uint32_t kWideColumns = 256;           // tensor memory: S of two steps (and P over it), O
 
-// Byte offset of 16-byte piece `piece` (0..15) of row `row` of an operand: 128-byte swizzle in each half.
+// Byte offset of 16-byte piece `piece` (0..15) of row `row` of an operand of ROWS rows: 128-byte swizzle in each half.
+template <uint32_t ROWS>
 __device__ __forceinline__ uint32_t wide_offset(uint32_t row, uint32_t piece) {
-  return (piece >> 3) * (kWideOperand / 2) + row * 128u + (((piece ^ row) & 7u) << 4);
+  return (piece >> 3) * (ROWS * 128u) + row * 128u + (((piece ^ row) & 7u) << 4);
 }
-// V as the B operand with its dimensions contiguous (N-major): 64 dimensions per 128-byte row, the other half 16 KB on, groups of
+// V as the B operand with its dimensions contiguous (N-major): 64 dimensions per 128-byte row, the other half 8 KB on, groups of
 // eight positions 1024 bytes apart.
 __device__ __forceinline__ uint64_t wide_desc_v(uint32_t smem_addr) {
-  return uint64_t((smem_addr >> 4) & 0x3FFFu) | (uint64_t(kWideOperand / 2 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
-      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
-      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+  return uint64_t((smem_addr >> 4) & 0x3FFFu) | (uint64_t(kWideStage / 2 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 // 32 bytes, a whole sector: a thread stores its own row, and 16 bytes at a time every sector went out twice (364 us for 16 trees of
 // 64 nodes behind 8192 positions instead of 352).
@@ -83,25 +81,27 @@ __global__ void __launch_bounds__(kWideThreads, 2)
 tree_wide_kernel(const TreeArgs a) {
   step_kernel_entry();
   extern __shared__ unsigned char wide_smem_raw[];
-  __shared__ __align__(8) uint64_t bars[6];                  // K stored, V stored, S done, P stored, O done, unit set up
+  __shared__ __align__(8) uint64_t bars[11];                 // of even and odd steps: K stored, V stored, S done, P stored, O done; unit set up
   __shared__ uint32_t tmem_at, aborted, next_unit;
   __shared__ uint32_t k_top, v_top, any_bad, any_absent;     // the loaders' own, while they set a unit up
   __shared__ WideInfo info[2];                               // of a unit and the next
-  __shared__ int64_t entries[2][kWideMostPart / kWideTile];  // entry (of the layer) of each step's first position; -1: no page
+  __shared__ int64_t entries[2][kWideMostPart / kWideStep];  // entry (of the layer) of each step's first position; -1: no page
   __shared__ uint32_t bad[2][kWideMostPart / 32];            // positions of the chunk whose key or value is not a number
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t smem = (smem_u32(wide_smem_raw) + 1023u) & ~1023u, qs = smem, ks = smem + kWideOperand, vs = smem + 2 * kWideOperand;
   const uint32_t k_scales = smem + kWideScalesAt, v_scales = k_scales + 2 * kWideMostPart;
-  const uint32_t bar_k = smem_u32(&bars[0]), bar_v = smem_u32(&bars[1]), bar_s = smem_u32(&bars[2]), bar_p = smem_u32(&bars[3]), bar_o = smem_u32(&bars[4]),
-                 bar_u = smem_u32(&bars[5]);
+  const uint32_t bar_k = smem_u32(&bars[0]), bar_v = smem_u32(&bars[2]), bar_s = smem_u32(&bars[4]), bar_o = smem_u32(&bars[6]), bar_p = smem_u32(&bars[8]),
+                 bar_u = smem_u32(&bars[10]);
   const uint32_t tiles = a.plan[2], units = a.plan[3];
   if (blockIdx.x >= units) return;
   if (tid == 0) {
-    mbar_init(bar_k, 4);
-    mbar_init(bar_v, 4);
-    mbar_init(bar_s, 1);
-    mbar_init(bar_p, 4);
-    mbar_init(bar_o, 1);
+    for (uint32_t b = 0; b < 16; b += 8) {
+      mbar_init(bar_k + b, 4);
+      mbar_init(bar_v + b, 4);
+      mbar_init(bar_s + b, 1);
+      mbar_init(bar_o + b, 1);
+      mbar_init(bar_p + b, 4);
+    }
     mbar_init(bar_u, 4);
     mbar_fence_init();
     aborted = 0u;
@@ -116,16 +116,19 @@ tree_wide_kernel(const TreeArgs a) {
   const uint32_t s_tmem = tmem_at, o_tmem = tmem_at + 128;
   // A wait that runs out is everybody's: nobody waits again, every loop runs to its end, and the status says so.
   auto wait = [&](uint32_t bar, uint32_t step) {
-    if (*reinterpret_cast<volatile uint32_t*>(&aborted)) return;
+    if (mbar_test_wait(bar, step & 1u) || *reinterpret_cast<volatile uint32_t*>(&aborted)) return;
     if (!mbar_wait(bar, step & 1u, false)) {
       *reinterpret_cast<volatile uint32_t*>(&aborted) = 1u;
       atomicOr(a.status, kStatusTimeout);
     }
   };
+  auto wait2 = [&](uint32_t bars2, uint32_t step) { wait(bars2 + 8 * (step & 1u), step >> 1); };
   // Units differ in length, so a CTA takes the next one when it is through with its own (who computes a unit changes nothing in it);
   // its loaders set the next one up while the last step of this one is multiplied and its result stored.
   uint32_t step0 = 0;                                        // steps this CTA has taken before the unit
-  if (warp >= 4) {
+  // registers, of the 240 that three threads of the launch have: 112 for the weights, 88 for loading, 40 for the products
+  if (warp >= 4 && warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
     // ---- loading ------------------------------------------------------------------------------------------------
     const uint32_t lt = tid - 128;
     uint32_t tile = 0, slot = 0, steps_before = 0;
@@ -154,8 +157,8 @@ tree_wide_kernel(const TreeArgs a) {
       }
       if (warp == 4) {                                       // (a step's positions lie in one page)
         int64_t place = 0;
-        if (lane < part_positions / kWideTile) {
-          place = kv_place(a.table, t.seq, t.start + int32_t(lane * kWideTile));
+        if (lane < part_positions / kWideStep) {
+          place = kv_place(a.table, t.seq, t.start + int32_t(lane * kWideStep));
           entries[slot][lane] = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
         }
         const bool absent = __any_sync(0xFFFFFFFFu, place < 0);
@@ -173,14 +176,14 @@ tree_wide_kernel(const TreeArgs a) {
         all = min(all, __shfl_xor_sync(0xFFFFFFFFu, all, off));
       }
       t.extent = min(extent, t.start + int32_t(part_positions));
-      steps = (uint32_t(t.extent - t.start) + kWideTile - 1) / kWideTile;       // (a unit has a position at least)
+      steps = (uint32_t(t.extent - t.start) + kWideStep - 1) / kWideStep;       // (a unit has a position at least)
       wide_loaders_meet();                                   // (the scales of the unit before have been read, too)
       u = next_unit;
-      plain = any_absent ? 0u : all >= t.extent ? steps : uint32_t(max(all - t.start, 0)) / kWideTile;
+      plain = any_absent ? 0u : all >= t.extent ? steps : uint32_t(max(all - t.start, 0)) / kWideStep;
       const int64_t* const at = entries[slot];
       // the queries, sixteen lanes a row, once the scores of the unit before are done
       auto queries = [&]() {
-        if (step0) wait(bar_s, step0 - 1);
+        if (step0) wait2(bar_s, step0 - 1);
 #pragma unroll 1
         for (int part = 0; part < 4; ++part) {
           uint4 x[4];
@@ -191,14 +194,14 @@ tree_wide_kernel(const TreeArgs a) {
                             : make_uint4(0u, 0u, 0u, 0u);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sts128(qs + wide_offset((lt >> 4) + (4 * part + i) * 8, lt & 15u), x[i]);
+          for (int i = 0; i < 4; ++i) sts128(qs + wide_offset<kWideTile>((lt >> 4) + (4 * part + i) * 8, lt & 15u), x[i]);
         }
       };
-      // everything is there: tells the weights' warps, who have all looked at the unit before by the time its second step's values
-      // were used (of a unit of one step: its only step's)
+      // everything is there: tells the weights' warps, who have all looked at the unit before once its first step's values have been
+      // used (storing the third step's waited for that)
       auto publish = [&]() {
         if (lt == 0) info[slot] = WideInfo{1u, t.first, t.rows, t.kvh, t.part, steps, plain, t.start, k_top, v_top, any_bad};
-        if (steps_before == 1) wait(bar_o, step0 - 1);
+        if (steps_before && steps_before <= 2) wait2(bar_o, step0 - 1);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_u);
@@ -207,19 +210,19 @@ tree_wide_kernel(const TreeArgs a) {
         // A thread's pieces: the same quarter of both halves of every 32nd row.  Eight lanes take four pieces of two neighbouring rows,
         // which the swizzle spreads over all banks when their sixteen values each are stored.
         const uint32_t row0 = lt >> 2;
-        uint4 k[8], v[8];
-        auto ask = [&](uint4 (&x)[8], const void* pool, uint32_t j) {
+        uint4 k[4], v[4];
+        auto ask = [&](uint4 (&x)[4], const void* pool, uint32_t j) {
           const int64_t entry = j < steps ? at[j] : -1;
-          const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
+          const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideStep);
           const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim) + row0 * 8 + (lt & 3u);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = int32_t(row0 + 32 * (i >> 1)) < npos ? src[256 * (i >> 1) + 4 * (i & 1)] : make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < 4; ++i) x[i] = int32_t(row0 + 32 * (i >> 1)) < npos ? src[256 * (i >> 1) + 4 * (i & 1)] : make_uint4(0u, 0u, 0u, 0u);
         };
-        const uint32_t to_lo = wide_offset(row0, 2 * (lt & 3u)), to_hi = wide_offset(row0, 2 * (lt & 3u) + 1);     // (32 rows on: 4096 bytes)
-        auto store = [&](const uint4 (&x)[8], uint32_t dst, uint32_t scales, uint32_t j, bool clean) {
+        const uint32_t to_lo = wide_offset<kWideStep>(row0, 2 * (lt & 3u)), to_hi = wide_offset<kWideStep>(row0, 2 * (lt & 3u) + 1);     // (32 rows on: 4096 bytes)
+        auto store = [&](const uint4 (&x)[4], uint32_t dst, uint32_t scales, uint32_t j, bool clean) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t s16 = lds_u16(scales + 2 * (j * kWideTile + row0 + 32 * (i >> 1))), s = s16 | (s16 << 16);
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t s16 = lds_u16(scales + 2 * (j * kWideStep + row0 + 32 * (i >> 1))), s = s16 | (s16 << 16);
             uint32_t h[8];
             e4m3_to_half4(x[i].x, h[0], h[1]);
             e4m3_to_half4(x[i].y, h[2], h[3]);
@@ -231,7 +234,7 @@ tree_wide_kernel(const TreeArgs a) {
             }
 #pragma unroll
             for (int q = 0; q < 8; ++q) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[q]) : "r"(s));
-            const uint32_t at = dst + 4096 * (i >> 1) + (kWideOperand / 2) * (i & 1);
+            const uint32_t at = dst + 4096 * (i >> 1) + (kWideStage / 2) * (i & 1);
             sts128(at + to_lo, make_uint4(h[0], h[1], h[2], h[3]));
             sts128(at + to_hi, make_uint4(h[4], h[5], h[6], h[7]));
           }
@@ -242,8 +245,8 @@ tree_wide_kernel(const TreeArgs a) {
         uint32_t w[2][4];
 #pragma unroll
         for (int of_v = 0; of_v < 2; ++of_v) {
-          const int64_t entry = lt < steps * 8 ? at[lt >> 3] : -1;
-          const uint4 x = entry >= 0 ? *reinterpret_cast<const uint4*>((of_v ? a.pages.v_exp : a.pages.k_exp) + entry + (lt & 7u) * 16) : make_uint4(0u, 0u, 0u, 0u);
+          const int64_t entry = lt < steps * 4 ? at[lt >> 2] : -1;
+          const uint4 x = entry >= 0 ? *reinterpret_cast<const uint4*>((of_v ? a.pages.v_exp : a.pages.k_exp) + entry + (lt & 3u) * 16) : make_uint4(0u, 0u, 0u, 0u);
           w[of_v][0] = x.x; w[of_v][1] = x.y; w[of_v][2] = x.z; w[of_v][3] = x.w;
         }
         const int32_t left = t.extent - t.start - int32_t(lt * 16);
@@ -286,51 +289,64 @@ tree_wide_kernel(const TreeArgs a) {
         wide_loaders_meet();                                 // the scales are complete
         for (uint32_t j = 0; j < steps; ++j) {
           const uint32_t g = step0 + j;
-          if (g) wait(bar_s, g - 1);                         // the scores of the step before have been taken from K
-          store(k, ks, k_scales, j, false);
+          const uint32_t stage = (g & 1u) * kWideStage;
+          if (g > 1) wait2(bar_s, g - 2);                    // scores have been taken from the stage's K
+          store(k, ks + stage, k_scales, j, false);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar_k);
+          if (lane == 0) mbar_arrive(bar_k + 8 * (g & 1u));
           ask(k, a.pages.k, j + 1);
-          if (g) wait(bar_o, g - 1);                         // the values of the step before have been used
-          store(v, vs, v_scales, j, j >= plain);
+          if (g > 1) wait2(bar_o, g - 2);                    // the stage's values have been used
+          store(v, vs + stage, v_scales, j, j >= plain);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar_v);
+          if (lane == 0) mbar_arrive(bar_v + 8 * (g & 1u));
           ask(v, a.pages.v, j + 1);
         }
       } else {
         auto ask = [&](uint32_t dst, const void* pool, uint32_t j) {
           const int64_t entry = at[j];
-          const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideTile);
+          const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideStep);
           const uint8_t* src = static_cast<const uint8_t*>(pool) + (entry < 0 ? 0 : entry) * kKvDim * 2;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const uint32_t c = lt + 128 * i;
             const bool in = int32_t(c >> 4) < npos;
-            cp_async_16(dst + wide_offset(c >> 4, c & 15u), src + (in ? c * 16 : 0u), in ? 16u : 0u);
+            cp_async_16(dst + wide_offset<kWideStep>(c >> 4, c & 15u), src + (in ? c * 16 : 0u), in ? 16u : 0u);
           }
           cp_async_commit();
         };
         wide_loaders_meet();                                 // (the unit after this one and its pages are known to all)
         queries();
         publish();
-        for (uint32_t j = 0; j < steps; ++j) {
-          const uint32_t g = step0 + j;
-          if (g) wait(bar_s, g - 1);
-          ask(ks, a.pages.k, j);
-          if (g) wait(bar_o, g - 1);
-          ask(vs, a.pages.v, j);
-          cp_async_wait<1>();
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_k);
-          cp_async_wait<0>();
-          if (j >= plain) {                                   // values that are not finite would reach, as 0 * infinity, rows that do not see them
+        // (a step's copies are on their way while the step before's land; behind the last one, groups of none keep the count)
+        for (uint32_t j = 0; j <= steps; ++j) {
+          const uint32_t g = step0 + j, stage = (g & 1u) * kWideStage, before = kWideStage - stage;
+          if (j < steps) {
+            if (g > 1) wait2(bar_s, g - 2);
+            ask(ks + stage, a.pages.k, j);
+          } else {
+            cp_async_commit();
+          }
+          if (j) {
+            cp_async_wait<2>();
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_k + 8 * (~g & 1u));
+          }
+          if (j < steps) {
+            if (g > 1) wait2(bar_o, g - 2);
+            ask(vs + stage, a.pages.v, j);
+          } else {
+            cp_async_commit();
+          }
+          if (!j) continue;
+          cp_async_wait<2>();
+          if (j > plain) {                                   // values that are not finite would reach, as 0 * infinity, rows that do not see them
             uint32_t mine = 0;                               // bit i: of the thread's piece i
 #pragma unroll 1
-            for (int i = 0; i < 16; ++i) {
-              const uint32_t c = lt + 128 * i, at = vs + wide_offset(c >> 4, c & 15u);
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t c = lt + 128 * i, at = vs + before + wide_offset<kWideStep>(c >> 4, c & 15u);
               const uint4 x = lds128(at);
               const uint32_t w[4] = {x.x, x.y, x.z, x.w};
               bool b = false;
@@ -341,29 +357,70 @@ tree_wide_kernel(const TreeArgs a) {
             }
             // piece i of this warp's lanes lies in positions 8 i + 2 (warp - 4) and the next
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 8; ++i) {
               const uint32_t m = __ballot_sync(0xFFFFFFFFu, mine >> i & 1u);
               const uint32_t p = 8 * i + 2 * (warp - 4);
-              if (lane == 0 && m) atomicOr(&bad[slot][j * (kWideTile / 32) + (p >> 5)], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
+              if (lane == 0 && m) atomicOr(&bad[slot][(j - 1) * (kWideStep / 32) + (p >> 5)], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
             }
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar_v);
+          if (lane == 0) mbar_arrive(bar_v + 8 * (~g & 1u));
         }
       }
+      if (steps == 1 && step0) wait2(bar_o, step0 - 1);      // (the unit before is over, whose tables the next one but one overwrites)
       step0 += steps;
       steps_before = steps;
     }
     // no unit is left
     if (lt == 0) info[slot].valid = 0u;
-    if (steps_before == 1) wait(bar_o, step0 - 1);
+    if (steps_before && steps_before <= 2) wait2(bar_o, step0 - 1);
     __syncwarp();
     if (lane == 0) mbar_arrive(bar_u);
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // ---- products -----------------------------------------------------------------------------------------------
+    // (a warp of its own: issuing a step's products takes it as long as the weights take theirs)
+    constexpr uint32_t kIdesc = umma_idesc_bf16(128) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);      // FP16 or BF16 operands
+    constexpr uint32_t kIdescS = umma_idesc_bf16(kWideStep) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);
+    auto scores = [&](uint32_t g) {
+      if (g > 1) wait2(bar_o, g - 2);                        // the weights there have been used (issue order alone does not say so:
+      wait2(bar_k, g);                                       // the two products differ in shape)
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d)                          // 16 dimensions each
+          umma_bf16(s_tmem + (g & 1u) * kWideStep, umma_desc_sw128(qs + (d >> 2) * (kWideOperand / 2) + (d & 3) * 32),
+                    umma_desc_sw128(ks + (g & 1u) * kWideStage + (d >> 2) * (kWideStage / 2) + (d & 3) * 32), kIdescS, d > 0);
+        umma_commit(bar_s + 8 * (g & 1u));
+      }
+      __syncwarp();
+    };
+    for (uint32_t n = 0; warp == 8; ++n) {
+      wait(bar_u, n);
+      if (!info[n & 1u].valid || *reinterpret_cast<volatile uint32_t*>(&aborted)) break;
+      const uint32_t steps = info[n & 1u].steps;
+      scores(step0);
+      for (uint32_t j = 0; j < steps; ++j) {
+        const uint32_t g = step0 + j;
+        if (j + 1 < steps) scores(g + 1);
+        wait2(bar_v, g);
+        wait2(bar_p, g);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d)                        // 16 positions each
+            umma_bf16_ts(o_tmem, s_tmem + (g & 1u) * kWideStep + 8 * d, wide_desc_v(vs + (g & 1u) * kWideStage + 2048 * d), kIdesc | (1u << 16), j > 0 || d > 0);
+          umma_commit(bar_o + 8 * (g & 1u));
+        }
+        __syncwarp();
+      }
+      step0 += steps;
+    }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ---- weights: thread = row m of the tile, lane m of tensor memory ------------------------------------------------
     constexpr float kSlack = 8.f, kBias = F8 ? 7.f : 0.f;    // FP16: weights up to 2^(7 + 8)
-    constexpr uint32_t kIdesc = umma_idesc_bf16(128) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);      // FP16 or BF16 operands
     const uint32_t m = tid, lanes = (warp * 32u) << 16;
     for (uint32_t n = 0;; ++n) {
       const uint32_t slot = n & 1u;
@@ -379,33 +436,22 @@ tree_wide_kernel(const TreeArgs a) {
       float ref = -INFINITY;
       float2 sum = make_float2(0.f, 0.f);
       for (uint32_t j = 0; j < steps; ++j) {
-        const uint32_t g = step0 + j;
-        const int32_t at = start + int32_t(j * kWideTile);
-        if (warp == 0) {                                     // (behind the values' product of the step before, in issue order)
-          wait(bar_k, g);
-          __syncwarp();
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {                    // 16 dimensions each
-              const uint32_t half = (s >> 2) * (kWideOperand / 2) + (s & 3) * 32;
-              umma_bf16(s_tmem, umma_desc_sw128(qs + half), umma_desc_sw128(ks + half), kIdesc, s > 0);
-            }
-            umma_commit(bar_s);
-          }
-          __syncwarp();
-        }
-        wait(bar_s, g);
+        const uint32_t g = step0 + j, s_at = s_tmem + lanes + (g & 1u) * kWideStep;
+        const int32_t at = start + int32_t(j * kWideStep);
+        wait2(bar_s, g);
         tc_fence_after();
+        uint32_t x[2][32];
+        tmem_ld32(s_at, x[0]);
+        tmem_ld32(s_at + 32, x[1]);
         // which of the step's positions the row sees
-        const bool there = entries[slot][j] >= 0;                 // (a page outside the pool: as if nobody saw its positions)
         const bool every = j < plain;
-        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+        uint32_t see[2] = {~0u, ~0u};
         bool poisoned = false;
         if (!every) {
-          wait(bar_v, g);                                    // (`bad` is complete)
+          wait2(bar_v, g);                                   // (`bad` is complete)
+          const bool there = entries[slot][j] >= 0;          // (a page outside the pool: as if nobody saw its positions)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < 2; ++w) {
             const int32_t p = at + 32 * w, most = min(max(mine - p, 0), 32);
             const uint32_t below = most == 32 ? ~0u : (1u << most) - 1u;            // up to the last position the row sees
             uint32_t bits = ~0u;
@@ -428,32 +474,19 @@ tree_wide_kernel(const TreeArgs a) {
         }
         if (F8 ? any_bad : !every) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&bad[slot][j * (kWideTile / 32) + w]) & see[w]);
+          for (int w = 0; w < 2; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&bad[slot][j * (kWideStep / 32) + w]) & see[w]);
         }
-        auto masked = [&](uint32_t (&x)[32], int w) {
-          if (!every) {
+        tmem_ld_wait();
+        if (!every) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = see[w] >> i & 1u ? x[i] : 0xFF800000u;
-          }
-        };
-        float top = -INFINITY;
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int w = 0; w < 4; w += 2) {
-          uint32_t x[32], y[32];
-          tmem_ld32(s_tmem + lanes + 32 * w, x);
-          tmem_ld32(s_tmem + lanes + 32 * w + 32, y);
-          tmem_ld_wait();
-          masked(x, w);
-          masked(y, w + 1);
-          float even = -INFINITY, odd = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            even = fmaxf(even, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
-            odd = fmaxf(odd, fmaxf(__uint_as_float(y[i]), __uint_as_float(y[i + 1])));
-          }
-          top = fmaxf(top, fmaxf(even, odd));
+            for (int i = 0; i < 32; ++i) x[w][i] = see[w] >> i & 1u ? x[w][i] : 0xFF800000u;
         }
-        top = __fmul_rn(top, scale);
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(tops[i >> 1 & 3], fmaxf(__uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i + 1) & 31])));
+        const float top = __fmul_rn(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), scale);
         const bool move = top > (ref == -INFINITY ? ref : __fadd_rn(ref, kSlack));
         if (__any_sync(0xFFFFFFFFu, move)) {
           const float to = move ? top : ref, f = move ? exp2_approx(__fsub_rn(ref, to)) : 1.f;        // (from -infinity: 0)
@@ -461,28 +494,28 @@ tree_wide_kernel(const TreeArgs a) {
           sum.y = __fmul_rn(sum.y, f);
           ref = to;
           if (j > 0) {
-            wait(bar_o, g - 1);
+            wait2(bar_o, g - 1);
             tc_fence_after();
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t x[32];
-              tmem_ld32(o_tmem + lanes + 32 * w, x);
+#pragma unroll 1
+            for (int w = 0; w < 8; ++w) {
+              uint32_t o[16];
+              tmem_ld16(o_tmem + lanes + 16 * w, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__fmul_rn(__uint_as_float(x[i]), f));
-              tmem_st32(o_tmem + lanes + 32 * w, x);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__fmul_rn(__uint_as_float(o[i]), f));
+              tmem_st16(o_tmem + lanes + 16 * w, o);
             }
           }
         }
         const float low = (ref == -INFINITY ? 0.f : ref) - kBias;
         const float2 scale2 = make_float2(scale, scale), low2 = make_float2(-low, -low);
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        auto weigh = [&](uint32_t (&x)[32], int w) {
-          masked(x, w);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 e = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, low2);
+            float2 e = fma2(make_float2(__uint_as_float(x[w][2 * i]), __uint_as_float(x[w][2 * i + 1])), scale2, low2);
             e.x = exp2_approx(e.x);
             e.y = exp2_approx(e.y);
             sums[i & 1] = add2(sums[i & 1], e);
@@ -493,42 +526,17 @@ tree_wide_kernel(const TreeArgs a) {
               p[i] = pack_bf(e.x, e.y);
             }
           }
-          tmem_st16(s_tmem + lanes + 16 * w, p);             // (over scores that have been read)
-        };
-        uint32_t x[32], y[32];
-        tmem_ld32(s_tmem + lanes, x);
-        tmem_ld32(s_tmem + lanes + 32, y);
-        tmem_ld_wait();
-        weigh(x, 0);
-        tmem_ld32(s_tmem + lanes + 64, x);
-        weigh(y, 1);
-        tmem_ld_wait();
-        tmem_ld32(s_tmem + lanes + 96, y);
-        weigh(x, 2);
-        tmem_ld_wait();
-        weigh(y, 3);
+          tmem_st16(s_at + 16 * w, p);                       // (over scores that have been read)
+        }
         sum = add2(sum, add2(sums[0], sums[1]));
         if (poisoned) sum.x = __uint_as_float(0x7FC00000u);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p);
-        if (warp == 0) {
-          wait(bar_p, g);
-          wait(bar_v, g);
-          __syncwarp();
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int s = 0; s < 8; ++s)                      // 16 positions each
-              umma_bf16_ts(o_tmem, s_tmem + 8 * s, wide_desc_v(vs + 2048 * s), kIdesc | (1u << 16), j > 0 || s > 0);
-            umma_commit(bar_o);
-          }
-          __syncwarp();
-        }
+        if (lane == 0) mbar_arrive(bar_p + 8 * (g & 1u));
       }
       // ---- the unit's partial result
-      wait(bar_o, step0 + steps - 1);
+      wait2(bar_o, step0 + steps - 1);
       tc_fence_after();
       const float back = F8 ? __uint_as_float((unit.v_top > 7u ? unit.v_top - 7u : 0u) << 23) : 1.f;
       const size_t out = pair * a.max_parts + unit.part;
