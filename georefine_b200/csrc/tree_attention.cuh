@@ -4,11 +4,12 @@
 //   out[r, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(q_rh . k_j / sqrt(128)),  j over the positions that row r sees:
 //   causal: j <= row_pos[r];  tree: j < base[r], or bit j - base[r] of the row's mask.  A row that sees nothing gives 0.
 //
-// Three launches, four where many rows of a sequence may come together.  tree_prep: rotates the queries (once rounded, to the type the matrix instruction takes), stores keys and
-// values, and one CTA lays down the plan: tiles of rows of one sequence, and units = (tile, part of the positions, kv head).
-// tree_part: persistent CTAs take units in turn.  tree_wide (tree_wide.cuh) does for runs of many rows.
-// tree_combine: merges a row's parts.  The parts of a row depend on its own sequence alone (in tree_part on its
-// own positions), and every sum runs in a fixed order, so a row's bits do not depend on the batch it is in.
+// Three launches, four where many rows of a sequence may come together.  tree_prep: rotates the queries (once rounded, to the type
+// the matrix instruction takes), stores keys and values, and one CTA lays down the plan: tiles of rows of one sequence, and units =
+// (tile, part of the positions, kv head).  tree_part: persistent CTAs take runs of units.  tree_wide (tree_wide.cuh): the same for
+// runs of many rows.  tree_combine: merges a row's parts.  Which kernel takes a row and where its parts lie depends on its own
+// sequence's rows alone (and on whether the caller's longest_run lets tree_wide run at all), and every sum runs in a fixed order:
+// a row's bits do not depend on what else is in the batch.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -20,12 +21,17 @@
 namespace grb {
 
 constexpr uint32_t kTreeMaxRows = 4096, kTreeMaskWords = 4;
-constexpr uint32_t kTreePrepThreads = 256, kTreePrepMost = 1024;   // of a CTA, up to 256 rows and beyond: the plan's CTA takes as many rows at a time
+// Threads of a tree_prep CTA, up to 256 rows and beyond: the plan's CTA takes as many rows at a time.
+constexpr uint32_t kTreePrepThreads = 256, kTreePrepMost = 1024;
 constexpr uint32_t kTreeRowAbsent = 0xFFFFFFFFu;             // row_parts of a row that is left out: its output stays as it was
 // Positions of a wide tile's unit: the most, for long contexts (a unit's result is as large as 256 positions of an 8-bit cache); fewer
-// for short ones, whose few units would leave SMs idle.
+// for short ones and for runs of one or two tiles, whose few units would leave SMs idle.  1024 instead of 2048 behind 8192 positions,
+// 8 bits, 40 heads of 8: one run of 16 rows 37 us instead of 53, 16 runs 127 instead of 140; 16 runs of 64 rows (three tiles) 347
+// instead of 318, which keep 2048.
 constexpr uint32_t kWideMostPart = 2048;
-__device__ __forceinline__ uint32_t wide_part(uint32_t extent) { return extent <= 1024 ? 256u : extent <= 4096 ? 512u : kWideMostPart; }
+__device__ __forceinline__ uint32_t wide_part(uint32_t extent, bool many) {
+  return extent <= 1024 ? 256u : extent <= 4096 ? 512u : extent <= 16384 && !many ? 1024u : kWideMostPart;
+}
 
 struct TreeArgs {
   const __nv_bfloat16* qkv;   // [rows][ldq]: nq query heads | nkv key heads | nkv value heads, 128 each
@@ -139,7 +145,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
       const uint32_t per = wide ? a.wide_rows : a.tile_rows;
       if ((r - first) % per == 0) {
         for (; n < per && r + n < a.rows && run_of[r + n] == first; ++n) extent = max(extent, extents[r + n]);
-        if (wide) positions = wide_part(uint32_t(extent));
+        if (wide) positions = wide_part(uint32_t(extent), first + 2 * a.wide_rows < a.rows && run_of[first + 2 * a.wide_rows] == first);
         parts = (uint32_t(extent) + positions - 1) / positions;
         if (wide)
           for (uint32_t i = 0; i < n; ++i) a.row_parts[r + i] = extents[r + i] < 0 ? kTreeRowAbsent : parts;
@@ -169,9 +175,9 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
 }
 
 // The first CTA lays down the plan; in the others a warp takes up to eight neighbouring heads of a row, all their loads on their
-// way together (one head a warp: 43 us for 1024 rows of 56 heads, eight: 27, a plan's CTA of 1024 threads: 15).  A lane owns dimensions 2 l, 2 l + 1 and the two that the
-// rotation pairs with them.  The products of BF16 values are exact in FP32, so the rotation rounds once before the result is
-// rounded to its type.
+// way together.  A lane owns dimensions 2 l, 2 l + 1 and the two that the rotation pairs with them.  The products of BF16 values are
+// exact in FP32, so the rotation rounds once before the result is rounded to its type.  1024 rows of 56 heads: 15 us (one head a
+// warp 43; 256 rows of the plan at a time 27).  One row: 7 us, the plan's chain of dependent loads.
 constexpr uint32_t kTreeHeadsPerWarp = 8;
 template <bool F8>
 __global__ void __launch_bounds__(kTreePrepMost)
@@ -267,6 +273,8 @@ tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
 // 8 bits: a code becomes FP16 exactly (one conversion for two), straight from shared memory to the MMA's B registers.
 // K's scale multiplies the score of its position.  V's goes into the weight: S' = S + e_v, so that the FP16 weights are
 // largest where the products are, whatever sizes the values have; the sum of the weights takes it out again.
+// 128 rows behind 2048 positions each, 40 heads of 8, 8 bits (410 MB): 100 us, 4.1 TB/s.  With one sequence's five heads in sixteen
+// MMA rows, what bounds it is the instructions that turn codes into operands and scores into weights, not their products.
 template <bool F8>
 struct TreePart {
   static constexpr int kThreads = 128;

@@ -121,7 +121,8 @@ struct VerifyOctet<true> {
 // Grid (8, rows): each CTA takes an eighth of the row, a thread up to ten octets of it at a time (all of its share of 152064
 // BF16 logits), loaded together: the CTA's maximum of them, then one multiply-add, one exponential and one addition each.
 // Bound by memory, the exponentials (16 per SM and cycle) not far behind.  The eighths are put together by whoever needs the
-// row: doing it here, in a cluster, left the SMs waiting for chains of exponentials and remote reads (54 us for 546 rows).
+// row: doing it here, in a cluster, left the SMs waiting for chains of exponentials and remote reads (546 rows of 152064 BF16
+// logits: 54 us, this 34, 4.9 TB/s).
 // The exponent l hi - c (hi: log2_scale rounded to 32 bits, c: that of the maximum m, rounded) is rounded once; what hi leaves
 // out, l (log2_scale - hi), is taken for m in R, which leaves (l - m) 2^-25 of a weight that falls with l - m.  Eight
 // exponentials are added in 32 bits, the eights in 64: a probability is off by the exponentials' 2^-22 at most.
@@ -184,7 +185,7 @@ verify_rows_kernel(const VerifyArgs a) {
 
 // 2^y for -101 < y < 1 to 2^-42: y = k / 16 + f, 2^(k / 16) from a table and a shift, 2^f by the first six terms of the
 // exponential series in f ln 2 (|f| <= 2^-5: the seventh is 1.4e-13).  Sixteen entries lie in as many pairs of banks, so a warp's
-// look-ups never collide; with 64 of them and one term less they did, and took three quarters of the kernel's time.
+// look-ups never collide; 64 of them and one term less took as long.
 constexpr uint32_t kExpTable = 16;
 __device__ __forceinline__ double exp2_f64(double y, const double* table) {
   constexpr double kRound = 6755399441055744.0;     // 1.5 * 2^52: what is added to it rounds to a whole number in its low bits
@@ -199,8 +200,7 @@ __device__ __forceinline__ double exp2_f64(double y, const double* table) {
   return __hiloint2double(__double2hiint(r) + ((k & -int(kExpTable)) << 16), __double2loint(r));
 }
 
-// x 2^-896 in 64 bits, for a finite x, by integer operations (conversions between the two widths run at a quarter of their rate);
-// a zero or a subnormal becomes some number below 2^-1022.
+// x 2^-896 in 64 bits, for a finite x, by integer operations in place of a conversion; a zero or a subnormal becomes some number below 2^-1022.
 __device__ __forceinline__ double widen(float x) {
   const int u = __float_as_int(x);
   return __hiloint2double((u >> 3) & int(0x8FFFFFFFu), int(uint32_t(u) << 29));
@@ -257,9 +257,10 @@ struct VerifyMasses {
 // Grid (CTAs of a sequence, sequences), a cluster per sequence: every warp of the cluster sums its regions of the row in 64 bits;
 // the sums are exchanged, and the warp in whose region the draw falls goes through it again, tile by tile.  All three passes
 // (the middle one for every draw, the first where q is subtracted, the last) run the same loop: unrolled, or written out for each,
-// the kernel was bound by the fetching of its own instructions (30 us for one sequence instead of 9).
-// The cluster is as large (8, 4 or 2 CTAs) as lets all sequences be resident at once: a CTA's chain of dependent loads and
-// barriers is 9 us long, so a second wave costs more than the larger share of a CTA in the first.
+// the kernel was slowed by the fetching of its own instructions.
+// One sequence: 13 us, a chain of dependent loads, barriers and the walk more than the sums.  128 sequences: 43 us, of which the
+// 64-bit operations, twelve a token, take 12.  The cluster is as large (8, 4 or 2 CTAs) as lets all sequences be resident at once:
+// with that chain a second wave costs more than the larger share of a CTA in the first.
 template <bool F32, bool VEC>
 __global__ void __launch_bounds__(kVerifyDrawThreads, 2)
 verify_draw_kernel(const VerifyArgs a) {

@@ -331,6 +331,66 @@ def test_a_long_context(dev):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+def test_more_wide_units_than_the_gpu_holds_at_a_time(dev, fmt):
+    """Trees of 64 and of 9 nodes behind contexts that end within and at the end of a part, of one step to forty: every row has the bits
+    of its tree alone and of the call before, and rows here and there agree with the definition."""
+    lengths = [6000, 4096, 1024, 1, 2047, 5000, 4100, 17, 8127, 63, 6144, 3000]
+    nodes = [64, 64, 9, 64, 64, 9, 64, 64, 64, 9, 64, 64]
+    s = Setup(dev, fmt, 40, 8, lengths, 33)
+    seq, pos, base, rope, mask = [], [], [], [], []
+    for slot, (n, count) in enumerate(zip(lengths, nodes)):
+        depth, masks = s.ops.TreeRows.masks([-1] + [(7 * i + slot) % (i + 1) for i in range(count - 1)])
+        seq += [slot] * count
+        pos += range(n, n + count)
+        base += [n] * count
+        rope += [n + d for d in depth]
+        mask += masks
+    qkv = s.qkv(len(seq))
+    out = torch.full((len(seq), 5120), float("nan"), device=dev, dtype=BF)
+    attn = s.ops.TreeAttention(40, 8, len(seq), 33, dev, kv_format=fmt)
+    tree = s.ops.TreeRows(_i32(base, dev), _i32(rope, dev), torch.tensor(mask, device=dev))
+    call = lambda at, to: attn(qkv[at], s.cos, s.sin, _i32(seq[at], dev), _i32(pos[at], dev), s.table, s.pages, to,
+                               tree=s.ops.TreeRows(tree.base[at], tree.rope[at], tree.mask[at]))
+    call(slice(0, None), out)
+    again = torch.empty_like(out)
+    call(slice(0, None), again)
+    assert attn.check_status() == 0 and torch.equal(out, again)
+    for slot in range(len(lengths)):
+        first = seq.index(slot)
+        at = slice(first, first + nodes[slot])
+        call(at, again[at].zero_())
+    assert attn.check_status() == 0 and torch.equal(out, again)
+    keep = [seq.index(slot) + i for slot in range(len(lengths)) for i in (0, nodes[slot] - 1)]
+
+    def seen(i, p):
+        node = p - base[keep[i]]
+        bits = torch.tensor([mask[keep[i]][0] >> b & 1 for b in range(64)], device=dev).bool()
+        return (node < 0) | ((node >= 0) & (node < 64) & bits[node.clamp(0, 63)])
+
+    s.check(qkv[keep], [seq[r] for r in keep], [pos[r] for r in keep], out[keep], seen, [rope[r] for r in keep])
+
+
+@pytest.mark.parametrize("rows", [1025, 4096])
+def test_as_many_rows_as_a_call_takes(dev, rows):
+    """Runs of 1, 2, 3 ... rows, and one of the rest that is cut into wide tiles: the plan takes 1024 rows at a time."""
+    counts, left = [], rows - 700
+    while left > 0:
+        counts.append(min(len(counts) % 40 + 1, left))
+        left -= counts[-1]
+    counts.insert(len(counts) // 2, 700)
+    s = Setup(dev, "e4m3", 4, 1, [200 if i % 3 else 0 for i in range(len(counts))], 4)
+    seq = [slot for slot, n in enumerate(counts) for _ in range(n)]
+    pos = [s.lengths[slot] + i for slot, n in enumerate(counts) for i in range(n)]
+    qkv = s.qkv(rows)
+    out = torch.full((rows, 512), float("nan"), device=dev, dtype=BF)
+    attn = s.ops.TreeAttention(4, 1, rows, 4, dev, kv_format="e4m3")
+    attn(qkv, s.cos, s.sin, _i32(seq, dev), _i32(pos, dev), s.table, s.pages, out, longest_run=700)
+    assert attn.check_status() == 0 and bool(torch.isfinite(out.float()).all())
+    keep = sorted({0, 1, 2, 255, 256, 1023, 1024, rows - 1} | set(range(5, rows, 97)))
+    s.check(qkv[keep], [seq[i] for i in keep], [pos[i] for i in keep], out[keep], _causal([pos[i] for i in keep]))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
 def test_captured_and_replayed_with_other_inputs_and_on_another_stream(dev, fmt):
     s = Setup(dev, fmt, 10, 2, [300, 17], 3)
     attn, plain = (s.ops.TreeAttention(10, 2, 8, 3, dev, kv_format=fmt) for _ in range(2))
