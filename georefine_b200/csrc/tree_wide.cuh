@@ -79,7 +79,6 @@ __device__ __forceinline__ void wide_loaders_meet() { asm volatile("bar.sync 1, 
 template <bool F8>
 __global__ void __launch_bounds__(kWideThreads, 2)
 tree_wide_kernel(const TreeArgs a) {
-  step_kernel_entry();
   extern __shared__ unsigned char wide_smem_raw[];
   __shared__ __align__(8) uint64_t bars[11];                 // of even and odd steps: K stored, V stored, S done, P stored, O done; unit set up
   __shared__ uint32_t tmem_at, aborted, next_unit;
@@ -92,8 +91,8 @@ tree_wide_kernel(const TreeArgs a) {
   const uint32_t k_scales = smem + kWideScalesAt, v_scales = k_scales + 2 * kWideMostPart;
   const uint32_t bar_k = smem_u32(&bars[0]), bar_v = smem_u32(&bars[2]), bar_s = smem_u32(&bars[4]), bar_o = smem_u32(&bars[6]), bar_p = smem_u32(&bars[8]),
                  bar_u = smem_u32(&bars[10]);
-  const uint32_t tiles = a.plan[2], units = a.plan[3];
-  if (blockIdx.x >= units) return;
+  // Tensor memory is taken before the kernels behind this one may start: a matrix product among them takes its own as it starts and
+  // keeps it until this kernel is through.
   if (tid == 0) {
     for (uint32_t b = 0; b < 16; b += 8) {
       mbar_init(bar_k + b, 4);
@@ -113,6 +112,12 @@ tree_wide_kernel(const TreeArgs a) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  step_kernel_entry();
+  const uint32_t tiles = a.plan[2], units = a.plan[3];
+  if (blockIdx.x >= units) {
+    if (warp == 4) tmem_dealloc(tmem_at, kWideColumns);
+    return;
+  }
   const uint32_t s_tmem = tmem_at, o_tmem = tmem_at + 128;
   // A wait that runs out is everybody's: nobody waits again, every loop runs to its end, and the status says so.
   auto wait = [&](uint32_t bar, uint32_t step) {
