@@ -68,7 +68,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GRB_ERR_CUDA;
   std::call_once(once[dev], [&] {
     prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_part_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
-    if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem)));
+    if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem<F8>)));
   });
   if (prepared[dev]) return prepared[dev];
   const int sms = device_sm_count(dev);
@@ -79,7 +79,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
   if (int st = launch_step(tree_part_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
   if (a.wide_from) {
-    if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem, stream, a)) return st;
+    if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * (F8 ? 2 : 1)))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
   }
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
   return launch_step(tree_combine_kernel, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a);
@@ -149,7 +149,7 @@ uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pa
   if (!rows || rows > kTreeMaxRows || !nq || !max_pages || format > GRB_KV_E4M3) return 0;
   const uint64_t parts = uint64_t(max_pages) * (format == GRB_KV_E4M3 ? kKvPage / TreePart<true>::kPositions : kKvPage / TreePart<false>::kPositions);
   const uint64_t pairs = uint64_t(rows) * nq;
-  return ((48 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * 2 + 16 + pairs * parts * (kKvDim * 4 + 8);
+  return ((48 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * (format == GRB_KV_E4M3 ? 2 : 4) + 16 + pairs * parts * (kKvDim * 4 + 8);
 }
 
 int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
@@ -207,7 +207,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.q_scale = reinterpret_cast<float*>(a.row_parts + a.rows);
   at += (48 + a.rows * 40ull + pairs * 4 + 255) & ~uint64_t(255);
   a.q = reinterpret_cast<uint16_t*>(at);
-  at += pairs * kKvDim * 2;
+  at += pairs * kKvDim * (f8 ? 2 : 4);
   at += reinterpret_cast<uintptr_t>(at) & 16;                // (the scratch starts on 16 bytes, the parts on 32)
   a.part_acc = reinterpret_cast<float*>(at);
   at += pairs * a.max_parts * kKvDim * 4;

@@ -48,7 +48,8 @@ struct TreeArgs {
   uint32_t mask_words;
   KvTable table;
   KvPagesArgs pages;          // of one layer
-  uint16_t* q;                // scratch: [rows][nq][128]: rotated queries, BF16 or (8-bit caches) FP16 times a power of two
+  uint16_t* q;                // scratch: rotated queries, (8-bit caches) [rows][nq][128] FP16 times a power of two, or [rows][nq][2][128]
+                              // BF16: rounded, and what the rounding left out, rounded
   float* q_scale;             // scratch: [rows][nq]: what a query's scores are multiplied by, in units of log 2
   uint32_t* status;           // scratch: kStatusTimeout where a wait ran out
   int32_t* extent;            // scratch: [rows]: positions up to the last one the row sees
@@ -87,6 +88,9 @@ __device__ __forceinline__ int32_t tree_extent(const TreeArgs& a, uint32_t r) {
 __device__ __forceinline__ bool tree_sees(const TreeArgs& a, uint32_t r, int32_t node) {
   return uint32_t(node) < a.mask_words * 64u && (a.row_mask[r * a.ldm + (node >> 6)] >> (node & 63) & 1u);
 }
+
+// What rounding two values to BF16 (`rounded`) left out of them, rounded to BF16.
+__device__ __forceinline__ uint32_t pack_bf_rest(float a, float b, uint32_t rounded) { return pack_bf(__fsub_rn(a, bf_lo(rounded)), __fsub_rn(b, bf_hi(rounded))); }
 
 // Inclusive scans over the CTA.  Op: sums and maxima of values >= 0 alone (the order is free, and 0 changes nothing).
 template <class T, class Op>
@@ -227,7 +231,7 @@ tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
     }
     if (query) {
       const size_t pair = size_t(row) * a.nq + head;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + pair * kKvDim) + lane;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + pair * (F8 ? kKvDim : 2 * kKvDim)) + lane;
       if constexpr (F8) {
         // FP16 times a power of two that brings the largest component to [2^14, 2^15): 11 bits where BF16 has 8, and what falls
         // below FP16's normal range is 2^-28 of the largest.
@@ -244,8 +248,11 @@ tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
         dst[32] = *reinterpret_cast<const uint32_t*>(&h1);
         if (lane == 0) a.q_scale[pair] = fine ? __fmul_rn(log2_scale, __uint_as_float(uint32_t(127 + e) << 23)) : __uint_as_float(0x7FC00000u);
       } else {
-        dst[0] = pack_bf(x[0], x[1]);
-        dst[32] = pack_bf(x[2], x[3]);
+        const uint32_t h0 = pack_bf(x[0], x[1]), h1 = pack_bf(x[2], x[3]);
+        dst[0] = h0;
+        dst[32] = h1;
+        dst[64] = pack_bf_rest(x[0], x[1], h0);
+        dst[96] = pack_bf_rest(x[2], x[3], h1);
         if (lane == 0) a.q_scale[pair] = log2_scale;
       }
       continue;
@@ -457,6 +464,20 @@ tree_part_kernel(const TreeArgs a) {
   tree_request_v<F8>(a, smem, t, tid);
   uint32_t qa[8][4];
   float scale0 = 0.f, scale1 = 0.f;
+  // BF16: the queries of a unit, or what their rounding left out (half 1)
+  auto ask_bf = [&](const TreeUnit& n, uint32_t half, uint32_t (&x)[8][4]) {
+    const uint32_t used = n.rows * a.group, rl0 = m0 / a.group, rl1 = m1 / a.group;
+    const bool ok0 = m0 < used, ok1 = m1 < used;
+    const uint16_t* s0 = a.q + (2 * (ok0 ? size_t(n.first + rl0) * a.nq + n.kvh * a.group + (m0 - rl0 * a.group) : 0) + half) * kKvDim + c * 2;
+    const uint16_t* s1 = a.q + (2 * (ok1 ? size_t(n.first + rl1) * a.nq + n.kvh * a.group + (m1 - rl1 * a.group) : 0) + half) * kKvDim + c * 2;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      x[k][0] = ok0 ? *reinterpret_cast<const uint32_t*>(s0 + 16 * k) : 0u;
+      x[k][1] = ok1 ? *reinterpret_cast<const uint32_t*>(s1 + 16 * k) : 0u;
+      x[k][2] = ok0 ? *reinterpret_cast<const uint32_t*>(s0 + 16 * k + 8) : 0u;
+      x[k][3] = ok1 ? *reinterpret_cast<const uint32_t*>(s1 + 16 * k + 8) : 0u;
+    }
+  };
   // the queries of a unit as A fragments, MMA row m = (row of the tile) * group + (query head of the group), and their scales
   auto ask_q = [&](const TreeUnit& n) {
     const uint32_t used = n.rows * a.group, rl0 = m0 / a.group, rl1 = m1 / a.group;
@@ -478,15 +499,7 @@ tree_part_kernel(const TreeArgs a) {
         }
       }
     } else {
-      const uint16_t* s0 = a.q + q0 * kKvDim + c * 2;
-      const uint16_t* s1 = a.q + q1 * kKvDim + c * 2;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        qa[k][0] = ok0 ? *reinterpret_cast<const uint32_t*>(s0 + 16 * k) : 0u;
-        qa[k][1] = ok1 ? *reinterpret_cast<const uint32_t*>(s1 + 16 * k) : 0u;
-        qa[k][2] = ok0 ? *reinterpret_cast<const uint32_t*>(s0 + 16 * k + 8) : 0u;
-        qa[k][3] = ok1 ? *reinterpret_cast<const uint32_t*>(s1 + 16 * k + 8) : 0u;
-      }
+      ask_bf(n, 0, qa);
     }
     scale0 = ok0 ? a.q_scale[q0] : 0.f;
     scale1 = ok1 ? a.q_scale[q1] : 0.f;
@@ -519,6 +532,8 @@ tree_part_kernel(const TreeArgs a) {
     const int32_t seen0 = ok0 ? min(a.row_base ? base0 : a.extent[row0], a.extent[row0]) - t.start : 0;
     const int32_t seen1 = ok1 ? min(a.row_base ? base1 : a.extent[row1], a.extent[row1]) - t.start : 0;
     // whether some row of the tile does not see the whole part
+    uint32_t rest[F8 ? 1 : 8][4];     // BF16: of the queries; needed for the scores alone, so asked for here
+    if constexpr (!F8) ask_bf(t, 1, rest);
     const bool holes = __syncthreads_or((ok0 && seen0 < int32_t(P::kPositions)) || (ok1 && seen1 < int32_t(P::kPositions)));
     if (!F8 && holes) {       // values that are not finite would reach, as 0 * infinity, the rows that do not see them
       if (tid < P::kPositions / 32) bad_sm[tid] = 0u;
@@ -580,6 +595,8 @@ tree_part_kernel(const TreeArgs a) {
         for (int nt = 0; nt < NT; ++nt) {
           uint32_t b[4];
           ldsm_x4(smem + P::offset(p_warp + 8 * nt + (lane & 7u), 4 * kq + (lane >> 3)), b);
+          mma_bf16_16816(sc[nt], rest[2 * kq], b[0], b[1]);
+          mma_bf16_16816(sc[nt], rest[2 * kq + 1], b[2], b[3]);
           mma_bf16_16816(sc[nt], qa[2 * kq], b[0], b[1]);
           mma_bf16_16816(sc[nt], qa[2 * kq + 1], b[2], b[3]);
         }
@@ -632,7 +649,7 @@ tree_part_kernel(const TreeArgs a) {
           if (n == nt) { sc[n][0] = x[0]; sc[n][1] = x[1]; sc[n][2] = x[2]; sc[n][3] = x[3]; }
       }
     }
-    uint32_t pa[NT / 2][4];
+    uint32_t pa[NT / 2][4], pr[F8 ? 1 : NT / 2][4];       // weights; BF16: and what their rounding left out
     float l0 = 0.f, l1 = 0.f;
     // one of the lane's two rows: its maximum over the warp's positions, its weights as A fragments, their sum
     auto weigh = [&](int r, float& mx, float& l) {
@@ -652,6 +669,7 @@ tree_part_kernel(const TreeArgs a) {
         } else {
           l = __fadd_rn(l, __fadd_rn(p0, p1));
           pa[nt >> 1][(nt & 1) * 2 + r] = pack_bf(p0, p1);
+          pr[nt >> 1][(nt & 1) * 2 + r] = pack_bf_rest(p0, p1, pa[nt >> 1][(nt & 1) * 2 + r]);
         }
       }
       l = __fadd_rn(l, __shfl_xor_sync(0xFFFFFFFFu, l, 1));
@@ -662,7 +680,10 @@ tree_part_kernel(const TreeArgs a) {
       weigh(1, mx1, l1);
     } else {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) pa[nt >> 1][(nt & 1) * 2 + 1] = 0u;
+      for (int nt = 0; nt < NT; ++nt) {
+        pa[nt >> 1][(nt & 1) * 2 + 1] = 0u;
+        if constexpr (!F8) pr[nt >> 1][(nt & 1) * 2 + 1] = 0u;
+      }
     }
     cp_async_wait<0>();
     __syncthreads();                                // V is in shared memory, and every warp is done with K
@@ -684,6 +705,8 @@ tree_part_kernel(const TreeArgs a) {
         for (int dn = 0; dn < 8; ++dn) {
           uint32_t b[4];
           ldsm_x4_trans(vs + P::offset(vrow, 2 * dn + (lane >> 4)), b);
+          mma_bf16_16816(o[2 * dn], pr[s], b[0], b[1]);
+          mma_bf16_16816(o[2 * dn + 1], pr[s], b[2], b[3]);
           mma_bf16_16816(o[2 * dn], pa[s], b[0], b[1]);
           mma_bf16_16816(o[2 * dn + 1], pa[s], b[2], b[3]);
         }

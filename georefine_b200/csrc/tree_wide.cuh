@@ -28,7 +28,9 @@ constexpr uint32_t kWideStep = 64;               // positions of a step
 constexpr uint32_t kWideOperand = 32768;         // Q: two halves of 64 dimensions, 128 rows of 128 bytes each; K or V of two steps
 constexpr uint32_t kWideStage = kWideOperand / 2;        // K or V of a step: two halves of 64 dimensions, 64 rows each
 constexpr uint32_t kWideScalesAt = 3 * kWideOperand;
-constexpr uint32_t kWideSmem = 3 * kWideOperand + 2 * 2 * kWideMostPart + 1024;   // operands, FP16 scales of a chunk's K and V, alignment
+// operands; FP16 scales of a chunk's K and V (8 bits) or what rounding left out of Q (BF16); alignment
+template <bool F8>
+constexpr uint32_t kWideSmem = 3 * kWideOperand + (F8 ? 2 * 2 * kWideMostPart : kWideOperand) + 1024;
 constexpr uint32_t kWideColumns = 256;           // tensor memory: S of two steps (and P over it), O
 
 // Byte offset of 16-byte piece `piece` (0..15) of row `row` of an operand of ROWS rows: 128-byte swizzle in each half.
@@ -189,17 +191,18 @@ tree_wide_kernel(const TreeArgs a) {
       // the queries, sixteen lanes a row, once the scores of the unit before are done
       auto queries = [&]() {
         if (step0) wait2(bar_s, step0 - 1);
+        constexpr uint32_t kHalves = F8 ? 1 : 2;
 #pragma unroll 1
-        for (int part = 0; part < 4; ++part) {
+        for (uint32_t part = 0; part < 4 * kHalves; ++part) {
           uint4 x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t m = (lt >> 4) + (4 * part + i) * 8, r = m / a.group;
-            x[i] = m < used ? reinterpret_cast<const uint4*>(a.q + ((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kKvDim)[lt & 15u]
+          for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t m = (lt >> 4) + (4 * (part & 3u) + i) * 8, r = m / a.group;
+            x[i] = m < used ? reinterpret_cast<const uint4*>(a.q + (((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kHalves + (part >> 2)) * kKvDim)[lt & 15u]
                             : make_uint4(0u, 0u, 0u, 0u);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sts128(qs + wide_offset<kWideTile>((lt >> 4) + (4 * part + i) * 8, lt & 15u), x[i]);
+          for (uint32_t i = 0; i < 4; ++i) sts128((part & 4u ? smem + kWideScalesAt : qs) + wide_offset<kWideTile>((lt >> 4) + (4 * (part & 3u) + i) * 8, lt & 15u), x[i]);
         }
       };
       // everything is there: tells the weights' warps, who have all looked at the unit before once its first step's values have been
@@ -394,9 +397,11 @@ tree_wide_kernel(const TreeArgs a) {
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int d = 0; d < 8; ++d)                          // 16 dimensions each
-          umma_bf16(s_tmem + (g & 1u) * kWideStep, umma_desc_sw128(qs + (d >> 2) * (kWideOperand / 2) + (d & 3) * 32),
-                    umma_desc_sw128(ks + (g & 1u) * kWideStage + (d >> 2) * (kWideStage / 2) + (d & 3) * 32), kIdescS, d > 0);
+        for (int d = 0; d < (F8 ? 8 : 16); ++d) {            // 16 dimensions each; BF16: of what Q's rounding left out, then of Q
+          const uint32_t q = F8 || d >= 8 ? qs : smem + kWideScalesAt, half = (d >> 2 & 1) * (kWideOperand / 2), k16 = (d & 3) * 32;
+          umma_bf16(s_tmem + (g & 1u) * kWideStep, umma_desc_sw128(q + half + k16),
+                    umma_desc_sw128(ks + (g & 1u) * kWideStage + half / 2 + k16), kIdescS, d > 0);
+        }
         umma_commit(bar_s + 8 * (g & 1u));
       }
       __syncwarp();
@@ -414,8 +419,8 @@ tree_wide_kernel(const TreeArgs a) {
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int d = 0; d < 4; ++d)                        // 16 positions each
-            umma_bf16_ts(o_tmem, s_tmem + (g & 1u) * kWideStep + 8 * d, wide_desc_v(vs + (g & 1u) * kWideStage + 2048 * d), kIdesc | (1u << 16), j > 0 || d > 0);
+          for (int d = 0; d < (F8 ? 4 : 8); ++d)             // 16 positions each; BF16: then of what the weights' rounding left out
+            umma_bf16_ts(o_tmem, s_tmem + (g & 1u) * kWideStep + 8 * d, wide_desc_v(vs + (g & 1u) * kWideStage + 2048 * (d & 3)), kIdesc | (1u << 16), j > 0 || d > 0);
           umma_commit(bar_o + 8 * (g & 1u));
         }
         __syncwarp();
@@ -517,7 +522,7 @@ tree_wide_kernel(const TreeArgs a) {
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          uint32_t p[16];
+          uint32_t p[16], rest[F8 ? 1 : 16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float2 e = fma2(make_float2(__uint_as_float(x[w][2 * i]), __uint_as_float(x[w][2 * i + 1])), scale2, low2);
@@ -529,9 +534,11 @@ tree_wide_kernel(const TreeArgs a) {
               p[i] = *reinterpret_cast<const uint32_t*>(&h);
             } else {
               p[i] = pack_bf(e.x, e.y);
+              rest[i] = pack_bf_rest(e.x, e.y, p[i]);
             }
           }
           tmem_st16(s_at + 16 * w, p);                       // (over scores that have been read)
+          if constexpr (!F8) tmem_st16(s_at + 32 + 16 * w, rest);
         }
         sum = add2(sum, add2(sums[0], sums[1]));
         if (poisoned) sum.x = __uint_as_float(0x7FC00000u);

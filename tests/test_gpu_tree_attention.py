@@ -56,7 +56,7 @@ class Setup:
 
     def check(self, qkv, seq, pos, out, seen, rope=None):
         """Every row against the definition over what the cache holds after the call; ``seen(row, positions)`` -> bool tensor."""
-        half = {"bf16": 2.0 ** -8, "e4m3": 2.0 ** -11}[self.fmt]
+        half = {"bf16": 2.0 ** -16, "e4m3": 2.0 ** -11}[self.fmt]     # (BF16: rounded twice, the second time what the first left out)
         for r, (s, p) in enumerate(zip(seq, pos)):
             if s < 0:
                 continue
