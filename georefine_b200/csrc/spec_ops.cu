@@ -79,7 +79,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
   if (int st = launch_step(tree_part_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
   if (a.wide_from) {
-    if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * (F8 ? 2 : 1)))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
+    if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
   }
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
   return launch_step(tree_combine_kernel, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a);

@@ -9,10 +9,14 @@
 // S of two steps are held, so a step's scores are computed while the step before is weighed, and the loaders set the next unit up
 // while this one ends.  256 columns of tensor memory and 105 KB of shared memory leave room for two CTAs on an SM.
 //
-// 16 trees of 64 nodes behind 8192 positions, 40 query heads of 8 kv heads: 317 us in 8 bits, 291 in BF16 (all launches), 0.42 PFLOP/s
-// - one step at a time and barriers between units: 438; steps of 128 with one S, the products issued by a weights' warp: 340.
-// What bounds it now is the loaders' chain of a step, 2500 cycles in which a CTA waits for a stage, converts 64 positions of K and
-// of V and asks for the next (without the loads 266 us; without the exponentials as long as with them).
+// 16 trees of 64 nodes behind 8192 positions, 40 query heads of 8 kv heads, all launches: 317 us in 8 bits, 0.42 PFLOP/s (one step
+// at a time and barriers between units: 438; steps of 128 with one S, the products issued by a weights' warp: 340).  What bounds it
+// is the loaders' chain of a step, 2500 cycles in which a CTA waits for a stage, converts 64 positions of K and of V and asks for
+// the next (without the loads 266 us; without the exponentials as long as with them).
+//
+// BF16: Q and the weights go into the products as two terms, what rounding to BF16 leaves and what it leaves out, so that the error
+// is the result's rounding (one term each: twice that).  416 us for the trees above, 291 with one term; with four stages of K and V
+// instead of three, and therefore one CTA an SM, 558.
 //
 // FP16 weights reach down to 2^-24 and V's entries to 2^-24 times a code of 1: both are scaled up as far as FP16 goes (weights at
 // most 2^15, values at most 57344), so what falls out at the bottom is 2^-39 of the largest - beyond what the 32-bit sums keep.
@@ -27,10 +31,6 @@ constexpr uint32_t kWideTile = 128;              // rows of a tile
 constexpr uint32_t kWideStep = 64;               // positions of a step
 constexpr uint32_t kWideOperand = 32768;         // Q: two halves of 64 dimensions, 128 rows of 128 bytes each; K or V of two steps
 constexpr uint32_t kWideStage = kWideOperand / 2;        // K or V of a step: two halves of 64 dimensions, 64 rows each
-constexpr uint32_t kWideScalesAt = 3 * kWideOperand;
-// operands; FP16 scales of a chunk's K and V (8 bits) or what rounding left out of Q (BF16); alignment
-template <bool F8>
-constexpr uint32_t kWideSmem = 3 * kWideOperand + (F8 ? 2 * 2 * kWideMostPart : kWideOperand) + 1024;
 constexpr uint32_t kWideColumns = 256;           // tensor memory: S of two steps (and P over it), O
 
 // Byte offset of 16-byte piece `piece` (0..15) of row `row` of an operand of ROWS rows: 128-byte swizzle in each half.
@@ -76,23 +76,34 @@ struct WideInfo {
   int32_t start;
   uint32_t k_top, v_top, any_bad;  // largest exponent bytes of the chunk; whether `bad` has bits
 };
+// Shared memory beside the operands.
+struct WideShared {
+  uint64_t bars[11];               // of even and odd steps: K stored, V stored, S done, O done, P stored; unit set up
+  WideInfo info[2];                // of a unit and the next
+  uint32_t bad[2][kWideMostPart / 32];     // positions of the chunk whose key or value is not a number
+  int32_t pages[2][kWideMostPart / kWideStep];     // page of each step; -1: none
+  uint32_t tmem_at, aborted, next_unit;
+  uint32_t k_top, v_top, any_bad, any_absent;      // the loaders' own, while they set a unit up
+};
+static_assert(sizeof(WideShared) <= 1024, "two CTAs of the BF16 kernel take all of an SM's shared memory");
+// Operands from 1024 on.  8 bits: Q, two stages of K, two of V, FP16 scales of a chunk's K and V.  BF16: Q, what its rounding left
+// out, a ring of three stages that K and V take in turn (K of step g where V of g - 2 was, V of g where K of g - 1 was).
+template <bool F8>
+constexpr uint32_t kWideSmem = 1024 + (F8 ? 3 * kWideOperand + 2 * 2 * kWideMostPart : 2 * kWideOperand + 3 * kWideStage);
 __device__ __forceinline__ void wide_loaders_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <bool F8>
 __global__ void __launch_bounds__(kWideThreads, 2)
 tree_wide_kernel(const TreeArgs a) {
-  extern __shared__ unsigned char wide_smem_raw[];
-  __shared__ __align__(8) uint64_t bars[11];                 // of even and odd steps: K stored, V stored, S done, P stored, O done; unit set up
-  __shared__ uint32_t tmem_at, aborted, next_unit;
-  __shared__ uint32_t k_top, v_top, any_bad, any_absent;     // the loaders' own, while they set a unit up
-  __shared__ WideInfo info[2];                               // of a unit and the next
-  __shared__ int64_t entries[2][kWideMostPart / kWideStep];  // entry (of the layer) of each step's first position; -1: no page
-  __shared__ uint32_t bad[2][kWideMostPart / 32];            // positions of the chunk whose key or value is not a number
+  extern __shared__ __align__(1024) unsigned char wide_smem[];
+  WideShared& sm = *reinterpret_cast<WideShared*>(wide_smem);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint32_t smem = (smem_u32(wide_smem_raw) + 1023u) & ~1023u, qs = smem, ks = smem + kWideOperand, vs = smem + 2 * kWideOperand;
-  const uint32_t k_scales = smem + kWideScalesAt, v_scales = k_scales + 2 * kWideMostPart;
-  const uint32_t bar_k = smem_u32(&bars[0]), bar_v = smem_u32(&bars[2]), bar_s = smem_u32(&bars[4]), bar_o = smem_u32(&bars[6]), bar_p = smem_u32(&bars[8]),
-                 bar_u = smem_u32(&bars[10]);
+  const uint32_t qs = smem_u32(wide_smem) + 1024, rs = qs + kWideOperand, ks = F8 ? rs : rs + kWideOperand, vs = ks + kWideOperand;
+  const uint32_t k_scales = vs + kWideOperand, v_scales = k_scales + 2 * kWideMostPart;
+  const uint32_t bar_k = smem_u32(&sm.bars[0]), bar_v = smem_u32(&sm.bars[2]), bar_s = smem_u32(&sm.bars[4]), bar_o = smem_u32(&sm.bars[6]),
+                 bar_p = smem_u32(&sm.bars[8]), bar_u = smem_u32(&sm.bars[10]);
+  auto k_stage = [&](uint32_t g) { return ks + (F8 ? g & 1u : 2 * g % 3) * kWideStage; };
+  auto v_stage = [&](uint32_t g) { return F8 ? vs + (g & 1u) * kWideStage : ks + (2 * g + 1) % 3 * kWideStage; };
   // Tensor memory is taken before the kernels behind this one may start: a matrix product among them takes its own as it starts and
   // keeps it until this kernel is through.
   if (tid == 0) {
@@ -105,10 +116,10 @@ tree_wide_kernel(const TreeArgs a) {
     }
     mbar_init(bar_u, 4);
     mbar_fence_init();
-    aborted = 0u;
+    sm.aborted = 0u;
   }
   if (warp == 4) {
-    tmem_alloc(smem_u32(&tmem_at), kWideColumns);
+    tmem_alloc(smem_u32(&sm.tmem_at), kWideColumns);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -117,15 +128,15 @@ tree_wide_kernel(const TreeArgs a) {
   step_kernel_entry();
   const uint32_t tiles = a.plan[2], units = a.plan[3];
   if (blockIdx.x >= units) {
-    if (warp == 4) tmem_dealloc(tmem_at, kWideColumns);
+    if (warp == 4) tmem_dealloc(sm.tmem_at, kWideColumns);
     return;
   }
-  const uint32_t s_tmem = tmem_at, o_tmem = tmem_at + 128;
+  const uint32_t s_tmem = sm.tmem_at, o_tmem = sm.tmem_at + 128;
   // A wait that runs out is everybody's: nobody waits again, every loop runs to its end, and the status says so.
   auto wait = [&](uint32_t bar, uint32_t step) {
-    if (mbar_test_wait(bar, step & 1u) || *reinterpret_cast<volatile uint32_t*>(&aborted)) return;
+    if (mbar_test_wait(bar, step & 1u) || *reinterpret_cast<volatile uint32_t*>(&sm.aborted)) return;
     if (!mbar_wait(bar, step & 1u, false)) {
-      *reinterpret_cast<volatile uint32_t*>(&aborted) = 1u;
+      *reinterpret_cast<volatile uint32_t*>(&sm.aborted) = 1u;
       atomicOr(a.status, kStatusTimeout);
     }
   };
@@ -133,9 +144,11 @@ tree_wide_kernel(const TreeArgs a) {
   // Units differ in length, so a CTA takes the next one when it is through with its own (who computes a unit changes nothing in it);
   // its loaders set the next one up while the last step of this one is multiplied and its result stored.
   uint32_t step0 = 0;                                        // steps this CTA has taken before the unit
-  // registers, of the 240 that three threads of the launch have: 112 for the weights, 88 for loading, 40 for the products
+  // registers, of the 240 that three threads of the launch have: 112 for the weights, 88 for loading, 40 for the products; BF16, whose
+  // loaders hold nothing: 128, 72, 40
   if (warp >= 4 && warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ---- loading ------------------------------------------------------------------------------------------------
     const uint32_t lt = tid - 128;
     uint32_t tile = 0, slot = 0, steps_before = 0;
@@ -157,19 +170,19 @@ tree_wide_kernel(const TreeArgs a) {
       t.seq = a.row_seq[t.first];
       t.start = int32_t(t.part * part_positions);
       const uint32_t used = t.rows * a.group;
-      if (lt < kWideMostPart / 32) bad[slot][lt] = 0u;
+      if (lt < kWideMostPart / 32) sm.bad[slot][lt] = 0u;
       if (lt == 0) {
-        k_top = v_top = any_bad = 0u;
-        next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
+        sm.k_top = sm.v_top = sm.any_bad = 0u;
+        sm.next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
       }
       if (warp == 4) {                                       // (a step's positions lie in one page)
         int64_t place = 0;
         if (lane < part_positions / kWideStep) {
           place = kv_place(a.table, t.seq, t.start + int32_t(lane * kWideStep));
-          entries[slot][lane] = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
+          sm.pages[slot][lane] = place < 0 ? -1 : int32_t(place / kKvPage);
         }
         const bool absent = __any_sync(0xFFFFFFFFu, place < 0);
-        if (lane == 0) any_absent = absent;
+        if (lane == 0) sm.any_absent = absent;
       }
       int32_t extent = 0, all = 0x7FFFFFFF;
       for (uint32_t i = lane; i < t.rows; i += 32) {
@@ -185,9 +198,13 @@ tree_wide_kernel(const TreeArgs a) {
       t.extent = min(extent, t.start + int32_t(part_positions));
       steps = (uint32_t(t.extent - t.start) + kWideStep - 1) / kWideStep;       // (a unit has a position at least)
       wide_loaders_meet();                                   // (the scales of the unit before have been read, too)
-      u = next_unit;
-      plain = any_absent ? 0u : all >= t.extent ? steps : uint32_t(max(all - t.start, 0)) / kWideStep;
-      const int64_t* const at = entries[slot];
+      u = sm.next_unit;
+      plain = sm.any_absent ? 0u : all >= t.extent ? steps : uint32_t(max(all - t.start, 0)) / kWideStep;
+      // entry (of the layer) of step j's first position; -1: none
+      auto entry_of = [&](uint32_t j) -> int64_t {
+        const int32_t page = sm.pages[slot][j];
+        return page < 0 ? -1 : int64_t(kv_entry(int64_t(page) * kKvPage + (uint32_t(t.start) + j * kWideStep) % kKvPage, a.nkv, t.kvh));
+      };
       // the queries, sixteen lanes a row, once the scores of the unit before are done
       auto queries = [&]() {
         if (step0) wait2(bar_s, step0 - 1);
@@ -202,13 +219,13 @@ tree_wide_kernel(const TreeArgs a) {
                             : make_uint4(0u, 0u, 0u, 0u);
           }
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) sts128((part & 4u ? smem + kWideScalesAt : qs) + wide_offset<kWideTile>((lt >> 4) + (4 * (part & 3u) + i) * 8, lt & 15u), x[i]);
+          for (uint32_t i = 0; i < 4; ++i) sts128((part & 4u ? rs : qs) + wide_offset<kWideTile>((lt >> 4) + (4 * (part & 3u) + i) * 8, lt & 15u), x[i]);
         }
       };
       // everything is there: tells the weights' warps, who have all looked at the unit before once its first step's values have been
       // used (storing the third step's waited for that)
       auto publish = [&]() {
-        if (lt == 0) info[slot] = WideInfo{1u, t.first, t.rows, t.kvh, t.part, steps, plain, t.start, k_top, v_top, any_bad};
+        if (lt == 0) sm.info[slot] = WideInfo{1u, t.first, t.rows, t.kvh, t.part, steps, plain, t.start, sm.k_top, sm.v_top, sm.any_bad};
         if (steps_before && steps_before <= 2) wait2(bar_o, step0 - 1);
         fence_proxy_async_smem();
         __syncwarp();
@@ -220,7 +237,7 @@ tree_wide_kernel(const TreeArgs a) {
         const uint32_t row0 = lt >> 2;
         uint4 k[4], v[4];
         auto ask = [&](uint4 (&x)[4], const void* pool, uint32_t j) {
-          const int64_t entry = j < steps ? at[j] : -1;
+          const int64_t entry = j < steps ? entry_of(j) : -1;
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideStep);
           const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim) + row0 * 8 + (lt & 3u);
 #pragma unroll
@@ -253,7 +270,7 @@ tree_wide_kernel(const TreeArgs a) {
         uint32_t w[2][4];
 #pragma unroll
         for (int of_v = 0; of_v < 2; ++of_v) {
-          const int64_t entry = lt < steps * 4 ? at[lt >> 2] : -1;
+          const int64_t entry = lt < steps * 4 ? entry_of(lt >> 2) : -1;
           const uint4 x = entry >= 0 ? *reinterpret_cast<const uint4*>((of_v ? a.pages.v_exp : a.pages.k_exp) + entry + (lt & 3u) * 16) : make_uint4(0u, 0u, 0u, 0u);
           w[of_v][0] = x.x; w[of_v][1] = x.y; w[of_v][2] = x.z; w[of_v][3] = x.w;
         }
@@ -270,16 +287,16 @@ tree_wide_kernel(const TreeArgs a) {
           }
 #pragma unroll
           for (int off = 16; off; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-          if (lane == 0 && top) atomicMax(of_v ? &v_top : &k_top, top);
+          if (lane == 0 && top) atomicMax(of_v ? &sm.v_top : &sm.k_top, top);
         }
         if (none) {
-          atomicOr(&bad[slot][lt >> 1], none << (16 * (lt & 1u)));
-          any_bad = 1u;
+          atomicOr(&sm.bad[slot][lt >> 1], none << (16 * (lt & 1u)));
+          sm.any_bad = 1u;
         }
         wide_loaders_meet();
 #pragma unroll
         for (int of_v = 0; of_v < 2; ++of_v) {
-          const uint32_t top = of_v ? v_top : k_top;
+          const uint32_t top = of_v ? sm.v_top : sm.k_top;
           uint32_t h[8];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -297,15 +314,14 @@ tree_wide_kernel(const TreeArgs a) {
         wide_loaders_meet();                                 // the scales are complete
         for (uint32_t j = 0; j < steps; ++j) {
           const uint32_t g = step0 + j;
-          const uint32_t stage = (g & 1u) * kWideStage;
           if (g > 1) wait2(bar_s, g - 2);                    // scores have been taken from the stage's K
-          store(k, ks + stage, k_scales, j, false);
+          store(k, k_stage(g), k_scales, j, false);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_k + 8 * (g & 1u));
           ask(k, a.pages.k, j + 1);
           if (g > 1) wait2(bar_o, g - 2);                    // the stage's values have been used
-          store(v, vs + stage, v_scales, j, j >= plain);
+          store(v, v_stage(g), v_scales, j, j >= plain);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_v + 8 * (g & 1u));
@@ -313,7 +329,7 @@ tree_wide_kernel(const TreeArgs a) {
         }
       } else {
         auto ask = [&](uint32_t dst, const void* pool, uint32_t j) {
-          const int64_t entry = at[j];
+          const int64_t entry = entry_of(j);
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideStep);
           const uint8_t* src = static_cast<const uint8_t*>(pool) + (entry < 0 ? 0 : entry) * kKvDim * 2;
 #pragma unroll
@@ -327,53 +343,55 @@ tree_wide_kernel(const TreeArgs a) {
         wide_loaders_meet();                                 // (the unit after this one and its pages are known to all)
         queries();
         publish();
-        // (a step's copies are on their way while the step before's land; behind the last one, groups of none keep the count)
-        for (uint32_t j = 0; j <= steps; ++j) {
-          const uint32_t g = step0 + j, stage = (g & 1u) * kWideStage, before = kWideStage - stage;
-          if (j < steps) {
-            if (g > 1) wait2(bar_s, g - 2);
-            ask(ks + stage, a.pages.k, j);
-          } else {
-            cp_async_commit();
+        // a step's values that are not finite would reach, as 0 * infinity, rows that do not see them
+        auto values = [&](uint32_t j) {
+          if (j < plain) return;
+          uint32_t mine = 0;                               // bit i: of the thread's piece i
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t c = lt + 128 * i, at = v_stage(step0 + j) + wide_offset<kWideStep>(c >> 4, c & 15u);
+            const uint4 x = lds128(at);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool b = false;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) b = b || (w[q] & 0x7F80u) == 0x7F80u || (w[q] & 0x7F800000u) == 0x7F800000u;
+            if (b) sts128(at, make_uint4(0u, 0u, 0u, 0u));
+            mine |= uint32_t(b) << i;
           }
+          // piece i of this warp's lanes lies in positions 8 i + 2 (warp - 4) and the next
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t m = __ballot_sync(0xFFFFFFFFu, mine >> i & 1u);
+            const uint32_t p = 8 * i + 2 * (warp - 4);
+            if (lane == 0 && m) atomicOr(&sm.bad[slot][j * (kWideStep / 32) + (p >> 5)], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
+          }
+        };
+        // (a step's copies are on their way while the step before's land; behind the last one, a group of none keeps the count)
+        for (uint32_t j = 0; j <= steps; ++j) {
+          const uint32_t g = step0 + j;
           if (j) {
-            cp_async_wait<2>();
+            cp_async_wait<1>();
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_k + 8 * (~g & 1u));
           }
           if (j < steps) {
             if (g > 1) wait2(bar_o, g - 2);
-            ask(vs + stage, a.pages.v, j);
+            ask(k_stage(g), a.pages.k, j);
           } else {
             cp_async_commit();
           }
-          if (!j) continue;
-          cp_async_wait<2>();
-          if (j > plain) {                                   // values that are not finite would reach, as 0 * infinity, rows that do not see them
-            uint32_t mine = 0;                               // bit i: of the thread's piece i
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t c = lt + 128 * i, at = vs + before + wide_offset<kWideStep>(c >> 4, c & 15u);
-              const uint4 x = lds128(at);
-              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-              bool b = false;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) b = b || (w[q] & 0x7F80u) == 0x7F80u || (w[q] & 0x7F800000u) == 0x7F800000u;
-              if (b) sts128(at, make_uint4(0u, 0u, 0u, 0u));
-              mine |= uint32_t(b) << i;
-            }
-            // piece i of this warp's lanes lies in positions 8 i + 2 (warp - 4) and the next
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t m = __ballot_sync(0xFFFFFFFFu, mine >> i & 1u);
-              const uint32_t p = 8 * i + 2 * (warp - 4);
-              if (lane == 0 && m) atomicOr(&bad[slot][(j - 1) * (kWideStep / 32) + (p >> 5)], (uint32_t((m & 0xFFFFu) != 0) | uint32_t((m >> 16) != 0) << 1) << (p & 31u));
-            }
+          if (j) {
+            cp_async_wait<1>();
+            values(j - 1);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_v + 8 * (~g & 1u));
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_v + 8 * (~g & 1u));
+          if (j < steps) {
+            if (g > 0) wait2(bar_s, g - 1);
+            ask(v_stage(g), a.pages.v, j);
+          }
         }
       }
       if (steps == 1 && step0) wait2(bar_o, step0 - 1);      // (the unit before is over, whose tables the next one but one overwrites)
@@ -381,7 +399,7 @@ tree_wide_kernel(const TreeArgs a) {
       steps_before = steps;
     }
     // no unit is left
-    if (lt == 0) info[slot].valid = 0u;
+    if (lt == 0) sm.info[slot].valid = 0u;
     if (steps_before && steps_before <= 2) wait2(bar_o, step0 - 1);
     __syncwarp();
     if (lane == 0) mbar_arrive(bar_u);
@@ -398,9 +416,9 @@ tree_wide_kernel(const TreeArgs a) {
       if (elect_one()) {
 #pragma unroll
         for (int d = 0; d < (F8 ? 8 : 16); ++d) {            // 16 dimensions each; BF16: of what Q's rounding left out, then of Q
-          const uint32_t q = F8 || d >= 8 ? qs : smem + kWideScalesAt, half = (d >> 2 & 1) * (kWideOperand / 2), k16 = (d & 3) * 32;
+          const uint32_t q = F8 || d >= 8 ? qs : rs, half = (d >> 2 & 1) * (kWideOperand / 2), k16 = (d & 3) * 32;
           umma_bf16(s_tmem + (g & 1u) * kWideStep, umma_desc_sw128(q + half + k16),
-                    umma_desc_sw128(ks + (g & 1u) * kWideStage + half / 2 + k16), kIdescS, d > 0);
+                    umma_desc_sw128(k_stage(g) + half / 2 + k16), kIdescS, d > 0);
         }
         umma_commit(bar_s + 8 * (g & 1u));
       }
@@ -408,8 +426,8 @@ tree_wide_kernel(const TreeArgs a) {
     };
     for (uint32_t n = 0; warp == 8; ++n) {
       wait(bar_u, n);
-      if (!info[n & 1u].valid || *reinterpret_cast<volatile uint32_t*>(&aborted)) break;
-      const uint32_t steps = info[n & 1u].steps;
+      if (!sm.info[n & 1u].valid || *reinterpret_cast<volatile uint32_t*>(&sm.aborted)) break;
+      const uint32_t steps = sm.info[n & 1u].steps;
       scores(step0);
       for (uint32_t j = 0; j < steps; ++j) {
         const uint32_t g = step0 + j;
@@ -420,7 +438,7 @@ tree_wide_kernel(const TreeArgs a) {
         if (elect_one()) {
 #pragma unroll
           for (int d = 0; d < (F8 ? 4 : 8); ++d)             // 16 positions each; BF16: then of what the weights' rounding left out
-            umma_bf16_ts(o_tmem, s_tmem + (g & 1u) * kWideStep + 8 * d, wide_desc_v(vs + (g & 1u) * kWideStage + 2048 * (d & 3)), kIdesc | (1u << 16), j > 0 || d > 0);
+            umma_bf16_ts(o_tmem, s_tmem + (g & 1u) * kWideStep + 8 * d, wide_desc_v(v_stage(g) + 2048 * (d & 3)), kIdesc | (1u << 16), j > 0 || d > 0);
           umma_commit(bar_o + 8 * (g & 1u));
         }
         __syncwarp();
@@ -428,15 +446,16 @@ tree_wide_kernel(const TreeArgs a) {
       step0 += steps;
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     // ---- weights: thread = row m of the tile, lane m of tensor memory ------------------------------------------------
     constexpr float kSlack = 8.f, kBias = F8 ? 7.f : 0.f;    // FP16: weights up to 2^(7 + 8)
     const uint32_t m = tid, lanes = (warp * 32u) << 16;
     for (uint32_t n = 0;; ++n) {
       const uint32_t slot = n & 1u;
       wait(bar_u, n);
-      const WideInfo unit = info[slot];
-      if (!unit.valid || *reinterpret_cast<volatile uint32_t*>(&aborted)) break;
+      const WideInfo unit = sm.info[slot];
+      if (!unit.valid || *reinterpret_cast<volatile uint32_t*>(&sm.aborted)) break;
       const uint32_t steps = unit.steps, plain = unit.plain, used = unit.rows * a.group, r = min(m, used - 1) / a.group, row = unit.first + r;
       const int32_t start = unit.start;
       const bool any_bad = unit.any_bad != 0u;
@@ -459,7 +478,7 @@ tree_wide_kernel(const TreeArgs a) {
         bool poisoned = false;
         if (!every) {
           wait2(bar_v, g);                                   // (`bad` is complete)
-          const bool there = entries[slot][j] >= 0;          // (a page outside the pool: as if nobody saw its positions)
+          const bool there = sm.pages[slot][j] >= 0;          // (a page outside the pool: as if nobody saw its positions)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const int32_t p = at + 32 * w, most = min(max(mine - p, 0), 32);
@@ -484,7 +503,7 @@ tree_wide_kernel(const TreeArgs a) {
         }
         if (F8 ? any_bad : !every) {
 #pragma unroll
-          for (int w = 0; w < 2; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&bad[slot][j * (kWideStep / 32) + w]) & see[w]);
+          for (int w = 0; w < 2; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&sm.bad[slot][j * (kWideStep / 32) + w]) & see[w]);
         }
         tmem_ld_wait();
         if (!every) {
@@ -574,14 +593,14 @@ tree_wide_kernel(const TreeArgs a) {
   }
   // (every product has been waited for, or its wait ran out: then the tensor memory is given back after a moment for what may
   // still be under way)
-  if (aborted) {
+  if (sm.aborted) {
     const unsigned long long t0 = global_ns();
     while (global_ns() - t0 < kLingerNs) {}
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 4) tmem_dealloc(tmem_at, kWideColumns);
+  if (warp == 4) tmem_dealloc(sm.tmem_at, kWideColumns);
 }
 
 }  // namespace grb
