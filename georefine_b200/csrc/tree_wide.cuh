@@ -22,6 +22,8 @@
 // most 2^15, values at most 57344), so what falls out at the bottom is 2^-39 of the largest - beyond what the 32-bit sums keep.
 // The reference of a row's weights moves only when its maximum has passed it by 2^8 (then O, in tensor memory, is scaled down).
 #pragma once
+#include <type_traits>
+
 #include "tree_attention.cuh"
 
 namespace grb {
@@ -77,28 +79,30 @@ struct WideInfo {
   uint32_t k_top, v_top, any_bad;  // largest exponent bytes of the chunk; whether `bad` has bits
 };
 // Shared memory beside the operands.
+template <bool F8>
 struct WideShared {
   uint64_t bars[11];               // of even and odd steps: K stored, V stored, S done, O done, P stored; unit set up
   WideInfo info[2];                // of a unit and the next
   uint32_t bad[2][kWideMostPart / 32];     // positions of the chunk whose key or value is not a number
-  int32_t pages[2][kWideMostPart / kWideStep];     // page of each step; -1: none
+  typename std::conditional<F8, int64_t, int32_t>::type where[2][kWideMostPart / kWideStep];     // first entry, or (BF16) page, of each step; -1: none
   uint32_t tmem_at, aborted, next_unit;
   uint32_t k_top, v_top, any_bad, any_absent;      // the loaders' own, while they set a unit up
 };
-static_assert(sizeof(WideShared) <= 1024, "two CTAs of the BF16 kernel take all of an SM's shared memory");
-// Operands from 1024 on.  8 bits: Q, two stages of K, two of V, FP16 scales of a chunk's K and V.  BF16: Q, what its rounding left
+static_assert(sizeof(WideShared<false>) <= 1024, "two CTAs of the BF16 kernel take all of an SM's shared memory");
+constexpr uint32_t kWideSharedBytes = 2048;
+// The operands follow.  8 bits: Q, two stages of K, two of V, FP16 scales of a chunk's K and V.  BF16: Q, what its rounding left
 // out, a ring of three stages that K and V take in turn (K of step g where V of g - 2 was, V of g where K of g - 1 was).
 template <bool F8>
-constexpr uint32_t kWideSmem = 1024 + (F8 ? 3 * kWideOperand + 2 * 2 * kWideMostPart : 2 * kWideOperand + 3 * kWideStage);
+constexpr uint32_t kWideSmem = F8 ? kWideSharedBytes + 3 * kWideOperand + 2 * 2 * kWideMostPart : 1024 + 2 * kWideOperand + 3 * kWideStage;
 __device__ __forceinline__ void wide_loaders_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <bool F8>
 __global__ void __launch_bounds__(kWideThreads, 2)
 tree_wide_kernel(const TreeArgs a) {
   extern __shared__ __align__(1024) unsigned char wide_smem[];
-  WideShared& sm = *reinterpret_cast<WideShared*>(wide_smem);
+  WideShared<F8>& sm = *reinterpret_cast<WideShared<F8>*>(wide_smem);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint32_t qs = smem_u32(wide_smem) + 1024, rs = qs + kWideOperand, ks = F8 ? rs : rs + kWideOperand, vs = ks + kWideOperand;
+  const uint32_t qs = smem_u32(wide_smem) + (F8 ? kWideSharedBytes : 1024u), rs = qs + kWideOperand, ks = F8 ? rs : rs + kWideOperand, vs = ks + kWideOperand;
   const uint32_t k_scales = vs + kWideOperand, v_scales = k_scales + 2 * kWideMostPart;
   const uint32_t bar_k = smem_u32(&sm.bars[0]), bar_v = smem_u32(&sm.bars[2]), bar_s = smem_u32(&sm.bars[4]), bar_o = smem_u32(&sm.bars[6]),
                  bar_p = smem_u32(&sm.bars[8]), bar_u = smem_u32(&sm.bars[10]);
@@ -179,7 +183,8 @@ tree_wide_kernel(const TreeArgs a) {
         int64_t place = 0;
         if (lane < part_positions / kWideStep) {
           place = kv_place(a.table, t.seq, t.start + int32_t(lane * kWideStep));
-          sm.pages[slot][lane] = place < 0 ? -1 : int32_t(place / kKvPage);
+          if constexpr (F8) sm.where[slot][lane] = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, t.kvh));
+          else sm.where[slot][lane] = place < 0 ? -1 : int32_t(place / kKvPage);
         }
         const bool absent = __any_sync(0xFFFFFFFFu, place < 0);
         if (lane == 0) sm.any_absent = absent;
@@ -202,7 +207,8 @@ tree_wide_kernel(const TreeArgs a) {
       plain = sm.any_absent ? 0u : all >= t.extent ? steps : uint32_t(max(all - t.start, 0)) / kWideStep;
       // entry (of the layer) of step j's first position; -1: none
       auto entry_of = [&](uint32_t j) -> int64_t {
-        const int32_t page = sm.pages[slot][j];
+        if constexpr (F8) return sm.where[slot][j];
+        const int32_t page = int32_t(sm.where[slot][j]);
         return page < 0 ? -1 : int64_t(kv_entry(int64_t(page) * kKvPage + (uint32_t(t.start) + j * kWideStep) % kKvPage, a.nkv, t.kvh));
       };
       // the queries, sixteen lanes a row, once the scores of the unit before are done
@@ -478,7 +484,7 @@ tree_wide_kernel(const TreeArgs a) {
         bool poisoned = false;
         if (!every) {
           wait2(bar_v, g);                                   // (`bad` is complete)
-          const bool there = sm.pages[slot][j] >= 0;          // (a page outside the pool: as if nobody saw its positions)
+          const bool there = sm.where[slot][j] >= 0;          // (a page outside the pool: as if nobody saw its positions)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const int32_t p = at + 32 * w, most = min(max(mine - p, 0), 32);

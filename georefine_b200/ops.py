@@ -227,7 +227,7 @@ def _kv_rows(name, k, v, row_seq, row_pos, page_table, pages):
 
 def kv_write(k, v, row_seq, row_pos, page_table, pages):
     """Stores rows of keys and values ([rows, kv heads, 128] BF16, as they are: rotated already) at positions ``row_pos`` of the
-    sequences in slots ``row_seq``, quantised when the pages are.  Rows of slot -1 are left out."""
+    sequences in slots ``row_seq``, quantised when the pages are.  Rows of slot -1 are left out; no two rows name the same place."""
     _kv_rows("grb_kv_write", k, v, row_seq, row_pos, page_table, pages)
 
 
@@ -321,7 +321,8 @@ class TreeAttention:
     def __call__(self, qkv, cos, sin, row_seq, row_pos, page_table, pages, out, *, tree=None, longest_run=None):
         """``qkv`` (BF16 [rows, (nq + 2 nkv) 128]) -> ``out`` (BF16 [rows, nq 128]).  Keys (rotated) and values are stored at
         ``row_pos`` of the sequences in slots ``row_seq`` before any row reads.  Without ``tree`` row r sees positions up to its
-        own; with ``TreeRows`` what they say, a row that sees nothing giving zeros.  Rows of slot -1 are left out.
+        own; with ``TreeRows`` what they say, a row that sees nothing giving zeros.  Rows of slot -1 are left out; no two rows name the
+        same place.
         ``longest_run``: how many rows of one sequence follow one another, at most, where the caller knows it; runs of 64 causal rows
         or of more than 32 tree rows and heads are multiplied together (without it: causal rows are taken to be spread evenly
         over the slots, tree rows to be anyhow)."""

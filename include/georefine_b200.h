@@ -397,7 +397,7 @@ int grb_attn_decode_bf16(const grb_attn_step* step, void* cuda_stream);
  *    reads as NaN throughout.
  *
  *    A row with slot -1, or one whose place is outside the table or the pool, is left out: nothing is stored or read for it
- *    and its output stays as it was.
+ *    and its output stays as it was.  No two rows of a call may name the same place to store at.
  * ------------------------------------------------------------------------------------------------- */
 #define GRB_KV_BF16 0
 #define GRB_KV_E4M3 1
