@@ -214,18 +214,19 @@ tree_wide_kernel(const TreeArgs a) {
       // the queries, sixteen lanes a row, once the scores of the unit before are done
       auto queries = [&]() {
         if (step0) wait2(bar_s, step0 - 1);
-        constexpr uint32_t kHalves = F8 ? 1 : 2;
+        constexpr uint32_t kHalves = F8 ? 1 : 2, kAtOnce = F8 ? 4 : 8;
 #pragma unroll 1
-        for (uint32_t part = 0; part < 4 * kHalves; ++part) {
-          uint4 x[4];
+        for (uint32_t i0 = 0; i0 < 16 * kHalves; i0 += kAtOnce) {
+          const uint32_t half = i0 >> 4, row0 = (lt >> 4) + (i0 & 15u) * 8;
+          uint4 x[kAtOnce];
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t m = (lt >> 4) + (4 * (part & 3u) + i) * 8, r = m / a.group;
-            x[i] = m < used ? reinterpret_cast<const uint4*>(a.q + (((size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group)) * kHalves + (part >> 2)) * kKvDim)[lt & 15u]
-                            : make_uint4(0u, 0u, 0u, 0u);
+          for (uint32_t i = 0; i < kAtOnce; ++i) {
+            const uint32_t m = row0 + 8 * i, r = m / a.group;
+            const size_t pair = (size_t(t.first + r)) * a.nq + t.kvh * a.group + (m - r * a.group);
+            x[i] = m < used ? reinterpret_cast<const uint4*>(a.q + (pair * kHalves + half) * kKvDim)[lt & 15u] : make_uint4(0u, 0u, 0u, 0u);
           }
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) sts128((part & 4u ? rs : qs) + wide_offset<kWideTile>((lt >> 4) + (4 * (part & 3u) + i) * 8, lt & 15u), x[i]);
+          for (uint32_t i = 0; i < kAtOnce; ++i) sts128((half ? rs : qs) + wide_offset<kWideTile>(row0 + 8 * i, lt & 15u), x[i]);
         }
       };
       // everything is there: tells the weights' warps, who have all looked at the unit before once its first step's values have been
