@@ -107,8 +107,9 @@ struct KvRowsArgs {
 
 // Rows into the cache (READ false) or out of it (READ true).  A warp takes eight neighbouring entries of a row (keys, then
 // values), two at a time with 16 bytes of BF16 a lane; all its loads are on their way before the first is used, which is what
-// keeps enough bytes in flight.  32768 rows of 8 heads, 8 bits: 45 us in, 42 out, 4.5 to 4.8 TB/s (one entry a warp, 8 bytes a
-// lane: 106 and 100).
+// keeps enough bytes in flight.  32768 rows of 8 heads, 8 bits: 45 us in, 36 out, 4.5 and 5.6 TB/s (one entry a warp, 8 bytes a
+// lane: 106 and 100).  On the way in, 118 instructions for two entries take two thirds of the issue slots; warps are numbered and
+// divided in 32 bits for their sake.
 constexpr uint32_t kKvEntriesPerWarp = 8;
 
 template <bool READ, bool F8>
@@ -118,11 +119,13 @@ kv_rows_kernel(const KvRowsArgs a) {
   constexpr int N = kKvEntriesPerWarp / 2;
   const uint32_t lane = threadIdx.x & 31u, half = lane >> 4, l = lane & 15u, heads = 2 * a.pages.nkv;
   const uint32_t per_row = (heads + kKvEntriesPerWarp - 1) / kKvEntriesPerWarp;
-  const uint64_t at = uint64_t(blockIdx.x) * kKvWarps + (threadIdx.x >> 5);
-  const uint32_t row = uint32_t(at / per_row), head0 = uint32_t(at % per_row) * kKvEntriesPerWarp + half;
+  const uint32_t at = blockIdx.x * kKvWarps + (threadIdx.x >> 5), row = at / per_row, head0 = (at - row * per_row) * kKvEntriesPerWarp + half;
   if (row >= a.rows) return;
   const int64_t place = kv_place(a.table, a.row_seq[row], a.row_pos[row]);
   if (place < 0) return;
+  const size_t first_entry = kv_entry(place, a.pages.nkv, 0);
+  uint4* const keys = reinterpret_cast<uint4*>(a.k + row * a.ldk) + l;
+  uint4* const values = reinterpret_cast<uint4*>(a.v + row * a.ldv) + l;
   size_t entry[N];
   bool value[N], in[N];
   uint4* rows[N];
@@ -131,9 +134,9 @@ kv_rows_kernel(const KvRowsArgs a) {
     const uint32_t head = head0 + 2 * i;
     in[i] = head < heads;
     value[i] = head >= a.pages.nkv;
-    const uint32_t h = value[i] ? head - a.pages.nkv : head;
-    entry[i] = kv_entry(place, a.pages.nkv, in[i] ? h : 0);
-    rows[i] = reinterpret_cast<uint4*>((value[i] ? a.v + row * a.ldv : a.k + row * a.ldk) + (in[i] ? h : 0) * kKvDim) + l;
+    const uint32_t h = in[i] ? value[i] ? head - a.pages.nkv : head : 0u;
+    entry[i] = first_entry + h * kKvPage;
+    rows[i] = (value[i] ? values : keys) + h * (kKvDim / 8);
   }
   if constexpr (!F8) {
     uint4 x[N];
@@ -179,11 +182,12 @@ kv_rows_kernel(const KvRowsArgs a) {
 #pragma unroll
         for (int off = 8; off; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
         const uint32_t byte = kv_exp_byte(__uint_as_float(m << 16), m < 0x7F80u);
+        const float s = kv_inverse(byte);
         uint32_t c[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = kv_codes(bf_lo(w[j]), bf_hi(w[j]), byte);
+        for (int j = 0; j < 4; ++j) c[j] = e4m3_pair(__fmul_rn(bf_lo(w[j]), s), __fmul_rn(bf_hi(w[j]), s));
         if (in[i]) {
-          *held(i) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+          *held(i) = byte == kKvNanByte ? make_uint2(0u, 0u) : make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
           if (l == 0) *exps(i) = uint8_t(byte);
         }
       }

@@ -54,7 +54,7 @@ int kv_rows(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t*
   a.ldv = ldv;
   a.rows = rows;
   const uint64_t warps = uint64_t(rows) * ((2 * a.pages.nkv + kKvEntriesPerWarp - 1) / kKvEntriesPerWarp), ctas = (warps + kKvWarps - 1) / kKvWarps;
-  if (ctas > 0x7FFFFFFFull) return GRB_ERR_UNSUPPORTED;
+  if (warps > 0xFFFFFF00ull) return GRB_ERR_UNSUPPORTED;   // (numbered in 32 bits)
   const auto kernel = pages->format == GRB_KV_E4M3 ? kv_rows_kernel<READ, true> : kv_rows_kernel<READ, false>;
   return launch_step(kernel, dim3(uint32_t(ctas)), dim3(kKvWarps * 32), 0, static_cast<cudaStream_t>(stream), a);
 }
