@@ -197,10 +197,10 @@ kv_rows_kernel(const KvRowsArgs a) {
 
 // What a draft tree keeps: entry base + path[i] of a sequence goes to base + i, for i = 1 .. count - 1, in every layer, keys
 // and values.  Paths ascend, so an entry never lands on one that is still to be read (base + i <= base + path[i] <
-// base + path[i + 1]) as long as each batch is read before it is written.  Grid (layers * 2 / 8, sequences): where an entry
-// lies is looked up once for eight planes, whose pieces are then in flight together (64 paths of 64 layers, 8 bits: 19 us; a plane a CTA: 29).
+// base + path[i + 1]) as long as each batch is read before it is written.  Grid (layers * 2 / 4, sequences): where an entry
+// lies is looked up once for four planes, whose pieces are then in flight together (64 paths of 64 layers, 8 bits: 19 us; a plane a CTA: 29).
 constexpr int kKeepThreads = 256;
-constexpr int kKeepPlanes = 8;      // planes (a layer's keys or values) of a CTA, one 16-byte piece of each a thread at a time
+constexpr int kKeepPlanes = 4;      // planes (a layer's keys or values) of a CTA, one 16-byte piece of each a thread at a time
 
 struct KvKeepArgs {
   KvPagesArgs pages;
