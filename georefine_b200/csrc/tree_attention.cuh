@@ -74,15 +74,23 @@ __device__ __forceinline__ int64_t tree_place(const TreeArgs& a, uint32_t r) {
 }
 // One past the last position that row r sees; -1: left out.
 __device__ __forceinline__ int32_t tree_extent(const TreeArgs& a, uint32_t r) {
+  int32_t base = 0;                                          // (asked for before the place is known: no load waits for another's check)
+  uint64_t mask[kTreeMaskWords] = {};
+  if (a.row_base) {
+    base = a.row_base[r];
+#pragma unroll
+    for (uint32_t w = 0; w < kTreeMaskWords; ++w)
+      if (w < a.mask_words) mask[w] = a.row_mask[r * a.ldm + w];
+  }
   if (tree_place(a, r) < 0) return -1;
   if (!a.row_base) return a.row_pos[r] + 1;
   const int32_t most = int32_t(a.table.max_pages * kKvPage);
-  const int32_t base = min(max(a.row_base[r], 0), most);
-  for (int w = int(a.mask_words) - 1; w >= 0; --w) {
-    const uint64_t m = a.row_mask[r * a.ldm + w];
-    if (m) return min(most, base + 64 * w + 64 - __clzll(m));
-  }
-  return base;
+  base = min(max(base, 0), most);
+  int32_t extent = base;
+#pragma unroll
+  for (uint32_t w = 0; w < kTreeMaskWords; ++w)
+    if (mask[w]) extent = min(most, base + 64 * int32_t(w) + 64 - __clzll(mask[w]));
+  return extent;
 }
 // Whether row r (of `base`) sees position p >= base.
 __device__ __forceinline__ bool tree_sees(const TreeArgs& a, uint32_t r, int32_t node) {
