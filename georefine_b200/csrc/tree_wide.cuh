@@ -204,7 +204,8 @@ tree_wide_kernel(const TreeArgs a) {
       steps = (uint32_t(t.extent - t.start) + kWideStep - 1) / kWideStep;       // (a unit has a position at least)
       wide_loaders_meet();                                   // (the scales of the unit before have been read, too)
       u = sm.next_unit;
-      plain = sm.any_absent ? 0u : all >= t.extent ? steps : uint32_t(max(all - t.start, 0)) / kWideStep;
+      // (whole steps alone: the last one may reach past what the tile's rows see, even where they all see as far)
+      plain = sm.any_absent ? 0u : uint32_t(max(min(all, t.extent) - t.start, 0)) / kWideStep;
       // entry (of the layer) of step j's first position; -1: none
       auto entry_of = [&](uint32_t j) -> int64_t {
         if constexpr (F8) return sm.where[slot][j];
