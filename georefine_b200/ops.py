@@ -124,6 +124,17 @@ def _vector(t, device, what, n=None):
     return t.data_ptr()
 
 
+def _ld(t, width, what):
+    """Elements from one row (of ``width``) to the next.  Rows that overlap - an expanded tensor's are all the same memory - would be
+    walked past its end; a single row has no distance to keep."""
+    ld = t.stride(0)
+    if ld < width:
+        if t.shape[0] > 1:
+            raise ValueError(f"{what}: rows overlap (they start {ld} elements apart and are {width} long)")
+        return width
+    return ld
+
+
 def _launch(device, name, *args):
     """The call on the device's current stream; a device that is not the current one is made so meanwhile."""
     import torch
@@ -206,7 +217,7 @@ def _table(page_table, device):
     if not slots or not pages or page_table.stride(1) != 1:
         raise ValueError("the page table is [slots, pages], its rows contiguous")
     _on(page_table, device, torch.int32, "page table")
-    return page_table.data_ptr(), page_table.stride(0), slots, pages
+    return page_table.data_ptr(), _ld(page_table, pages, "page table"), slots, pages
 
 
 def _kv_rows(name, k, v, row_seq, row_pos, page_table, pages):
@@ -221,8 +232,9 @@ def _kv_rows(name, k, v, row_seq, row_pos, page_table, pages):
         if rows and not (t.is_contiguous() or (t.stride(2) == 1 and t.stride(1) == HEAD_DIM)):
             raise ValueError(f"{what}: the heads of a row have to lie side by side")
     args = _native.KV_TABLE.pack(*_table(page_table, device)), _vector(row_seq, device, "row_seq"), _vector(row_pos, device, "row_pos", rows)
+    ldk, ldv = _ld(k, width, "keys"), _ld(v, width, "values")
     if rows:
-        _launch(device, name, pages._packed, *args, k.data_ptr(), max(k.stride(0), width), v.data_ptr(), max(v.stride(0), width), rows)
+        _launch(device, name, pages._packed, *args, k.data_ptr(), ldk, v.data_ptr(), ldv, rows)
 
 
 def kv_write(k, v, row_seq, row_pos, page_table, pages):
@@ -248,9 +260,9 @@ def kv_keep(slots, base, path, count, page_table, pages):
     _on(path, pages.device, torch.int32, "path")
     device = pages.device
     args = _native.KV_TABLE.pack(*_table(page_table, device)), _vector(slots, device, "slots"), _vector(base, device, "base", n)
-    kept = _vector(count, device, "count", n)
+    kept, ldp = _vector(count, device, "count", n), _ld(path, path.shape[1], "path")
     if n and path.shape[1]:
-        _launch(device, "grb_kv_keep", pages._packed, *args, path.data_ptr(), max(path.stride(0), path.shape[1]), kept, n, path.shape[1])
+        _launch(device, "grb_kv_keep", pages._packed, *args, path.data_ptr(), ldp, kept, n, path.shape[1])
 
 
 class TreeRows:
@@ -270,7 +282,7 @@ class TreeRows:
         self.rows, self.device = rows, base.device
         self.base, self.rope, self.mask = base, rope, mask
         # (fields of the C structure)
-        self._fields = base.data_ptr(), rope.data_ptr(), mask.data_ptr(), max(mask.stride(0), mask.shape[1]), mask.shape[1]
+        self._fields = base.data_ptr(), rope.data_ptr(), mask.data_ptr(), _ld(mask, mask.shape[1], "mask"), mask.shape[1]
 
     @staticmethod
     def masks(parents, words=None):
@@ -350,7 +362,7 @@ class TreeAttention:
                 raise ValueError("tree rows: one for each row, on the same device")
             nodes = tree._fields
         step = _native.TREE_STEP.pack(
-            qkv.data_ptr(), max(qkv.stride(0), wide), cos.data_ptr(), sin.data_ptr(), cos.shape[0], _vector(row_seq, device, "row_seq", rows),
+            qkv.data_ptr(), _ld(qkv, wide, "qkv"), cos.data_ptr(), sin.data_ptr(), cos.shape[0], _vector(row_seq, device, "row_seq", rows),
             _vector(row_pos, device, "row_pos", rows), *nodes, *pages._fields, *_table(page_table, device), self.scratch.data_ptr(), self.scratch_bytes,
-            out.data_ptr(), max(out.stride(0), narrow), rows, self.nq, HEAD_DIM, self._scaling, longest_run or 0)
+            out.data_ptr(), _ld(out, narrow, "out"), rows, self.nq, HEAD_DIM, self._scaling, longest_run or 0)
         _launch(device, "grb_attn_tree", step)

@@ -139,7 +139,7 @@ class DraftVerifier:
         import torch
 
         from . import _native
-        from .ops import _launch, _on, _vector
+        from .ops import _launch, _ld, _on, _vector
 
         device, n = self.device, starts.shape[0] - 1
         kind = 0 if logits.dtype is torch.bfloat16 else 1 if logits.dtype is torch.float32 else None
@@ -161,12 +161,12 @@ class DraftVerifier:
             _on(draft_probs, device, torch.float32, "draft_probs", (rows, vocab))
             if vocab > 1 and draft_probs.stride(1) != 1:
                 raise ValueError("rows of draft_probs have to be contiguous")
-            q, ldq = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
+            q, ldq = draft_probs.data_ptr(), _ld(draft_probs, vocab, "draft_probs")
         above = 0 if parent is None else _vector(parent, device, "parent", rows)
         tokens_at, starts_at = _vector(tokens, device, "tokens", rows), _vector(starts, device, "starts")
         out = (self.tokens, self.rows, self.count) if n == self.max_seqs else (self.tokens[:n], self.rows[:n], self.count[:n])
         if n:
-            step = _native.VERIFY_STEP.pack(logits.data_ptr(), max(logits.stride(0), vocab), tokens_at, above, starts_at, u_keep.data_ptr(), u_draw.data_ptr(), q, ldq,
+            step = _native.VERIFY_STEP.pack(logits.data_ptr(), _ld(logits, vocab, "logits"), tokens_at, above, starts_at, u_keep.data_ptr(), u_draw.data_ptr(), q, ldq,
                                             *self._places, rows, n, vocab, self.width, kind, float(temperature))
             _launch(device, "grb_verify_drafts", step)
         return out
