@@ -219,7 +219,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
 int grb_verify_drafts(const grb_verify_step* s, void* cuda_stream) {
   if (!s || !s->logits || !s->tokens || !s->starts || !s->u_keep || !s->u_draw || !s->stats || !s->out_tokens || !s->out_rows || !s->out_count)
     return GRB_ERR_ARGUMENT;
-  if (!s->vocab || !s->width || s->ldl < int64_t(s->vocab) || !(s->temperature > 0.0) || s->temperature > 1e30 || s->dtype > 1 || (reinterpret_cast<uintptr_t>(s->stats) & 15))
+  if (!s->vocab || !s->width || s->ldl < int64_t(s->vocab) || !(s->temperature >= kVerifyLeastTemperature) || s->temperature > kVerifyMostTemperature || s->dtype > 1 || (reinterpret_cast<uintptr_t>(s->stats) & 15))
     return GRB_ERR_ARGUMENT;
   if (s->draft_probs && (s->parent || s->ldq < int64_t(s->vocab))) return GRB_ERR_ARGUMENT;
   if (s->vocab > kVerifyMaxVocab || s->rows > 65535 || s->seqs > 65535 || s->width > kVerifyMaxNodes) return GRB_ERR_UNSUPPORTED;

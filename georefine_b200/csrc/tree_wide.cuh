@@ -53,20 +53,6 @@ __device__ __forceinline__ void stg256(float* p, const float (&v)[8]) {
 // 2^e in FP16, e <= 15; below its range 0.
 __device__ __forceinline__ uint32_t half_power(int e) { return e >= -14 ? uint32_t(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u; }
 
-// Two values at a time: a * b + c, a + b.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-
 struct WideUnit {
   uint32_t first, rows, kvh, part;
   int32_t seq, start, extent;      // positions start .. extent - 1 (at most a chunk): what some row sees, up to the last such

@@ -26,6 +26,8 @@ constexpr uint32_t kVerifyThreads = 256;
 constexpr uint32_t kVerifyDrawThreads = 512;
 constexpr uint32_t kVerifyTile = 256;          // tokens a warp takes at a time, eight consecutive ones a lane
 constexpr uint32_t kVerifyMaxVocab = 524288;
+// log2(e) / T fits 32 bits with room, 2^104 of it is above 100 (see widen)
+constexpr double kVerifyLeastTemperature = 1e-30, kVerifyMostTemperature = 1e20;
 
 struct VerifyArgs {
   const void* logits;       // [rows][ldl] BF16 or FP32
@@ -37,7 +39,7 @@ struct VerifyArgs {
   const float* u_draw;      // [seqs]
   const float* q;           // [rows][ldq] or null: what row i's token was drawn from
   int64_t ldq;
-  double2* stats;           // scratch [rows][8]: (R, Z) of an eighth of the row: Z = sum of 2^(l[t] log2_scale - R) over it
+  double2* stats;           // scratch [rows][8]: (m, Z) of an eighth of the row: its largest logit, Z = sum of 2^((l[t] - m) log2_scale) over it
   int32_t* out_tokens;      // [seqs][width]
   int32_t* out_rows;        // [seqs][width]
   int32_t* out_count;       // [seqs]
@@ -123,9 +125,10 @@ struct VerifyOctet<true> {
 // Bound by memory, the exponentials (16 per SM and cycle) not far behind.  The eighths are put together by whoever needs the
 // row: doing it here, in a cluster, left the SMs waiting for chains of exponentials and remote reads (546 rows of 152064 BF16
 // logits: 54 us, this 34, 4.9 TB/s).
-// The exponent l hi - c (hi: log2_scale rounded to 32 bits, c: that of the maximum m, rounded) is rounded once; what hi leaves
-// out, l (log2_scale - hi), is taken for m in R, which leaves (l - m) 2^-25 of a weight that falls with l - m.  Eight
-// exponentials are added in 32 bits, the eights in 64: a probability is off by the exponentials' 2^-22 at most.
+// The exponent is (l - m) hi, the difference first: whatever the logits' size (a mask of the type's lowest value) and however small
+// the temperature, it is 0 for the maximum and negative or -infinity for the others.  Two roundings and what hi (log2_scale in 32 bits)
+// leaves out are 2.5 2^-24 of an exponent whose weight falls with it.  Eight exponentials are added in 32 bits, the eights in 64: a
+// probability is off by the exponentials' 2^-22 at most.
 template <bool F32, bool VEC>
 __global__ void __launch_bounds__(kVerifyThreads)
 verify_rows_kernel(const VerifyArgs a) {
@@ -138,7 +141,8 @@ verify_rows_kernel(const VerifyArgs a) {
   const float hi = float(a.log2_scale);
   const uint32_t octets = (a.vocab + 7) / 8, per = (octets + kVerifySlices - 1) / kVerifySlices;
   const uint32_t first = min(octets, blockIdx.x * per), last = min(octets, first + per);
-  float m = -INFINITY, c = -INFINITY;
+  const float2 hi2 = make_float2(hi, hi);
+  float m = -INFINITY;
   double sum = 0.0;
 #pragma unroll 1
   for (uint32_t o0 = first + tid; o0 < last; o0 += B * kVerifyThreads) {
@@ -150,27 +154,28 @@ verify_rows_kernel(const VerifyArgs a) {
     for (int b = 0; b < B; ++b) top = x[b].max(top);
     if (top == -INFINITY) continue;
     if (top > m) {
-      const float was = c;
+      sum *= double(exp2_approx(__fmul_rn(__fsub_rn(m, top), hi)));      // (from -infinity: 0)
       m = top;
-      c = __fmul_rn(m, hi);
-      sum *= double(exp2_approx(__fsub_rn(was, c)));
     }
+    const float2 less = make_float2(-m, -m);
 #pragma unroll
     for (int b = 0; b < B; ++b) {
       float eight = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) eight = __fadd_rn(eight, exp2_approx(__fmaf_rn(x[b][i], hi, -c)));
+      for (int i = 0; i < 8; i += 2) {
+        const float2 e = mul2(add2(make_float2(x[b][i], x[b][i + 1]), less), hi2);
+        eight = __fadd_rn(__fadd_rn(eight, exp2_approx(e.x)), exp2_approx(e.y));
+      }
       sum += double(eight);
     }
   }
-  // all under the CTA's maximum (c belongs to m: the same m gives the same c)
+  // all under the CTA's maximum
   float top = warp_max(m);
   if (lane == 0) tops[warp] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < int(kVerifyThreads / 32); ++w) top = fmaxf(top, tops[w]);
-  const float all = __fmul_rn(top, hi);
-  if (m < top) sum *= double(exp2_approx(__fsub_rn(c, all)));
+  if (m < top) sum *= double(exp2_approx(__fmul_rn(__fsub_rn(m, top), hi)));
 #pragma unroll
   for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
   if (lane == 0) sums[warp] = sum;
@@ -179,28 +184,30 @@ verify_rows_kernel(const VerifyArgs a) {
     sum = 0.0;
 #pragma unroll
     for (int w = 0; w < int(kVerifyThreads / 32); ++w) sum += sums[w];
-    a.stats[size_t(row) * kVerifySlices + blockIdx.x] = make_double2(top == -INFINITY ? -INFINITY : double(all) + double(top) * (a.log2_scale - double(hi)), sum);
+    a.stats[size_t(row) * kVerifySlices + blockIdx.x] = make_double2(double(top), sum);
   }
 }
 
-// 2^y for -101 < y < 1 to 2^-42: y = k / 16 + f, 2^(k / 16) from a table and a shift, 2^f by the first six terms of the
-// exponential series in f ln 2 (|f| <= 2^-5: the seventh is 1.4e-13).  Sixteen entries lie in as many pairs of banks, so a warp's
-// look-ups never collide; 64 of them and one term less took as long.
+// 2^(d scale16 / 16) to 2^-42, for exponents in (-101, 0]: d scale16 = k + f with k whole, 2^(k / 16) from a table and a shift, 2^(f / 16) by
+// the first six terms of the exponential series in f ln 2 / 16 (|f| <= 1 / 2: the seventh is 1.4e-13).  Sixteen entries lie in as many
+// pairs of banks, so a warp's look-ups never collide; 64 of them and one term less took as long.  (The exponent comes as a product so
+// that no operation goes into it alone.)
 constexpr uint32_t kExpTable = 16;
-__device__ __forceinline__ double exp2_f64(double y, const double* table) {
+__device__ __forceinline__ double exp2_f64(double d, double scale16, const double* table) {
   constexpr double kRound = 6755399441055744.0;     // 1.5 * 2^52: what is added to it rounds to a whole number in its low bits
-  const double t = __fma_rn(y, double(kExpTable), kRound);
+  const double t = __fma_rn(d, scale16, kRound);
   const int k = __double2loint(t);                  // (whole and fraction: the bits above and below the table's)
-  const double f = __fma_rn(t - kRound, -1.0 / kExpTable, y);
-  double q = __fma_rn(f, 0.0013333558146428441, 0.009618129107628477);  // ln2^5 / 120, ln2^4 / 24
-  q = __fma_rn(f, q, 0.05550410866482158);                              // ln2^3 / 6
-  q = __fma_rn(f, q, 0.2402265069591007);                               // ln2^2 / 2
-  q = __fma_rn(f, q, 0.6931471805599453);
+  const double f = __fma_rn(d, scale16, -(t - kRound));
+  double q = __fma_rn(f, 1.2715871950558131e-09, 1.467610032291943e-07);      // L^5 / 120, L^4 / 24 with L = ln 2 / 16
+  q = __fma_rn(f, q, 1.3550807779497457e-05);                               // L^3 / 6
+  q = __fma_rn(f, q, 0.0009383847928089872);                               // L^2 / 2
+  q = __fma_rn(f, q, 0.04332169878499658);
   const double r = table[k & int(kExpTable - 1)] * __fma_rn(f, q, 1.0);
   return __hiloint2double(__double2hiint(r) + ((k & -int(kExpTable)) << 16), __double2loint(r));
 }
 
-// x 2^-896 in 64 bits, for a finite x, by integer operations in place of a conversion; a zero or a subnormal becomes some number below 2^-1022.
+// x 2^-896 in 64 bits, exactly, for a finite x, by integer operations in place of a conversion; -infinity becomes -2^128 2^-896, which is
+// 2^104 2^-896 below every number.
 __device__ __forceinline__ double widen(float x) {
   const int u = __float_as_int(x);
   return __hiloint2double((u >> 3) & int(0x8FFFFFFFu), int(uint32_t(u) << 29));
@@ -221,7 +228,8 @@ __device__ __forceinline__ double warp_scan_f64(double v, uint32_t lane) {
 }
 
 // What verify_draw draws from: masses of a row's tokens.  A mass below 2^-100 of the likeliest token's counts as that much, which no
-// draw can feel (a draw's target is at least 2^-75): that saves a comparison and a selection a token.
+// draw can feel (a draw's target is at least 2^-75).  The bound is put on the difference l - top in 64 bits: one on the logit, rounded
+// to its 32 bits, may be the top itself where the logits are large or the temperature is small.
 constexpr double kLeastMass = 8.077935669463161e-28, kLeastTarget = 2.6469779601696886e-23;    // 2^-90, 2^-75
 struct VerifyMasses {
   const float* q;           // refused draft's distribution, or null
@@ -229,15 +237,19 @@ struct VerifyMasses {
   const double* table;
   uint32_t tried_count, vocab;
   bool q_vec;               // rows of q start on 16-byte boundaries
-  float least;              // the logit of 2^-100 of the likeliest
-  double ref, scale, inverse;   // scale: times 2^896; inverse: of the sum of the masses without q, where q is subtracted
+  uint32_t least;           // upper half of the difference that stands for 2^-100
+  double top, scale16, inverse;   // top: the likeliest token's logit, times 2^-896; scale16: 16 log2_scale, times 2^896; inverse: of the sum of the masses without q, where q is subtracted
 
   // Eight consecutive tokens from t.  `plain`: without q.  `some`: of them were tried.  (No branch between the exponentials: each
   // is a chain of a dozen dependent operations, and only side by side do they keep the unit busy.)
   template <bool F32>
   __device__ __forceinline__ void eight(const VerifyOctet<F32>& x, uint32_t t, bool plain, bool some, double (&m)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = exp2_f64(__fma_rn(widen(fmaxf(x[i], least)), scale, -ref), table);
+    for (int i = 0; i < 8; ++i) {
+      const double d = widen(x[i]) - top;
+      // from the bound to 0: of numbers that are not positive, the bits of the larger magnitude are the larger integer (positive is a NaN's alone)
+      m[i] = exp2_f64(__hiloint2double(int(min(max(uint32_t(__double2hiint(d)), 0x80000000u), least)), __double2loint(d)), scale16, table);
+    }
     if (q && !plain) {
       float o[8];
       if (q_vec) verify_load8<true, true>(q, t, vocab, o, 0.f);
@@ -267,7 +279,7 @@ verify_draw_kernel(const VerifyArgs a) {
   step_kernel_entry();
   extern __shared__ uint32_t struck[];              // ceil(vocab / 256) words: one bit for every eight tokens that hold a tried one
   __shared__ int32_t token[kVerifyMaxNodes], up[kVerifyMaxNodes], next[kVerifyMaxNodes], tried[kVerifyMaxNodes];
-  __shared__ double node_ref[kVerifyMaxNodes], node_sum[kVerifyMaxNodes];
+  __shared__ double node_top[kVerifyMaxNodes], node_sum[kVerifyMaxNodes];
   __shared__ double node_mass[kVerifyMaxNodes];     // the parent's probability of a node's token; 0 for one tried before
   __shared__ __align__(128) double table[kExpTable];
   __shared__ double sums[kVerifyRegions], region[kVerifyRegions];
@@ -298,13 +310,13 @@ verify_draw_kernel(const VerifyArgs a) {
     double2 part[kVerifySlices];
 #pragma unroll
     for (int i = 0; i < int(kVerifySlices); ++i) part[i] = a.stats[size_t(first + tid) * kVerifySlices + i];
-    double ref = part[0].x, sum = 0.0;
+    double top = part[0].x, sum = 0.0;
 #pragma unroll
-    for (int i = 1; i < int(kVerifySlices); ++i) ref = fmax(ref, part[i].x);
+    for (int i = 1; i < int(kVerifySlices); ++i) top = fmax(top, part[i].x);
 #pragma unroll
     for (int i = 0; i < int(kVerifySlices); ++i)
-      if (part[i].x > -INFINITY) sum += part[i].y * double(exp2_approx(float(part[i].x - ref)));
-    node_ref[tid] = ref;
+      if (part[i].x > -INFINITY) sum += part[i].y * double(exp2_approx(float((part[i].x - top) * a.log2_scale)));
+    node_top[tid] = top;
     node_sum[tid] = sum;
     token[tid] = t;
     up[tid] = p;
@@ -319,7 +331,7 @@ verify_draw_kernel(const VerifyArgs a) {
   double mass = 0.0;
   if (mine_up >= 0 && uint32_t(token[tid]) < a.vocab) {
     if (a.q) q_mine = a.q[int64_t(first + tid) * a.ldq + token[tid]];
-    mass = exp2(__fma_rn(double(verify_logit<F32>(verify_row<F32>(a, first + mine_up), uint32_t(token[tid]))), a.log2_scale, -node_ref[mine_up])) / node_sum[mine_up];
+    mass = exp2((double(verify_logit<F32>(verify_row<F32>(a, first + mine_up), uint32_t(token[tid]))) - node_top[mine_up]) * a.log2_scale) / node_sum[mine_up];
   }
   if (a.parent && mine_up >= 0)                     // a token tried before at this node
     for (uint32_t j = uint32_t(mine_up) + 1; j < tid; ++j)
@@ -368,10 +380,10 @@ verify_draw_kernel(const VerifyArgs a) {
   masses.table = table;
   masses.tried_count = tried_count;
   masses.vocab = a.vocab;
-  masses.scale = a.log2_scale * 5.282945311356653e+269;    // 2^896
-  masses.ref = node_ref[node];
+  masses.scale16 = a.log2_scale * 16 * 0x1p896;
+  masses.least = uint32_t(__double2hiint(-100.0 / a.log2_scale * 0x1p-896));
+  masses.top = node_top[node] * 0x1p-896;
   masses.inverse = 1.0;
-  masses.least = float((masses.ref - 100.0) / a.log2_scale);
   const void* const row = verify_row<F32>(a, first + node);
   constexpr uint32_t kWarps = kVerifyDrawThreads / 32, kLane = kVerifyRegions / 32;     // regions of a lane, where one looks them over
   const uint32_t of_cta = kVerifyRegions / gridDim.x, of_warp = of_cta / kWarps;
@@ -433,7 +445,7 @@ verify_draw_kernel(const VerifyArgs a) {
     }
     // the region where the running mass passes the target, or the last one with any mass
     target = fmax(double(u_draw) * whole, kLeastTarget);
-    if (!(whole > kLeastTarget)) {                           // nothing left to draw from (a drafted token of probability 1 that was refused)
+    if (!(whole > kLeastTarget) || masses.top == -INFINITY) {      // nothing left to draw from (a drafted token of probability 1 that was refused), or no token in the row
       if (blockIdx.x == 0 && tid == 0) out_tokens[count - 1] = last_tried >= 0 ? token[last_tried] : 0;
       return;
     }

@@ -148,8 +148,8 @@ class DraftVerifier:
         rows, vocab = logits.shape
         if not 0 <= n <= self.max_seqs or rows > self.max_rows:
             raise ValueError("more rows or sequences than the verifier was made for")
-        if not temperature > 0:
-            raise ValueError("temperature must be positive; temperature 0 is the arg-max path")
+        if not 1e-30 <= temperature <= 1e20:
+            raise ValueError("temperature must be from 1e-30 to 1e20; temperature 0 is the arg-max path")
         for t, size, what in ((u_keep, rows, "u_keep"), (u_draw, n, "u_draw")):
             _on(t, device, torch.float32, what, (size,))
             if not t.is_contiguous():

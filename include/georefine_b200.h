@@ -480,7 +480,7 @@ typedef struct grb_verify_step {
   int32_t* out_rows;          /* [seqs][width]: the walk's nodes (0 first), then -1 */
   int32_t* out_count;         /* [seqs]: nodes of the walk = emitted tokens; 0 for a sequence without rows */
   uint32_t rows, seqs, vocab, width, dtype;   /* vocab <= 524288, width <= 256, at most 256 rows a sequence are looked at */
-  double temperature;
+  double temperature;         /* 1e-30 to 1e20 */
 } grb_verify_step;
 int grb_verify_drafts(const grb_verify_step* step, void* cuda_stream);
 
