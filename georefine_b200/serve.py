@@ -325,8 +325,9 @@ class BatchDecoder:
         if self.attn is not None and not tree:
             self.attn(qkv, self.cos, self.sin, seq, pos, self.page_table, self.kv[layer, 0], self.kv[layer, 1], out)
         else:
+            attention = self._tree_attention()                # (the rows' bases and masks are made with it)
             nodes = ops.TreeRows(self.row_base[rows], self.row_rope[rows], self.row_mask[rows]) if tree else None
-            self._tree_attention()(qkv, self.cos, self.sin, seq, pos, self.page_table, self._pages[layer], out, tree=nodes, longest_run=longest)
+            attention(qkv, self.cos, self.sin, seq, pos, self.page_table, self._pages[layer], out, tree=nodes, longest_run=longest)
 
     # ---- sequence slots and pages (host bookkeeping; the device sees only the page table) ---------------------
     def open_slot(self) -> int:
@@ -424,7 +425,10 @@ class BatchDecoder:
     def capture(self, kinds) -> None:
         """Captures the given (kind, rows) steps ahead of time (the reference's ``FastDecoder.capture``)."""
         for kind, n in kinds:
-            self.set_rows([self.pad_slot] * n, [0] * n, [0] * n)
+            if kind == "tree":                  # rows of no sequence: nodes may not share a place
+                self.set_tree_rows([-1] * n, [0] * n, [0] * n, [0] * n, [0] * n, [[0]] * n)
+            else:
+                self.set_rows([self.pad_slot] * n, [0] * n, [0] * n)
             self.run(kind, n)
 
     def set_rows(self, slots, positions, tokens) -> None:
