@@ -336,8 +336,8 @@ class TreeAttention:
         own; with ``TreeRows`` what they say, a row that sees nothing giving zeros.  Rows of slot -1 are left out; no two rows name the
         same place.
         ``longest_run``: how many rows of one sequence follow one another, at most, where the caller knows it; runs of 64 causal rows
-        or of more than 32 tree rows and heads are multiplied together (without it: causal rows are taken to be spread evenly
-        over the slots, tree rows to be anyhow)."""
+        or of more than 32 tree rows and heads are multiplied together (without it: tree rows are, causal rows are taken as steps
+        of decoding - a prompt's rows are as right, and slower)."""
         device, bf, (wide, narrow) = self.device, self._bf16, self._width
         rows = qkv.shape[0]
         if rows > self.max_rows or page_table.shape[1] > self.max_pages:

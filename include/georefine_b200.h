@@ -453,8 +453,8 @@ typedef struct grb_attn_tree_step {
   float scaling;              /* 1 / sqrt(head_dim) */
   uint32_t longest_run;       /* rows of one sequence that follow one another, at most; 0: not known.  Runs of 64 causal rows, or of
                                  more than 32 tree rows x query heads per kv head, go through the tensor cores together; not
-                                 known, causal rows are taken to be spread evenly over the table's slots.  A row has the same bits
-                                 whatever else is in the call, if this says alike whether such runs may come */
+                                 known, causal rows are taken as steps of decoding (right for any run, slow for a prompt).  A row
+                                 has the same bits whatever else is in the call, if this says alike whether such runs may come */
 } grb_attn_tree_step;
 uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pages, uint32_t format);
 int grb_attn_tree(const grb_attn_tree_step* step, void* cuda_stream);
