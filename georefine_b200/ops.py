@@ -319,15 +319,14 @@ class TreeAttention:
         self.scratch_bytes = _native.lib().grb_attn_tree_scratch_bytes(self.max_rows, nq, self.max_pages, KV_FORMATS.index(kv_format))
         self.scratch = torch.empty(self.scratch_bytes, device=device, dtype=torch.uint8)
         self.scratch[:16].zero_()
+        self.status = self.scratch[:4].view(torch.int32)
         self.device = self.scratch.device
         self._bf16, self._scaling, self._width = torch.bfloat16, 1.0 / math.sqrt(HEAD_DIM), ((nq + 2 * nkv) * HEAD_DIM, nq * HEAD_DIM)
 
     def check_status(self) -> int:
         """GRB_STATUS_* bits of the calls since the last check (0: their outputs can be trusted).  Synchronises."""
-        import torch
-
-        bits = int(self.scratch[:4].view(torch.int32).item())
-        self.scratch[:4].zero_()
+        bits = int(self.status.item())
+        self.status.zero_()
         return bits
 
     def __call__(self, qkv, cos, sin, row_seq, row_pos, page_table, pages, out, *, tree=None, longest_run=None):

@@ -264,7 +264,7 @@ class BatchDecoder:
         self._free_pages = list(range(n_pages - 2, -1, -1))
         self._free_slots = list(range(self.max_slots - 1, -1, -1))
         self.cos, self.sin = ops.rope_tables(self.max_context, cfg.rope_theta, self.dev)
-        self._tree_attn = None
+        self._tree_attn = self._status_host = None
         self.attn = self._pages = None
         if kv_format == "bf16":
             self.attn = ops.PagedAttention(cfg.local_heads, cfg.local_kv_heads, self.max_rows, self.pages_per_seq, self.dev)
@@ -317,6 +317,7 @@ class BatchDecoder:
             self._tree_staging = [(torch.zeros(2, R, dtype=torch.int32).pin_memory(), torch.zeros(R, words, dtype=torch.int64).pin_memory(), torch.cuda.Event())
                                   for _ in range(STAGING)]
             self._tree_staged = 0
+            self._status_host = torch.zeros(1, dtype=torch.int32).pin_memory()
         return self._tree_attn
 
     def attend(self, layer: int, rows: slice, tree: bool = False, longest: int | None = None) -> None:
@@ -328,6 +329,15 @@ class BatchDecoder:
             attention = self._tree_attention()                # (the rows' bases and masks are made with it)
             nodes = ops.TreeRows(self.row_base[rows], self.row_rope[rows], self.row_mask[rows]) if tree else None
             attention(qkv, self.cos, self.sin, seq, pos, self.page_table, self._pages[layer], out, tree=nodes, longest_run=longest)
+
+    def check_status(self) -> None:
+        """Raises when an attention over an 8-bit cache, or of draft trees, gave up a wait in the passes so far: their tokens and
+        the cache entries behind them are not to be used (retire the sequences).  Every such pass leaves its status in pinned memory, so
+        a caller that has read a pass's tokens asks without waiting again."""
+        if self._status_host is not None and self._status_host.item():
+            bits = self._tree_attn.check_status()            # (waits for the stream, and clears the word)
+            self._status_host.zero_()
+            raise RuntimeError(f"attention reported status {bits}: the tokens since the last check are to be discarded")
 
     # ---- sequence slots and pages (host bookkeeping; the device sees only the page table) ---------------------
     def open_slot(self) -> int:
@@ -377,6 +387,8 @@ class BatchDecoder:
             self._row_parallel(layer.down, "down", self.act[:n], self.down_out[:n])
             delta = self.down_out[:n]
         ops.rmsnorm(h, w.final_norm, x, delta=delta, eps=cfg.eps)          # h now holds the final residual stream
+        if tree or self.attn is None:
+            self._status_host.copy_(self._tree_attn.status, non_blocking=True)
         if head is None:
             return
         logits, token = self.logits[:n - head], self.next_token[:n - head]
@@ -524,6 +536,7 @@ class Batcher:
         # prompt where ``absorb`` gives no logits)
         self._rows, self._absorb = getattr(decoder, "queue_rows", decoder.set_rows), getattr(decoder, "absorb", None)
         self._absorb_head = self._absorb is not None and "head" in inspect.signature(self._absorb).parameters
+        self._check = getattr(decoder, "check_status", lambda: None)      # (asked once a pass's tokens are on the host, before they count)
 
     def admit(self, prompt_ids, *, sampler=None) -> int:
         """Processes a prompt and returns the sequence's slot; its first generated token is in ``active[slot]['tokens']``
@@ -536,6 +549,11 @@ class Batcher:
         slot = d.open_slot()
         d.ensure_pages(slot, len(ids))
         first = int(d.next_token[self._take_in(slot, 0, ids) - 1].item())
+        try:
+            self._check()
+        except RuntimeError:
+            d.close_slot(slot)
+            raise
         if sampler is not None:
             first = int(sampler.draw(d.logits[(len(ids) - 1) % d.max_rows][None])[0])
         self.active[slot] = {"pos": len(ids), "tokens": [first]}
@@ -582,6 +600,7 @@ class Batcher:
         if not rows:
             return
         pending = self.d.tokens[:len(self._order)].tolist()
+        self._check()
         for i, s in enumerate(self._order):
             if s in self.active and self.active[s]["tokens"][-1] is None:
                 self.active[s]["tokens"][-1] = int(pending[i])
@@ -625,6 +644,13 @@ class Batcher:
                 self.active[s]["tokens"].append(None)
             return None
         got = chosen[:n].tolist()
+        try:
+            self._check()
+        except RuntimeError:
+            for s in self._order:
+                self.active[s]["pos"] -= 1
+            self._dirty = True
+            raise
         for s, t in zip(self._order, got):
             self.active[s]["tokens"].append(int(t))
         return dict(zip(self._order, got))
@@ -652,6 +678,8 @@ class Batcher:
         self._rows(slots, positions, tokens)
         d.run("verify", len(slots))
         argmax_rows = d.next_token[:len(slots)].tolist()
+        self._dirty = True                   # (the rows of the last step are gone, whatever comes)
+        self._check()
         for slot, ds in drafts.items():
             k = len(ds)
             if sampler is None:
@@ -667,7 +695,6 @@ class Batcher:
             s["pos"] += len(emitted)
             out[slot] = emitted
             at += k + 1
-        self._dirty = True
         return out
 
 
@@ -710,9 +737,11 @@ class Batcher:
         pad = bucket_for(rows, self.buckets) - rows
         d.set_tree_rows(slots + [-1] * pad, positions + [0] * pad, tokens + [0] * pad, base + [0] * pad, rope + [0] * pad,
                         masks + [[0] * len(masks[0])] * pad)
+        self._dirty = True
         d.run("tree", rows + pad)
         if sampler is None:
             best = d.next_token[:rows].tolist()
+            self._check()
             emitted, walks = [], []
             for lo, hi in zip(starts, starts[1:]):
                 walk, got = [0], []
@@ -730,6 +759,7 @@ class Batcher:
         else:
             got, path, count = sampler.verify(d.logits[:rows], tokens, parents, starts)
             emitted = [g[:n] for g, n in zip(got.tolist(), count.tolist())]
+            self._check()
         first = torch.tensor([[slots[lo], base[lo]] for lo in starts[:-1]], dtype=torch.int32).to(d.dev)
         ops.kv_keep(first[:, 0].contiguous(), first[:, 1].contiguous(), path, count, d.page_table, d.pages)
         for slot, new in zip(trees, emitted):
@@ -737,7 +767,6 @@ class Batcher:
             s["tokens"] += new
             s["pos"] += len(new)
             out[slot] = new
-        self._dirty = True
         return out
 
 
