@@ -720,7 +720,6 @@ class Batcher:
                 raise ValueError("a draft hangs below the pending token (0) or an earlier draft")
             depth, seen = ops.TreeRows.masks(up, words=min(ops.MASK_WORDS, -(-d.max_rows // 64)))
             n, at = len(up), s["pos"]
-            d.ensure_pages(slot, at + n)
             slots += [slot] * n
             positions += range(at, at + n)
             tokens += [s["tokens"][-1]] + [int(t) for t in ts]
@@ -734,6 +733,8 @@ class Batcher:
             return out
         if rows > d.max_rows:
             raise ValueError("verify pass larger than the decoder's row buffers")
+        for slot, lo, hi in zip(trees, starts, starts[1:]):
+            d.ensure_pages(slot, base[lo] + hi - lo)
         pad = bucket_for(rows, self.buckets) - rows
         d.set_tree_rows(slots + [-1] * pad, positions + [0] * pad, tokens + [0] * pad, base + [0] * pad, rope + [0] * pad,
                         masks + [[0] * len(masks[0])] * pad)
