@@ -159,7 +159,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   if (int st = table_of(&s->table, a.pages, a.table)) return st;
   a.nkv = s->pages.nkv;
   a.nq = s->nq;
-  if (!s->nq || s->nq % a.nkv || s->head_dim != kKvDim || !s->rope_rows) return GRB_ERR_ARGUMENT;
+  if (!s->nq || s->nq % a.nkv || s->head_dim != kKvDim || !s->rope_rows || !(s->scaling > 0.f) || s->scaling > 1e30f) return GRB_ERR_ARGUMENT;
   a.group = a.nq / a.nkv;
   if (a.group > 16 || s->rows > kTreeMaxRows || s->nq + 2 * a.nkv > 65535 || s->mask_words > kTreeMaskWords) return GRB_ERR_UNSUPPORTED;
   if (s->row_base && (!s->row_rope || !s->row_mask || !s->mask_words || s->ldm < int64_t(s->mask_words))) return GRB_ERR_ARGUMENT;

@@ -450,7 +450,7 @@ typedef struct grb_attn_tree_step {
   void* out;                  /* BF16 [rows][ldo]: nq * 128 */
   int64_t ldo;
   uint32_t rows, nq, head_dim;   /* rows <= 4096; head_dim must be 128; nq / nkv <= 16 */
-  float scaling;              /* 1 / sqrt(head_dim) */
+  float scaling;              /* 1 / sqrt(head_dim); positive */
   uint32_t longest_run;       /* rows of one sequence that follow one another, at most; 0: not known.  Runs of 64 causal rows, or of
                                  more than 32 tree rows x query heads per kv head, go through the tensor cores together; not
                                  known, causal rows are taken as steps of decoding (right for any run, slow for a prompt).  A row
