@@ -97,8 +97,10 @@ class Sampler:
 
         rows, seqs = logits.shape[0], len(starts) - 1
         width = max(hi - lo for lo, hi in zip(starts, starts[1:]))
+        if width > 256:
+            raise ValueError(f"a draft tree of {width} nodes: at most 256 are looked at")
         if self._verifier is None or rows > self._verifier.max_rows or seqs > self._verifier.max_seqs or width > self._verifier.width:
-            self._verifier = DraftVerifier(max(rows, 128), max(seqs, 128), min(256, max(width, 16)), logits.device)
+            self._verifier = DraftVerifier(max(rows, 128), max(seqs, 128), max(width, 16), logits.device)
         if self.top_p < 1:          # the nucleus renormalised is the soft-max over its tokens alone
             logits = logits.float().masked_fill(self.probabilities(logits) == 0, float("-inf"))
         i32 = lambda v: torch.tensor(list(v), dtype=torch.int32).to(logits.device)
@@ -132,7 +134,7 @@ class DraftVerifier:
         tokens tried before; where none is kept, the last token is drawn from p without the tried ones: the lowest whose
         cumulative mass exceeds u_draw[s] times what is left.  ``draft_probs`` (FP32 [rows, vocabulary], chains): row i is the
         distribution that token i was drawn from; it is kept when u q[t] < p[t], else the draw is from max(p - q, 0).  Both leave
-        the tokens distributed as draws from the target.
+        the tokens distributed as draws from the target.  A sequence has at most 256 rows: those behind them are not looked at.
 
         Returns int32 (tokens [seqs, width]: the kept drafts, then the drawn token; rows [seqs, width]: the walk's nodes, the
         root first; count [seqs]: how many of each), padded with -1."""
