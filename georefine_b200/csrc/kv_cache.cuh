@@ -19,7 +19,7 @@
 namespace grb {
 
 constexpr uint32_t kKvDim = 128, kKvPage = 256;
-constexpr uint32_t kKvNanByte = 255;
+constexpr uint32_t kKvNanByte = 255, kKvLeastByte = 127 - 40;
 
 struct KvPagesArgs {
   void* k;                  // [layers][pages][nkv][256][128] BF16 or e4m3; layers `layer_stride` elements apart

@@ -5,21 +5,22 @@
 //   S = Q K^T (Q, K in shared memory, S in tensor memory);  weights P = exp2(S scale - reference), written over S;
 //   O += P V (P from tensor memory, V in shared memory, O in tensor memory).
 // Four warps, a thread per row, turn scores into weights; four bring K and V: BF16 as it is, 8 bits through registers, where a code
-// becomes FP16 (one conversion for two) times its entry's scale relative to the chunk's largest; one issues the products.  K, V and
+// becomes FP16, exactly (one conversion for two); one issues the products.  K, V and
 // S of two steps are held, so a step's scores are computed while the step before is weighed, and the loaders set the next unit up
 // while this one ends.  256 columns of tensor memory and 105 KB of shared memory leave room for two CTAs on an SM.
 //
-// 16 trees of 64 nodes behind 8192 positions, 40 query heads of 8 kv heads, all launches: 317 us in 8 bits, 0.42 PFLOP/s (one step
+// 16 trees of 64 nodes behind 8192 positions, 40 query heads of 8 kv heads, all launches: 322 us in 8 bits, 0.41 PFLOP/s (one step
 // at a time and barriers between units: 438; steps of 128 with one S, the products issued by a weights' warp: 340).  What bounds it
-// is the loaders' chain of a step, 2500 cycles in which a CTA waits for a stage, converts 64 positions of K and of V and asks for
-// the next (without the loads 266 us; without the exponentials as long as with them).
+// is the chain of a step, in which the loaders wait for a stage, convert 64 positions of K and of V and ask for the next, and the
+// weights' warps go through 64 scores a thread: without the scales' arithmetic 307 us.
 //
 // BF16: Q and the weights go into the products as two terms, what rounding to BF16 leaves and what it leaves out, so that the error
 // is the result's rounding (one term each: twice that).  416 us for the trees above, 291 with one term; with four stages of K and V
 // instead of three, and therefore one CTA an SM, 558.
 //
-// FP16 weights reach down to 2^-24 and V's entries to 2^-24 times a code of 1: both are scaled up as far as FP16 goes (weights at
-// most 2^15, values at most 57344), so what falls out at the bottom is 2^-39 of the largest - beyond what the 32-bit sums keep.
+// 8 bits: K's scale multiplies the score of its position, V's goes into the weight, as in the narrow kernel: S' = S 2^e_k scale + e_v, so
+// that the FP16 weights (2^15 at most, down to 2^-24) are largest where the row's own products are, whatever else the chunk holds; the
+// sum of the weights takes V's scale out again.
 // The reference of a row's weights moves only when its maximum has passed it by 2^8 (then O, in tensor memory, is scaled down).
 #pragma once
 #include <type_traits>
@@ -50,9 +51,6 @@ __device__ __forceinline__ uint64_t wide_desc_v(uint32_t smem_addr) {
 __device__ __forceinline__ void stg256(float* p, const float (&v)[8]) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
 }
-// 2^e in FP16, e <= 15; below its range 0.
-__device__ __forceinline__ uint32_t half_power(int e) { return e >= -14 ? uint32_t(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u; }
-
 struct WideUnit {
   uint32_t first, rows, kvh, part;
   int32_t seq, start, extent;      // positions start .. extent - 1 (at most a chunk): what some row sees, up to the last such
@@ -62,24 +60,29 @@ struct WideInfo {
   uint32_t valid, first, rows, kvh, part, steps;
   uint32_t plain;                  // steps, from the first on, whose positions every row sees
   int32_t start;
-  uint32_t k_top, v_top, any_bad;  // largest exponent bytes of the chunk; whether `bad` has bits
+};
+// What the exponents of a step's positions mean: 2^e of K; e and 2^-e (BF16, exact) of V.  (Half as many loads for the last, whose
+// latency the weights wait for: 322 us for the trees above instead of 326.)
+struct WideScales {
+  float k[kWideStep], v[kWideStep];
+  uint16_t v_inverse[kWideStep];
 };
 // Shared memory beside the operands.
 template <bool F8>
 struct WideShared {
-  uint64_t bars[11];               // of even and odd steps: K stored, V stored, S done, O done, P stored; unit set up
+  uint64_t bars[F8 ? 15 : 11];     // of even and odd steps: K stored, V stored, S done, O done, P stored; unit set up; 8 bits, of every fourth step: scales
   WideInfo info[2];                // of a unit and the next
-  uint32_t bad[2][kWideMostPart / 32];     // positions of the chunk whose key or value is not a number
+  uint32_t bad[2][F8 ? 1 : kWideMostPart / 32];        // BF16: positions of the chunk whose value is not a number
   typename std::conditional<F8, int64_t, int32_t>::type where[2][kWideMostPart / kWideStep];     // first entry, or (BF16) page, of each step; -1: none
   uint32_t tmem_at, aborted, next_unit;
-  uint32_t k_top, v_top, any_bad, any_absent;      // the loaders' own, while they set a unit up
+  uint32_t any_absent;             // the loaders' own, while they set a unit up
 };
 static_assert(sizeof(WideShared<false>) <= 1024, "two CTAs of the BF16 kernel take all of an SM's shared memory");
 constexpr uint32_t kWideSharedBytes = 2048;
-// The operands follow.  8 bits: Q, two stages of K, two of V, FP16 scales of a chunk's K and V.  BF16: Q, what its rounding left
+// The operands follow.  8 bits: Q, two stages of K, two of V, scales of four steps.  BF16: Q, what its rounding left
 // out, a ring of three stages that K and V take in turn (K of step g where V of g - 2 was, V of g where K of g - 1 was).
 template <bool F8>
-constexpr uint32_t kWideSmem = F8 ? kWideSharedBytes + 3 * kWideOperand + 2 * 2 * kWideMostPart : 1024 + 2 * kWideOperand + 3 * kWideStage;
+constexpr uint32_t kWideSmem = F8 ? kWideSharedBytes + 3 * kWideOperand + 4 * uint32_t(sizeof(WideScales)) : 1024 + 2 * kWideOperand + 3 * kWideStage;
 __device__ __forceinline__ void wide_loaders_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 template <bool F8>
@@ -89,9 +92,9 @@ tree_wide_kernel(const TreeArgs a) {
   WideShared<F8>& sm = *reinterpret_cast<WideShared<F8>*>(wide_smem);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t qs = smem_u32(wide_smem) + (F8 ? kWideSharedBytes : 1024u), rs = qs + kWideOperand, ks = F8 ? rs : rs + kWideOperand, vs = ks + kWideOperand;
-  const uint32_t k_scales = vs + kWideOperand, v_scales = k_scales + 2 * kWideMostPart;
+  WideScales* const scales = reinterpret_cast<WideScales*>(wide_smem + kWideSharedBytes + 3 * kWideOperand);     // (8 bits)
   const uint32_t bar_k = smem_u32(&sm.bars[0]), bar_v = smem_u32(&sm.bars[2]), bar_s = smem_u32(&sm.bars[4]), bar_o = smem_u32(&sm.bars[6]),
-                 bar_p = smem_u32(&sm.bars[8]), bar_u = smem_u32(&sm.bars[10]);
+                 bar_p = smem_u32(&sm.bars[8]), bar_u = smem_u32(&sm.bars[10]), bar_t = smem_u32(&sm.bars[F8 ? 11 : 10]);
   auto k_stage = [&](uint32_t g) { return ks + (F8 ? g & 1u : 2 * g % 3) * kWideStage; };
   auto v_stage = [&](uint32_t g) { return F8 ? vs + (g & 1u) * kWideStage : ks + (2 * g + 1) % 3 * kWideStage; };
   // Tensor memory is taken before the kernels behind this one may start: a matrix product among them takes its own as it starts and
@@ -105,6 +108,9 @@ tree_wide_kernel(const TreeArgs a) {
       mbar_init(bar_p + b, 4);
     }
     mbar_init(bar_u, 4);
+    if constexpr (F8) {
+      for (uint32_t b = 0; b < 32; b += 8) mbar_init(bar_t + b, 4);
+    }
     mbar_fence_init();
     sm.aborted = 0u;
   }
@@ -160,11 +166,10 @@ tree_wide_kernel(const TreeArgs a) {
       t.seq = a.row_seq[t.first];
       t.start = int32_t(t.part * part_positions);
       const uint32_t used = t.rows * a.group;
-      if (lt < kWideMostPart / 32) sm.bad[slot][lt] = 0u;
-      if (lt == 0) {
-        sm.k_top = sm.v_top = sm.any_bad = 0u;
-        sm.next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
+      if constexpr (!F8) {
+        if (lt < kWideMostPart / 32) sm.bad[slot][lt] = 0u;
       }
+      if (lt == 0) sm.next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
       if (warp == 4) {                                       // (a step's positions lie in one page)
         int64_t place = 0;
         if (lane < part_positions / kWideStep) {
@@ -188,7 +193,7 @@ tree_wide_kernel(const TreeArgs a) {
       }
       t.extent = min(extent, t.start + int32_t(part_positions));
       steps = (uint32_t(t.extent - t.start) + kWideStep - 1) / kWideStep;       // (a unit has a position at least)
-      wide_loaders_meet();                                   // (the scales of the unit before have been read, too)
+      wide_loaders_meet();
       u = sm.next_unit;
       // (whole steps alone: the last one may reach past what the tile's rows see, even where they all see as far)
       plain = sm.any_absent ? 0u : uint32_t(max(min(all, t.extent) - t.start, 0)) / kWideStep;
@@ -219,7 +224,7 @@ tree_wide_kernel(const TreeArgs a) {
       // everything is there: tells the weights' warps, who have all looked at the unit before once its first step's values have been
       // used (storing the third step's waited for that)
       auto publish = [&]() {
-        if (lt == 0) sm.info[slot] = WideInfo{1u, t.first, t.rows, t.kvh, t.part, steps, plain, t.start, sm.k_top, sm.v_top, sm.any_bad};
+        if (lt == 0) sm.info[slot] = WideInfo{1u, t.first, t.rows, t.kvh, t.part, steps, plain, t.start};
         if (steps_before && steps_before <= 2) wait2(bar_o, step0 - 1);
         fence_proxy_async_smem();
         __syncwarp();
@@ -238,10 +243,9 @@ tree_wide_kernel(const TreeArgs a) {
           for (int i = 0; i < 4; ++i) x[i] = int32_t(row0 + 32 * (i >> 1)) < npos ? src[256 * (i >> 1) + 4 * (i & 1)] : make_uint4(0u, 0u, 0u, 0u);
         };
         const uint32_t to_lo = wide_offset<kWideStep>(row0, 2 * (lt & 3u)), to_hi = wide_offset<kWideStep>(row0, 2 * (lt & 3u) + 1);     // (32 rows on: 4096 bytes)
-        auto store = [&](const uint4 (&x)[4], uint32_t dst, uint32_t scales, uint32_t j, bool clean) {
+        auto store = [&](const uint4 (&x)[4], uint32_t dst, bool clean) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t s16 = lds_u16(scales + 2 * (j * kWideStep + row0 + 32 * (i >> 1))), s = s16 | (s16 << 16);
             uint32_t h[8];
             e4m3_to_half4(x[i].x, h[0], h[1]);
             e4m3_to_half4(x[i].y, h[2], h[3]);
@@ -251,71 +255,50 @@ tree_wide_kernel(const TreeArgs a) {
 #pragma unroll
               for (int q = 0; q < 8; ++q) h[q] = half2_number(h[q]);
             }
-#pragma unroll
-            for (int q = 0; q < 8; ++q) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[q]) : "r"(s));
             const uint32_t at = dst + 4096 * (i >> 1) + (kWideStage / 2) * (i & 1);
             sts128(at + to_lo, make_uint4(h[0], h[1], h[2], h[3]));
             sts128(at + to_hi, make_uint4(h[4], h[5], h[6], h[7]));
           }
         };
+        // exponents: half of the threads a position's of K, the others one's of V.  A byte below what an entry has (0, where nobody wrote)
+        // stands for zeros of the smallest size.
+        const uint32_t at = lt & (kWideStep - 1);
+        const uint8_t* const exps = lt < kWideStep ? a.pages.k_exp : a.pages.v_exp;
+        uint32_t byte;
+        auto ask_exp = [&](uint32_t j) {
+          const int64_t entry = j < steps ? entry_of(j) : -1;
+          byte = entry < 0 ? 127u : exps[entry + at];
+        };
+        auto store_exp = [&](WideScales& s) {
+          if (lt < kWideStep) {
+            s.k[at] = kv_scale(byte);
+          } else {
+            const uint32_t b = max(byte, kKvLeastByte);
+            s.v[at] = b == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(b) - 127);
+            s.v_inverse[at] = uint16_t(__float_as_uint(kv_inverse(b)) >> 16);
+          }
+        };
+        ask_exp(0);
         ask(k, a.pages.k, 0);
-        // exponents of the chunk: a thread takes sixteen positions' of K and of V; bytes of no entry (135 to 254, where nobody wrote)
-        // do not count, nor do those behind the last position
-        uint32_t w[2][4];
-#pragma unroll
-        for (int of_v = 0; of_v < 2; ++of_v) {
-          const int64_t entry = lt < steps * 4 ? entry_of(lt >> 2) : -1;
-          const uint4 x = entry >= 0 ? *reinterpret_cast<const uint4*>((of_v ? a.pages.v_exp : a.pages.k_exp) + entry + (lt & 3u) * 16) : make_uint4(0u, 0u, 0u, 0u);
-          w[of_v][0] = x.x; w[of_v][1] = x.y; w[of_v][2] = x.z; w[of_v][3] = x.w;
-        }
-        const int32_t left = t.extent - t.start - int32_t(lt * 16);
-        uint32_t none = 0;
-#pragma unroll
-        for (int of_v = 0; of_v < 2; ++of_v) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t b = w[of_v][i >> 2] >> (8 * (i & 3)) & 0xFFu;
-            if (i < left && b == kKvNanByte) none |= 1u << i;
-            if (i < left && b <= 134u) top = max(top, b);
-          }
-#pragma unroll
-          for (int off = 16; off; off >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-          if (lane == 0 && top) atomicMax(of_v ? &sm.v_top : &sm.k_top, top);
-        }
-        if (none) {
-          atomicOr(&sm.bad[slot][lt >> 1], none << (16 * (lt & 1u)));
-          sm.any_bad = 1u;
-        }
-        wide_loaders_meet();
-#pragma unroll
-        for (int of_v = 0; of_v < 2; ++of_v) {
-          const uint32_t top = of_v ? sm.v_top : sm.k_top;
-          uint32_t h[8];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t b = w[of_v][i >> 2] >> (8 * (i & 3)) & 0xFFu;
-            const uint32_t p = b > 134u ? 0u : half_power(min(int(b) - int(top) + 7, 7));
-            h[i >> 1] = i & 1 ? h[i >> 1] | p << 16 : p;
-          }
-          const uint32_t dst = (of_v ? v_scales : k_scales) + lt * 32;
-          sts128(dst, make_uint4(h[0], h[1], h[2], h[3]));
-          sts128(dst + 16, make_uint4(h[4], h[5], h[6], h[7]));
-        }
         ask(v, a.pages.v, 0);
+        wide_loaders_meet();                                 // (the unit after this one and its pages are known to all)
         queries();
         publish();
-        wide_loaders_meet();                                 // the scales are complete
         for (uint32_t j = 0; j < steps; ++j) {
           const uint32_t g = step0 + j;
           if (g > 1) wait2(bar_s, g - 2);                    // scores have been taken from the stage's K
-          store(k, k_stage(g), k_scales, j, false);
+          store(k, k_stage(g), false);
+          store_exp(scales[g & 3u]);                         // (the step four before has been weighed: the one after it was waited for)
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar_k + 8 * (g & 1u));
+          if (lane == 0) {
+            mbar_arrive(bar_t + 8 * (g & 3u));
+            mbar_arrive(bar_k + 8 * (g & 1u));
+          }
+          ask_exp(j + 1);
           ask(k, a.pages.k, j + 1);
           if (g > 1) wait2(bar_o, g - 2);                    // the stage's values have been used
-          store(v, v_stage(g), v_scales, j, j >= plain);
+          store(v, v_stage(g), j >= plain);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_v + 8 * (g & 1u));
@@ -452,9 +435,8 @@ tree_wide_kernel(const TreeArgs a) {
       if (!unit.valid || *reinterpret_cast<volatile uint32_t*>(&sm.aborted)) break;
       const uint32_t steps = unit.steps, plain = unit.plain, used = unit.rows * a.group, r = min(m, used - 1) / a.group, row = unit.first + r;
       const int32_t start = unit.start;
-      const bool any_bad = unit.any_bad != 0u;
       const size_t pair = size_t(row) * a.nq + unit.kvh * a.group + (min(m, used - 1) - r * a.group);
-      const float scale = F8 ? __fmul_rn(a.q_scale[pair], __uint_as_float((unit.k_top > 7u ? unit.k_top - 7u : 127u) << 23)) : a.q_scale[pair];
+      const float scale = a.q_scale[pair];
       const int32_t base = a.row_base ? a.row_base[row] : 0, mine = a.extent[row];
       float ref = -INFINITY;
       float2 sum = make_float2(0.f, 0.f);
@@ -471,7 +453,7 @@ tree_wide_kernel(const TreeArgs a) {
         uint32_t see[2] = {~0u, ~0u};
         bool poisoned = false;
         if (!every) {
-          wait2(bar_v, g);                                   // (`bad` is complete)
+          if constexpr (!F8) wait2(bar_v, g);                // (`bad` is complete)
           const bool there = sm.where[slot][j] >= 0;          // (a page outside the pool: as if nobody saw its positions)
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
@@ -495,11 +477,26 @@ tree_wide_kernel(const TreeArgs a) {
             see[w] = there ? bits & below : 0u;
           }
         }
-        if (F8 ? any_bad : !every) {
+        if (!F8 && !every) {
 #pragma unroll
           for (int w = 0; w < 2; ++w) poisoned = poisoned || (*reinterpret_cast<volatile uint32_t*>(&sm.bad[slot][j * (kWideStep / 32) + w]) & see[w]);
         }
         tmem_ld_wait();
+        const float2 scale2 = make_float2(scale, scale);
+        const WideScales& of_step = scales[g & 3u];
+        if constexpr (F8) {                                  // S' (a NaN entry's is NaN)
+          wait(bar_t + 8 * (g & 3u), g >> 2);
+#pragma unroll
+          for (int i = 0; i < 64; i += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(&of_step.k[i]), v4 = *reinterpret_cast<const float4*>(&of_step.v[i]);
+            const float2 s0 = fma2(mul2(make_float2(__uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i & 31) + 1])), make_float2(k4.x, k4.y)), scale2, make_float2(v4.x, v4.y));
+            const float2 s1 = fma2(mul2(make_float2(__uint_as_float(x[i >> 5][(i & 31) + 2]), __uint_as_float(x[i >> 5][(i & 31) + 3])), make_float2(k4.z, k4.w)), scale2, make_float2(v4.z, v4.w));
+            x[i >> 5][i & 31] = __float_as_uint(s0.x);
+            x[i >> 5][(i & 31) + 1] = __float_as_uint(s0.y);
+            x[i >> 5][(i & 31) + 2] = __float_as_uint(s1.x);
+            x[i >> 5][(i & 31) + 3] = __float_as_uint(s1.y);
+          }
+        }
         if (!every) {
 #pragma unroll
           for (int w = 0; w < 2; ++w)
@@ -509,7 +506,7 @@ tree_wide_kernel(const TreeArgs a) {
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(tops[i >> 1 & 3], fmaxf(__uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i + 1) & 31])));
-        const float top = __fmul_rn(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), scale);
+        const float raw = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), top = F8 ? raw : __fmul_rn(raw, scale);
         const bool move = top > (ref == -INFINITY ? ref : __fadd_rn(ref, kSlack));
         if (__any_sync(0xFFFFFFFFu, move)) {
           const float to = move ? top : ref, f = move ? exp2_approx(__fsub_rn(ref, to)) : 1.f;        // (from -infinity: 0)
@@ -531,21 +528,31 @@ tree_wide_kernel(const TreeArgs a) {
           }
         }
         const float low = (ref == -INFINITY ? 0.f : ref) - kBias;
-        const float2 scale2 = make_float2(scale, scale), low2 = make_float2(-low, -low);
+        const float2 low2 = make_float2(-low, -low);
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           uint32_t p[16], rest[F8 ? 1 : 16];
+          uint32_t inverse[F8 ? 16 : 1];
+          if constexpr (F8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 q = *reinterpret_cast<const uint4*>(&of_step.v_inverse[32 * w + 8 * i]);
+              inverse[4 * i] = q.x; inverse[4 * i + 1] = q.y; inverse[4 * i + 2] = q.z; inverse[4 * i + 3] = q.w;
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 e = fma2(make_float2(__uint_as_float(x[w][2 * i]), __uint_as_float(x[w][2 * i + 1])), scale2, low2);
+            const float2 s = make_float2(__uint_as_float(x[w][2 * i]), __uint_as_float(x[w][2 * i + 1]));
+            float2 e = F8 ? add2(s, low2) : fma2(s, scale2, low2);
             e.x = exp2_approx(e.x);
             e.y = exp2_approx(e.y);
-            sums[i & 1] = add2(sums[i & 1], e);
             if constexpr (F8) {
+              sums[i & 1] = fma2(e, make_float2(bf_lo(inverse[i]), bf_hi(inverse[i])), sums[i & 1]);
               const __half2 h = __floats2half2_rn(e.x, e.y);
               p[i] = *reinterpret_cast<const uint32_t*>(&h);
             } else {
+              sums[i & 1] = add2(sums[i & 1], e);
               p[i] = pack_bf(e.x, e.y);
               rest[i] = pack_bf_rest(e.x, e.y, p[i]);
             }
@@ -563,7 +570,6 @@ tree_wide_kernel(const TreeArgs a) {
       // ---- the unit's partial result
       wait2(bar_o, step0 + steps - 1);
       tc_fence_after();
-      const float back = F8 ? __uint_as_float((unit.v_top > 7u ? unit.v_top - 7u : 0u) << 23) : 1.f;
       const size_t out = pair * a.max_parts + unit.part;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -575,7 +581,7 @@ tree_wide_kernel(const TreeArgs a) {
           for (int i = 0; i < 32; i += 8) {
             float o[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = __fmul_rn(__uint_as_float(x[i + e]), back);
+            for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(x[i + e]);
             stg256(a.part_acc + out * kKvDim + 32 * w + i, o);
           }
         }
