@@ -574,7 +574,8 @@ tree_part_kernel(const TreeArgs a) {
       // what the positions' exponents mean, a thread two positions of K or of V: 2^e; e and 2^-e
       {
         const uint32_t pair = lds_u16(smem + P::kExpAt + tid * 2), b0 = pair & 0xFFu, b1 = pair >> 8;        // K: this thread's two positions
-        const uint32_t vpair = lds_u16(smem + P::kExpAt + 256 + tid * 2), v0 = vpair & 0xFFu, v1 = vpair >> 8;
+        // (V's bytes below what an entry has - 0, where nobody wrote - stand for zeros of the smallest size: 2^127 would leave the sums' range)
+        const uint32_t vpair = lds_u16(smem + P::kExpAt + 256 + tid * 2), v0 = max(vpair & 0xFFu, kKvLeastByte), v1 = max(vpair >> 8, kKvLeastByte);
         *reinterpret_cast<float2*>(&scales_sm[0][2 * tid]) = make_float2(kv_scale(b0), kv_scale(b1));
         *reinterpret_cast<float2*>(&scales_sm[1][2 * tid]) = make_float2(v0 == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(v0) - 127),
                                                                          v1 == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(v1) - 127));
