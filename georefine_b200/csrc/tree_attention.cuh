@@ -704,7 +704,8 @@ tree_part_kernel(const TreeArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
     if constexpr (F8) {
-      if (holes && a.row_base) tree_values_f8<true>(o, pa, vs, p_warp, lane);
+      // (a tile of one causal row has nothing behind what the row sees; between several rows there may be places that nobody wrote)
+      if (holes && (a.row_base || t.rows > 1)) tree_values_f8<true>(o, pa, vs, p_warp, lane);
       else tree_values_f8<false>(o, pa, vs, p_warp, lane);
     } else {
 #pragma unroll

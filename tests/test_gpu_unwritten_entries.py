@@ -35,3 +35,16 @@ def test_empty_pages_that_a_row_sees_hold_zeros(dev, fmt, rows, q_scale):
     want, bound = _all_rows(s, qkv, pos, 0, torch.arange(512, device=dev) <= pos[:, None])
     off = ((out.view(rows, 8, 128).double() - want).abs() / bound).amax()
     assert attn.check_status() == 0 and float(off) <= 1
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "bf16"])
+def test_causal_rows_with_places_between_them_that_hold_anything(dev, fmt):
+    """Rows of one call at positions far apart: a row's answer is that of the positions up to its own."""
+    s = Setup(dev, fmt, 4, 1, [20], 2)                 # (the places behind 20 hold NaN)
+    qkv = s.qkv(3)
+    out = torch.full((3, 512), float("nan"), device=dev, dtype=BF)
+    attn = s.ops.TreeAttention(4, 1, 3, 2, dev, kv_format=fmt)
+    pos = [20, 21, 100]
+    attn(qkv, s.cos, s.sin, _i32([0] * 3, dev), _i32(pos, dev), s.table, s.pages, out)
+    s.check(qkv[:2], [0, 0], pos[:2], out[:2], lambda r, p: p <= pos[r])
+    assert bool(out[2].isnan().all())                  # (it sees the places that nobody wrote)
