@@ -735,7 +735,7 @@ class Batcher:
             raise ValueError("verify pass larger than the decoder's row buffers")
         for slot, lo, hi in zip(trees, starts, starts[1:]):
             d.ensure_pages(slot, base[lo] + hi - lo)
-        pad = bucket_for(rows, self.buckets) - rows
+        pad = next((b for b in self.buckets if b >= rows), rows) - rows       # (a decoder may take more rows than its largest bucket)
         d.set_tree_rows(slots + [-1] * pad, positions + [0] * pad, tokens + [0] * pad, base + [0] * pad, rope + [0] * pad,
                         masks + [[0] * len(masks[0])] * pad)
         self._dirty = True
