@@ -492,14 +492,14 @@ class BatchDecoder:
 
         self._tree_attention()
         n = len(slots)
+        given, most = torch.tensor(masks, dtype=torch.int64), self.row_mask.shape[1]
+        if given.dim() != 2 or given.shape[0] != n or given.shape[1] > most:
+            raise ValueError(f"masks of {n} rows with up to {most} words")
         self._queue(slots, positions, tokens, self.max_rows)
         places, words, copied = self._tree_staging[self._tree_staged % STAGING]
         self._tree_staged += 1
         copied.synchronize()
         places[:, :n].copy_(torch.tensor([list(base), list(rope)], dtype=torch.int32))
-        given = torch.tensor(masks, dtype=torch.int64)
-        if given.dim() != 2 or given.shape[0] != n or given.shape[1] > words.shape[1]:
-            raise ValueError(f"masks of {n} rows with up to {words.shape[1]} words")
         words[:n].zero_()[:, :given.shape[1]].copy_(given)
         self.row_base[:n].copy_(places[0, :n], non_blocking=True)
         self.row_rope[:n].copy_(places[1, :n], non_blocking=True)

@@ -47,3 +47,15 @@ def test_run_before_any_tree_was_queued(dev, weights, fmt, graph):
     d = serve.BatchDecoder(weights, max_rows=64, max_slots=4, max_context=512, device=dev, kv_format=fmt)
     d.run("tree", 2, graph=graph)
     assert bool((d.ctx[:2] == 0).all()) and bool(torch.isfinite(d.logits[:2].float()).all())
+
+
+def test_masks_that_are_refused_leave_the_rows_as_they_were(dev, weights):
+    from georefine_b200 import serve
+
+    d = serve.BatchDecoder(weights, max_rows=64, max_slots=4, max_context=512, device=dev)
+    d.set_tree_rows([0, 1], [3, 4], [5, 6], [3, 4], [3, 4], [[1], [1]])
+    held = [t.clone() for t in (d.row_seq, d.row_pos, d.tokens, d.row_base, d.row_rope, d.row_mask)]
+    for bad in ([[1, 1], [1, 1]], [[1]], [1, 1]):
+        with pytest.raises(ValueError, match="masks"):
+            d.set_tree_rows([2, 3], [7, 8], [9, 9], [7, 8], [7, 8], bad)
+        assert all(torch.equal(a, b) for a, b in zip(held, (d.row_seq, d.row_pos, d.tokens, d.row_base, d.row_rope, d.row_mask)))
