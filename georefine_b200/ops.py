@@ -339,7 +339,7 @@ class TreeAttention:
         of decoding - a prompt's rows are as right, and slower)."""
         device, bf, (wide, narrow) = self.device, self._bf16, self._width
         rows = qkv.shape[0]
-        if rows > self.max_rows or page_table.shape[1] > self.max_pages:
+        if rows > self.max_rows or (page_table.dim() == 2 and page_table.shape[1] > self.max_pages):
             raise ValueError("more rows or pages than the scratch was sized for")
         if pages.format != self.format or pages.stacked or pages.kv_heads != self.nkv or pages.device != device:
             raise ValueError("pages of one layer, in this object's format, heads and device")

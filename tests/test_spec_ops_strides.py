@@ -95,3 +95,11 @@ def test_the_distances_that_are_passed_on(launched):
     step = _native.VerifyStep.from_buffer_copy(launched.pop()[1][0])
     assert (step.ldl, step.ldq, step.rows, step.vocab) == (20, 12, 3, 10)
     assert not launched
+
+
+def test_a_page_table_that_is_a_vector(launched):
+    attn = ops.TreeAttention(4, 2, 8, 4, "cpu")
+    seq = torch.zeros(2, dtype=I32)
+    with pytest.raises(ValueError, match="page table"):
+        attn(torch.zeros(2, 1024, dtype=BF), torch.zeros(64, 128, dtype=BF), torch.zeros(64, 128, dtype=BF), seq, seq, torch.zeros(4, dtype=I32), _pages(), torch.zeros(2, 512, dtype=BF))
+    assert not launched
