@@ -188,8 +188,9 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.wide_rows = kWideTile / a.group;
   // Runs for the wide kernel: trees of more rows than two tiles of the narrow one take; of causal rows prompt chunks, so that the
   // rows of a speculative chain keep the bits of single steps.  A run's rows alone decide, whatever else is in the call, so one run
-  // pays for what many gain.  Eight nodes of five heads a kv head, 8 bits, us narrow / wide: one tree behind 1000 positions 18 / 23,
-  // four behind 2000 36 / 29, sixteen behind 4000 129 / 76; 16 nodes: 20 / 25, 48 / 29, 214 / 86.
+  // pays for what many gain.  Eight nodes of five heads a kv head, 8 bits, us narrow / wide: one tree behind 1000 positions 18 / 21,
+  // four behind 2000 37 / 27, sixteen behind 4000 127 / 69; 16 nodes: 20 / 22, 48 / 28, 214 / 80.  128 rows of a prompt: behind 2000
+  // 67 / 37, behind 8000 190 / 75; at its start 20 / 22.
   // Causal rows are taken to be decode rows where the caller does not say (an empty launch of the wide kernel costs a batch of 128 rows
   // behind 2048 positions 148 us instead of 135); guessing from the other rows of the call would have them change a run's bits.
   const uint32_t longest = s->longest_run ? s->longest_run : s->row_base ? s->rows : 1u;

@@ -26,8 +26,8 @@ constexpr uint32_t kTreePrepThreads = 256, kTreePrepMost = 1024;
 constexpr uint32_t kTreeRowAbsent = 0xFFFFFFFFu;             // row_parts of a row that is left out: its output stays as it was
 // Positions of a wide tile's unit: the most, for long contexts (a unit's result is as large as 256 positions of an 8-bit cache); fewer
 // for short ones and for runs of one or two tiles, whose few units would leave SMs idle.  1024 instead of 2048 behind 8192 positions,
-// 8 bits, 40 heads of 8: one run of 16 rows 37 us instead of 53, 16 runs 127 instead of 140; 16 runs of 64 rows (three tiles) 347
-// instead of 318, which keep 2048.
+// 8 bits, 40 heads of 8: one run of 16 rows 35 us instead of 51, 16 runs 120 instead of 138; 16 runs of 64 rows (three tiles) 337
+// instead of 320, which keep 2048.
 constexpr uint32_t kWideMostPart = 2048;
 __device__ __forceinline__ uint32_t wide_part(uint32_t extent, bool many) {
   return extent <= 1024 ? 256u : extent <= 4096 ? 512u : extent <= 16384 && !many ? 1024u : kWideMostPart;

@@ -563,8 +563,9 @@ class Batcher:
     def _take_in(self, slot: int, first: int, ids) -> int:
         """Runs the tokens ``ids`` at positions ``first``.. of a sequence through the decoder in chunks; returns the number of
         rows that got logits: what a whole number of ``max_rows`` leaves of them, or ``max_rows``.  The chunks follow one another
-        on the stream without the host waiting for any of them, and may be wider than a step (a row's bits do not depend on
-        the chunk it is in); the output head runs for the rows that get logits alone."""
+        on the stream without the host waiting for any of them, and may be wider than a step (over a BF16 cache a row's bits do not
+        depend on the chunk it is in; over an 8-bit one, 64 rows or more of a slice are multiplied together, with other roundings
+        than fewer); the output head runs for the rows that get logits alone."""
         d = self.d
         last = (len(ids) - 1) // d.max_rows * d.max_rows
         lo, head = 0, self._absorb is not None and self._absorb_head
@@ -704,7 +705,9 @@ class Batcher:
         from the root goes, at each node, to the first child that is kept, and emits one more token where none is.  Without a
         sampler a child is kept when it is the target's arg-max there; with a ``sampling.Sampler`` with the probability the target
         gives it among what was not refused before, on the GPU (``sampling.DraftVerifier``), which leaves the emitted tokens
-        distributed as plain sampling.  The cache entries of the walk move to consecutive positions in every layer.  Returns {slot:
+        distributed as plain sampling.  (The attention of a tree rounds elsewhere than that of a step - over a BF16 cache always, over
+        an 8-bit one where a tree has more than 32 rows x query heads per KV head - so a walk equals plain decoding but where two logits are
+        within that rounding; chains of fewer than 64 rows, in ``verify``, equal it bit for bit.)  The cache entries of the walk move to consecutive positions in every layer.  Returns {slot:
         emitted tokens}."""
         import torch
 
@@ -837,7 +840,7 @@ class FastSession:
         """Yields up to ``max_tokens`` new tokens (the token the prefill produced counts as the first).  ``temperature``
         > 0 samples (``top_p`` < 1: from the nucleus); ``seed`` makes the draws reproducible, and a tensor-parallel
         decoder needs one, the same on every rank, for the ranks to stay in step.  ``tree_drafter(state)`` proposes a tree of drafts
-        instead of a chain: (tokens, parents) as ``Batcher.verify_trees`` takes them."""
+        instead of a chain: (tokens, parents) as ``Batcher.verify_trees`` takes them, which also says how near to plain decoding it is."""
         from .sampling import Sampler
 
         sampler = None
