@@ -549,16 +549,20 @@ class Batcher:
         slot = d.open_slot()
         d.ensure_pages(slot, len(ids))
         first = int(d.next_token[self._take_in(slot, 0, ids) - 1].item())
-        try:
-            self._check()
-        except RuntimeError:
-            d.close_slot(slot)
-            raise
+        self._check_prompt(slot)
         if sampler is not None:
             first = int(sampler.draw(d.logits[(len(ids) - 1) % d.max_rows][None])[0])
         self.active[slot] = {"pos": len(ids), "tokens": [first]}
         self._dirty = True
         return slot
+
+    def _check_prompt(self, slot: int) -> None:
+        """Gives the slot back where the prompt's passes are not to be trusted."""
+        try:
+            self._check()
+        except RuntimeError:
+            self.d.close_slot(slot)
+            raise
 
     def _take_in(self, slot: int, first: int, ids) -> int:
         """Runs the tokens ``ids`` at positions ``first``.. of a sequence through the decoder in chunks; returns the number of
@@ -1036,6 +1040,7 @@ class MTPSpeculator:
             d.set_rows([slot] * len(chunk), range(lo, lo + len(chunk)), chunk)
             d.run("verify", len(chunk), graph=False)
             first = int(d.next_token[len(chunk) - 1].item())
+            self.b._check_prompt(slot)
             if sampler is not None and lo + len(chunk) == len(ids):
                 first = int(sampler.draw(d.logits[len(chunk) - 1][None])[0])
             hidden = d.h[:len(chunk)].clone()

@@ -116,3 +116,18 @@ def test_a_status_that_the_host_sets(fmt):
         with pytest.raises(RuntimeError, match="status 16"):
             b.verify_trees({slot: ([1], [0])})
     b.step()
+
+
+def test_a_failed_prompt_of_a_sequence_with_a_draft_head(monkeypatch):
+    d = Reporting(monkeypatch, max_rows=16)
+    d.h = torch.zeros(16, 4)
+    absorbed = []
+    head = types.SimpleNamespace(absorb=lambda slots, *rest: absorbed.append(slots) or [0] * len(slots), z=torch.zeros(16, 4))
+    spec = serve.MTPSpeculator(serve.Batcher(d), head, k=2)
+    free = len(d._free)
+    d.fail = True
+    with pytest.raises(RuntimeError, match="status"):
+        spec.admit([5, 6, 7])
+    assert len(d._free) == free and not spec.b.active and not spec.first
+    slot = spec.admit([5, 6, 7])
+    assert spec.b.active[slot]["tokens"] == greedy([5, 6, 7], 1) and slot in spec.first
