@@ -1,4 +1,4 @@
-// A paged KV cache in BF16 or in 8 bits: storing rows, reading them back, and moving what a draft tree keeps.
+// A paged KV cache in BF16, in 8 or in 4 bits: storing rows, reading them back, and moving what a draft tree keeps.
 //
 // A page holds 256 positions of one sequence as [kv head][position][128]; an entry is the 128 values of one key or value head
 // at one position.  In 8 bits an entry is 128 e4m3 codes and one exponent byte (pages of exponents: [kv head][position]):
@@ -7,6 +7,18 @@
 // step, 2^-4 of the value - whatever its size, and the same input gives the same codes everywhere.  The scale goes with the
 // entry because a cache is appended to one entry at a time: nothing stored before is touched again.  An entry with an
 // infinity or a NaN is stored as byte 255 with codes 0 and reads as NaN throughout.
+//
+// In 4 bits an entry is 128 whole numbers in -7 .. 7, a scale byte for each 32 of them and an exponent byte: 69 bytes.  With a = max |x|
+// of the entry, e = clamp(floor(log2(a / 7)) + 9, -40, 22), kept as e + 127; a group's scale F is the number nearest to (its max |x|) / 7 2^(24 - e)
+// among (16 + m) 2^k, m 0 .. 15, k 0 .. 11, kept as the byte 64 + 16 k + m; code = x / (F 2^(e - 24)) to the nearest (ties to even) in -7 .. 7;
+// value = code F 2^(e - 24).  Uniform steps, because the largest of 32 values is about two standard deviations: a normal entry is held to
+// 20.2 dB (e2m1 codes under the same scales: 19.9).  A nibble holds code + 8: nibbles masked out of a word are FP16 subnormals, so that one
+// fused multiply-add makes two FP16 operands of them - u 2^-24 F - 8 F 2^-24, exact, as F is a whole number of at most 16 bits, five of them
+// significant, which is also why the scales stay in twelve binades.  The exponent keeps the operands of an entry near the top of that range
+// whatever its size, as in 8 bits.  A scale byte below 16 reads as byte / 8, so that memory of zeros reads as zeros.
+// A page of one head is 17664 bytes in a piece: the codes of its 256 positions, 64 bytes each, then their scales, 4 bytes each, then their
+// exponents.  The codes of dimensions 8 w .. 8 w + 7 are 32-bit word w: nibble j of the lower half is dimension 2 j of the eight, of the upper
+// half 2 j + 1 - the two that share an operand register.
 //
 // The kernels here move bytes, and memory bounds them; nothing is kept between calls.
 #pragma once
@@ -21,8 +33,12 @@ namespace grb {
 constexpr uint32_t kKvDim = 128, kKvPage = 256;
 constexpr uint32_t kKvNanByte = 255, kKvLeastByte = 127 - 40;
 
+enum : int { kKvBf16 = 0, kKvE4m3 = 1, kKvQ4 = 4 };      // formats, numbered as in the C interface
+constexpr uint32_t kQ4Codes = kKvDim / 2;                // bytes of an entry's codes
+constexpr uint32_t kQ4ScalesAt = kKvPage * kQ4Codes, kQ4ExpsAt = kQ4ScalesAt + kKvPage * 4, kQ4Page = kQ4ExpsAt + kKvPage;    // of one head's page
+
 struct KvPagesArgs {
-  void* k;                  // [layers][pages][nkv][256][128] BF16 or e4m3; layers `layer_stride` elements apart
+  void* k;                  // [layers][pages][nkv][256][128] BF16 or e4m3, [layers][pages][nkv][17664] in 4 bits; layers `layer_stride` elements apart
   void* v;
   uint8_t* k_exp;           // [layers][pages][nkv][256], layers `exp_stride` bytes apart (8-bit caches)
   uint8_t* v_exp;
@@ -92,6 +108,34 @@ __device__ __forceinline__ uint32_t kv_codes(float lo, float hi, uint32_t byte) 
   return e4m3_pair(__fmul_rn(lo, s), __fmul_rn(hi, s));
 }
 
+
+// ---- 4 bits ---------------------------------------------------------------------------------------------------------
+// Exponent byte of an entry whose largest magnitude is `amax`.  (A quotient by 7 that is no power of two does not round to one: below
+// 7 2^k values are 2^(k - 21) apart, a seventh of which is more than half of a step of the quotient.)
+__device__ __forceinline__ uint32_t q4_exp_byte(float amax, bool finite) {
+  const int e = int(__float_as_uint(__fdiv_rn(amax, 7.f)) >> 23) - 127 + 9;
+  return finite ? uint32_t(min(max(e, -40), 22) + 127) : kKvNanByte;
+}
+// Scale byte of a group whose largest magnitude is `amax`, and the scale times the entry's unit, 2^(e - 24).
+__device__ __forceinline__ uint32_t q4_scale_byte(float amax, uint32_t exp_byte, float& step) {
+  const float want = fminf(fmaxf(__fmul_rn(__fdiv_rn(amax, 7.f), __uint_as_float((127u + 24u + 127u - exp_byte) << 23)), 16.f), 63488.f);
+  const uint32_t bits = __float_as_uint(want), five = (bits + 0x3FFFFu + (bits >> 19 & 1u)) >> 19;     // five bits, ties to even
+  step = __fmul_rn(__uint_as_float(five << 19), __uint_as_float((exp_byte - 24u) << 23));
+  return five - 127u * 16u;
+}
+// code + 8 of a value whose quotient by the step is q.
+__device__ __forceinline__ uint32_t q4_nibble(float q) { return uint32_t(__float2int_rn(fminf(fmaxf(q, -7.f), 7.f)) + 8); }
+// What a scale byte stands for.
+__device__ __forceinline__ float q4_scale(uint32_t byte) {
+  return byte < 16u ? __fmul_rn(float(byte), 0.125f) : __uint_as_float((byte + 127u * 16u) << 19);
+}
+// 2^(e - 24) of an exponent byte; bytes below what an entry has (0, where nobody wrote) stand for the smallest.
+__device__ __forceinline__ float q4_unit(uint32_t byte) {
+  return byte == kKvNanByte ? __uint_as_float(0x7FC00000u) : __uint_as_float((max(byte, kKvLeastByte) - 24u) << 23);
+}
+// Bytes from the pool's start to the page of one head that entry `entry` is in.
+__device__ __forceinline__ size_t q4_page_at(size_t entry) { return entry / kKvPage * kQ4Page; }
+
 constexpr int kKvWarps = 8;
 
 struct KvRowsArgs {
@@ -112,7 +156,7 @@ struct KvRowsArgs {
 // divided in 32 bits for their sake.
 constexpr uint32_t kKvEntriesPerWarp = 8;
 
-template <bool READ, bool F8>
+template <bool READ, int FORMAT>
 __global__ void __launch_bounds__(kKvWarps * 32)
 kv_rows_kernel(const KvRowsArgs a) {
   step_kernel_entry();
@@ -138,7 +182,7 @@ kv_rows_kernel(const KvRowsArgs a) {
     entry[i] = first_entry + h * kKvPage;
     rows[i] = (value[i] ? values : keys) + h * (kKvDim / 8);
   }
-  if constexpr (!F8) {
+  if constexpr (FORMAT == kKvBf16) {
     uint4 x[N];
     auto held = [&](int i) { return reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(value[i] ? a.pages.v : a.pages.k) + entry[i] * kKvDim) + l; };
 #pragma unroll
@@ -147,6 +191,65 @@ kv_rows_kernel(const KvRowsArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (in[i]) *(READ ? rows[i] : held(i)) = x[i];
+  } else if constexpr (FORMAT == kKvQ4) {
+    // a lane holds word l of the entry's codes, dimensions 8 l .. 8 l + 7; four lanes share a scale
+    auto page = [&](int i) { return static_cast<uint8_t*>(value[i] ? a.pages.v : a.pages.k) + q4_page_at(entry[i]); };
+    auto at = [&](int i) { return uint32_t(entry[i] % kKvPage); };
+    if constexpr (READ) {
+      uint32_t code[N], scale[N], exp[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (in[i]) {
+          code[i] = reinterpret_cast<const uint32_t*>(page(i))[at(i) * (kQ4Codes / 4) + l];
+          scale[i] = page(i)[kQ4ScalesAt + at(i) * 4 + (l >> 2)];
+          exp[i] = page(i)[kQ4ExpsAt + at(i)];
+        }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (!in[i]) continue;
+        const float step = __fmul_rn(q4_scale(scale[i]), q4_unit(exp[i]));      // (exact, as is its product with a code: eight bits)
+        auto one = [&](uint32_t nibble) { return __fmul_rn(float(int(code[i] >> (4 * nibble) & 15u) - 8), step); };
+        *rows[i] = make_uint4(pack_bf(one(0), one(4)), pack_bf(one(1), one(5)), pack_bf(one(2), one(6)), pack_bf(one(3), one(7)));
+      }
+    } else {
+      uint4 x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = in[i] ? *rows[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t m = 0;                               // (magnitudes of BF16 values compare as integers)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+        m = max(m & 0xFFFFu, m >> 16);
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+        const float group = __uint_as_float(m << 16);
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
+        const bool finite = m < 0x7F80u;
+        const uint32_t exp = q4_exp_byte(__uint_as_float(m << 16), finite);
+        float step;
+        uint32_t scale = q4_scale_byte(finite ? group : 0.f, finite ? exp : 127u, step), code = 0;
+        // A product with the rounded reciprocal is 2^-19 of the quotient at most off.  The quotient of a value of eight bits and a step of
+        // five lies on a border between two codes, or 2^-11 or more from all of them; rounded to 2^-13 first, it lands on the right side.
+        const float inverse = __frcp_rn(step);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          auto nibble = [&](float v) {                // code + 8 in the lowest bits
+            const float q = fminf(fmaxf(__fmul_rn(v, inverse), -7.f), 7.f);
+            return __float_as_uint(__fadd_rn(__fadd_rn(__fadd_rn(q, 1536.f), -1536.f), 12582920.f)) & 15u;
+          };
+          code |= (nibble(bf_lo(w[j])) | nibble(bf_hi(w[j])) << 16) << (4 * j);
+        }
+        if (!finite) { code = 0x88888888u; scale = 64u; }
+        if (in[i]) {
+          reinterpret_cast<uint32_t*>(page(i))[at(i) * (kQ4Codes / 4) + l] = code;
+          if ((l & 3u) == 0) page(i)[kQ4ScalesAt + at(i) * 4 + (l >> 2)] = uint8_t(scale);
+          if (l == 0) page(i)[kQ4ExpsAt + at(i)] = uint8_t(exp);
+        }
+      }
+    }
   } else {
     auto held = [&](int i) { return reinterpret_cast<uint2*>(static_cast<uint8_t*>(value[i] ? a.pages.v : a.pages.k) + entry[i] * kKvDim) + l; };
     auto exps = [&](int i) { return (value[i] ? a.pages.v_exp : a.pages.k_exp) + entry[i]; };
@@ -213,18 +316,23 @@ struct KvKeepArgs {
   uint32_t width;
 };
 
-template <bool F8>
+template <int FORMAT>
 __global__ void __launch_bounds__(kKeepThreads)
 kv_keep_kernel(const KvKeepArgs a) {
   step_kernel_entry();
   const uint32_t s = blockIdx.y, tid = threadIdx.x, plane0 = blockIdx.x * kKeepPlanes, planes = min(uint32_t(kKeepPlanes), 2 * a.pages.layers - plane0);
   const int32_t count = min(a.count[s], int32_t(a.width)), seq = a.seqs[s], base = a.base[s];
-  constexpr uint32_t kPieces = (F8 ? 1 : 2) * kKvDim / 16;       // of an entry
+  constexpr bool F8 = FORMAT == kKvE4m3, Q4 = FORMAT == kKvQ4;
+  constexpr uint32_t kPieces = (Q4 ? kQ4Codes : (F8 ? 1 : 2) * kKvDim) / 16;       // of an entry
   const uint32_t per_node = a.pages.nkv * kPieces, nodes = max(1u, kKeepThreads / per_node);
   // plane p: keys (even) or values of layer p / 2
   auto pieces = [&](uint32_t p) {
-    return reinterpret_cast<uint4*>(static_cast<uint8_t*>(p & 1u ? a.pages.v : a.pages.k) + int64_t(p >> 1) * a.pages.layer_stride * (F8 ? 1 : 2));
+    return reinterpret_cast<uint4*>(static_cast<uint8_t*>(p & 1u ? a.pages.v : a.pages.k) + int64_t(p >> 1) * a.pages.layer_stride * (FORMAT == kKvBf16 ? 2 : 1));
   };
+  // index of an entry's first piece (4 bits: in its plane, whose pages hold scales and exponents behind the codes)
+  auto first_piece = [&](size_t entry) { return Q4 ? (q4_page_at(entry) + entry % kKvPage * kQ4Codes) / 16 : entry * kPieces; };
+  auto scales = [&](uint32_t p, size_t entry) { return reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(pieces(p)) + q4_page_at(entry) + kQ4ScalesAt) + entry % kKvPage; };
+  auto q4_exps = [&](uint32_t p, size_t entry) { return reinterpret_cast<uint8_t*>(pieces(p)) + q4_page_at(entry) + kQ4ExpsAt + entry % kKvPage; };
   auto exps = [&](uint32_t p) { return (p & 1u ? a.pages.v_exp : a.pages.k_exp) + int64_t(p >> 1) * a.pages.exp_stride; };
   for (int32_t first = 1; first < count; first += nodes) {
     const uint32_t items = min(nodes, uint32_t(count - first)) * per_node;
@@ -244,12 +352,16 @@ kv_keep_kernel(const KvKeepArgs a) {
       }
       uint4 x[kKeepPlanes];
       uint8_t byte[kKeepPlanes];
+      uint32_t scale[Q4 ? kKeepPlanes : 1];
       if (on) {
 #pragma unroll
         for (int p = 0; p < kKeepPlanes; ++p)
           if (uint32_t(p) < planes) {
-            x[p] = pieces(plane0 + p)[src * kPieces + piece];
+            x[p] = pieces(plane0 + p)[first_piece(src) + piece];
             if (F8 && piece == 0) byte[p] = exps(plane0 + p)[src];
+            if constexpr (Q4) {
+              if (piece == 0) { scale[p] = *scales(plane0 + p, src); byte[p] = *q4_exps(plane0 + p, src); }
+            }
           }
       }
       __syncthreads();
@@ -257,8 +369,11 @@ kv_keep_kernel(const KvKeepArgs a) {
 #pragma unroll
         for (int p = 0; p < kKeepPlanes; ++p)
           if (uint32_t(p) < planes) {
-            pieces(plane0 + p)[dst * kPieces + piece] = x[p];
+            pieces(plane0 + p)[first_piece(dst) + piece] = x[p];
             if (F8 && piece == 0) exps(plane0 + p)[dst] = byte[p];
+            if constexpr (Q4) {
+              if (piece == 0) { *scales(plane0 + p, dst) = scale[p]; *q4_exps(plane0 + p, dst) = byte[p]; }
+            }
           }
       }
       __syncthreads();

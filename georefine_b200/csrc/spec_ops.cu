@@ -1,4 +1,4 @@
-// extern "C" entry points of speculative serving over a BF16 or 8-bit KV cache: argument validation and launch geometry.
+// extern "C" entry points of serving over a paged KV cache in BF16, 8 or 4 bits, and of speculation: argument validation and launch geometry.
 // No allocation and no host synchronisation happen here; errors are returned, never thrown.
 #include <cuda_runtime.h>
 
@@ -9,6 +9,7 @@
 #include "kv_cache.cuh"
 #include "launch_utils.h"
 #include "tree_attention.cuh"
+#include "tree_q4.cuh"
 #include "tree_wide.cuh"
 #include "verify_ops.cuh"
 
@@ -20,10 +21,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 int pages_of(const grb_kv_pages* p, KvPagesArgs& a) {
   if (!p || !p->k || !p->v || !p->layers || !p->pages || !p->nkv) return GRB_ERR_ARGUMENT;
-  if (p->format > GRB_KV_E4M3) return GRB_ERR_UNSUPPORTED;
+  if (p->format > GRB_KV_E4M3 && p->format != GRB_KV_Q4) return GRB_ERR_UNSUPPORTED;
   if (p->format == GRB_KV_E4M3 ? !p->k_exp || !p->v_exp || !aligned16(p->k_exp) || !aligned16(p->v_exp) : p->k_exp || p->v_exp) return GRB_ERR_ARGUMENT;
-  const int64_t entries = int64_t(p->pages) * p->nkv * kKvPage;
-  if (!aligned16(p->k) || !aligned16(p->v) || (p->layers > 1 && (p->layer_stride < entries * int64_t(kKvDim) || (p->layer_stride & 15)))) return GRB_ERR_ARGUMENT;
+  const int64_t entries = int64_t(p->pages) * p->nkv * kKvPage, elements = p->format == GRB_KV_Q4 ? int64_t(p->pages) * p->nkv * kQ4Page : entries * int64_t(kKvDim);
+  if (!aligned16(p->k) || !aligned16(p->v) || (p->layers > 1 && (p->layer_stride < elements || (p->layer_stride & 15)))) return GRB_ERR_ARGUMENT;
   if (p->format == GRB_KV_E4M3 && p->layers > 1 && p->exp_stride < entries) return GRB_ERR_ARGUMENT;
   if (p->pages > 0x7FFFFFu || p->nkv > 4096) return GRB_ERR_UNSUPPORTED;
   a = KvPagesArgs{p->k, p->v, p->k_exp, p->v_exp, p->layer_stride, p->exp_stride, p->layers, p->pages, p->nkv};
@@ -55,19 +56,29 @@ int kv_rows(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t*
   a.rows = rows;
   const uint64_t warps = uint64_t(rows) * ((2 * a.pages.nkv + kKvEntriesPerWarp - 1) / kKvEntriesPerWarp), ctas = (warps + kKvWarps - 1) / kKvWarps;
   if (warps > 0xFFFFFF00ull) return GRB_ERR_UNSUPPORTED;   // (numbered in 32 bits)
-  const auto kernel = pages->format == GRB_KV_E4M3 ? kv_rows_kernel<READ, true> : kv_rows_kernel<READ, false>;
+  const auto kernel = pages->format == GRB_KV_E4M3 ? kv_rows_kernel<READ, kKvE4m3> : pages->format == GRB_KV_Q4 ? kv_rows_kernel<READ, kKvQ4> : kv_rows_kernel<READ, kKvBf16>;
   return launch_step(kernel, dim3(uint32_t(ctas)), dim3(kKvWarps * 32), 0, static_cast<cudaStream_t>(stream), a);
 }
 
-template <bool F8>
+// Positions of a part of the narrow kernels.
+constexpr uint32_t part_positions(uint32_t format) {
+  return format == GRB_KV_Q4 ? TreeQ4::kPositions : format == GRB_KV_E4M3 ? TreePart<true>::kPositions : TreePart<false>::kPositions;
+}
+uint64_t parts_of(uint32_t max_pages, uint32_t format) { return (uint64_t(max_pages) * kKvPage + part_positions(format) - 1) / part_positions(format); }
+
+template <int FORMAT>
 int tree_launch(const TreeArgs& a, cudaStream_t stream) {
-  using P = TreePart<F8>;
+  constexpr bool F8 = FORMAT != kKvBf16;
+  using P = std::conditional_t<FORMAT == kKvQ4, TreeQ4, TreePart<F8>>;
+  void (*part)(TreeArgs);
+  if constexpr (FORMAT == kKvQ4) part = tree_q4_kernel;
+  else part = tree_part_kernel<F8>;
   static std::once_flag once[64];
   static int prepared[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GRB_ERR_CUDA;
   std::call_once(once[dev], [&] {
-    prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_part_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
+    prepared[dev] = cuda_status(cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
     if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem<F8>)));
   });
   if (prepared[dev]) return prepared[dev];
@@ -75,9 +86,9 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   if (sms <= 0) return GRB_ERR_CUDA;
   const uint32_t warps = a.rows * ((a.nq + 2 * a.nkv + kTreeHeadsPerWarp - 1) / kTreeHeadsPerWarp);
   const uint32_t threads = a.rows > kTreePrepThreads ? kTreePrepMost : kTreePrepThreads;
-  if (int st = launch_step(tree_prep_kernel<F8>, dim3((warps + threads / 32 - 1) / (threads / 32) + 1), dim3(threads), a.rows * 6, stream, a, P::kPositions)) return st;
+  if (int st = launch_step(tree_prep_kernel<FORMAT>, dim3((warps + threads / 32 - 1) / (threads / 32) + 1), dim3(threads), a.rows * 6, stream, a, P::kPositions)) return st;
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
-  if (int st = launch_step(tree_part_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
+  if (int st = launch_step(part, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
   if (a.wide_from) {
     if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
   }
@@ -141,15 +152,15 @@ int grb_kv_keep(const grb_kv_pages* pages, const grb_kv_table* table, const int3
   a.count = count;
   a.ldp = ldp;
   a.width = width;
-  const auto kernel = pages->format == GRB_KV_E4M3 ? kv_keep_kernel<true> : kv_keep_kernel<false>;
+  const auto kernel = pages->format == GRB_KV_E4M3 ? kv_keep_kernel<kKvE4m3> : pages->format == GRB_KV_Q4 ? kv_keep_kernel<kKvQ4> : kv_keep_kernel<kKvBf16>;
   return launch_step(kernel, dim3((a.pages.layers * 2 + kKeepPlanes - 1) / kKeepPlanes, n), dim3(kKeepThreads), 0, static_cast<cudaStream_t>(cuda_stream), a);
 }
 
 uint64_t grb_attn_tree_scratch_bytes(uint32_t rows, uint32_t nq, uint32_t max_pages, uint32_t format) {
-  if (!rows || rows > kTreeMaxRows || !nq || !max_pages || format > GRB_KV_E4M3) return 0;
-  const uint64_t parts = uint64_t(max_pages) * (format == GRB_KV_E4M3 ? kKvPage / TreePart<true>::kPositions : kKvPage / TreePart<false>::kPositions);
+  if (!rows || rows > kTreeMaxRows || !nq || !max_pages || (format > GRB_KV_E4M3 && format != GRB_KV_Q4)) return 0;
+  const uint64_t parts = parts_of(max_pages, format);
   const uint64_t pairs = uint64_t(rows) * nq;
-  return ((48 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * (format == GRB_KV_E4M3 ? 2 : 4) + 16 + pairs * parts * (kKvDim * 4 + 8);
+  return ((48 + rows * 40ull + pairs * 4 + 255) & ~uint64_t(255)) + pairs * kKvDim * (format == GRB_KV_BF16 ? 4 : 2) + 16 + pairs * parts * (kKvDim * 4 + 8);
 }
 
 int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
@@ -169,7 +180,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
     return GRB_ERR_ARGUMENT;
   if (!s->rows) return GRB_OK;
   if (s->scratch_bytes < grb_attn_tree_scratch_bytes(s->rows, s->nq, s->table.max_pages, s->pages.format)) return GRB_ERR_WORKSPACE;
-  const bool f8 = s->pages.format == GRB_KV_E4M3;
+  const uint32_t format = s->pages.format;
   a.qkv = static_cast<const __nv_bfloat16*>(s->qkv);
   a.ldq = s->ldq;
   a.cos_table = static_cast<const __nv_bfloat16*>(s->cos_table);
@@ -183,7 +194,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.ldm = s->ldm;
   a.mask_words = s->mask_words;
   a.rows = s->rows;
-  a.max_parts = s->table.max_pages * (f8 ? kKvPage / TreePart<true>::kPositions : kKvPage / TreePart<false>::kPositions);
+  a.max_parts = uint32_t(parts_of(s->table.max_pages, format));
   a.tile_rows = 16 / a.group;
   a.wide_rows = kWideTile / a.group;
   // Runs for the wide kernel: trees of more rows than two tiles of the narrow one take; of causal rows prompt chunks, so that the
@@ -195,7 +206,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   // behind 2048 positions 148 us instead of 135); guessing from the other rows of the call would have them change a run's bits.
   const uint32_t longest = s->longest_run ? s->longest_run : s->row_base ? s->rows : 1u;
   a.wide_from = s->row_base ? 32 / a.group + 1 : 64;
-  if (a.wide_from > s->rows || a.wide_from > longest) a.wide_from = 0;
+  if (a.wide_from > s->rows || a.wide_from > longest || s->pages.format == GRB_KV_Q4) a.wide_from = 0;
   a.scaling = s->scaling;
   a.out = static_cast<__nv_bfloat16*>(s->out);
   a.ldo = s->ldo;
@@ -210,13 +221,13 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.q_scale = reinterpret_cast<float*>(a.row_parts + a.rows);
   at += (48 + a.rows * 40ull + pairs * 4 + 255) & ~uint64_t(255);
   a.q = reinterpret_cast<uint16_t*>(at);
-  at += pairs * kKvDim * (f8 ? 2 : 4);
+  at += pairs * kKvDim * (format == GRB_KV_BF16 ? 4 : 2);
   at += reinterpret_cast<uintptr_t>(at) & 16;                // (the scratch starts on 16 bytes, the parts on 32)
   a.part_acc = reinterpret_cast<float*>(at);
   at += pairs * a.max_parts * kKvDim * 4;
   a.part_ml = reinterpret_cast<float2*>(at);
   const auto stream = static_cast<cudaStream_t>(cuda_stream);
-  return f8 ? tree_launch<true>(a, stream) : tree_launch<false>(a, stream);
+  return format == GRB_KV_Q4 ? tree_launch<kKvQ4>(a, stream) : format == GRB_KV_E4M3 ? tree_launch<kKvE4m3>(a, stream) : tree_launch<kKvBf16>(a, stream);
 }
 
 int grb_verify_drafts(const grb_verify_step* s, void* cuda_stream) {

@@ -186,14 +186,46 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
   if (tid == 0) a.plan[0] = uint32_t(done >> 32), a.plan[1] = uint32_t(done), a.plan[2] = uint32_t(wide_done >> 32), a.plan[3] = uint32_t(wide_done);
 }
 
+// An entry of a 4-bit page from a warp whose lanes hold dimensions 2 l, 2 l + 1, 64 + 2 l and 64 + 2 l + 1.
+__device__ __forceinline__ void tree_store_q4(uint8_t* page, uint32_t at, float (&x)[4], uint32_t lane) {
+  bool fine = true;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) fine = fine && fabsf(x[k]) <= 3.4028234e38f;
+  fine = __all_sync(0xFFFFFFFFu, fine);
+  float group[2];                                            // of dimensions 32 (l / 16) .. and 64 + 32 (l / 16) ..
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    group[h] = fine ? fmaxf(fabsf(x[2 * h]), fabsf(x[2 * h + 1])) : 0.f;
+#pragma unroll
+    for (int off = 8; off; off >>= 1) group[h] = fmaxf(group[h], __shfl_xor_sync(0xFFFFFFFFu, group[h], off));
+  }
+  const float top = fmaxf(group[0], group[1]);
+  const uint32_t exp = q4_exp_byte(fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16)), true);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float step;
+    const uint32_t scale = q4_scale_byte(group[h], exp, step);
+    // dimensions 2 l and 2 l + 1 are nibble l % 4 of either half of word l / 4
+    uint32_t code = 0x00080008u;
+    if (fine) code = q4_nibble(__fdiv_rn(x[2 * h], step)) | q4_nibble(__fdiv_rn(x[2 * h + 1], step)) << 16;
+    code <<= 4 * (lane & 3u);
+    code |= __shfl_xor_sync(0xFFFFFFFFu, code, 1);
+    code |= __shfl_xor_sync(0xFFFFFFFFu, code, 2);
+    if ((lane & 3u) == 0) reinterpret_cast<uint32_t*>(page)[at * (kQ4Codes / 4) + 8 * h + (lane >> 2)] = code;
+    if ((lane & 15u) == 0) page[kQ4ScalesAt + at * 4 + 2 * h + (lane >> 4)] = uint8_t(scale);
+  }
+  if (lane == 0) page[kQ4ExpsAt + at] = uint8_t(fine ? exp : kKvNanByte);
+}
+
 // The first CTA lays down the plan; in the others a warp takes up to eight neighbouring heads of a row, all their loads on their
 // way together.  A lane owns dimensions 2 l, 2 l + 1 and the two that the rotation pairs with them.  The products of BF16 values are
 // exact in FP32, so the rotation rounds once before the result is rounded to its type.  1024 rows of 56 heads: 15 us (one head a
 // warp 43; 256 rows of the plan at a time 27).  One row: 7 us, the plan's chain of dependent loads.
 constexpr uint32_t kTreeHeadsPerWarp = 8;
-template <bool F8>
+template <int FORMAT>
 __global__ void __launch_bounds__(kTreePrepMost)
 tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
+  constexpr bool F8 = FORMAT != kKvBf16;                   // queries in FP16, as for all caches that are decoded to it
   step_kernel_entry();
   if (blockIdx.x == 0) return tree_plan(a, part_positions);
   const uint32_t heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 31u, per_row = (heads + kTreeHeadsPerWarp - 1) / kTreeHeadsPerWarp;
@@ -267,7 +299,9 @@ tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
     }
     const size_t entry = kv_entry(place, a.nkv, value ? head - a.nq - a.nkv : head - a.nq);
     void* const pages = value ? a.pages.v : a.pages.k;
-    if constexpr (F8) {
+    if constexpr (FORMAT == kKvQ4) {
+      tree_store_q4(static_cast<uint8_t*>(pages) + q4_page_at(entry), uint32_t(entry % kKvPage), x, lane);
+    } else if constexpr (F8) {
       const uint32_t byte = kv_warp_byte(x);
       uint16_t* dst = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(pages) + entry * kKvDim) + lane;
       dst[0] = uint16_t(kv_codes(x[0], x[1], byte));
@@ -348,10 +382,8 @@ template <bool F8>
 __device__ __forceinline__ void tree_locate(const TreeArgs& a, TreeUnit& t) {
   t.k = t.npos ? int64_t(kv_entry(t.place, a.nkv, t.kvh)) * TreePart<F8>::kRowBytes : 0;
 }
-// The unit of number u.  Whole warp.
-template <bool F8>
-__device__ __forceinline__ TreeUnit tree_unit(const TreeArgs& a, uint32_t u, uint32_t tiles) {
-  TreeUnit t;
+// The tile of unit number u.  Whole warp.
+__device__ __forceinline__ uint32_t tree_tile_of(const TreeArgs& a, uint32_t u, uint32_t tiles) {
   const uint32_t lane = threadIdx.x & 31u;
   uint32_t lo = 0, n = tiles;                              // the tile is one of n from lo on
   while (n > 1) {
@@ -361,8 +393,14 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeArgs& a, uint32_t u, uin
     lo += k * step;
     n = min(step, n - k * step);
   }
-  t.tile = lo;
-  const int4 d = a.tiles[lo];
+  return lo;
+}
+// The unit of number u.  Whole warp.
+template <bool F8>
+__device__ __forceinline__ TreeUnit tree_unit(const TreeArgs& a, uint32_t u, uint32_t tiles) {
+  TreeUnit t;
+  t.tile = tree_tile_of(a, u, tiles);
+  const int4 d = a.tiles[t.tile];
   tree_set_tile<F8>(a, t, d);
   const uint32_t local = u - uint32_t(d.z);
   t.kvh = local % a.nkv;

@@ -99,9 +99,11 @@ class PagedAttention:
         _native.check(st, "grb_attn_decode_bf16")
 
 
-# ---- a cache in BF16 or in 8 bits, and attention of causal rows and draft trees over it ---------------------------------
+# ---- a cache in BF16, 8 or 4 bits, and attention of causal rows and draft trees over it --------------------------------
 
-KV_FORMATS = ("bf16", "e4m3")
+KV_FORMATS = ("bf16", "e4m3")                       # of 128 numbers an entry
+KV_CODES = {"bf16": 0, "e4m3": 1, "q4": 4}          # all formats, and their numbers in the C interface
+Q4_ROWS = 69          # rows of 256 bytes of a 4-bit page of one head; bytes of an entry
 MASK_WORDS = 4        # of 64 nodes: the largest tree a row's mask describes
 TREE_ROWS = 4096      # rows of one call
 
@@ -152,20 +154,21 @@ def _launch(device, name, *args):
 class KVPages:
     """Keys and values of one layer, [pages, kv heads, 256, 128], or of a stack of layers ([layers, pages, ...], layers may be
     strided): BF16, or ``float8_e4m3fn`` codes with an exponent byte per entry (128 values of one head at one position) in
-    ``k_exp`` and ``v_exp``, [pages, kv heads, 256] (see ``csrc/kv_cache.cuh`` for the format).  An object holds no copies."""
+    ``k_exp`` and ``v_exp``, [pages, kv heads, 256].  In 4 bits (``"q4"``: 69 bytes for an entry of 256) pages are ``uint8`` [pages, kv heads,
+    69, 256] and hold codes, scales and exponents together.  The formats are in ``csrc/kv_cache.cuh``.  An object holds no copies."""
 
     def __init__(self, k, v, k_exp=None, v_exp=None):
         import torch
 
-        if k.dim() not in (4, 5) or tuple(k.shape[-2:]) != (PAGE, HEAD_DIM):
-            raise ValueError("pages are [pages, kv heads, 256, 128], or that with the layers in front")
+        if k.dim() not in (4, 5) or tuple(k.shape[-2:]) != ((Q4_ROWS, PAGE) if k.dtype == torch.uint8 else (PAGE, HEAD_DIM)):
+            raise ValueError("pages are [pages, kv heads, 256, 128] (4 bits: [pages, kv heads, 69, 256]), or that with the layers in front")
         if k.device.type != "cuda":
             raise ValueError("pages live on a CUDA device")
-        self.format = {torch.bfloat16: "bf16", torch.float8_e4m3fn: "e4m3"}.get(k.dtype)
+        self.format = {torch.bfloat16: "bf16", torch.float8_e4m3fn: "e4m3", torch.uint8: "q4"}.get(k.dtype)
         if self.format is None:
-            raise ValueError(f"pages are BF16 or e4m3, not {k.dtype}")
+            raise ValueError(f"pages are BF16, e4m3 or bytes of 4-bit pages, not {k.dtype}")
         _on(v, k.device, k.dtype, "values", tuple(k.shape))
-        if (k_exp is None) != (self.format == "bf16") or (v_exp is None) != (self.format == "bf16"):
+        if (k_exp is None) != (self.format != "e4m3") or (v_exp is None) != (self.format != "e4m3"):
             raise ValueError("exponents go with e4m3 pages, and with those alone")
         for t, what in ((k, "keys"), (v, "values"), (k_exp, "exponents of keys"), (v_exp, "exponents of values")):
             if t is None:
@@ -182,7 +185,7 @@ class KVPages:
         stride = (k.stride(0), 0 if k_exp is None else k_exp.stride(0)) if self.stacked else (0, 0)
         # (fields of the C structure)
         self._fields = (k.data_ptr(), v.data_ptr(), 0 if k_exp is None else k_exp.data_ptr(), 0 if v_exp is None else v_exp.data_ptr(), *stride,
-                        k.shape[0] if self.stacked else 1, self.pages, self.kv_heads, KV_FORMATS.index(self.format))
+                        k.shape[0] if self.stacked else 1, self.pages, self.kv_heads, KV_CODES[self.format])
         self._packed = _native.KV_PAGES.pack(*self._fields)
 
     @classmethod
@@ -190,9 +193,11 @@ class KVPages:
         """Empty pages (zeros)."""
         import torch
 
-        if kv_format not in KV_FORMATS:
-            raise ValueError(f"the cache's format is one of {KV_FORMATS}")
+        if kv_format not in KV_CODES:
+            raise ValueError(f"the cache's format is one of {tuple(KV_CODES)}")
         shape = (() if layers is None else (int(layers),)) + (int(pages), int(kv_heads), PAGE, HEAD_DIM)
+        if kv_format == "q4":
+            return cls(*(torch.zeros(*shape[:-2], Q4_ROWS, PAGE, device=device, dtype=torch.uint8) for _ in range(2)))
         if kv_format == "bf16":
             return cls(*(torch.zeros(shape, device=device, dtype=torch.bfloat16) for _ in range(2)))
         return cls(*(torch.zeros(shape, device=device, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)),
@@ -206,7 +211,7 @@ class KVPages:
     @property
     def entry_bytes(self) -> int:
         """Bytes of the cache per position, key or value head."""
-        return 2 * HEAD_DIM if self.format == "bf16" else HEAD_DIM + 1
+        return {"bf16": 2 * HEAD_DIM, "e4m3": HEAD_DIM + 1, "q4": Q4_ROWS}[self.format]
 
 
 def _table(page_table, device):
@@ -302,21 +307,21 @@ class TreeRows:
 
 
 class TreeAttention:
-    """Attention over a cache in BF16 or 8 bits, for causal rows and for nodes of draft trees: scratch and geometry for up to
+    """Attention over a cache in BF16, 8 or 4 bits, for causal rows and for nodes of draft trees: scratch and geometry for up to
     ``max_rows`` rows a call and ``max_pages`` pages a sequence; ``__call__`` runs rotary embedding, append and attention for one
     layer.  Up to 16 query heads per kv head.  Calls that may run at the same time need an object each: they share its scratch."""
 
     def __init__(self, nq: int, nkv: int, max_rows: int, max_pages: int, device, *, kv_format="bf16"):
         import torch
 
-        if kv_format not in KV_FORMATS:
-            raise ValueError(f"the cache's format is one of {KV_FORMATS}")
+        if kv_format not in KV_CODES:
+            raise ValueError(f"the cache's format is one of {tuple(KV_CODES)}")
         if nq < 1 or nkv < 1 or nq % nkv or nq // nkv > 16:
             raise ValueError("query heads per kv head: a whole number up to 16")
         if not 1 <= max_rows <= TREE_ROWS or max_pages < 1:
             raise ValueError(f"1 to {TREE_ROWS} rows and at least one page")
         self.nq, self.nkv, self.max_rows, self.max_pages, self.format = nq, nkv, int(max_rows), int(max_pages), kv_format
-        self.scratch_bytes = _native.lib().grb_attn_tree_scratch_bytes(self.max_rows, nq, self.max_pages, KV_FORMATS.index(kv_format))
+        self.scratch_bytes = _native.lib().grb_attn_tree_scratch_bytes(self.max_rows, nq, self.max_pages, KV_CODES[kv_format])
         self.scratch = torch.empty(self.scratch_bytes, device=device, dtype=torch.uint8)
         self.scratch[:16].zero_()
         self.status = self.scratch[:4].view(torch.int32)

@@ -221,11 +221,13 @@ class DecoderWeights:
 
 
 def kv_buffers(shape, device, kv_format):
-    """A cache [..., 256, 128] of zeros and, in 8 bits, its exponents [..., 256] (else None)."""
+    """A cache [..., 256, 128] (4 bits: [..., 69, 256]) of zeros and, in 8 bits, its exponents [..., 256] (else None)."""
     import torch
 
     if kv_format == "bf16":
         return torch.zeros(*shape, PAGE, ops.HEAD_DIM, device=device, dtype=torch.bfloat16), None
+    if kv_format == "q4":
+        return torch.zeros(*shape, ops.Q4_ROWS, PAGE, device=device, dtype=torch.uint8), None
     z = lambda *s: torch.zeros(*s, device=device, dtype=torch.uint8)
     return z(*shape, PAGE, ops.HEAD_DIM).view(torch.float8_e4m3fn), z(*shape, PAGE)
 
@@ -240,7 +242,8 @@ class BatchDecoder:
     (``set_tree_rows``), no advance.
 
     ``kv_format`` "e4m3" holds the KV cache in 8 bits (129 bytes for an entry of 256, each value off by at most 2^-4 of
-    itself; the format is in ``csrc/kv_cache.cuh``)."""
+    itself), "q4" in 4 (69 bytes, each value off by a fourteenth of the largest of its 32 neighbours, give or take a thirtieth of
+    that); the formats are in ``csrc/kv_cache.cuh``."""
 
     def __init__(self, weights: DecoderWeights, *, max_rows=128, max_slots=128, max_context=2304, device="cuda:0", kv_format="bf16"):
         import torch
@@ -248,8 +251,8 @@ class BatchDecoder:
         cfg = weights.config
         if cfg.head_dim != ops.HEAD_DIM:
             raise ValueError("the attention kernels are written for head dimension 128")
-        if kv_format not in ops.KV_FORMATS:
-            raise ValueError(f"the cache's format is one of {ops.KV_FORMATS}")
+        if kv_format not in ops.KV_CODES:
+            raise ValueError(f"the cache's format is one of {tuple(ops.KV_CODES)}")
         self.w, self.cfg, self.dev = weights, cfg, torch.device(device)
         self.max_rows, self.max_slots = int(max_rows), int(max_slots)
         self.pages_per_seq = -(-int(max_context) // PAGE)
@@ -508,7 +511,7 @@ class BatchDecoder:
 
     def streamed_bytes(self, rows_context) -> dict:
         """Bytes one step streams: the compressed weights, and the KV cache of rows whose contexts are given."""
-        entry = self.cfg.head_dim + 1 if self.kv_format == "e4m3" else 2 * self.cfg.head_dim
+        entry = {"bf16": 2 * self.cfg.head_dim, "e4m3": self.cfg.head_dim + 1, "q4": ops.Q4_ROWS}[self.kv_format]
         kv = sum(int(c) for c in rows_context) * self.cfg.local_kv_heads * entry * 2 * self.cfg.layers
         return {"weights": self.w.streamed_bytes(), "kv": kv}
 

@@ -401,8 +401,10 @@ int grb_attn_decode_bf16(const grb_attn_step* step, void* cuda_stream);
  * ------------------------------------------------------------------------------------------------- */
 #define GRB_KV_BF16 0
 #define GRB_KV_E4M3 1
+#define GRB_KV_Q4 4
 typedef struct grb_kv_pages {
-  void* k;                    /* [layers][pages][nkv][256][128] BF16 or e4m3 codes, layers layer_stride elements apart */
+  void* k;                    /* [layers][pages][nkv][256][128] BF16 or e4m3 codes, [layers][pages][nkv][17664] bytes (GRB_KV_Q4);
+                                 layers layer_stride elements apart */
   void* v;
   uint8_t* k_exp;             /* GRB_KV_E4M3: [layers][pages][nkv][256], layers exp_stride bytes apart; else NULL */
   uint8_t* v_exp;
