@@ -71,14 +71,19 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   constexpr bool F8 = FORMAT != kKvBf16;
   using P = std::conditional_t<FORMAT == kKvQ4, TreeQ4, TreePart<F8>>;
   void (*part)(TreeArgs);
-  if constexpr (FORMAT == kKvQ4) part = tree_q4_kernel;
+  if constexpr (FORMAT == kKvQ4) part = a.tile_rows * a.group <= 8 ? tree_q4_kernel<1> : tree_q4_kernel<2>;
   else part = tree_part_kernel<F8>;
   static std::once_flag once[64];
   static int prepared[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GRB_ERR_CUDA;
   std::call_once(once[dev], [&] {
-    prepared[dev] = cuda_status(cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
+    if constexpr (FORMAT == kKvQ4) {
+      for (auto kernel : {tree_q4_kernel<1>, tree_q4_kernel<2>})
+        if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
+    } else {
+      prepared[dev] = cuda_status(cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
+    }
     if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem<F8>)));
   });
   if (prepared[dev]) return prepared[dev];
@@ -195,7 +200,8 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.mask_words = s->mask_words;
   a.rows = s->rows;
   a.max_parts = uint32_t(parts_of(s->table.max_pages, format));
-  a.tile_rows = 16 / a.group;
+  // (4 bits: a tile of eight columns where the caller says that one row of a sequence comes at a time, whatever comes then; a row's bits are the same)
+  a.tile_rows = (format == GRB_KV_Q4 && s->longest_run == 1 && a.group <= 8 ? 8 : 16) / a.group;
   a.wide_rows = kWideTile / a.group;
   // Runs for the wide kernel: trees of more rows than two tiles of the narrow one take; of causal rows prompt chunks, so that the
   // rows of a speculative chain keep the bits of single steps.  A run's rows alone decide, whatever else is in the call, so one run

@@ -54,7 +54,7 @@ struct TreeArgs {
   uint32_t* status;           // scratch: kStatusTimeout where a wait ran out
   int32_t* extent;            // scratch: [rows]: positions up to the last one the row sees
   uint32_t* row_parts;        // scratch: [rows]: parts of the row
-  int4* tiles;                // scratch: [rows]: first row, rows, first unit, positions up to the last one its rows see
+  int4* tiles;                // scratch: [rows]: first row, rows, units (4 bits: weight of the units) before it, positions up to the last one its rows see
   int4* wide_tiles;           // scratch: [rows]: first row, rows, first unit, positions of a unit
   uint32_t* plan;             // scratch: tiles, units, wide tiles, wide units, wide units taken
   float* part_acc;            // scratch: [rows][nq][max_parts][128]
@@ -121,8 +121,13 @@ __device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
   return warp ? op(before, v) : v;
 }
 
+// Weight of a unit of so many positions in the 4-bit kernel: its steps of 128 positions, and a step's time for its beginning and end.
+__device__ __forceinline__ uint32_t tree_q4_weight(uint32_t positions) { return (positions + 127) / 128 + 1; }
+
 // A tile is up to tile_rows (wide_rows) consecutive rows of one sequence; rows that are left out or see nothing may be among them.
 // What it needs of the rows is read once, side by side; the rest runs in shared memory.
+// A tile's units have a weight each, one in the kernels that deal them out by number.
+template <int FORMAT>
 __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_positions) {
   extern __shared__ int32_t extents[];                       // [rows]; -1: left out
   uint16_t* const run_of = reinterpret_cast<uint16_t*>(extents + a.rows);      // [rows]: first row of the row's run (rows of one sequence in a row)
@@ -164,7 +169,11 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
       }
       if (!wide) a.row_parts[r] = extents[r] < 0 ? kTreeRowAbsent : (uint32_t(extents[r]) + part_positions - 1) / part_positions;
     }
-    const unsigned long long mine = parts ? (1ull << 32) + parts * a.nkv : 0ull;
+    uint32_t weight = parts;
+    if constexpr (FORMAT == kKvQ4) {
+      if (!wide && parts) weight = (parts - 1) * tree_q4_weight(part_positions) + tree_q4_weight(uint32_t(extent) - (parts - 1) * part_positions);
+    }
+    const unsigned long long mine = parts ? (1ull << 32) + weight * a.nkv : 0ull;
     auto scan = [&](bool counts, unsigned long long before) {
       const auto sum = [](unsigned long long x, unsigned long long y) { return x + y; };
       const unsigned long long upto = before + cta_scan(counts ? mine : 0ull, sums, sum);
@@ -172,7 +181,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
       return upto;
     };
     const unsigned long long upto = scan(!wide, done);
-    if (parts && !wide) a.tiles[(upto >> 32) - 1] = make_int4(int32_t(r), int32_t(n), int32_t(uint32_t(upto) - parts * a.nkv), extent);
+    if (parts && !wide) a.tiles[(upto >> 32) - 1] = make_int4(int32_t(r), int32_t(n), int32_t(uint32_t(upto) - weight * a.nkv), extent);
     __syncthreads();
     done = total;
     if (a.wide_from) {
@@ -227,7 +236,7 @@ __global__ void __launch_bounds__(kTreePrepMost)
 tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
   constexpr bool F8 = FORMAT != kKvBf16;                   // queries in FP16, as for all caches that are decoded to it
   step_kernel_entry();
-  if (blockIdx.x == 0) return tree_plan(a, part_positions);
+  if (blockIdx.x == 0) return tree_plan<FORMAT>(a, part_positions);
   const uint32_t heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 31u, per_row = (heads + kTreeHeadsPerWarp - 1) / kTreeHeadsPerWarp;
   const uint32_t at = (blockIdx.x - 1) * (blockDim.x / 32) + (threadIdx.x >> 5), row = at / per_row, head0 = at % per_row * kTreeHeadsPerWarp;
   if (row >= a.rows) return;

@@ -19,13 +19,17 @@ struct TreeQ4 {
   static constexpr int kThreads = 128;
   static constexpr uint32_t kPositions = 512;                // of a part
   static constexpr uint32_t kChunk = 32;                     // positions of a warp's step
-  static constexpr uint32_t kStages = 4;
+  static constexpr uint32_t kStages = 4;                     // a warp's chunks of a unit
   static constexpr uint32_t kVAt = kChunk * kQ4Codes, kKScalesAt = 2 * kVAt, kVScalesAt = kKScalesAt + kChunk * 4, kKExpsAt = kVScalesAt + kChunk * 4,
                             kVExpsAt = kKExpsAt + kChunk, kStage = kVExpsAt + kChunk;
-  static constexpr uint32_t kSmem = 4 * kStages * kStage;
+  static constexpr uint32_t kWarp = kStages * kStage + kChunk * 16;    // and what the exponents of the chunk at hand mean
+  static constexpr uint32_t kSmem = 4 * kWarp;
 };
+static_assert(TreeQ4::kStages * 4 * TreeQ4::kChunk == TreeQ4::kPositions && TreeQ4::kPositions == 2 * kKvPage, "a unit is two pages, four chunks a warp");
 static_assert(TreeQ4::kStage >= 8 * kKvDim * 4, "a warp's stage holds its part of the merge, eight columns at a time");
 static_assert(TreeQ4::kStage % 16 == 0 && kKvPage % TreeQ4::kChunk == 0, "copies of 16 bytes; a chunk lies in one page");
+
+constexpr float kQ4Bias = 7.f;                               // FP16 weights: up to 2^(7 + the 8 by which a score may pass the reference)
 
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
@@ -37,6 +41,15 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// The product of mma_f16_16816, and loads from shared memory, that the compiler may move: a tile's loads go before the products of the tile
+// before it.
+__device__ __forceinline__ void mma_q4(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <class T>
+__device__ __forceinline__ T q4_ld(const unsigned char* p) { return *reinterpret_cast<const T*>(p); }
 // An 8 x 8 matrix of 16-bit values across the warp, transposed.
 __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   uint32_t r;
@@ -61,9 +74,10 @@ __device__ __forceinline__ void q4_operands(uint32_t w, const Q4Factors& f, uint
   y[3] = fma_f16x2(upper & 0x00F000F0u, f.high, f.offset);
 }
 
-// Units are numbered as in tree_part_kernel: tile by tile, part by part, kv head by kv head; a CTA takes a run of them.
+// Units follow one another tile by tile, part by part, kv head by kv head; a CTA takes those that start in its share of the plan's weights.
 struct Q4Unit {
   uint32_t tile, first, rows, kvh, part, parts;
+  uint32_t at;              // where the unit starts, in weights
   int32_t seq, extent;
 };
 __device__ __forceinline__ void q4_set_tile(const TreeArgs& a, Q4Unit& t) {
@@ -74,13 +88,32 @@ __device__ __forceinline__ void q4_set_tile(const TreeArgs& a, Q4Unit& t) {
   t.parts = (uint32_t(t.extent) + TreeQ4::kPositions - 1) / TreeQ4::kPositions;
   t.seq = a.row_seq[t.first];
 }
-__device__ __forceinline__ void q4_next(const TreeArgs& a, Q4Unit& t) {
-  if (++t.kvh < a.nkv) return;
+__device__ __forceinline__ uint32_t q4_unit_weight(const Q4Unit& t) { return tree_q4_weight(min(TreeQ4::kPositions, uint32_t(t.extent) - t.part * TreeQ4::kPositions)); }
+__device__ __forceinline__ void q4_next(const TreeArgs& a, Q4Unit& t, uint32_t end) {
+  t.at += q4_unit_weight(t);
+  if (++t.kvh < a.nkv || t.at >= end) return;
   t.kvh = 0;
   if (++t.part < t.parts) return;
   t.part = 0;
   ++t.tile;
   q4_set_tile(a, t);
+}
+// The first unit that starts at weight `from` or behind it, below `end`; none: one that starts at `end` or behind it.  Whole warp.
+__device__ __forceinline__ Q4Unit q4_first(const TreeArgs& a, uint32_t from, uint32_t end, uint32_t tiles) {
+  Q4Unit t;
+  t.tile = tree_tile_of(a, from, tiles);
+  q4_set_tile(a, t);
+  const uint32_t before = uint32_t(a.tiles[t.tile].z), part = tree_q4_weight(TreeQ4::kPositions) * a.nkv;     // (of all parts but the last)
+  t.part = (from - before) / part;
+  t.kvh = 0;
+  t.at = before + t.part * part;
+  const uint32_t unit = q4_unit_weight(t), skip = (from - t.at + unit - 1) / unit;
+  if (skip) {
+    t.kvh = skip - 1;
+    t.at += (skip - 1) * unit;
+    q4_next(a, t, end);
+  }
+  return t;
 }
 // Chunks that a warp takes of the unit: positions 512 part + 128 i + 32 warp .. + 31 for i below this.
 __device__ __forceinline__ uint32_t q4_chunks(const Q4Unit& t, uint32_t warp) {
@@ -88,17 +121,21 @@ __device__ __forceinline__ uint32_t q4_chunks(const Q4Unit& t, uint32_t warp) {
   return uint32_t(max(n, 0) + 4 * TreeQ4::kChunk - 1) / (4 * TreeQ4::kChunk);
 }
 
-// What a lane keeps of a unit's columns: of block b, the queries of column 8 b + lane / 4 as B operands, and of its score columns
-// 8 b + 2 (lane % 4) + j the factor, the row, and the position below which the row sees everything.
+// What a lane keeps of a unit's columns: of block b, the queries of column 8 b + lane / 4 as B operands, the factors of its score columns
+// 8 b + 2 (lane % 4) and the next; and the position below which all rows see everything.
 template <int NB>
 struct Q4Columns {
   uint4 q[NB][4];
-  float scale[NB][2];
-  int32_t below[NB][2];            // behind it, in a tree, the mask decides; columns that are nobody's see everything
+  float2 scale[NB];
+  int32_t plain;
 };
+constexpr float kQ4Nothing = -3.4028234e38f;       // the reference of a column that has seen nothing
 
 struct Q4Warp {                    // a lane's places, the same for all units
   uint32_t warp, lane, r, c, place;      // place: of MMA row r (and, 8 further, of row r + 8) among a tile's 16 positions
+  uint32_t per_group;                    // a number below 16 over the group, in units of 2^-16
+  unsigned char* meaning;                // the warp's table of what exponents mean
+  __device__ __forceinline__ uint32_t row_of(uint32_t column) const { return column * per_group >> 16; }
 };
 
 template <int NB>
@@ -106,26 +143,33 @@ __device__ __forceinline__ void q4_ask_columns(const TreeArgs& a, const Q4Unit& 
   const uint32_t used = t.rows * a.group;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const uint32_t n = 8 * b + w.r, rl = n / a.group;
+    const uint32_t n = 8 * b + w.r, rl = w.row_of(n);
     const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t(t.first + rl) * a.nq + t.kvh * a.group + (n - rl * a.group)) * kKvDim + 32 * w.c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) k.q[b][i] = n < used ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t m = 8 * b + 2 * w.c + j, ml = m / a.group, row = t.first + ml;
-      const bool in = m < used;
-      k.scale[b][j] = in ? a.q_scale[size_t(row) * a.nq + t.kvh * a.group + (m - ml * a.group)] : 0.f;
-      k.below[b][j] = in ? a.row_base ? min(a.row_base[row], a.extent[row]) : a.extent[row] : 0x7FFFFFFF;
-    }
+    const uint32_t m = 8 * b + 2 * w.c, m0 = w.row_of(m), m1 = w.row_of(m + 1), head = t.kvh * a.group;
+    k.scale[b] = make_float2(m < used ? a.q_scale[size_t(t.first + m0) * a.nq + head + (m - m0 * a.group)] : 0.f,
+                             m + 1 < used ? a.q_scale[size_t(t.first + m1) * a.nq + head + (m + 1 - m1 * a.group)] : 0.f);
+  }
+  k.plain = 0x7FFFFFFF;
+  for (uint32_t i = 0; i < t.rows; ++i) {
+    const int32_t e = a.extent[t.first + i];
+    k.plain = min(k.plain, a.row_base ? min(a.row_base[t.first + i], e) : e);
   }
 }
 
 // One warp's 32 positions from `at` on, against NB blocks of eight columns.
 template <int NB>
-__device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, const Q4Warp& w, uint32_t stage, int32_t at, const Q4Columns<NB>& k, float (&ref)[NB][2],
-                                         float (&sum)[NB][2], float (&o)[NB][8][4]) {
-  constexpr float kSlack = 8.f, kBias = 7.f;                 // FP16 weights: up to 2^(7 + 8)
+__device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, const Q4Warp& w, unsigned char* stage, int32_t at, const Q4Columns<NB>& k, float2 (&ref)[NB],
+                                         float2 (&sum)[NB], float (&o)[NB][8][4]) {
+  constexpr float kSlack = 8.f;
   using P = TreeQ4;
+  {                                                          // each lane a position: 2^e of K; e and 2^-e of V
+    const uint32_t kb = q4_ld<uint8_t>(stage + P::kKExpsAt + w.lane), vb = max(uint32_t(q4_ld<uint8_t>(stage + P::kVExpsAt + w.lane)), kKvLeastByte);
+    const float add = vb == kKvNanByte ? __uint_as_float(0x7FC00000u) : __fsub_rn(__uint_as_float(0x4B000000u | vb), 8388735.f);      // 2^23 + 127
+    *reinterpret_cast<uint4*>(w.meaning + 16 * w.lane) = make_uint4(kb << 23, __float_as_uint(add), __float_as_uint(kv_inverse(vb)), 0u);
+    __syncwarp();
+  }
   float s[2][NB][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {                              // 16 positions
@@ -134,9 +178,9 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[i][b][e] = 0.f;
     const uint32_t p = 16 * i + w.place;
-    const uint4 k0 = lds128(stage + p * kQ4Codes + 16 * w.c), k1 = lds128(stage + (p + 8) * kQ4Codes + 16 * w.c);
+    const uint4 k0 = q4_ld<uint4>(stage + p * kQ4Codes + 16 * w.c), k1 = q4_ld<uint4>(stage + (p + 8) * kQ4Codes + 16 * w.c);
     // (a lane's 16 bytes are a group of 32 dimensions of one position: one scale)
-    const Q4Factors f0 = q4_factors(lds_u8(stage + P::kKScalesAt + 4 * p + w.c) * 0x10001u), f1 = q4_factors(lds_u8(stage + P::kKScalesAt + 4 * (p + 8) + w.c) * 0x10001u);
+    const Q4Factors f0 = q4_factors(q4_ld<uint8_t>(stage + P::kKScalesAt + 4 * p + w.c) * 0x10001u), f1 = q4_factors(q4_ld<uint8_t>(stage + P::kKScalesAt + 4 * (p + 8) + w.c) * 0x10001u);
     const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -146,45 +190,42 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
       const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        mma_f16_16816(s[i][b], a0, k.q[b][j].x, k.q[b][j].y);
-        mma_f16_16816(s[i][b], a1, k.q[b][j].z, k.q[b][j].w);
+        mma_q4(s[i][b], a0, k.q[b][j].x, k.q[b][j].y);
+        mma_q4(s[i][b], a1, k.q[b][j].z, k.q[b][j].w);
       }
     }
   }
   // scores in units of log 2, with V's exponent; masked where some row does not see the whole chunk
   float inverse[2][2];                                       // 2^-e of V
-  bool hole = false;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) hole = hole || min(k.below[b][0], k.below[b][1]) < at + int32_t(P::kChunk);
-  const bool holes = __any_sync(0xFFFFFFFFu, hole);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t p = 16 * i + 8 * h + w.place;
-      const uint32_t kb = lds_u8(stage + P::kKExpsAt + p), vb = max(lds_u8(stage + P::kVExpsAt + p), kKvLeastByte);
-      const float up = kv_scale(kb), add = vb == kKvNanByte ? __uint_as_float(0x7FC00000u) : __fsub_rn(__uint_as_float(0x4B000000u | vb), 8388735.f);      // 2^23 + 127
-      inverse[i][h] = kv_inverse(vb);
+      const uint4 e = q4_ld<uint4>(w.meaning + 16 * (16 * i + 8 * h + w.place));
+      const float2 up = make_float2(__uint_as_float(e.x), __uint_as_float(e.x)), add = make_float2(__uint_as_float(e.y), __uint_as_float(e.y));
+      inverse[i][h] = __uint_as_float(e.z);
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) s[i][b][2 * h + j] = __fmaf_rn(__fmul_rn(s[i][b][2 * h + j], k.scale[b][j]), up, add);
+      for (int b = 0; b < NB; ++b) {
+        const float2 x = fma2(mul2(make_float2(s[i][b][2 * h], s[i][b][2 * h + 1]), k.scale[b]), up, add);
+        s[i][b][2 * h] = x.x;
+        s[i][b][2 * h + 1] = x.y;
+      }
     }
-  if (holes) {
+  if (at + int32_t(P::kChunk) > k.plain) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t m = 8 * b + 2 * w.c + j;
         if (m >= t.rows * a.group) continue;
-        const uint32_t row = t.first + m / a.group;
-        const int32_t base = a.row_base ? a.row_base[row] : 0;
+        const uint32_t row = t.first + w.row_of(m);
+        const int32_t base = a.row_base ? a.row_base[row] : 0, below = a.row_base ? min(base, a.extent[row]) : a.extent[row];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int32_t pos = at + int32_t(16 * i + 8 * h + w.place);
-            if (pos >= k.below[b][j] && !(a.row_base && tree_sees(a, row, pos - base))) s[i][b][2 * h + j] = -INFINITY;
+            if (pos >= below && !(a.row_base && tree_sees(a, row, pos - base))) s[i][b][2 * h + j] = -INFINITY;
           }
       }
   }
@@ -195,7 +236,7 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       top[b][j] = fmaxf(fmaxf(s[0][b][j], s[0][b][2 + j]), fmaxf(s[1][b][j], s[1][b][2 + j]));
-      move = move || top[b][j] > (ref[b][j] == -INFINITY ? ref[b][j] : __fadd_rn(ref[b][j], kSlack));
+      move = move || top[b][j] > __fadd_rn(j ? ref[b].y : ref[b].x, kSlack);
     }
   if (__any_sync(0xFFFFFFFFu, move)) {
 #pragma unroll
@@ -205,10 +246,12 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
         float v = top[b][j];
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
-        if (!(v > (ref[b][j] == -INFINITY ? ref[b][j] : __fadd_rn(ref[b][j], kSlack)))) continue;
-        const float f = exp2_approx(__fsub_rn(ref[b][j], v));      // (from -infinity: 0)
-        ref[b][j] = v;
-        sum[b][j] = __fmul_rn(sum[b][j], f);
+        float& r = j ? ref[b].y : ref[b].x;
+        float& l = j ? sum[b].y : sum[b].x;
+        if (!(v > __fadd_rn(r, kSlack))) continue;
+        const float f = exp2_approx(__fsub_rn(r, v));        // (from nothing: 0)
+        r = v;
+        l = __fmul_rn(l, f);
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
           o[b][d][j] = __fmul_rn(o[b][d][j], f);
@@ -219,15 +262,16 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
   uint32_t weights[2][NB][2];                                // B operands: positions by columns
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const float low0 = (ref[b][0] == -INFINITY ? 0.f : ref[b][0]) - kBias, low1 = (ref[b][1] == -INFINITY ? 0.f : ref[b][1]) - kBias;
+    const float2 up = make_float2(kQ4Bias - ref[b].x, kQ4Bias - ref[b].y);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float e0 = exp2_approx(__fsub_rn(s[i][b][2 * h], low0)), e1 = exp2_approx(__fsub_rn(s[i][b][2 * h + 1], low1));
-        sum[b][0] = __fmaf_rn(e0, inverse[i][h], sum[b][0]);
-        sum[b][1] = __fmaf_rn(e1, inverse[i][h], sum[b][1]);
-        const __half2 pair = __floats2half2_rn(e0, e1);
+        float2 e = add2(make_float2(s[i][b][2 * h], s[i][b][2 * h + 1]), up);
+        e.x = exp2_approx(e.x);
+        e.y = exp2_approx(e.y);
+        sum[b] = fma2(e, make_float2(inverse[i][h], inverse[i][h]), sum[b]);
+        const __half2 pair = __floats2half2_rn(e.x, e.y);
         weights[i][b][h] = movmatrix(*reinterpret_cast<const uint32_t*>(&pair));
       }
   }
@@ -235,9 +279,10 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t p0 = 16 * i + w.c, p1 = 16 * i + 4 + (w.c ^ 1u);      // places of MMA rows 2 c and 2 c + 1; 8 further those of 2 c + 8 and 2 c + 9
-    const uint32_t codes = stage + P::kVAt + 8 * w.r, scales = stage + P::kVScalesAt + (w.r >> 1);
-    const uint2 x0 = lds64(codes + p0 * kQ4Codes), x1 = lds64(codes + p1 * kQ4Codes), x2 = lds64(codes + (p0 + 8) * kQ4Codes), x3 = lds64(codes + (p1 + 8) * kQ4Codes);
-    const Q4Factors f01 = q4_factors(lds_u8(scales + 4 * p0) | lds_u8(scales + 4 * p1) << 16), f23 = q4_factors(lds_u8(scales + 4 * (p0 + 8)) | lds_u8(scales + 4 * (p1 + 8)) << 16);
+    const unsigned char* const codes = stage + P::kVAt + 8 * w.r;
+    const unsigned char* const scales = stage + P::kVScalesAt + (w.r >> 1);
+    const uint2 x0 = q4_ld<uint2>(codes + p0 * kQ4Codes), x1 = q4_ld<uint2>(codes + p1 * kQ4Codes), x2 = q4_ld<uint2>(codes + (p0 + 8) * kQ4Codes), x3 = q4_ld<uint2>(codes + (p1 + 8) * kQ4Codes);
+    const Q4Factors f01 = q4_factors(q4_ld<uint8_t>(scales + 4 * p0) | q4_ld<uint8_t>(scales + 4 * p1) << 16), f23 = q4_factors(q4_ld<uint8_t>(scales + 4 * (p0 + 8)) | q4_ld<uint8_t>(scales + 4 * (p1 + 8)) << 16);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {                            // eight dimensions
       const uint32_t y0 = h ? x0.y : x0.x, y1 = h ? x1.y : x1.x, y2 = h ? x2.y : x2.x, y3 = h ? x3.y : x3.x;
@@ -250,7 +295,7 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
         for (int q = 0; q < 2; ++q) {
           const uint32_t x[4] = {u[2 * q], u[2 * q + 1], v[2 * q], v[2 * q + 1]};
 #pragma unroll
-          for (int b = 0; b < NB; ++b) mma_f16_16816(o[b][4 * h + 2 * odd + q], x, weights[i][b][0], weights[i][b][1]);
+          for (int b = 0; b < NB; ++b) mma_q4(o[b][4 * h + 2 * odd + q], x, weights[i][b][0], weights[i][b][1]);
         }
       }
     }
@@ -260,12 +305,14 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
 // Float index of (column m of eight, 16-byte piece i of its 128 outputs) in a warp's block of the merge, spread over the banks.
 __device__ __forceinline__ uint32_t q4_merge_index(uint32_t m, uint32_t piece) { return m * 128u + ((piece ^ (m >> 1)) << 2); }
 
+// NB: blocks of eight columns.  Calls whose tiles have eight at most - decode rows - take one.
+template <int NB>
 __global__ void __launch_bounds__(TreeQ4::kThreads, 3)
 tree_q4_kernel(const TreeArgs a) {
   step_kernel_entry();
   using P = TreeQ4;
   extern __shared__ __align__(128) unsigned char tree_smem[];
-  __shared__ float ml_sm[4][16][2];
+  __shared__ float ml_sm[4][8][2];
   const uint32_t tid = threadIdx.x;
   Q4Warp w;
   w.warp = tid >> 5;
@@ -274,139 +321,134 @@ tree_q4_kernel(const TreeArgs a) {
   w.c = w.lane & 3u;
   // Places are dealt so that neighbouring MMA rows lie in entries of different parity: 64-byte rows, two of which share all banks.
   w.place = w.r & 1u ? 4u + ((w.r >> 1) ^ 1u) : w.r >> 1;
-  const uint32_t tiles = a.plan[0], units = a.plan[1];
-  const uint32_t u0 = uint32_t(uint64_t(units) * blockIdx.x / gridDim.x), u1 = uint32_t(uint64_t(units) * (blockIdx.x + 1) / gridDim.x);
-  if (u0 == u1) return;
-  const uint32_t ring = smem_u32(tree_smem) + w.warp * P::kStages * P::kStage;
-  Q4Unit t;
-  t.tile = tree_tile_of(a, u0, tiles);
-  q4_set_tile(a, t);
-  {
-    const uint32_t local = u0 - uint32_t(a.tiles[t.tile].z);
-    t.kvh = local % a.nkv;
-    t.part = local / a.nkv;
-  }
-  // The chunks of the run in their order: where the next one to be copied lies is looked up while the one before is on its way.
-  Q4Unit ahead = t;
-  uint32_t left = u1 - u0, chunk = 0, asked = 0, there = 0;  // units left; of the unit; chunks asked for; whether the last 32 of them have a page
-  int32_t page = -1;                                         // (looked at a chunk later: nothing waits for the load)
-  auto position = [&]() { return ahead.part * P::kPositions + chunk * 4 * P::kChunk + w.warp * P::kChunk; };
-  auto find = [&]() {                                        // the next chunk, from (ahead, chunk) on
-    while (left && chunk >= q4_chunks(ahead, w.warp)) {
-      chunk = 0;
-      if (--left) q4_next(a, ahead);
-    }
-    const uint32_t p = position() / kKvPage;
-    page = left && uint32_t(ahead.seq) < a.table.slots && p < a.table.max_pages ? a.table.table[ahead.seq * a.table.ld + p] : -1;
+  w.per_group = 65536u / a.group + 1u;
+  const uint32_t tiles = a.plan[0], weights = a.plan[1];
+  const uint32_t from = uint32_t(uint64_t(weights) * blockIdx.x / gridDim.x), end = uint32_t(uint64_t(weights) * (blockIdx.x + 1) / gridDim.x);
+  if (from == end) return;
+  Q4Unit t = q4_first(a, from, end, tiles);
+  if (t.at >= end) return;
+  const uint32_t ring = smem_u32(tree_smem) + w.warp * P::kWarp;
+  unsigned char* const stages = tree_smem + w.warp * P::kWarp;
+  w.meaning = stages + P::kStages * P::kStage;
+  // a lane's places in a chunk's copies: 16-byte pieces of codes; the first 20 lanes take the scales (8 pieces of either) and the exponents (2)
+  const bool of_scales = w.lane < 16, of_k = of_scales ? w.lane < 8 : w.lane < 18;
+  const uint8_t* const k_codes = static_cast<const uint8_t*>(a.pages.k) + w.warp * P::kChunk * kQ4Codes + w.lane * 16;
+  const uint8_t* const v_codes = static_cast<const uint8_t*>(a.pages.v) + w.warp * P::kChunk * kQ4Codes + w.lane * 16;
+  const uint8_t* const others = static_cast<const uint8_t*>(of_k ? a.pages.k : a.pages.v) +
+                                (of_scales ? kQ4ScalesAt + w.warp * P::kChunk * 4 + (w.lane & 7u) * 16 : kQ4ExpsAt + w.warp * P::kChunk + (w.lane & 1u) * 16);
+  const uint32_t to_others = of_scales ? P::kKScalesAt + w.lane * 16 : P::kKExpsAt + (w.lane - 16) * 16, page_bytes = a.nkv * kQ4Page;
+  const uint32_t half = of_scales ? 4 * P::kChunk * 4 : 4 * P::kChunk;       // to the second 128 positions of a page
+  // Chunk i of a unit goes to stage i.  Stages are asked for a unit ahead, as they are left; where the next unit's pages lie is looked up
+  // while the first chunk of this one is at hand.
+  int32_t page0, page1;
+  auto look_up = [&](const Q4Unit& u) {
+    const uint32_t p = u.part * 2;
+    const bool in = u.at < end && uint32_t(u.seq) < a.table.slots;
+    page0 = in && p < a.table.max_pages ? a.table.table[u.seq * a.table.ld + p] : -1;
+    page1 = in && p + 1 < a.table.max_pages ? a.table.table[u.seq * a.table.ld + p + 1] : -1;
   };
-  auto request = [&]() {
-    if (left) {
-      const bool in = uint32_t(page) < a.table.pages;
-      there = (there & ~(1u << (asked & 31u))) | uint32_t(in) << (asked & 31u);
-      if (in) {
-        const size_t block = (size_t(page) * a.nkv + ahead.kvh) * kQ4Page;
-        const uint32_t at = position() % kKvPage, dst = ring + (asked % P::kStages) * P::kStage;
-        const uint8_t* const k = static_cast<const uint8_t*>(a.pages.k) + block;
-        const uint8_t* const v = static_cast<const uint8_t*>(a.pages.v) + block;
+  uint32_t chunks = 0, there = 0;                            // of the unit asked for: how many, and which of its pages are in the pool
+  auto request = [&](const Q4Unit& u, uint32_t i) {
+    if (i < chunks && there >> (i >> 1) & 1u) {
+      const uint64_t block = uint64_t(uint32_t(i >> 1 ? page1 : page0)) * page_bytes + u.kvh * kQ4Page;
+      const uint32_t dst = ring + i * P::kStage + w.lane * 16, up = (i & 1u) * (4 * P::kChunk * kQ4Codes);
+      const uint8_t* const k = k_codes + block + up;
+      const uint8_t* const v = v_codes + block + up;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cp_async_16(dst + (w.lane + 32 * i) * 16, k + at * kQ4Codes + (w.lane + 32 * i) * 16, 16u);
+      for (int x = 0; x < 4; ++x) cp_async_16(dst + 512 * x, k + 512 * x, 16u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cp_async_16(dst + P::kVAt + (w.lane + 32 * i) * 16, v + at * kQ4Codes + (w.lane + 32 * i) * 16, 16u);
-        if (w.lane < 20) {                                   // 8 pieces of either's scales, 2 of either's exponents
-          const bool scales = w.lane < 16;
-          const uint32_t i = scales ? w.lane : w.lane - 16, half = scales ? 8u : 2u, piece = i % half;
-          const uint8_t* const src = (i < half ? k : v) + (scales ? kQ4ScalesAt + at * 4 : kQ4ExpsAt + at) + piece * 16;
-          cp_async_16(dst + (scales ? P::kKScalesAt : P::kKExpsAt) + i * 16, src, 16u);
-        }
-      }
-      ++asked;
-      ++chunk;
-      find();
+      for (int x = 0; x < 4; ++x) cp_async_16(dst + P::kVAt + 512 * x, v + 512 * x, 16u);
+      if (w.lane < 20) cp_async_16(ring + i * P::kStage + to_others, others + block + (i & 1u) * half, 16u);
     }
     cp_async_commit();
   };
-  find();
-  for (uint32_t i = 0; i + 1 < P::kStages; ++i) request();
-
-  uint32_t g = 0;                                            // chunks this warp has taken
-  auto run = [&](auto blocks, const Q4Unit& unit) {
-    constexpr int NB = decltype(blocks)::value;
-    Q4Columns<NB> columns;
-    q4_ask_columns<NB>(a, unit, w, columns);
-    float ref[NB][2], sum[NB][2], o[NB][8][4];
+  auto begin = [&](const Q4Unit& u) {                        // the pages have come
+    chunks = u.at < end ? q4_chunks(u, w.warp) : 0u;
+    there = uint32_t(uint32_t(page0) < a.table.pages) | uint32_t(uint32_t(page1) < a.table.pages) << 1;
+  };
+  look_up(t);
+  begin(t);
+#pragma unroll
+  for (uint32_t i = 0; i < P::kStages; ++i) request(t, i);
+  Q4Columns<NB> columns;
+  q4_ask_columns<NB>(a, t, w, columns);
+  while (t.at < end) {
+    float2 ref[NB], sum[NB];
+    float o[NB][8][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) { ref[b][j] = -INFINITY; sum[b][j] = 0.f; }
+      ref[b] = make_float2(kQ4Nothing, kQ4Nothing);
+      sum[b] = make_float2(0.f, 0.f);
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[b][d][e] = 0.f;
     }
-    const uint32_t n = q4_chunks(unit, w.warp);
-    const int32_t start = int32_t(unit.part * P::kPositions + w.warp * P::kChunk);
-    for (uint32_t i = 0; i < n; ++i, ++g) {
-      request();                                             // (into the stage that the chunk before has left)
+    const uint32_t n = chunks, mine = there;
+    Q4Unit next = t;
+    q4_next(a, next, end);
+    look_up(next);
+    int32_t at = int32_t(t.part * P::kPositions + w.warp * P::kChunk);
+#pragma unroll 1
+    for (uint32_t i = 0; i < P::kStages; ++i, at += 4 * P::kChunk) {
       cp_async_wait<P::kStages - 1>();
       __syncwarp();
-      // a page outside the pool: as if nobody saw the chunk
-      if (there >> (g & 31u) & 1u) q4_chunk<NB>(a, unit, w, ring + (g % P::kStages) * P::kStage, start + int32_t(i * 4 * P::kChunk), columns, ref, sum, o);
+      // (a page outside the pool: as if nobody saw the chunk)
+      if (i < n && mine >> (i >> 1) & 1u) q4_chunk<NB>(a, t, w, stages + i * P::kStage, at, columns, ref, sum, o);
       __syncwarp();
+      if (i == 0) begin(next);
+      if (i + 1 < P::kStages) request(next, i);              // (the last stage serves the merge first)
     }
-    // the warps' results merged, eight columns at a time, through the stage of each that is free
-    const uint32_t used = unit.rows * a.group, free_stage = (g + P::kStages - 1) % P::kStages;
+    // the next unit's columns are on their way while the warps' results are merged, eight columns at a time
+    const uint32_t used = t.rows * a.group, first = t.first, heads = t.kvh * a.group, part = t.part;
+    t = next;
+    if (t.at < end) q4_ask_columns<NB>(a, t, w, columns);
+    constexpr uint32_t kMergeAt = (P::kStages - 1) * P::kStage;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+      if (b && 8u * b >= used) break;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float l = sum[b][j];
+        float l = j ? sum[b].y : sum[b].x;
+        const float r = j ? ref[b].y : ref[b].x;
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l = __fadd_rn(l, __shfl_xor_sync(0xFFFFFFFFu, l, off));
-        if (w.r == 0) {
-          ml_sm[w.warp][8 * b + 2 * w.c + j][0] = ref[b][j] == -INFINITY ? ref[b][j] : ref[b][j] - 7.f;
-          ml_sm[w.warp][8 * b + 2 * w.c + j][1] = l;
-        }
+        if (w.r == 0) *reinterpret_cast<float2*>(ml_sm[w.warp][2 * w.c + j]) = make_float2(r == kQ4Nothing ? -INFINITY : r - kQ4Bias, l);
       }
-      float* const mine = reinterpret_cast<float*>(tree_smem + (w.warp * P::kStages + free_stage) * P::kStage);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {                        // dimensions 16 r + 4 q ..: of word q / 2, 4 (q % 2) on
           const int d = 4 * (q >> 1) + (q & 1);
-          *reinterpret_cast<float4*>(mine + q4_merge_index(2 * w.c + j, 4 * w.r + q)) = make_float4(o[b][d][j], o[b][d + 2][j], o[b][d][2 + j], o[b][d + 2][2 + j]);
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(tree_smem + w.warp * P::kWarp + kMergeAt) + q4_merge_index(2 * w.c + j, 4 * w.r + q)) =
+              make_float4(o[b][d][j], o[b][d + 2][j], o[b][d][2 + j], o[b][d + 2][2 + j]);
         }
-      // (where the other warps put theirs: their own free stages)
-      __shared__ uint32_t stage_sm[4];
-      if (w.lane == 0) stage_sm[w.warp] = (w.warp * P::kStages + free_stage) * P::kStage;
       __syncthreads();
       for (uint32_t m = w.warp; m < 8 && 8 * b + m < used; m += 4) {
-        float wm[4], mx = -INFINITY, den = 0.f;
+        float2 ml[4];
+        float mx = -INFINITY, den = 0.f;
         float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) { wm[x] = ml_sm[x][8 * b + m][0]; mx = fmaxf(mx, wm[x]); }
+        for (int x = 0; x < 4; ++x) { ml[x] = *reinterpret_cast<const float2*>(ml_sm[x][m]); mx = fmaxf(mx, ml[x].x); }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           // (a warp that saw nothing adds zeros; one whose scores were all NaN has no reference either and adds NaN)
-          const float e = wm[x] == -INFINITY ? 1.f : exp2_approx(__fsub_rn(wm[x], mx));
-          den = __fmaf_rn(e, ml_sm[x][8 * b + m][1], den);
-          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tree_smem + stage_sm[x]) + q4_merge_index(m, w.lane));
+          const float e = ml[x].x == -INFINITY ? 1.f : exp2_approx(__fsub_rn(ml[x].x, mx));
+          den = __fmaf_rn(e, ml[x].y, den);
+          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tree_smem + x * P::kWarp + kMergeAt) + q4_merge_index(m, w.lane));
           num.x = __fmaf_rn(e, v.x, num.x);
           num.y = __fmaf_rn(e, v.y, num.y);
           num.z = __fmaf_rn(e, v.z, num.z);
           num.w = __fmaf_rn(e, v.w, num.w);
         }
-        const uint32_t col = 8 * b + m, rl = col / a.group;
-        const size_t at = (size_t(unit.first + rl) * a.nq + unit.kvh * a.group + (col - rl * a.group)) * a.max_parts + unit.part;
-        *reinterpret_cast<float4*>(a.part_acc + at * kKvDim + w.lane * 4) = num;
-        if (w.lane == 0) a.part_ml[at] = make_float2(mx, den);
+        const uint32_t col = 8 * b + m, rl = w.row_of(col);
+        const size_t to = (size_t(first + rl) * a.nq + heads + (col - rl * a.group)) * a.max_parts + part;
+        *reinterpret_cast<float4*>(a.part_acc + to * kKvDim + w.lane * 4) = num;
+        if (w.lane == 0) a.part_ml[to] = make_float2(mx, den);
       }
       __syncthreads();                                       // the stages are free again
     }
-  };
-  for (uint32_t u = u0; u < u1; ++u) {
-    if (t.rows * a.group > 8) run(std::integral_constant<int, 2>{}, t);
-    else run(std::integral_constant<int, 1>{}, t);
-    if (u + 1 < u1) q4_next(a, t);
+    request(t, P::kStages - 1);
   }
   cp_async_wait<0>();
 }
