@@ -84,7 +84,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
     } else {
       prepared[dev] = cuda_status(cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
     }
-    if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem<F8>)));
+    if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<FORMAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem<F8>)));
   });
   if (prepared[dev]) return prepared[dev];
   const int sms = device_sm_count(dev);
@@ -95,7 +95,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
   if (int st = launch_step(part, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
   if (a.wide_from) {
-    if (int st = launch_step(tree_wide_kernel<F8>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
+    if (int st = launch_step(tree_wide_kernel<FORMAT>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
   }
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
   return launch_step(tree_combine_kernel, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a);
@@ -212,7 +212,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   // behind 2048 positions 148 us instead of 135); guessing from the other rows of the call would have them change a run's bits.
   const uint32_t longest = s->longest_run ? s->longest_run : s->row_base ? s->rows : 1u;
   a.wide_from = s->row_base ? 32 / a.group + 1 : 64;
-  if (a.wide_from > s->rows || a.wide_from > longest || s->pages.format == GRB_KV_Q4) a.wide_from = 0;
+  if (a.wide_from > s->rows || a.wide_from > longest) a.wide_from = 0;
   a.scaling = s->scaling;
   a.out = static_cast<__nv_bfloat16*>(s->out);
   a.ldo = s->ldo;

@@ -27,10 +27,11 @@ constexpr uint32_t kTreeRowAbsent = 0xFFFFFFFFu;             // row_parts of a r
 // Positions of a wide tile's unit: the most, for long contexts (a unit's result is as large as 256 positions of an 8-bit cache); fewer
 // for short ones and for runs of one or two tiles, whose few units would leave SMs idle.  1024 instead of 2048 behind 8192 positions,
 // 8 bits, 40 heads of 8: one run of 16 rows 35 us instead of 51, 16 runs 120 instead of 138; 16 runs of 64 rows (three tiles) 337
-// instead of 320, which keep 2048.
+// instead of 320, which keep 2048.  (4 bits: never fewer than a part of the narrow kernel has, for as many parts there is room.)
 constexpr uint32_t kWideMostPart = 2048;
+template <int FORMAT>
 __device__ __forceinline__ uint32_t wide_part(uint32_t extent, bool many) {
-  return extent <= 1024 ? 256u : extent <= 4096 ? 512u : extent <= 16384 && !many ? 1024u : kWideMostPart;
+  return extent <= 1024 && FORMAT != kKvQ4 ? 256u : extent <= 4096 ? 512u : extent <= 16384 && !many ? 1024u : kWideMostPart;
 }
 
 struct TreeArgs {
@@ -162,7 +163,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
       const uint32_t per = wide ? a.wide_rows : a.tile_rows;
       if ((r - first) % per == 0) {
         for (; n < per && r + n < a.rows && run_of[r + n] == first; ++n) extent = max(extent, extents[r + n]);
-        if (wide) positions = wide_part(uint32_t(extent), first + 2 * a.wide_rows < a.rows && run_of[first + 2 * a.wide_rows] == first);
+        if (wide) positions = wide_part<FORMAT>(uint32_t(extent), first + 2 * a.wide_rows < a.rows && run_of[first + 2 * a.wide_rows] == first);
         parts = (uint32_t(extent) + positions - 1) / positions;
         if (wide)
           for (uint32_t i = 0; i < n; ++i) a.row_parts[r + i] = extents[r + i] < 0 ? kTreeRowAbsent : parts;
