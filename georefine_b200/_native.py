@@ -33,6 +33,7 @@ EXPORTS = (
     "grb_peer_alloc", "grb_peer_free", "grb_peer_open", "grb_peer_close",
     "grb_rmsnorm_bf16", "grb_silu_mul_bf16", "grb_argmax_bf16", "grb_attn_decode_bf16",
     "grb_kv_write", "grb_kv_read", "grb_kv_keep", "grb_attn_tree_scratch_bytes", "grb_attn_tree", "grb_verify_drafts",
+    "grb_rotary", "grb_kv_copy", "grb_kv_fork", "grb_kv_free", "grb_kv_compact_scratch_bytes", "grb_kv_compact",
 )
 
 
@@ -98,11 +99,18 @@ class VerifyStep(ctypes.Structure):
                 ("temperature", ctypes.c_double)]
 
 
+class RotaryStep(ctypes.Structure):
+    _fields_ = [("x", VOIDP), ("ldx", ctypes.c_int64), ("ldx_head", ctypes.c_int64), ("out", VOIDP), ("ldo", ctypes.c_int64), ("ldo_head", ctypes.c_int64),
+                ("positions", VOIDP), ("turns", VOIDP), ("rows", ctypes.c_uint32), ("heads", ctypes.c_uint32), ("dim", ctypes.c_uint32), ("turned", ctypes.c_uint32),
+                ("layout", ctypes.c_uint32), ("dtype", ctypes.c_uint32), ("positions_64", ctypes.c_uint32), ("backward", ctypes.c_uint32), ("factor", ctypes.c_float)]
+
+
 # The same structures in one go: filling a ctypes structure field by field costs a third of a small call.  (Native alignment, as
 # the fields above have it; bytes are the call's own, so calls from several threads do not meet.)
 KV_PAGES, KV_TABLE = struct.Struct("@PPPPqqIIII"), struct.Struct("@PqII")
 TREE_STEP = struct.Struct("@PqPPIPPPPPqIPPPPqqIIIIPqIIPQPqIIIfI4x")
 VERIFY_STEP = struct.Struct("@PqPPPPPPqPPPPIIIII4xd")
+ROTARY_STEP = struct.Struct("@PqqPqqPPIIIIIIIIf4x")
 _PACKED = {}
 
 
@@ -173,6 +181,14 @@ def _declare(lib):
     lib.grb_attn_tree_scratch_bytes.restype = u64
     lib.grb_attn_tree.argtypes = [ctypes.POINTER(TreeStep), VOIDP]
     lib.grb_verify_drafts.argtypes = [ctypes.POINTER(VerifyStep), VOIDP]
+    pages, table, i32 = ctypes.POINTER(KvPages), ctypes.POINTER(KvTable), ctypes.c_int32
+    lib.grb_rotary.argtypes = [ctypes.POINTER(RotaryStep), VOIDP]
+    lib.grb_kv_copy.argtypes = [pages, VOIDP, VOIDP, VOIDP, u32, VOIDP]
+    lib.grb_kv_fork.argtypes = [pages, table, VOIDP, VOIDP, VOIDP, VOIDP, VOIDP, i32, u32, VOIDP]
+    lib.grb_kv_free.argtypes = [table, VOIDP, VOIDP, u32, i32, u32, VOIDP]
+    lib.grb_kv_compact_scratch_bytes.argtypes = [u32]
+    lib.grb_kv_compact_scratch_bytes.restype = u64
+    lib.grb_kv_compact.argtypes = [pages, table, VOIDP, VOIDP, VOIDP, VOIDP, u64, VOIDP]
     lib.grb_peer_control_bytes.argtypes = []
     lib.grb_peer_control_bytes.restype = u64
     lib.grb_peer_enable.argtypes = [ci]
@@ -183,7 +199,7 @@ def _declare(lib):
     lib.grb_peer_allreduce_bf16.argtypes = [VOIDP, ctypes.POINTER(VOIDP), ctypes.POINTER(VOIDP), u64, u32, u32, VOIDP, u64, u64, VOIDP, VOIDP]
     for name in EXPORTS:
         if name not in ("bcx_free", "bxr_free", "grb_bxr_workspace_bytes", "grb_static_scratch_bytes", "grb_peer_control_bytes",
-                        "grb_attn_tree_scratch_bytes", "bxr_layout_version", "bxr_partition_version"):
+                        "grb_attn_tree_scratch_bytes", "grb_kv_compact_scratch_bytes", "bxr_layout_version", "bxr_partition_version"):
             getattr(lib, name).restype = ci
 
 

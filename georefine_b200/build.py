@@ -20,7 +20,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT = PKG / "_build" / "libgeorefine_b200.so"
-SOURCES = [CSRC / "capi.cu", CSRC / "spec_ops.cu", CSRC / "bcx_host.cpp", CSRC / "bcx_frame.cpp", CSRC / "bxr_build.cpp"]
+SOURCES = [CSRC / "capi.cu", CSRC / "spec_ops.cu", CSRC / "page_ops.cu", CSRC / "bcx_host.cpp", CSRC / "bcx_frame.cpp", CSRC / "bxr_build.cpp"]
 FASTCALL_SOURCE = CSRC / "fastcall.c"
 FASTCALL = PKG / "_build" / ("_fastcall" + sysconfig.get_config_var("EXT_SUFFIX"))     # (named for the interpreter's ABI)
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",

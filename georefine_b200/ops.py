@@ -6,8 +6,10 @@ the current stream, without allocating or synchronising, so a whole step can be 
 place of the reference's step kernels (``glc_serve/fastdec_kernels.cu:83-110,324-488``) for a plain grouped-query
 decoder with head dimension 128.
 
-``KVPages``, ``kv_write``, ``kv_read``, ``kv_keep`` and ``TreeAttention`` are speculative serving over a cache in BF16 or in 8 bits
-(``csrc/kv_cache.cuh``, ``csrc/tree_attention.cuh``); the reference has no counterparts.
+``KVPages``, ``kv_write``, ``kv_read``, ``kv_keep`` and ``TreeAttention`` are speculative serving over a cache in BF16, 8 or 4 bits
+(``csrc/kv_cache.cuh``, ``csrc/tree_attention.cuh``, ``csrc/tree_q4.cuh``); ``Rope`` and ``rotary`` are rotary positions in every layout and scaling
+(``csrc/rotary.cuh``); ``kv_copy``, ``kv_fork``, ``kv_free`` and ``kv_compact`` are pages shared and moved (``csrc/kv_pages.cuh``).  The
+reference has no counterparts.
 """
 from __future__ import annotations
 
@@ -268,6 +270,186 @@ def kv_keep(slots, base, path, count, page_table, pages):
     kept, ldp = _vector(count, device, "count", n), _ld(path, path.shape[1], "path")
     if n and path.shape[1]:
         _launch(device, "grb_kv_keep", pages._packed, *args, path.data_ptr(), ldp, kept, n, path.shape[1])
+
+
+# ---- pages as a whole -------------------------------------------------------------------------------------------------------
+
+
+def _refs(refs, pages):
+    return _vector(refs, pages.device, "refs", pages.pages)
+
+
+def _empty(empty):
+    if not -(1 << 31) <= empty < 1 << 31:
+        raise ValueError("empty is a number of 32 bits")
+    return int(empty)
+
+
+def kv_copy(src, dst, pages, *, positions=None):
+    """Entries of page ``src[i]`` to page ``dst[i]`` (int32 vectors), keys and values, in every layer of ``pages``: all 256, or the first
+    ``positions[i]``.  A page of -1 is left out; no page is a destination twice, or a source and a destination."""
+    n, device = src.shape[0], pages.device
+    args = _vector(src, device, "src"), _vector(dst, device, "dst", n), 0 if positions is None else _vector(positions, device, "positions", n)
+    if n:
+        _launch(device, "grb_kv_copy", pages._packed, *args, n)
+
+
+def kv_fork(parents, children, lengths, fresh, page_table, refs, pages, *, empty=-1):
+    """Sequences that begin as others: slot ``children[i]`` gets the first ``lengths[i]`` positions of slot ``parents[i]``.  Whole pages are
+    shared, and are not to be written to while they are; the positions behind them are copied to page ``fresh[i]``, in every layer.
+    ``refs`` (int32 [pages]) counts the places of the table that name a page and goes up for every page the child gets; the places behind
+    its pages hold ``empty``.  What the child's slot held before is not given back (``kv_free`` it first).  A parent may have many children; no
+    slot is a child twice, or a parent and a child, and no fresh page is in use.  Forks of slot -1 are left out."""
+    n, device = parents.shape[0], pages.device
+    args = _native.KV_TABLE.pack(*_table(page_table, device)), _vector(parents, device, "parents"), *(
+        _vector(t, device, what, n) for t, what in ((children, "children"), (lengths, "lengths"), (fresh, "fresh"))), _refs(refs, pages), _empty(empty)
+    if n:
+        _launch(device, "grb_kv_fork", pages._packed, *args, n)
+
+
+def kv_free(slots, page_table, refs, *, empty=-1):
+    """Gives the pages of the sequences in ``slots`` back: their places in the table become ``empty``, and the counts in ``refs`` go down;
+    a page is free when its count is 0.  Slots of -1 are left out."""
+    device, n = refs.device, slots.shape[0]
+    if device.type != "cuda":
+        raise ValueError("refs live on a CUDA device")
+    args = _native.KV_TABLE.pack(*_table(page_table, device)), _vector(slots, device, "slots"), _vector(refs, device, "refs")
+    if n and refs.shape[0]:
+        _launch(device, "grb_kv_free", *args, refs.shape[0], _empty(empty), n)
+
+
+def kv_compact(page_table, refs, pages, where, used, *, scratch=None):
+    """Moves the pages in use (``refs`` above 0) to the front of the pool, entries, counts and the places that name them: with u in use, the i-th
+    at u or behind goes to the i-th free one before u.  ``where`` (int32 [pages]) receives each page's new number, -1 for pages that are not
+    in use, and ``used`` (int32 [1]) u.  ``scratch``: uint8, ``kv_compact_scratch_bytes`` of it; allocated by the call if not given."""
+    import torch
+
+    device = pages.device
+    args = _native.KV_TABLE.pack(*_table(page_table, device)), _refs(refs, pages), _vector(where, device, "where", pages.pages), _vector(used, device, "used", 1)
+    size = kv_compact_scratch_bytes(pages)
+    if scratch is None:
+        with torch.cuda.device(device):
+            scratch = torch.empty(size, device=device, dtype=torch.uint8)
+    _on(scratch, device, torch.uint8, "scratch")
+    if not scratch.is_contiguous():
+        raise ValueError("scratch has to be contiguous")
+    _launch(device, "grb_kv_compact", pages._packed, *args, scratch.data_ptr(), scratch.numel())
+
+
+def kv_compact_scratch_bytes(pages) -> int:
+    return _native.lib().grb_kv_compact_scratch_bytes(pages.pages)
+
+
+# ---- rotary positions ---------------------------------------------------------------------------------------------------
+
+
+ROPE_LAYOUTS = ("half", "interleaved")
+_ROPE_KEYS = {"linear": ("factor",), "ntk": ("factor",), "yarn": ("factor", "original"), "bands": ("factor", "original", "low", "high")}
+_ROPE_MORE = {"yarn": {"fast": 32.0, "slow": 1.0, "attention": None}}
+
+
+def rope_frequencies(dim: int, theta: float = 1e4, scaling=None):
+    """Radians a position of the dim / 2 pairs (Python floats), theta^(-2 i / dim) scaled for contexts longer than the trained one, and the
+    factor on both components of a turned pair.  ``scaling`` is None or a dict:
+      kind "linear", factor: every pair slower by the factor (positions interpolated);
+      kind "ntk", factor: theta factor^(dim / (dim - 2)), under which the slowest pair is slower by the factor and the fastest as it was;
+      kind "yarn", factor, original (the trained context), fast=32, slow=1, attention=None: pairs that turn ``fast`` times or more within the
+        trained context stay, those that turn ``slow`` times or fewer are slower by the factor, between the pairs' numbers it is a ramp; both
+        components are multiplied by ``attention``, 0.1 ln(factor) + 1 where it is None (Peng et al., 2023);
+      kind "bands", factor, original, low, high: the same with the ramp over the turns themselves, between ``low`` and ``high``, and no factor."""
+    if dim < 2 or dim % 2:
+        raise ValueError("the turned dimensions are an even number of two or more")
+    if not 0 < theta < float("inf"):
+        raise ValueError("theta is positive")
+    given = dict(scaling or {"kind": None})
+    kind = given.pop("kind", None)
+    if kind is not None:
+        if kind not in _ROPE_KEYS:
+            raise ValueError(f"the scaling's kind is one of {tuple(_ROPE_KEYS)}")
+        given = {**_ROPE_MORE.get(kind, {}), **given}
+        if set(given) != {*_ROPE_KEYS[kind], *_ROPE_MORE.get(kind, {})}:
+            raise ValueError(f"scaling {kind!r} takes {(*_ROPE_KEYS[kind], *_ROPE_MORE.get(kind, {}))}")
+        if any(not 0 < v < float("inf") for v in given.values() if v is not None):
+            raise ValueError("the numbers of a scaling are positive")
+    elif given:
+        raise ValueError("a scaling has a kind")
+    if kind == "ntk" and dim > 2:
+        theta = theta * given["factor"] ** (dim / (dim - 2))
+    inv = [theta ** (-2 * i / dim) for i in range(dim // 2)]
+    if kind == "linear":
+        return [f / given["factor"] for f in inv], 1.0
+    if kind == "yarn":
+        if theta == 1 or given["fast"] <= given["slow"]:
+            raise ValueError("yarn needs a theta other than 1 and fast above slow")
+        number = lambda turns: dim / 2 * math.log(given["original"] / (2 * math.pi * turns)) / math.log(theta)
+        lo, hi = max(math.floor(number(given["fast"])), 0), min(math.ceil(number(given["slow"])), dim - 1)
+        slow = [min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0) for i in range(dim // 2)]
+        return [f / given["factor"] * s + f * (1 - s) for f, s in zip(inv, slow)], 0.1 * math.log(given["factor"]) + 1 if given["attention"] is None else float(given["attention"])
+    if kind == "bands":
+        if given["low"] >= given["high"]:
+            raise ValueError("low lies below high")
+        keep = [min(max((given["original"] * f / (2 * math.pi) - given["low"]) / (given["high"] - given["low"]), 0.0), 1.0) for f in inv]
+        return [f / given["factor"] * (1 - k) + f * k for f, k in zip(inv, keep)], 1.0
+    return inv, 1.0
+
+
+class Rope:
+    """Rotary positions of the first ``dim`` dimensions of a head: pairs (i, i + dim / 2) (``layout`` "half") or (2 i, 2 i + 1)
+    ("interleaved"), frequencies by ``theta`` and ``scaling`` (``rope_frequencies``), held on the device as 64-bit fractions of a turn."""
+
+    def __init__(self, dim: int, theta: float = 1e4, *, layout="half", scaling=None, device="cuda:0"):
+        import torch
+
+        if layout not in ROPE_LAYOUTS:
+            raise ValueError(f"the layout is one of {ROPE_LAYOUTS}")
+        self.dim, self.layout = int(dim), layout
+        self.frequencies, self.factor = rope_frequencies(self.dim, theta, scaling)
+        turns = [round(f / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for f in self.frequencies]
+        self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64).to(device)
+        self.device = self.turns.device
+
+    def tables(self, positions: int):
+        """BF16 cos / sin tables [positions, 128] as the attention takes them, with the factor: for all 128 dimensions in halves."""
+        import torch
+
+        if self.dim != HEAD_DIM or self.layout != "half":
+            raise ValueError("the attention's tables are of 128 dimensions in halves")
+        angle = torch.arange(positions, dtype=torch.float64)[:, None] * torch.tensor(self.frequencies, dtype=torch.float64)
+        angle = torch.cat([angle, angle], dim=1)
+        return tuple((f(angle) * self.factor).to(torch.bfloat16).to(self.device) for f in (torch.cos, torch.sin))
+
+
+def rotary(x, positions, rope, *, out=None, backward=False):
+    """Turns the first ``rope.dim`` dimensions of every head of ``x`` ([rows, heads, head dim] BF16, FP16 or FP32; rows and heads may be any distance apart) by
+    ``positions`` (int32 or int64 [rows]), into ``out`` or, without it, in place.  Angles are exact for positions of any size; a value is rounded
+    once.  ``backward``: turned the other way - the gradient of the call, given that of its result, and where ``rope.factor`` is 1 its inverse."""
+    import torch
+
+    device = rope.device
+    out = x if out is None else out
+    kinds = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+    if x.dim() != 3 or x.dtype not in kinds or x.device != device or device.type != "cuda":
+        raise ValueError("x is BF16, FP16 or FP32 [rows, heads, head dim] on the rope's device, a CUDA device")
+    rows, heads, dim = x.shape
+    if rope.dim > dim:
+        raise ValueError(f"{rope.dim} dimensions are turned, a head has {dim}")
+    _on(out, device, x.dtype, "out", x.shape)
+    if positions.dim() != 1 or positions.shape[0] != rows or not positions.is_contiguous() or positions.device != device or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions: a contiguous int32 or int64 vector of {rows} is wanted")
+    if not rows or not heads:
+        return out
+    for t, what in ((x, "x"), (out, "out")):
+        if dim > 1 and t.stride(2) != 1:
+            raise ValueError(f"{what}: the dimensions of a head have to be contiguous")
+    if out is not x:
+        span = [(t.data_ptr(), t.data_ptr() + t.element_size() * (t.stride(0) * (rows - 1) + t.stride(1) * (heads - 1) + dim)) for t in (x, out)]
+        if span[0][0] < span[1][1] and span[1][0] < span[0][1] and (x.data_ptr() != out.data_ptr() or x.stride() != out.stride()):
+            raise ValueError("x and out overlap: give the same tensor, or tensors apart")
+    wide = positions.dtype == torch.int64
+    step = _native.ROTARY_STEP.pack(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), positions.data_ptr(), rope.turns.data_ptr(),
+                                    rows, heads, dim, rope.dim, ROPE_LAYOUTS.index(rope.layout), kinds[x.dtype], wide, bool(backward), rope.factor)
+    _launch(device, "grb_rotary", step)
+    return out
 
 
 class TreeRows:

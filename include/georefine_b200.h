@@ -387,7 +387,7 @@ typedef struct grb_attn_step {
 int grb_attn_decode_bf16(const grb_attn_step* step, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------------------------------
- * 6. Speculative serving over a paged KV cache in BF16 or in 8 bits: storing and reading entries, attention of causal rows and
+ * 6. Speculative serving over a paged KV cache in BF16, 8 or 4 bits: storing and reading entries, attention of causal rows and
  *    of draft trees, verification of drafted tokens from given random numbers, keeping an accepted path.  The reference has no
  *    counterparts.  No allocation, no host synchronisation; rows and sequences do not depend on what shares the call.
  *
@@ -395,6 +395,13 @@ int grb_attn_decode_bf16(const grb_attn_step* step, void* cuda_stream);
  *    byte: with a = max |x|, e = clamp(ceil(log2(a / 448)), -40, 7), the code is the e4m3 number nearest to x 2^-e (ties to
  *    even, at most 448), the byte e + 127, the value code 2^e.  An entry with an infinity or a NaN has byte 255 and codes 0 and
  *    reads as NaN throughout.
+ *
+ *    In 4 bits it is 128 codes, a scale byte for each 32 of them and an exponent byte, 69 bytes: with a as before, e = clamp(floor(log2(a / 7))
+ *    + 9, -40, 22), the byte e + 127; a group's scale is the number nearest to (its max |x|) / 7 2^(24 - e) among (16 + m) 2^k, m 0 .. 15, k 0 .. 11, the
+ *    byte 64 + 16 k + m; a code is x / (scale 2^(e - 24)) to the nearest (ties to even) in -7 .. 7, the value code scale 2^(e - 24).  A page of one
+ *    head is 17664 bytes in a piece: the codes of its 256 positions, 64 bytes each, their scales, 4 bytes each, their exponents.  A nibble holds
+ *    code + 8; of dimensions 8 w .. 8 w + 7, in the 32-bit word w of the codes, nibble j < 4 is dimension 2 j and nibble 4 + j dimension 2 j + 1.  Not
+ *    finite: byte 255, codes 0, reads as NaN.  A scale byte below 16 stands for byte / 8: memory of zeros reads as zeros.
  *
  *    A row with slot -1, or one whose place is outside the table or the pool, is left out: nothing is stored or read for it
  *    and its output stays as it was.  No two rows of a call may name the same place to store at.
@@ -485,6 +492,49 @@ typedef struct grb_verify_step {
   double temperature;         /* 1e-30 to 1e20 */
 } grb_verify_step;
 int grb_verify_drafts(const grb_verify_step* step, void* cuda_stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * 7. Long contexts and shared prompts: rotary positions of any layout and scaling, and the pages of a cache as a whole.  The
+ *    reference has no counterparts.  No allocation, no host synchronisation.
+ * ------------------------------------------------------------------------------------------------- */
+#define GRB_ROTARY_BF16 0
+#define GRB_ROTARY_FP32 1
+#define GRB_ROTARY_FP16 2
+#define GRB_ROTARY_HALF 0             /* pairs (i, i + turned / 2) */
+#define GRB_ROTARY_INTERLEAVED 1      /* pairs (2 i, 2 i + 1) */
+/* (a, b) -> factor (a cos - b sin, b cos + a sin) for the pairs of the first `turned` dimensions of every head, by position x frequency; the
+ * others are copied (nothing is done to them where out == x, which needs the same distances).  x and out may not overlap otherwise. */
+typedef struct grb_rotary_step {
+  const void* x;              /* [rows][heads][dim], rows ldx and heads ldx_head elements apart */
+  int64_t ldx, ldx_head;
+  void* out;                  /* the same; rows and heads may not overlap */
+  int64_t ldo, ldo_head;
+  const void* positions;      /* [rows], int32 or (positions_64) int64; negative ones turn backwards */
+  const uint64_t* turns;      /* [turned / 2]: turns that one position adds, in units of 2^-64 */
+  uint32_t rows, heads, dim, turned, layout, dtype, positions_64;    /* turned even; dim <= 1024, heads <= 65535 */
+  uint32_t backward;          /* 1: turned the other way, the gradient of this (its inverse where factor is 1) */
+  float factor;
+} grb_rotary_step;
+int grb_rotary(const grb_rotary_step* step, void* cuda_stream);
+
+/* Entries of page src[i] to page dst[i], in all layers, keys and values: the first positions[i] of them (NULL: all 256).  A page outside the pool, or
+ * one onto itself, is left out; no page may be a destination twice, or a source and a destination. */
+int grb_kv_copy(const grb_kv_pages* pages, const int32_t* src, const int32_t* dst, const int32_t* positions, uint32_t n, void* cuda_stream);
+
+/* Forks: slot children[i] begins with the first lengths[i] positions of slot parents[i].  Its places name the parent's whole pages, then page
+ * fresh[i] with the positions behind them, copied in all layers (not looked at where there are none), then `empty`; refs[p], how many places
+ * of the table name page p, goes up by one for each.  What the child's places held before is not given back: free the slot first.  A slot may
+ * have many children in a call; no slot is a child twice, or a parent and a child, and no fresh page is in use.  A fork that names slots or lengths outside the
+ * table is left out; without a fresh page in the pool the child gets the whole pages alone. */
+int grb_kv_fork(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t* parents, const int32_t* children, const int32_t* lengths, const int32_t* fresh,
+                int32_t* refs, int32_t empty, uint32_t n, void* cuda_stream);
+/* The slots' places become `empty` and the counts of the pages they named go down.  A slot outside the table is left out; one named twice is freed once. */
+int grb_kv_free(const grb_kv_table* table, const int32_t* slots, int32_t* refs, uint32_t pages, int32_t empty, uint32_t n, void* cuda_stream);
+/* Pages in use (refs > 0) to the front of the pool: with *used of them, the i-th at *used or behind goes to the i-th free one before it, entries and
+ * count, in all layers, and the table's places follow.  where[p] (as many as there are pages) is the new number of page p, -1 for one that is not in use. */
+uint64_t grb_kv_compact_scratch_bytes(uint32_t pages);
+int grb_kv_compact(const grb_kv_pages* pages, const grb_kv_table* table, int32_t* refs, int32_t* where, int32_t* used, void* scratch, uint64_t scratch_bytes,
+                   void* cuda_stream);
 
 #ifdef __cplusplus
 }
