@@ -31,7 +31,7 @@
 namespace grb {
 
 constexpr uint32_t kKvDim = 128, kKvPage = 256;
-constexpr uint32_t kKvNanByte = 255, kKvLeastByte = 127 - 40;
+constexpr uint32_t kKvNanByte = 255, kKvLeastByte = 127 - 40, kQ4MostByte = 127 + 22;
 
 enum : int { kKvBf16 = 0, kKvE4m3 = 1, kKvQ4 = 4 };      // formats, numbered as in the C interface
 constexpr uint32_t kQ4Codes = kKvDim / 2;                // bytes of an entry's codes
@@ -110,16 +110,23 @@ __device__ __forceinline__ uint32_t kv_codes(float lo, float hi, uint32_t byte) 
 
 
 // ---- 4 bits ---------------------------------------------------------------------------------------------------------
-// Exponent byte of an entry whose largest magnitude is `amax`.  (A quotient by 7 that is no power of two does not round to one: below
-// 7 2^k values are 2^(k - 21) apart, a seventh of which is more than half of a step of the quotient.)
+// Exponent byte of an entry whose largest magnitude is `amax` = 1.f 2^(E - 127): 7 = 1.75 2^2, so floor(log2(amax / 7)) = E - 127 - 3 + (1.f >= 1.75).
 __device__ __forceinline__ uint32_t q4_exp_byte(float amax, bool finite) {
-  const int e = int(__float_as_uint(__fdiv_rn(amax, 7.f)) >> 23) - 127 + 9;
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = int(bits >> 23) - 127 - 3 + ((bits & 0x7FFFFFu) >= 0x600000u) + 9;
   return finite ? uint32_t(min(max(e, -40), 22) + 127) : kKvNanByte;
 }
-// Scale byte of a group whose largest magnitude is `amax`, and the scale times the entry's unit, 2^(e - 24).
+// Scale byte of a group whose largest magnitude is `amax`, and the scale times the entry's unit, 2^(e - 24).  (A quotient by 7 that lies on no border
+// between two scales does not round to one: values next to seven times a border are farther apart than seven halves of a step of the quotient.)
+// EIGHT: amax has eight significant bits.  Then the quotient lies on a border, or 2^-9 of it or more from all of them, and the product with
+// the rounded seventh, taken to 12 bits first, lands where the quotient does (all 128 fractions agree).
+template <bool EIGHT>
 __device__ __forceinline__ uint32_t q4_scale_byte(float amax, uint32_t exp_byte, float& step) {
-  const float want = fminf(fmaxf(__fmul_rn(__fdiv_rn(amax, 7.f), __uint_as_float((127u + 24u + 127u - exp_byte) << 23)), 16.f), 63488.f);
-  const uint32_t bits = __float_as_uint(want), five = (bits + 0x3FFFFu + (bits >> 19 & 1u)) >> 19;     // five bits, ties to even
+  const float to_unit = __uint_as_float((127u + 24u + 127u - exp_byte) << 23);
+  const float want = fminf(fmaxf(__fmul_rn(EIGHT ? __fmul_rn(amax, 0.14285715f) : __fdiv_rn(amax, 7.f), to_unit), 16.f), 63488.f);
+  uint32_t bits = __float_as_uint(want);
+  if constexpr (EIGHT) bits = (bits + 0x400u) & ~0x7FFu;
+  const uint32_t five = (bits + 0x3FFFFu + (bits >> 19 & 1u)) >> 19;     // five bits, ties to even
   step = __fmul_rn(__uint_as_float(five << 19), __uint_as_float((exp_byte - 24u) << 23));
   return five - 127u * 16u;
 }
@@ -230,17 +237,24 @@ kv_rows_kernel(const KvRowsArgs a) {
         const bool finite = m < 0x7F80u;
         const uint32_t exp = q4_exp_byte(__uint_as_float(m << 16), finite);
         float step;
-        uint32_t scale = q4_scale_byte(finite ? group : 0.f, finite ? exp : 127u, step), code = 0;
-        // A product with the rounded reciprocal is 2^-19 of the quotient at most off.  The quotient of a value of eight bits and a step of
-        // five lies on a border between two codes, or 2^-11 or more from all of them; rounded to 2^-13 first, it lands on the right side.
-        const float inverse = __frcp_rn(step);
+        uint32_t scale = q4_scale_byte<true>(finite ? group : 0.f, finite ? exp : 127u, step);
+        if (exp == kQ4MostByte) {                     // (the only entries with values beyond 7 steps and a half; 7 steps are a BF16 number)
+          const __nv_bfloat162 most = __float2bfloat162_rn(__fmul_rn(step, 7.f)), least = __hneg2(most);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          auto nibble = [&](float v) {                // code + 8 in the lowest bits
-            const float q = fminf(fmaxf(__fmul_rn(v, inverse), -7.f), 7.f);
-            return __float_as_uint(__fadd_rn(__fadd_rn(__fadd_rn(q, 1536.f), -1536.f), 12582920.f)) & 15u;
-          };
-          code |= (nibble(bf_lo(w[j])) | nibble(bf_hi(w[j])) << 16) << (4 * j);
+          for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 v = __hmax2(__hmin2(*reinterpret_cast<__nv_bfloat162*>(&w[j]), most), least);
+            w[j] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+        }
+        // The quotient of a value of eight bits and a step of five lies on a border between two codes, or 2^-11 or more from all of them.  A product with the
+        // reciprocal, 2^-19 of it off at most, rounded to 2^-13 - by adding 1536 - lands on the right side; added to 2^23 1.5 + 8, it is the code.
+        float inverse;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(step));
+        uint32_t code = 0;
+#pragma unroll
+        for (int j = 3; j >= 0; --j) {
+          auto nibble = [&](float v) { return __float_as_uint(__fadd_rn(__fmaf_rn(v, inverse, 1536.f), 12582920.f - 1536.f)); };     // code + 8 in the lowest byte, 0 in the next
+          code = code * 16 + __byte_perm(nibble(bf_lo(w[j])), nibble(bf_hi(w[j])), 0x5410);
         }
         if (!finite) { code = 0x88888888u; scale = 64u; }
         if (in[i]) {

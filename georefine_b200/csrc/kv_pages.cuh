@@ -6,7 +6,8 @@
 // to the i-th free one before u, so every page moves once at most and nothing moves onto a page that is still to be read.
 //
 // Memory bounds the copies.  A piece of work is one head's part of one page in one plane (a layer's keys or values), whose bytes lie together;
-// CTAs stay and take the pieces in turn, forks of one parent side by side, so that its bytes come from L2 after the first.
+// warps take the pieces, eight loads of 16 bytes a lane on their way; forks of one parent run side by side, so that its bytes come from L2
+// after the first.  (A CTA a piece, which looks up where the piece lies before its first byte can move: 204 us for the forks that take ??.)
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -17,39 +18,41 @@ namespace grb {
 
 constexpr int kPageThreads = 256;
 
-// The first `count` positions of one head's part of a page of plane p (keys, even, or values of layer p / 2).  Whole CTA.
+// Bytes between addresses that are multiples of 16.  Whole warp.
+__device__ __forceinline__ void kv_copy_bytes(uint8_t* dst, const uint8_t* src, uint32_t bytes, uint32_t lane) {
+  const uint32_t pieces = bytes / 16;
+  constexpr uint32_t kAtOnce = 8;
+  for (uint32_t i0 = lane; i0 < pieces; i0 += kAtOnce * 32) {
+    uint4 x[kAtOnce];
+#pragma unroll
+    for (uint32_t i = 0; i < kAtOnce; ++i)
+      if (i0 + i * 32 < pieces) x[i] = reinterpret_cast<const uint4*>(src)[i0 + i * 32];
+#pragma unroll
+    for (uint32_t i = 0; i < kAtOnce; ++i)
+      if (i0 + i * 32 < pieces) reinterpret_cast<uint4*>(dst)[i0 + i * 32] = x[i];
+  }
+  if (lane < bytes % 16) dst[pieces * 16 + lane] = src[pieces * 16 + lane];
+}
+// The first `count` positions of one head's part of a page of plane p (keys, even, or values of layer p / 2).  Whole warp.
 template <int FORMAT>
-__device__ __forceinline__ void kv_copy_head(const KvPagesArgs& a, uint32_t p, uint32_t head, uint32_t from, uint32_t to, uint32_t count) {
+__device__ __forceinline__ void kv_copy_head(const KvPagesArgs& a, uint32_t p, uint32_t head, uint32_t from, uint32_t to, uint32_t count, uint32_t lane) {
   constexpr uint32_t kEntry = FORMAT == kKvQ4 ? kQ4Codes : FORMAT == kKvE4m3 ? kKvDim : 2 * kKvDim, kBlock = FORMAT == kKvQ4 ? kQ4Page : kEntry * kKvPage;
   uint8_t* const plane = static_cast<uint8_t*>(p & 1u ? a.v : a.k) + int64_t(p >> 1) * a.layer_stride * (FORMAT == kKvBf16 ? 2 : 1);
   const size_t from_block = size_t(from) * a.nkv + head, to_block = size_t(to) * a.nkv + head;
   const uint8_t* const src = plane + from_block * kBlock;
   uint8_t* const dst = plane + to_block * kBlock;
-  const uint32_t tid = threadIdx.x;
   // (4 bits: a whole page is one piece of memory, scales and exponents behind the codes)
-  const uint32_t pieces = (FORMAT == kKvQ4 && count == kKvPage ? kQ4Page : count * kEntry) / 16;
-  constexpr uint32_t kAtOnce = 8;
-  for (uint32_t i0 = tid; i0 < pieces; i0 += kAtOnce * kPageThreads) {
-    uint4 x[kAtOnce];
-#pragma unroll
-    for (uint32_t i = 0; i < kAtOnce; ++i)
-      if (i0 + i * kPageThreads < pieces) x[i] = reinterpret_cast<const uint4*>(src)[i0 + i * kPageThreads];
-#pragma unroll
-    for (uint32_t i = 0; i < kAtOnce; ++i)
-      if (i0 + i * kPageThreads < pieces) reinterpret_cast<uint4*>(dst)[i0 + i * kPageThreads] = x[i];
-  }
-  if constexpr (FORMAT == kKvQ4) {
-    if (count < kKvPage && tid < count) {
-      reinterpret_cast<uint32_t*>(dst + kQ4ScalesAt)[tid] = reinterpret_cast<const uint32_t*>(src + kQ4ScalesAt)[tid];
-      dst[kQ4ExpsAt + tid] = src[kQ4ExpsAt + tid];
-    }
+  const bool whole = FORMAT == kKvQ4 && count == kKvPage;
+  kv_copy_bytes(dst, src, whole ? kQ4Page : count * kEntry, lane);
+  if (FORMAT == kKvQ4 && !whole) {
+    kv_copy_bytes(dst + kQ4ScalesAt, src + kQ4ScalesAt, count * 4, lane);
+    kv_copy_bytes(dst + kQ4ExpsAt, src + kQ4ExpsAt, count, lane);
   }
   if constexpr (FORMAT == kKvE4m3) {
     uint8_t* const exps = (p & 1u ? a.v_exp : a.k_exp) + int64_t(p >> 1) * a.exp_stride;
-    if (tid < count) exps[to_block * kKvPage + tid] = exps[from_block * kKvPage + tid];
+    for (uint32_t i = lane; i < count; i += 32) exps[to_block * kKvPage + i] = exps[from_block * kKvPage + i];
   }
 }
-static_assert(kPageThreads == kKvPage, "a thread for each position's scales and exponents");
 
 struct KvCopyArgs {
   KvPagesArgs pages;
@@ -61,16 +64,17 @@ struct KvCopyArgs {
 };
 
 template <int FORMAT>
-__global__ void __launch_bounds__(kPageThreads)
+__global__ void __launch_bounds__(kPageThreads, 4)
 kv_copy_kernel(const KvCopyArgs a) {
   step_kernel_entry();
   const uint32_t n = a.moves ? min(uint32_t(max(*a.moves, 0)), a.n) : a.n, parts = 2 * a.pages.layers * a.pages.nkv;
-  for (uint64_t item = blockIdx.x; item < uint64_t(n) * parts; item += gridDim.x) {
+  const uint64_t warps = uint64_t(gridDim.x) * (kPageThreads / 32);
+  for (uint64_t item = uint64_t(blockIdx.x) * (kPageThreads / 32) + (threadIdx.x >> 5); item < uint64_t(n) * parts; item += warps) {
     const uint32_t part = uint32_t(item / n), i = uint32_t(item - uint64_t(part) * n);
     const uint32_t from = uint32_t(a.src[i]), to = uint32_t(a.dst[i]);
     if (from >= a.pages.pages || to >= a.pages.pages || from == to) continue;
     const int32_t count = a.positions ? min(max(a.positions[i], 0), int32_t(kKvPage)) : int32_t(kKvPage);
-    kv_copy_head<FORMAT>(a.pages, part / a.pages.nkv, part % a.pages.nkv, from, to, uint32_t(count));
+    kv_copy_head<FORMAT>(a.pages, part / a.pages.nkv, part % a.pages.nkv, from, to, uint32_t(count), threadIdx.x & 31u);
   }
 }
 
@@ -89,30 +93,28 @@ struct KvForkArgs {
 };
 
 template <int FORMAT>
-__global__ void __launch_bounds__(kPageThreads)
+__global__ void __launch_bounds__(kPageThreads, 4)
 kv_fork_kernel(const KvForkArgs a) {
   step_kernel_entry();
-  const uint32_t parts = 2 * a.pages.layers * a.pages.nkv;
-  for (uint64_t item = blockIdx.x; item < uint64_t(a.n) * parts; item += gridDim.x) {
-    const uint32_t part = uint32_t(item / a.n), i = uint32_t(item - uint64_t(part) * a.n);
-    const uint32_t parent = uint32_t(a.parents[i]), child = uint32_t(a.children[i]), length = uint32_t(a.lengths[i]);
-    // a fork that names what is not there is left out
-    if (parent >= a.slots || child >= a.slots || parent == child || length > a.max_pages * kKvPage) continue;
-    const int32_t* const from = a.table + parent * a.ld;
-    const uint32_t whole = length / kKvPage, rest = length % kKvPage;
-    const uint32_t fresh = rest ? uint32_t(a.fresh[i]) : 0xFFFFFFFFu;
-    if (part == 0) {
-      int32_t* const to = a.table + child * a.ld;
-      for (uint32_t p = threadIdx.x; p < a.max_pages; p += kPageThreads) {
-        const int32_t page = p < whole ? from[p] : p == whole && fresh < a.pages.pages ? int32_t(fresh) : a.empty;
-        to[p] = page;
-        if (page != a.empty && uint32_t(page) < a.pages.pages) atomicAdd(a.refs + page, 1);
-      }
+  // a CTA is one fork's: where it lies is looked up once for all of the CTA's pieces
+  const uint32_t parts = 2 * a.pages.layers * a.pages.nkv, i = blockIdx.x % a.n, slice = blockIdx.x / a.n, slices = gridDim.x / a.n;
+  const uint32_t parent = uint32_t(a.parents[i]), child = uint32_t(a.children[i]), length = uint32_t(a.lengths[i]);
+  // a fork that names what is not there is left out
+  if (parent >= a.slots || child >= a.slots || parent == child || length > a.max_pages * kKvPage) return;
+  const int32_t* const from = a.table + parent * a.ld;
+  const uint32_t whole = length / kKvPage, rest = length % kKvPage;
+  const uint32_t fresh = rest ? uint32_t(a.fresh[i]) : 0xFFFFFFFFu, source = rest ? uint32_t(from[whole]) : 0xFFFFFFFFu;
+  if (slice == 0) {
+    int32_t* const to = a.table + child * a.ld;
+    for (uint32_t p = threadIdx.x; p < a.max_pages; p += kPageThreads) {
+      const int32_t page = p < whole ? from[p] : p == whole && fresh < a.pages.pages ? int32_t(fresh) : a.empty;
+      to[p] = page;
+      if (page != a.empty && uint32_t(page) < a.pages.pages) atomicAdd(a.refs + page, 1);
     }
-    if (!rest || fresh >= a.pages.pages) continue;
-    const uint32_t source = uint32_t(from[whole]);
-    if (source < a.pages.pages && source != fresh) kv_copy_head<FORMAT>(a.pages, part / a.pages.nkv, part % a.pages.nkv, source, fresh, rest);
   }
+  if (fresh >= a.pages.pages || source >= a.pages.pages || source == fresh) return;
+  for (uint32_t part = slice * (kPageThreads / 32) + (threadIdx.x >> 5); part < parts; part += slices * (kPageThreads / 32))
+    kv_copy_head<FORMAT>(a.pages, part / a.pages.nkv, part % a.pages.nkv, source, fresh, rest, threadIdx.x & 31u);
 }
 
 // A slot's pages counted down and its places emptied.  (An exchange: a slot named twice gives its pages back once.)
@@ -125,7 +127,7 @@ struct KvFreeArgs {
   uint32_t pages, n;
   int32_t empty;
 };
-__global__ void __launch_bounds__(kPageThreads)
+__global__ void __launch_bounds__(kPageThreads, 4)
 kv_free_kernel(const KvFreeArgs a) {
   step_kernel_entry();
   const uint64_t places = uint64_t(a.n) * a.max_pages;
@@ -182,7 +184,7 @@ kv_compact_plan_kernel(const KvCompactArgs a) {
   if (tid == 0) { *a.used = int32_t(used); *a.moves = int32_t(sources); }
 }
 // Behind the copies: the table names the new places, and the counts go along.
-__global__ void __launch_bounds__(kPageThreads)
+__global__ void __launch_bounds__(kPageThreads, 4)
 kv_compact_table_kernel(const KvCompactArgs a) {
   step_kernel_entry();
   const uint64_t places = uint64_t(a.slots) * a.max_pages, stride = uint64_t(gridDim.x) * kPageThreads, first = uint64_t(blockIdx.x) * kPageThreads + threadIdx.x;

@@ -15,22 +15,22 @@ namespace {
 
 using namespace grb;
 
-// CTAs of a copy: as many as stay resident, or one for each piece.
-uint32_t copy_ctas(uint64_t pieces) {
+// So many CTAs, or as many as stay resident.
+uint32_t copy_ctas(uint64_t ctas) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  return uint32_t(std::min<uint64_t>(pieces, uint64_t(std::max(device_sm_count(dev), 0)) * 8));
+  return uint32_t(std::min<uint64_t>(ctas, uint64_t(std::max(device_sm_count(dev), 0)) * 4));
 }
 uint64_t parts_of(const KvPagesArgs& p) { return 2ull * p.layers * p.nkv; }
 
 template <class Args>
-int launch_copies(void (*bf16)(Args), void (*e4m3)(Args), void (*q4)(Args), uint32_t format, uint64_t pieces, cudaStream_t stream, const Args& a) {
-  const uint32_t ctas = copy_ctas(pieces);
+int launch_copies(void (*bf16)(Args), void (*e4m3)(Args), void (*q4)(Args), uint32_t format, uint32_t ctas, cudaStream_t stream, const Args& a) {
   if (!ctas) return GRB_ERR_CUDA;
   return launch_step(format == GRB_KV_Q4 ? q4 : format == GRB_KV_E4M3 ? e4m3 : bf16, dim3(ctas), dim3(kPageThreads), 0, stream, a);
 }
+constexpr uint32_t kWarps = kPageThreads / 32;
 int copies(uint32_t format, uint64_t pieces, cudaStream_t stream, const KvCopyArgs& a) {
-  return launch_copies(kv_copy_kernel<kKvBf16>, kv_copy_kernel<kKvE4m3>, kv_copy_kernel<kKvQ4>, format, pieces, stream, a);
+  return launch_copies(kv_copy_kernel<kKvBf16>, kv_copy_kernel<kKvE4m3>, kv_copy_kernel<kKvQ4>, format, copy_ctas((pieces + kWarps - 1) / kWarps), stream, a);
 }
 // A table that a call writes to.
 int own_table_of(const grb_kv_table* t) {
@@ -42,11 +42,11 @@ bool layers_fit(const KvPagesArgs& p) { return parts_of(p) <= 0x7FFFFFFFull; }
 template <class T, int V, bool HALF>
 int rotary_launch(RotaryArgs a, bool copy, cudaStream_t stream) {
   a.items = a.turned / 2 / (HALF || V == 1 ? V : V / 2) + (copy ? (a.dim - a.turned) / V : 0);
-  const uint32_t per_row = std::min<uint32_t>(a.items, kRotaryThreads), slots = kRotaryThreads / per_row;
-  a.heads_at_once = std::min(a.heads, slots);
-  a.rows_per_cta = std::min(slots / a.heads_at_once, a.rows);
-  const uint32_t ctas = (a.rows + a.rows_per_cta - 1) / a.rows_per_cta;
-  return launch_step(rotary_kernel<T, V, HALF>, dim3(ctas), dim3(kRotaryThreads), a.rows_per_cta * (a.turned / 2) * uint32_t(sizeof(float2)), stream, a);
+  a.groups = (a.heads + kRotaryHeads - 1) / kRotaryHeads;
+  a.groups_per_cta = kRotaryThreads / std::min<uint32_t>(a.items, kRotaryThreads);
+  const uint64_t ctas = (uint64_t(a.rows) * a.groups + a.groups_per_cta - 1) / a.groups_per_cta;
+  if (ctas > 0x7FFFFFFFull) return GRB_ERR_UNSUPPORTED;
+  return launch_step(rotary_kernel<T, V, HALF>, dim3(uint32_t(ctas)), dim3(kRotaryThreads), 0, stream, a);
 }
 template <class T, bool HALF>
 int rotary_width(const RotaryArgs& a, bool copy, cudaStream_t stream) {
@@ -135,7 +135,10 @@ int grb_kv_fork(const grb_kv_pages* pages, const grb_kv_table* table, const int3
   a.refs = refs;
   a.empty = empty;
   a.n = n;
-  return launch_copies(kv_fork_kernel<kKvBf16>, kv_fork_kernel<kKvE4m3>, kv_fork_kernel<kKvQ4>, pages->format, n * parts_of(a.pages), static_cast<cudaStream_t>(cuda_stream), a);
+  // CTAs of a fork: as many as there are pieces for their warps, and as stay resident together
+  const uint64_t most = (parts_of(a.pages) + kWarps - 1) / kWarps, slices = std::max<uint64_t>(1, std::min<uint64_t>(most, copy_ctas(~0ull) / n));
+  if (n * slices > 0x7FFFFFFFull) return GRB_ERR_UNSUPPORTED;
+  return launch_copies(kv_fork_kernel<kKvBf16>, kv_fork_kernel<kKvE4m3>, kv_fork_kernel<kKvQ4>, pages->format, uint32_t(n * slices), static_cast<cudaStream_t>(cuda_stream), a);
 }
 
 int grb_kv_free(const grb_kv_table* table, const int32_t* slots, int32_t* refs, uint32_t pages, int32_t empty, uint32_t n, void* cuda_stream) {

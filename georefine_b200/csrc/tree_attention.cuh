@@ -214,7 +214,7 @@ __device__ __forceinline__ void tree_store_q4(uint8_t* page, uint32_t at, float 
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float step;
-    const uint32_t scale = q4_scale_byte(group[h], exp, step);
+    const uint32_t scale = q4_scale_byte<false>(group[h], exp, step);
     // dimensions 2 l and 2 l + 1 are nibble l % 4 of either half of word l / 4
     uint32_t code = 0x00080008u;
     if (fine) code = q4_nibble(__fdiv_rn(x[2 * h], step)) | q4_nibble(__fdiv_rn(x[2 * h + 1], step)) << 16;
