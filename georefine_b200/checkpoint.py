@@ -62,11 +62,48 @@ def decoder_config(config, **overrides):
                       rope_theta=float(config.get("rope_theta", 10000.0)), eps=float(config.get("rms_norm_eps", 1e-6)))
     except (KeyError, TypeError, ValueError) as exc:
         raise ContextServingError(f"model config lacks a decoder field: {exc}") from exc
+    fields.update(_rotary_fields(config, fields["head_dim"]))
     for flag in ("attention_bias", "mlp_bias"):
         if config.get(flag):
             raise ContextServingError(f"unsupported decoder family: {flag} is set")
     fields.update(overrides)
     return DecoderConfig(**fields)
+
+
+def _rotary_fields(config, head_dim):
+    """Rotary positions of a ``config.json``: which part of a head turns, and the scaling for long contexts."""
+    given = dict(config.get("rope_scaling") or config.get("rope_parameters") or {})
+    fields = {}
+    part = config.get("partial_rotary_factor", given.pop("partial_rotary_factor", None))
+    if "rope_theta" in given:
+        theta = float(given.pop("rope_theta"))
+        if "rope_theta" not in config:
+            fields["rope_theta"] = theta
+    kind = given.pop("rope_type", given.pop("type", "default") if "type" in given else "default")
+    given.pop("type", None)
+    try:
+        if part is not None and float(part) != 1.0:
+            fields["rope_dim"] = int(head_dim * float(part))
+        original = given.pop("original_max_position_embeddings", None) or config.get("max_position_embeddings")
+        if "low_freq_factor" in given:
+            scaling = {"kind": "bands", "factor": float(given.pop("factor")), "original": float(original), "low": float(given.pop("low_freq_factor")),
+                       "high": float(given.pop("high_freq_factor"))}
+        elif kind == "linear":
+            scaling = {"kind": "linear", "factor": float(given.pop("factor"))}
+        elif kind == "yarn":
+            scaling = {"kind": "yarn", "factor": float(given.pop("factor")), "original": float(original), "fast": float(given.pop("beta_fast", None) or 32.0),
+                       "slow": float(given.pop("beta_slow", None) or 1.0), "attention": given.pop("attention_factor", None)}
+        elif kind == "default":
+            scaling = None
+        else:
+            raise ContextServingError(f"unsupported rotary positions: type {kind!r}")
+    except (KeyError, TypeError, ValueError) as exc:
+        raise ContextServingError(f"model config lacks a number of its rotary positions: {exc}") from exc
+    if any(v is not None for v in given.values()):
+        raise ContextServingError(f"unsupported rotary positions: {sorted(given)}")
+    if scaling is not None:
+        fields["rope_scaling"] = scaling
+    return fields
 
 
 def mtp_shapes(cfg):

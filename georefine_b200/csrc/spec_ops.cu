@@ -51,8 +51,14 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   constexpr bool F8 = FORMAT != kKvBf16;
   using P = std::conditional_t<FORMAT == kKvQ4, TreeQ4, TreePart<F8>>;
   void (*part)(TreeArgs);
-  if constexpr (FORMAT == kKvQ4) part = a.tile_rows * a.group <= 8 ? tree_q4_kernel<1> : tree_q4_kernel<2>;
-  else part = tree_part_kernel<F8>;
+  int resident = 3;                                          // CTAs an SM
+  if constexpr (FORMAT == kKvQ4) {
+    const bool one = a.tile_rows * a.group <= 8;
+    part = one ? tree_q4_kernel<1> : tree_q4_kernel<2>;
+    resident = one ? 4 : 3;
+  } else {
+    part = tree_part_kernel<F8>;
+  }
   static std::once_flag once[64];
   static int prepared[64];
   int dev = 0;
@@ -73,7 +79,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   const uint32_t threads = a.rows > kTreePrepThreads ? kTreePrepMost : kTreePrepThreads;
   if (int st = launch_step(tree_prep_kernel<FORMAT>, dim3((warps + threads / 32 - 1) / (threads / 32) + 1), dim3(threads), a.rows * 6, stream, a, P::kPositions)) return st;
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
-  if (int st = launch_step(part, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 3))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
+  if (int st = launch_step(part, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * resident))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
   if (a.wide_from) {
     if (int st = launch_step(tree_wide_kernel<FORMAT>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
   }

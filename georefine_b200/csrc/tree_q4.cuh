@@ -19,13 +19,14 @@ struct TreeQ4 {
   static constexpr int kThreads = 128;
   static constexpr uint32_t kPositions = 512;                // of a part
   static constexpr uint32_t kChunk = 32;                     // positions of a warp's step
-  static constexpr uint32_t kStages = 4;                     // a warp's chunks of a unit
+  static constexpr uint32_t kChunks = 4;                     // of a warp and unit
+  static constexpr uint32_t kStages = 3;
   static constexpr uint32_t kVAt = kChunk * kQ4Codes, kKScalesAt = 2 * kVAt, kVScalesAt = kKScalesAt + kChunk * 4, kKExpsAt = kVScalesAt + kChunk * 4,
                             kVExpsAt = kKExpsAt + kChunk, kStage = kVExpsAt + kChunk;
   static constexpr uint32_t kWarp = kStages * kStage + kChunk * 16;    // and what the exponents of the chunk at hand mean
   static constexpr uint32_t kSmem = 4 * kWarp;
 };
-static_assert(TreeQ4::kStages * 4 * TreeQ4::kChunk == TreeQ4::kPositions && TreeQ4::kPositions == 2 * kKvPage, "a unit is two pages, four chunks a warp");
+static_assert(TreeQ4::kChunks * 4 * TreeQ4::kChunk == TreeQ4::kPositions && TreeQ4::kPositions == 2 * kKvPage, "a unit is two pages, four chunks a warp");
 static_assert(TreeQ4::kStage >= 8 * kKvDim * 4, "a warp's stage holds its part of the merge, eight columns at a time");
 static_assert(TreeQ4::kStage % 16 == 0 && kKvPage % TreeQ4::kChunk == 0, "copies of 16 bytes; a chunk lies in one page");
 
@@ -151,16 +152,18 @@ __device__ __forceinline__ void q4_ask_columns(const TreeArgs& a, const Q4Unit& 
     k.scale[b] = make_float2(m < used ? a.q_scale[size_t(t.first + m0) * a.nq + head + (m - m0 * a.group)] : 0.f,
                              m + 1 < used ? a.q_scale[size_t(t.first + m1) * a.nq + head + (m + 1 - m1 * a.group)] : 0.f);
   }
-  k.plain = 0x7FFFFFFF;
-  for (uint32_t i = 0; i < t.rows; ++i) {
-    const int32_t e = a.extent[t.first + i];
-    k.plain = min(k.plain, a.row_base ? min(a.row_base[t.first + i], e) : e);
+  k.plain = t.extent;
+  if (t.rows > 1 || a.row_base) {
+    for (uint32_t i = 0; i < t.rows; ++i) {
+      const int32_t e = a.extent[t.first + i];
+      k.plain = min(k.plain, a.row_base ? min(a.row_base[t.first + i], e) : e);
+    }
   }
 }
 
 // One warp's 32 positions from `at` on, against NB blocks of eight columns.
 template <int NB>
-__device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, const Q4Warp& w, unsigned char* stage, int32_t at, const Q4Columns<NB>& k, float2 (&ref)[NB],
+__device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, const Q4Warp& w, unsigned char* stage, int32_t at, bool first, const Q4Columns<NB>& k, float2 (&ref)[NB],
                                          float2 (&sum)[NB], float (&o)[NB][8][4]) {
   constexpr float kSlack = 8.f;
   using P = TreeQ4;
@@ -251,6 +254,7 @@ __device__ __forceinline__ void q4_chunk(const TreeArgs& a, const Q4Unit& t, con
         if (!(v > __fadd_rn(r, kSlack))) continue;
         const float f = exp2_approx(__fsub_rn(r, v));        // (from nothing: 0)
         r = v;
+        if (first) continue;                                 // (nothing to scale)
         l = __fmul_rn(l, f);
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
@@ -307,7 +311,7 @@ __device__ __forceinline__ uint32_t q4_merge_index(uint32_t m, uint32_t piece) {
 
 // NB: blocks of eight columns.  Calls whose tiles have eight at most - decode rows - take one.
 template <int NB>
-__global__ void __launch_bounds__(TreeQ4::kThreads, 3)
+__global__ void __launch_bounds__(TreeQ4::kThreads, NB == 1 ? 4 : 3)
 tree_q4_kernel(const TreeArgs a) {
   step_kernel_entry();
   using P = TreeQ4;
@@ -338,38 +342,31 @@ tree_q4_kernel(const TreeArgs a) {
                                 (of_scales ? kQ4ScalesAt + w.warp * P::kChunk * 4 + (w.lane & 7u) * 16 : kQ4ExpsAt + w.warp * P::kChunk + (w.lane & 1u) * 16);
   const uint32_t to_others = of_scales ? P::kKScalesAt + w.lane * 16 : P::kKExpsAt + (w.lane - 16) * 16, page_bytes = a.nkv * kQ4Page;
   const uint32_t half = of_scales ? 4 * P::kChunk * 4 : 4 * P::kChunk;       // to the second 128 positions of a page
-  // Chunk i of a unit goes to stage i.  Stages are asked for a unit ahead, as they are left; where the next unit's pages lie is looked up
-  // while the first chunk of this one is at hand.
-  int32_t page0, page1;
-  auto look_up = [&](const Q4Unit& u) {
-    const uint32_t p = u.part * 2;
-    const bool in = u.at < end && uint32_t(u.seq) < a.table.slots;
-    page0 = in && p < a.table.max_pages ? a.table.table[u.seq * a.table.ld + p] : -1;
-    page1 = in && p + 1 < a.table.max_pages ? a.table.table[u.seq * a.table.ld + p + 1] : -1;
-  };
-  uint32_t chunks = 0, there = 0;                            // of the unit asked for: how many, and which of its pages are in the pool
-  auto request = [&](const Q4Unit& u, uint32_t i) {
-    if (i < chunks && there >> (i >> 1) & 1u) {
-      const uint64_t block = uint64_t(uint32_t(i >> 1 ? page1 : page0)) * page_bytes + u.kvh * kQ4Page;
-      const uint32_t dst = ring + i * P::kStage + w.lane * 16, up = (i & 1u) * (4 * P::kChunk * kQ4Codes);
+  // Two chunks are on their way while a third is at hand; units with fewer chunks, and pages outside the pool, leave their stages empty.  Where the
+  // next unit's pages lie is looked up at this unit's beginning, two chunks before it is needed.
+  auto request = [&](uint32_t stage, int32_t page, uint32_t kvh, uint32_t i, uint32_t chunks) {
+    if (i < chunks && uint32_t(page) < a.table.pages) {
+      const uint64_t block = uint64_t(uint32_t(page)) * page_bytes + kvh * kQ4Page;
+      const uint32_t dst = ring + stage + w.lane * 16, up = (i & 1u) * (4 * P::kChunk * kQ4Codes);
       const uint8_t* const k = k_codes + block + up;
       const uint8_t* const v = v_codes + block + up;
 #pragma unroll
       for (int x = 0; x < 4; ++x) cp_async_16(dst + 512 * x, k + 512 * x, 16u);
 #pragma unroll
       for (int x = 0; x < 4; ++x) cp_async_16(dst + P::kVAt + 512 * x, v + 512 * x, 16u);
-      if (w.lane < 20) cp_async_16(ring + i * P::kStage + to_others, others + block + (i & 1u) * half, 16u);
+      if (w.lane < 20) cp_async_16(ring + stage + to_others, others + block + (i & 1u) * half, 16u);
     }
     cp_async_commit();
   };
-  auto begin = [&](const Q4Unit& u) {                        // the pages have come
-    chunks = u.at < end ? q4_chunks(u, w.warp) : 0u;
-    there = uint32_t(uint32_t(page0) < a.table.pages) | uint32_t(uint32_t(page1) < a.table.pages) << 1;
+  auto page_of = [&](const Q4Unit& u, uint32_t i) {
+    const uint32_t p = u.part * 2 + i;
+    return u.at < end && uint32_t(u.seq) < a.table.slots && p < a.table.max_pages ? a.table.table[u.seq * a.table.ld + p] : -1;
   };
-  look_up(t);
-  begin(t);
-#pragma unroll
-  for (uint32_t i = 0; i < P::kStages; ++i) request(t, i);
+  auto after = [&](uint32_t stage) { return stage == (P::kStages - 1) * P::kStage ? 0u : stage + P::kStage; };
+  int32_t page0 = page_of(t, 0), page1 = page_of(t, 1);
+  uint32_t stage = 0, chunks = q4_chunks(t, w.warp);
+  request(0, page0, t.kvh, 0, chunks);
+  request(P::kStage, page0, t.kvh, 1, chunks);
   Q4Columns<NB> columns;
   q4_ask_columns<NB>(a, t, w, columns);
   while (t.at < end) {
@@ -384,26 +381,34 @@ tree_q4_kernel(const TreeArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[b][d][e] = 0.f;
     }
-    const uint32_t n = chunks, mine = there;
     Q4Unit next = t;
     q4_next(a, next, end);
-    look_up(next);
+    const int32_t next0 = page_of(next, 0), next1 = page_of(next, 1);
+    const uint32_t next_chunks = next.at < end ? q4_chunks(next, w.warp) : 0u;
     int32_t at = int32_t(t.part * P::kPositions + w.warp * P::kChunk);
+    bool first = true;
 #pragma unroll 1
-    for (uint32_t i = 0; i < P::kStages; ++i, at += 4 * P::kChunk) {
+    for (uint32_t i = 0; i < P::kChunks; ++i, at += 4 * P::kChunk) {
+      // (into the stage that the chunk before has left)
+      const bool same = i < 2;
+      request(after(after(stage)), same ? page1 : next0, same ? t.kvh : next.kvh, i ^ 2u, same ? chunks : next_chunks);
       cp_async_wait<P::kStages - 1>();
       __syncwarp();
       // (a page outside the pool: as if nobody saw the chunk)
-      if (i < n && mine >> (i >> 1) & 1u) q4_chunk<NB>(a, t, w, stages + i * P::kStage, at, columns, ref, sum, o);
+      if (i < chunks && uint32_t(same ? page0 : page1) < a.table.pages) {
+        q4_chunk<NB>(a, t, w, stages + stage, at, first, columns, ref, sum, o);
+        first = false;
+      }
+      stage = after(stage);
       __syncwarp();
-      if (i == 0) begin(next);
-      if (i + 1 < P::kStages) request(next, i);              // (the last stage serves the merge first)
     }
-    // the next unit's columns are on their way while the warps' results are merged, eight columns at a time
-    const uint32_t used = t.rows * a.group, first = t.first, heads = t.kvh * a.group, part = t.part;
+    // the next unit's columns are on their way while the warps' results are merged, eight columns at a time, in the stage that was left last
+    const uint32_t used = t.rows * a.group, first_row = t.first, heads = t.kvh * a.group, part = t.part, merge_at = after(after(stage));
     t = next;
+    page0 = next0;
+    page1 = next1;
+    chunks = next_chunks;
     if (t.at < end) q4_ask_columns<NB>(a, t, w, columns);
-    constexpr uint32_t kMergeAt = (P::kStages - 1) * P::kStage;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       if (b && 8u * b >= used) break;
@@ -420,7 +425,7 @@ tree_q4_kernel(const TreeArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {                        // dimensions 16 r + 4 q ..: of word q / 2, 4 (q % 2) on
           const int d = 4 * (q >> 1) + (q & 1);
-          *reinterpret_cast<float4*>(reinterpret_cast<float*>(tree_smem + w.warp * P::kWarp + kMergeAt) + q4_merge_index(2 * w.c + j, 4 * w.r + q)) =
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(tree_smem + w.warp * P::kWarp + merge_at) + q4_merge_index(2 * w.c + j, 4 * w.r + q)) =
               make_float4(o[b][d][j], o[b][d + 2][j], o[b][d][2 + j], o[b][d + 2][2 + j]);
         }
       __syncthreads();
@@ -435,20 +440,19 @@ tree_q4_kernel(const TreeArgs a) {
           // (a warp that saw nothing adds zeros; one whose scores were all NaN has no reference either and adds NaN)
           const float e = ml[x].x == -INFINITY ? 1.f : exp2_approx(__fsub_rn(ml[x].x, mx));
           den = __fmaf_rn(e, ml[x].y, den);
-          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tree_smem + x * P::kWarp + kMergeAt) + q4_merge_index(m, w.lane));
+          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tree_smem + x * P::kWarp + merge_at) + q4_merge_index(m, w.lane));
           num.x = __fmaf_rn(e, v.x, num.x);
           num.y = __fmaf_rn(e, v.y, num.y);
           num.z = __fmaf_rn(e, v.z, num.z);
           num.w = __fmaf_rn(e, v.w, num.w);
         }
         const uint32_t col = 8 * b + m, rl = w.row_of(col);
-        const size_t to = (size_t(first + rl) * a.nq + heads + (col - rl * a.group)) * a.max_parts + part;
+        const size_t to = (size_t(first_row + rl) * a.nq + heads + (col - rl * a.group)) * a.max_parts + part;
         *reinterpret_cast<float4*>(a.part_acc + to * kKvDim + w.lane * 4) = num;
         if (w.lane == 0) a.part_ml[to] = make_float2(mx, den);
       }
       __syncthreads();                                       // the stages are free again
     }
-    request(t, P::kStages - 1);
   }
   cp_async_wait<0>();
 }

@@ -16,9 +16,10 @@ tokens alone, inside any batch, and as rows of a speculative verify pass.
 
 All per-sequence state is indexed by absolute position (KV pages), so a rewind is "set the position".
 
-Beyond the reference: the KV cache may be held in 8 bits (``BatchDecoder(kv_format="e4m3")``: about half the memory and traffic
-of a long context), and drafts may form trees that one pass checks (``Batcher.verify_trees``), both through
-``georefine_b200.ops.TreeAttention``.
+Beyond the reference: the KV cache may be held in 8 or in 4 bits (``BatchDecoder(kv_format="e4m3")``, ``"q4"``: about half or a quarter of
+the memory and traffic of a long context), and drafts may form trees that one pass checks (``Batcher.verify_trees``), both through
+``georefine_b200.ops.TreeAttention``; a sequence may go on in several ways from one cached prompt (``Batcher.fork``: whole pages are shared, and
+copied where one of them is to be written to); rotary positions may be paired, partial or scaled as ``DecoderConfig`` says.
 """
 from __future__ import annotations
 
@@ -53,11 +54,25 @@ class DecoderConfig:
     eps: float = 1e-6
     tp_world: int = 1        # tensor parallelism over the GPUs of one node: this process is rank tp_rank of tp_world
     tp_rank: int = 0
+    rope_layout: str = "half"          # pairs of the rotary positions, how many of a head's dimensions turn (None: all), and their
+    rope_dim: int | None = None        # scaling for long contexts: see ``ops.Rope``
+    rope_scaling: object = None
 
     def __post_init__(self):
+        if self.rope_scaling is not None:
+            object.__setattr__(self, "rope_scaling", tuple(sorted(dict(self.rope_scaling).items())))
+        if self.rope_layout not in ops.ROPE_LAYOUTS or (self.rope_dim is not None and not 2 <= self.rope_dim <= self.head_dim):
+            raise ValueError(f"rotary positions: the layout is one of {ops.ROPE_LAYOUTS}, and 2 to {self.head_dim} dimensions turn")
+        if self.rope_scaling is not None or self.rope_dim is not None:
+            ops.rope_frequencies(self.rope_dim or self.head_dim, self.rope_theta, self.rope_options)        # (refuses what it does not know)
         w = self.tp_world
         if w < 1 or not 0 <= self.tp_rank < w or self.heads % w or self.kv_heads % w or self.ffn % w or (self.ffn // w) % 128:
             raise ValueError("tensor parallelism needs the query heads, the KV heads and the FFN width (in 128-column chunks) to divide evenly")
+
+    @property
+    def rope_options(self) -> dict | None:
+        """The scaling as ``ops.Rope`` takes it."""
+        return None if self.rope_scaling is None else dict(self.rope_scaling)
 
     @property
     def qkv_rows(self) -> int:
@@ -241,6 +256,8 @@ class BatchDecoder:
     rows (prompt chunks, speculative drafts), no advance.  ``kind`` "tree": rows that are nodes of draft trees
     (``set_tree_rows``), no advance.
 
+    Slots may share pages (``fork_slot``); who is about to write positions of a slot asks for ``own_pages`` first.
+
     ``kv_format`` "e4m3" holds the KV cache in 8 bits (129 bytes for an entry of 256, each value off by at most 2^-4 of
     itself), "q4" in 4 (69 bytes, each value off by a fourteenth of the largest of its 32 neighbours, give or take a thirtieth of
     that); the formats are in ``csrc/kv_cache.cuh``."""
@@ -266,7 +283,20 @@ class BatchDecoder:
         self._table_host = np.full((self.max_slots + 1, self.pages_per_seq), -1, dtype=np.int64)
         self._free_pages = list(range(n_pages - 2, -1, -1))
         self._free_slots = list(range(self.max_slots - 1, -1, -1))
-        self.cos, self.sin = ops.rope_tables(self.max_context, cfg.rope_theta, self.dev)
+        # The attention turns all of a head in halves, by tables; other rotary positions are applied to its rows before, and its tables are ones and zeros.
+        self.rope = None
+        if cfg.rope_layout == "half" and cfg.rope_dim in (None, cfg.head_dim):
+            if cfg.rope_scaling is None:
+                self.cos, self.sin = ops.rope_tables(self.max_context, cfg.rope_theta, self.dev)
+            else:
+                self.cos, self.sin = ops.Rope(cfg.head_dim, cfg.rope_theta, scaling=cfg.rope_options, device=self.dev).tables(self.max_context)
+        else:
+            self.rope = ops.Rope(cfg.rope_dim or cfg.head_dim, cfg.rope_theta, layout=cfg.rope_layout, scaling=cfg.rope_options, device=self.dev)
+            self.cos, self.sin = (torch.full((self.max_context, ops.HEAD_DIM), v, device=self.dev, dtype=bf) for v in (1.0, 0.0))
+        # how many slots' places name a page; the same on the device, brought up to date where pages are shared or moved
+        self._refs = np.zeros(n_pages, dtype=np.int32)
+        self._refs_dev = self._stack = None
+        self.page_sets = []          # caches beside the stack's under the same page table, of one layer each (a draft head's)
         self._tree_attn = self._status_host = None
         self.attn = self._pages = None
         if kv_format == "bf16":
@@ -326,12 +356,19 @@ class BatchDecoder:
     def attend(self, layer: int, rows: slice, tree: bool = False, longest: int | None = None) -> None:
         """Attention of rows ``rows`` over one layer's cache, into ``ctx``.  ``longest``: see ``ops.TreeAttention``."""
         qkv, seq, pos, out = self.qkv[rows], self.row_seq[rows], self.row_pos[rows], self.ctx[rows]
+        if self.rope is not None:
+            self.rotate(qkv, self.row_rope[rows] if tree else pos, self.cfg.local_heads, self.cfg.local_kv_heads)
         if self.attn is not None and not tree:
             self.attn(qkv, self.cos, self.sin, seq, pos, self.page_table, self.kv[layer, 0], self.kv[layer, 1], out)
         else:
             attention = self._tree_attention()                # (the rows' bases and masks are made with it)
             nodes = ops.TreeRows(self.row_base[rows], self.row_rope[rows], self.row_mask[rows]) if tree else None
             attention(qkv, self.cos, self.sin, seq, pos, self.page_table, self._pages[layer], out, tree=nodes, longest_run=longest)
+
+    def rotate(self, qkv, positions, heads: int, kv_heads: int) -> None:
+        """Turns the queries and keys of rows ``qkv`` where the attention's own tables do not (``rope``)."""
+        if self.rope is not None:
+            ops.rotary(qkv.unflatten(1, (heads + 2 * kv_heads, ops.HEAD_DIM))[:, :heads + kv_heads], positions, self.rope)
 
     def check_status(self) -> None:
         """Raises when an attention over an 8-bit cache, or of draft trees, gave up a wait in the passes so far: their tokens and
@@ -351,7 +388,7 @@ class BatchDecoder:
     def close_slot(self, slot: int) -> None:
         for p in range(self.pages_per_seq):
             if self._table_host[slot, p] >= 0:
-                self._free_pages.append(int(self._table_host[slot, p]))
+                self._drop_page(int(self._table_host[slot, p]))
                 self._table_host[slot, p] = -1
         self.page_table[slot].fill_(self.scratch_page)
         self._free_slots.append(slot)
@@ -362,11 +399,107 @@ class BatchDecoder:
             raise ValueError(f"position {upto_position} exceeds the context of {self.max_context}")
         for p in range(upto_position // PAGE + 1):
             if self._table_host[slot, p] < 0:
-                if not self._free_pages:
-                    raise RuntimeError("KV page pool exhausted")
-                page = self._free_pages.pop()
+                page = self._take_page()
                 self._table_host[slot, p] = page
                 self.page_table[slot, p] = page
+
+    def _take_page(self) -> int:
+        if not self._free_pages:
+            raise RuntimeError("KV page pool exhausted")
+        page = self._free_pages.pop()
+        self._refs[page] = 1
+        return page
+
+    def _drop_page(self, page: int) -> None:
+        """One slot fewer names the page."""
+        self._refs[page] -= 1
+        if self._refs[page] == 0:
+            self._free_pages.append(page)
+
+    def _pool(self):
+        """The stack's pages without the one that padding rows write to, and the counts of their sharers, up to date on the device."""
+        import torch
+
+        if self._stack is None:
+            cut = lambda x: None if x is None else x[:, :self.scratch_page]
+            exps = (None, None) if self.kv_exp is None else (self.kv_exp[:, 0], self.kv_exp[:, 1])
+            self._stack = ops.KVPages(cut(self.kv[:, 0]), cut(self.kv[:, 1]), *map(cut, exps))
+            self._refs_dev = torch.zeros(self.scratch_page, device=self.dev, dtype=torch.int32)
+        self._refs_dev.copy_(torch.from_numpy(self._refs[:self.scratch_page]))
+        return self._stack, self._refs_dev
+
+    def _vectors(self, *lists):
+        import torch
+
+        return torch.tensor([list(x) for x in lists], dtype=torch.int32).to(self.dev).unbind()
+
+    def fork_slot(self, slot: int, length: int, n: int = 1) -> list:
+        """``n`` more slots whose sequences begin with the first ``length`` positions of the one in ``slot``: its whole pages are shared, the
+        positions behind them copied, in every layer, on the current stream."""
+        whole, rest = divmod(int(length), PAGE)
+        held = self._table_host[slot, :whole + (rest > 0)]
+        if n < 1 or not 0 < length <= self.max_context or (held < 0).any():
+            raise ValueError(f"slot {slot} does not hold {length} positions")
+        if len(self._free_slots) < n:
+            raise RuntimeError("no free sequence slot")
+        if rest and len(self._free_pages) < n:
+            raise RuntimeError("KV page pool exhausted")
+        pool, refs = self._pool()
+        children = [self.open_slot() for _ in range(n)]
+        fresh = [self._take_page() if rest else -1 for _ in children]
+        source = int(held[whole]) if rest else -1
+        parents, slots, lengths, pages, sources, counts = self._vectors([slot] * n, children, [length] * n, fresh, [source] * n, [rest] * n)
+        ops.kv_fork(parents, slots, lengths, pages, self.page_table, refs, pool, empty=self.scratch_page)
+        for other in self.page_sets if rest else ():
+            ops.kv_copy(sources, pages, other, positions=counts)
+        for child, page in zip(children, fresh):
+            self._table_host[child, :whole] = held[:whole]
+            self._refs[held[:whole]] += 1
+            if rest:
+                self._table_host[child, whole] = page
+        return children
+
+    def own_pages(self, slot: int, first: int, upto: int) -> None:
+        """Before the slot's positions ``first`` .. ``upto`` are written: pages of theirs that other slots share are copied, as far as ``first``."""
+        moves = []
+        for p in range(first // PAGE, min(upto // PAGE + 1, self.pages_per_seq)):
+            page = int(self._table_host[slot, p])
+            if page >= 0 and self._refs[page] > 1:
+                moves.append((p, page, max(first - p * PAGE, 0)))
+        if not moves:
+            return
+        if len(self._free_pages) < len(moves):
+            raise RuntimeError("KV page pool exhausted")
+        pool, _ = self._pool()
+        fresh = [self._take_page() for _ in moves]
+        src, dst, counts = self._vectors([page for _, page, _ in moves], fresh, [n for _, _, n in moves])
+        for pages in (pool, *self.page_sets):
+            ops.kv_copy(src, dst, pages, positions=counts)
+        for (p, page, _), own in zip(moves, fresh):
+            self._drop_page(page)
+            self._table_host[slot, p] = own
+            self.page_table[slot, p] = own
+
+    def compact_pages(self) -> int:
+        """Moves the pages in use to the front of the pool and returns how many there are (what lies behind them may be given to others)."""
+        import torch
+
+        pool, refs = self._pool()
+        where, used = (torch.empty(n, device=self.dev, dtype=torch.int32) for n in (self.scratch_page, 1))
+        ops.kv_compact(self.page_table, refs, pool, where, used)
+        where = where.cpu().numpy().astype(np.int64)
+        moved = np.flatnonzero((where >= 0) & (where != np.arange(where.size)))
+        if moved.size:
+            src, dst = self._vectors(moved.tolist(), where[moved].tolist())
+            for pages in self.page_sets:
+                ops.kv_copy(src, dst, pages)
+            held = self._table_host >= 0
+            self._table_host[held] = where[self._table_host[held]]
+            counts = self._refs.copy()
+            self._refs[where[moved]] = counts[moved]
+            self._refs[moved] = 0
+            self._free_pages = [p for p in range(self.scratch_page - 1, -1, -1) if self._refs[p] == 0]
+        return int(used.item())
 
     # ---- the step ----------------------------------------------------------------------------------------------
     def _trunk(self, n: int, advance: bool, head: int | None = 0, tree: bool = False) -> None:
@@ -559,6 +692,24 @@ class Batcher:
         self._dirty = True
         return slot
 
+    def room(self, slot: int, first: int, upto: int) -> None:
+        """Pages of the slot's own for positions ``first`` .. ``upto``, before the pass that writes them."""
+        own = getattr(self.d, "own_pages", None)
+        if own is not None:
+            own(slot, first, upto)
+        self.d.ensure_pages(slot, upto)
+
+    def fork(self, slot: int, n: int = 1) -> list:
+        """``n`` more sequences that go on from where the one in ``slot`` is: same tokens, same pending input, one cache for what they have in common
+        (several continuations of a prompt; a beam).  Returns their slots."""
+        self.sync_tokens()
+        s = self.active[slot]
+        children = self.d.fork_slot(slot, s["pos"], n)
+        for c in children:
+            self.active[c] = {"pos": s["pos"], "tokens": list(s["tokens"])}
+        self._dirty = True
+        return children
+
     def _check_prompt(self, slot: int) -> None:
         """Gives the slot back where the prompt's passes are not to be trusted."""
         try:
@@ -630,7 +781,7 @@ class Batcher:
         n = len(wanted)
         b = bucket_for(n, self.buckets)
         for slot in wanted:
-            d.ensure_pages(slot, self.active[slot]["pos"])
+            self.room(slot, self.active[slot]["pos"], self.active[slot]["pos"])
         if self._dirty or wanted != self._order:
             self.sync_tokens()
             self._order = wanted
@@ -675,7 +826,7 @@ class Batcher:
         slots, positions, tokens = [], [], []
         for slot, ds in drafts.items():
             s = self.active[slot]
-            d.ensure_pages(slot, s["pos"] + len(ds))
+            self.room(slot, s["pos"], s["pos"] + len(ds))
             seq = [s["tokens"][-1]] + [int(t) for t in ds]
             slots += [slot] * len(seq)
             positions += list(range(s["pos"], s["pos"] + len(seq)))
@@ -744,7 +895,7 @@ class Batcher:
         if rows > d.max_rows:
             raise ValueError("verify pass larger than the decoder's row buffers")
         for slot, lo, hi in zip(trees, starts, starts[1:]):
-            d.ensure_pages(slot, base[lo] + hi - lo)
+            self.room(slot, base[lo], base[lo] + hi - lo)
         pad = next((b for b in self.buckets if b >= rows), rows) - rows       # (a decoder may take more rows than its largest bucket)
         d.set_tree_rows(slots + [-1] * pad, positions + [0] * pad, tokens + [0] * pad, base + [0] * pad, rope + [0] * pad,
                         masks + [[0] * len(masks[0])] * pad)
@@ -890,7 +1041,7 @@ class FastSession:
             return
         seq, d = self.batcher.active[st.slot], self.d
         feed = [seq["tokens"][-1]] + ids[:-1]
-        d.ensure_pages(st.slot, seq["pos"] + len(ids))
+        self.batcher.room(st.slot, seq["pos"], seq["pos"] + len(ids))
         self.batcher._take_in(st.slot, seq["pos"], feed)
         seq["tokens"] += ids
         seq["pos"] += len(ids)
@@ -906,6 +1057,13 @@ class FastSession:
         del seq["tokens"][-n:]
         seq["pos"] -= n
         self.batcher._dirty = True
+
+    def fork(self, st: State, n: int = 1) -> list:
+        """``n`` more states that go on from where ``st`` is, over one cache for what they have in common."""
+        children = [State(slot, st.plen, self.batcher.active[slot]["tokens"], st.first_logits) for slot in self.batcher.fork(st.slot, n)]
+        for c in children:
+            c._first_out = getattr(st, "_first_out", False)
+        return children
 
     def close(self, st: State) -> None:
         self.batcher.retire(st.slot)
@@ -931,7 +1089,11 @@ class MTPHead:
         bf, R, H = torch.bfloat16, d.max_rows, cfg.hidden
         z = lambda *shape, dtype=bf: torch.zeros(*shape, device=d.dev, dtype=dtype)
         self.kv, exps = kv_buffers((2, d.kv.shape[2], cfg.kv_heads), d.dev, getattr(d, "kv_format", "bf16"))
-        self.pages = None if exps is None else ops.KVPages(self.kv[0], self.kv[1], exps[0], exps[1])
+        paged = getattr(d, "kv_format", "bf16") != "bf16" or hasattr(d, "page_sets")
+        pages = ops.KVPages(self.kv[0], self.kv[1], *((None, None) if exps is None else exps)) if paged else None
+        self.pages = None if getattr(d, "kv_format", "bf16") == "bf16" else pages
+        if hasattr(d, "page_sets"):
+            d.page_sets.append(pages)
         self.tok, self.hid = z(R, dtype=torch.int32), z(R, H)
         self.e, self.cat, self.z, self.x = z(R, H), z(R, 2 * H), z(R, H), z(R, H)
         self.qkv, self.ctx, self.o_out = z(R, cfg.qkv_rows), z(R, cfg.heads * cfg.head_dim), z(R, H)
@@ -973,6 +1135,8 @@ class MTPHead:
         z, x = self.z[:n], self.x[:n]
         ops.rmsnorm(z, L.norm1, x, eps=cfg.eps)
         L.qkv(x, self.qkv[:n])
+        if getattr(d, "rope", None) is not None:
+            d.rotate(self.qkv[:n], d.row_pos[:n], cfg.heads, cfg.kv_heads)
         rows = self.qkv[:n], d.cos, d.sin, d.row_seq[:n], d.row_pos[:n], d.page_table
         if self.pages is None:
             d.attn(*rows, self.kv[0], self.kv[1], self.ctx[:n])
@@ -1070,7 +1234,7 @@ class MTPSpeculator:
         order = sorted(b.active)
         n = len(order)
         for s in order:
-            d.ensure_pages(s, b.active[s]["pos"] + k + 1)
+            b.room(s, b.active[s]["pos"], b.active[s]["pos"] + k + 1)
         # drafts 2..k chained on the head's own state, starting from the rows of the pending first drafts
         drafts = {s: [self.first[s]] for s in order}
         if k > 1:
@@ -1104,6 +1268,13 @@ class MTPSpeculator:
             self.stats["emitted"] += len(out[s])
             self.stats["drafts_accepted"] += len(out[s]) - 1
         return out
+
+    def fork(self, slot: int, n: int = 1) -> list:
+        """``Batcher.fork`` with the head's pending draft and hidden state."""
+        children = self.b.fork(slot, n)
+        for c in children:
+            self.first[c], self.hidden[c] = self.first[slot], self.hidden[slot].clone()
+        return children
 
     def retire(self, slot: int) -> None:
         self.b.retire(slot)
