@@ -10,6 +10,7 @@
 #include "kv_cache.cuh"
 #include "launch_utils.h"
 #include "tree_attention.cuh"
+#include "tree_pair.cuh"
 #include "tree_q4.cuh"
 #include "tree_wide.cuh"
 #include "verify_ops.cuh"
@@ -59,6 +60,19 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   } else {
     part = tree_part_kernel<F8>;
   }
+  void (*wide)(TreeArgs);
+  uint32_t wide_smem, wide_threads, wide_resident;
+  if constexpr (FORMAT == kKvQ4) {
+    wide = tree_pair_kernel;
+    wide_smem = kPairSmem;
+    wide_threads = kPairThreads;
+    wide_resident = 1;
+  } else {
+    wide = tree_wide_kernel<F8>;
+    wide_smem = kWideSmem<F8>;
+    wide_threads = kWideThreads;
+    wide_resident = 2;
+  }
   static std::once_flag once[64];
   static int prepared[64];
   int dev = 0;
@@ -70,7 +84,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
     } else {
       prepared[dev] = cuda_status(cudaFuncSetAttribute(part, cudaFuncAttributeMaxDynamicSharedMemorySize, int(P::kSmem)));
     }
-    if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(tree_wide_kernel<FORMAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kWideSmem<F8>)));
+    if (!prepared[dev]) prepared[dev] = cuda_status(cudaFuncSetAttribute(wide, cudaFuncAttributeMaxDynamicSharedMemorySize, int(wide_smem)));
   });
   if (prepared[dev]) return prepared[dev];
   const int sms = device_sm_count(dev);
@@ -81,7 +95,7 @@ int tree_launch(const TreeArgs& a, cudaStream_t stream) {
   const uint64_t units = uint64_t(a.rows) * a.max_parts * a.nkv;      // at most
   if (int st = launch_step(part, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * resident))), dim3(P::kThreads), P::kSmem, stream, a)) return st;
   if (a.wide_from) {
-    if (int st = launch_step(tree_wide_kernel<FORMAT>, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * 2))), dim3(kWideThreads), kWideSmem<F8>, stream, a)) return st;
+    if (int st = launch_step(wide, dim3(uint32_t(std::min<uint64_t>(units, uint64_t(sms) * wide_resident))), dim3(wide_threads), wide_smem, stream, a)) return st;
   }
   const uint64_t pairs = uint64_t(a.rows) * a.nq;
   return launch_step(tree_combine_kernel, dim3(uint32_t((pairs + kTreeCombineWarps - 1) / kTreeCombineWarps)), dim3(kTreeCombineWarps * 32), 0, stream, a);
@@ -188,7 +202,7 @@ int grb_attn_tree(const grb_attn_tree_step* s, void* cuda_stream) {
   a.max_parts = uint32_t(parts_of(s->table.max_pages, format));
   // (4 bits: a tile of eight columns where the caller says that one row of a sequence comes at a time, whatever comes then; a row's bits are the same)
   a.tile_rows = (format == GRB_KV_Q4 && s->longest_run == 1 && a.group <= 8 ? 8 : 16) / a.group;
-  a.wide_rows = kWideTile / a.group;
+  a.wide_rows = (format == GRB_KV_Q4 ? 2 : 1) * (kWideTile / a.group);       // (4 bits: tiles in pairs)
   // Runs for the wide kernel: trees of more rows than two tiles of the narrow one take; of causal rows prompt chunks, so that the
   // rows of a speculative chain keep the bits of single steps.  A run's rows alone decide, whatever else is in the call, so one run
   // pays for what many gain.  Eight nodes of five heads a kv head, 8 bits, us narrow / wide: one tree behind 1000 positions 18 / 21,

@@ -56,14 +56,14 @@ struct TreeArgs {
   int32_t* extent;            // scratch: [rows]: positions up to the last one the row sees
   uint32_t* row_parts;        // scratch: [rows]: parts of the row
   int4* tiles;                // scratch: [rows]: first row, rows, units (4 bits: weight of the units) before it, positions up to the last one its rows see
-  int4* wide_tiles;           // scratch: [rows]: first row, rows, first unit, positions of a unit
+  int4* wide_tiles;           // scratch: [rows]: first row, rows (4 bits: of a pair of tiles), first unit, positions of a unit
   uint32_t* plan;             // scratch: tiles, units, wide tiles, wide units, wide units taken
   float* part_acc;            // scratch: [rows][nq][max_parts][128]
   float2* part_ml;            // scratch: [rows][nq][max_parts]: maximum and sum of a part
   __nv_bfloat16* out;         // [rows][ldo]: nq * 128
   int64_t ldo;
   uint32_t rows, nq, nkv, group, tile_rows, max_parts;
-  uint32_t wide_rows, wide_from;   // rows of a wide tile; a run of so many rows (0: none) is cut into wide tiles
+  uint32_t wide_rows, wide_from;   // rows of a wide tile (4 bits: of a pair of them); a run of so many rows (0: none) is cut into wide tiles
   float scaling;
 };
 

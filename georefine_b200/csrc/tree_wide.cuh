@@ -26,7 +26,6 @@
 #include <type_traits>
 
 #include "tree_attention.cuh"
-#include "tree_q4.cuh"
 
 namespace grb {
 
@@ -86,10 +85,9 @@ template <bool F8>
 constexpr uint32_t kWideSmem = F8 ? kWideSharedBytes + 3 * kWideOperand + 4 * uint32_t(sizeof(WideScales)) : 1024 + 2 * kWideOperand + 3 * kWideStage;
 __device__ __forceinline__ void wide_loaders_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-template <int FORMAT>
+template <bool F8>
 __global__ void __launch_bounds__(kWideThreads, 2)
 tree_wide_kernel(const TreeArgs a) {
-  constexpr bool F8 = FORMAT != kKvBf16, Q4 = FORMAT == kKvQ4;        // F8: decoded to FP16, with exponents on scores and weights
   extern __shared__ __align__(1024) unsigned char wide_smem[];
   WideShared<F8>& sm = *reinterpret_cast<WideShared<F8>*>(wide_smem);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -233,64 +231,33 @@ tree_wide_kernel(const TreeArgs a) {
         if (lane == 0) mbar_arrive(bar_u);
       };
       if constexpr (F8) {
+        // A thread's pieces: the same quarter of both halves of every 32nd row.  Eight lanes take four pieces of two neighbouring rows,
+        // which the swizzle spreads over all banks when their sixteen values each are stored.
         const uint32_t row0 = lt >> 2;
-        constexpr int kPieces = Q4 ? 2 : 4;                  // of 16 bytes that a thread brings of K, and of V, each step
-        uint4 k[kPieces], v[kPieces];
-        uint32_t k_scale = 0, v_scale = 0;                   // 4 bits: of the thread's two pieces, which are groups of 32 dimensions, in bits 0-7 and 16-23
-        // 8 bits: the same quarter of both halves of every 32nd row.  Eight lanes take four pieces of two neighbouring rows, which the swizzle
-        // spreads over all banks when their sixteen values each are stored.  4 bits: the same group of every 32nd row; the lanes of the upper
-        // two groups take their words in another order, so that no two of eight lanes store to the same banks.
-        const uint32_t swapped = Q4 ? lt & 2u : 0u;
-        auto ask = [&](uint4 (&x)[kPieces], uint32_t& scale, const void* pool, uint32_t j) {
+        uint4 k[4], v[4];
+        auto ask = [&](uint4 (&x)[4], const void* pool, uint32_t j) {
           const int64_t entry = j < steps ? entry_of(j) : -1;
           const int32_t npos = entry < 0 ? 0 : t.extent - t.start - int32_t(j * kWideStep);
-          if constexpr (Q4) {
-            const uint8_t* const page = static_cast<const uint8_t*>(pool) + (entry < 0 ? 0 : q4_page_at(size_t(entry)));
-            const uint32_t at = uint32_t(entry) % kKvPage + row0;
-            scale = 0;
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim) + row0 * 8 + (lt & 3u);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const bool in = int32_t(row0 + 32 * i) < npos;
-              const uint4 p = in ? reinterpret_cast<const uint4*>(page)[(at + 32 * i) * (kQ4Codes / 16) + (lt & 3u)] : make_uint4(0u, 0u, 0u, 0u);
-              x[i] = swapped ? make_uint4(p.z, p.w, p.x, p.y) : p;
-              if (in) scale |= uint32_t(page[kQ4ScalesAt + (at + 32 * i) * 4 + (lt & 3u)]) << (16 * i);
-            }
-          } else {
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pool) + entry * kKvDim) + row0 * 8 + (lt & 3u);
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) x[i] = int32_t(row0 + 32 * (i >> 1)) < npos ? src[256 * (i >> 1) + 4 * (i & 1)] : make_uint4(0u, 0u, 0u, 0u);
-          }
+          for (int i = 0; i < 4; ++i) x[i] = int32_t(row0 + 32 * (i >> 1)) < npos ? src[256 * (i >> 1) + 4 * (i & 1)] : make_uint4(0u, 0u, 0u, 0u);
         };
         const uint32_t to_lo = wide_offset<kWideStep>(row0, 2 * (lt & 3u)), to_hi = wide_offset<kWideStep>(row0, 2 * (lt & 3u) + 1);     // (32 rows on: 4096 bytes)
-        uint32_t to_word[4];                                 // 4 bits: where the piece's words, eight dimensions each, go
+        auto store = [&](const uint4 (&x)[4], uint32_t dst, bool clean) {
 #pragma unroll
-        for (uint32_t q = 0; q < 4; ++q) to_word[q] = wide_offset<kWideStep>(row0, 4 * (lt & 3u) + (q ^ swapped));
-        auto store = [&](const uint4 (&x)[kPieces], uint32_t scale, uint32_t dst, bool clean) {
+          for (int i = 0; i < 4; ++i) {
+            uint32_t h[8];
+            e4m3_to_half4(x[i].x, h[0], h[1]);
+            e4m3_to_half4(x[i].y, h[2], h[3]);
+            e4m3_to_half4(x[i].z, h[4], h[5]);
+            e4m3_to_half4(x[i].w, h[6], h[7]);
+            if (clean) {
 #pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            if constexpr (Q4) {
-              const Q4Factors f = q4_factors((scale >> (16 * i) & 0xFFu) * 0x10001u);
-              const uint32_t words[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t y[4];
-                q4_operands(words[q], f, y);
-                sts128(dst + 4096 * i + to_word[q], make_uint4(y[0], y[1], y[2], y[3]));
-              }
-            } else {
-              uint32_t h[8];
-              e4m3_to_half4(x[i].x, h[0], h[1]);
-              e4m3_to_half4(x[i].y, h[2], h[3]);
-              e4m3_to_half4(x[i].z, h[4], h[5]);
-              e4m3_to_half4(x[i].w, h[6], h[7]);
-              if (clean) {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) h[q] = half2_number(h[q]);
-              }
-              const uint32_t at = dst + 4096 * (i >> 1) + (kWideStage / 2) * (i & 1);
-              sts128(at + to_lo, make_uint4(h[0], h[1], h[2], h[3]));
-              sts128(at + to_hi, make_uint4(h[4], h[5], h[6], h[7]));
+              for (int q = 0; q < 8; ++q) h[q] = half2_number(h[q]);
             }
+            const uint32_t at = dst + 4096 * (i >> 1) + (kWideStage / 2) * (i & 1);
+            sts128(at + to_lo, make_uint4(h[0], h[1], h[2], h[3]));
+            sts128(at + to_hi, make_uint4(h[4], h[5], h[6], h[7]));
           }
         };
         // exponents: half of the threads a position's of K, the others one's of V.  A byte below what an entry has (0, where nobody wrote)
@@ -300,8 +267,7 @@ tree_wide_kernel(const TreeArgs a) {
         uint32_t byte;
         auto ask_exp = [&](uint32_t j) {
           const int64_t entry = j < steps ? entry_of(j) : -1;
-          if constexpr (Q4) byte = entry < 0 ? 127u : (static_cast<const uint8_t*>(lt < kWideStep ? a.pages.k : a.pages.v) + q4_page_at(size_t(entry)))[kQ4ExpsAt + uint32_t(entry) % kKvPage + at];
-          else byte = entry < 0 ? 127u : exps[entry + at];
+          byte = entry < 0 ? 127u : exps[entry + at];
         };
         auto store_exp = [&](WideScales& s) {
           if (lt < kWideStep) {
@@ -313,15 +279,15 @@ tree_wide_kernel(const TreeArgs a) {
           }
         };
         ask_exp(0);
-        ask(k, k_scale, a.pages.k, 0);
-        ask(v, v_scale, a.pages.v, 0);
+        ask(k, a.pages.k, 0);
+        ask(v, a.pages.v, 0);
         wide_loaders_meet();                                 // (the unit after this one and its pages are known to all)
         queries();
         publish();
         for (uint32_t j = 0; j < steps; ++j) {
           const uint32_t g = step0 + j;
           if (g > 1) wait2(bar_s, g - 2);                    // scores have been taken from the stage's K
-          store(k, k_scale, k_stage(g), false);
+          store(k, k_stage(g), false);
           store_exp(scales[g & 3u]);                         // (the step four before has been weighed: the one after it was waited for)
           fence_proxy_async_smem();
           __syncwarp();
@@ -330,13 +296,13 @@ tree_wide_kernel(const TreeArgs a) {
             mbar_arrive(bar_k + 8 * (g & 1u));
           }
           ask_exp(j + 1);
-          ask(k, k_scale, a.pages.k, j + 1);
+          ask(k, a.pages.k, j + 1);
           if (g > 1) wait2(bar_o, g - 2);                    // the stage's values have been used
-          store(v, v_scale, v_stage(g), j >= plain);
+          store(v, v_stage(g), j >= plain);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_v + 8 * (g & 1u));
-          ask(v, v_scale, a.pages.v, j + 1);
+          ask(v, a.pages.v, j + 1);
         }
       } else {
         auto ask = [&](uint32_t dst, const void* pool, uint32_t j) {
