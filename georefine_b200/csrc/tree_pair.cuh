@@ -1,33 +1,41 @@
 // The wide attention of tree_wide.cuh over a 4-bit cache: two tiles of 128 rows (row of the step, query head of the group) share each step's K and V.
 //
-// A CTA takes all of an SM.  Two warpgroups turn scores into weights, one for each tile, a thread per row; one brings K and V, which it decodes to FP16 in shared
-// memory once for both tiles; two warps issue the products, one for each tile:
+// A CTA takes all of an SM.  Two warpgroups turn scores into weights, one for each tile, a thread per row; one brings K and one V, which they decode to FP16 in
+// shared memory once for both tiles, their codes asked for two steps ahead; two warps issue the products, one for each tile; one looks up where the next unit lies:
 //   S = Q K^T (S in tensor memory, two steps of each tile);  weights P = exp2(S' - reference), written over S;  O += P V (P and O in tensor memory).
 // A step is 64 positions; K and V of three steps are held.  Arithmetic is that of tree_wide.cuh: K's exponent multiplies the score of its position, V's goes
 // into the weight, the sum of the weights takes it out again; the reference of a row moves when its maximum has passed it by 2^8.
 //
-// A unit is a pair of tiles and a part of the positions.  Where a run's last tile has no partner, its products' warp and its weights' warps stand still, and
-// keep the count of the steps.  Barriers of a step are numbered by the step modulo three: nobody can be a whole round ahead of one who still
-// waits, as the loaders wait for the products of the step whose place they take.
+// A unit is a pair of tiles and a part of the positions.  Where a run's last tile has no partner, the products' and the weights' warps of the other half go through
+// all waits and arrivals without anything between them.  Barriers of a step are numbered by the step modulo three.  A wait tells a phase from the one before it and
+// no more, so nobody may be a round ahead of one who still waits, and nobody waits for a phase whose predecessor is open: everybody waits for every step in turn,
+// and the loaders for the products of the step whose place they take.  (Schedules of all roles in any order, run on the CPU, end and mistake no phase.)
 #pragma once
 #include "tree_q4.cuh"
 #include "tree_wide.cuh"
 
 namespace grb {
 
-constexpr int kPairThreads = 512;                // weights of tile 0, of tile 1: warps 0-3, 4-7; loading: 8-11; products: 12, 13
+constexpr int kPairThreads = 640;                // weights of tile 0, of tile 1: warps 0-3, 4-7; K and the queries: 8-11; V: 12-15; products: 16, 17; units: 18
 constexpr uint32_t kPairRing = 3;
+constexpr uint32_t kPairScales = 8;              // steps whose exponents are held: the one five before a step whose K may be stored has been weighed
 constexpr uint32_t kPairColumns = 512;           // tensor memory: S of two steps (and P over it) of tile 0, of tile 1, O of either
 
+// What everybody is told of a unit.
+struct PairInfo {
+  uint32_t valid, first, rows, kvh, part, steps;
+  uint32_t plain;                  // steps, from the first on, whose positions every row sees
+  int32_t start, extent;           // positions start .. extent - 1: what some row sees, up to the last such
+};
 struct PairShared {
-  uint64_t bars[2 * kPairRing + 3 * 2 * kPairRing + 2 + 4];      // K stored, V stored; S done, O done, P stored, of either tile; unit set up, unit seen; scales of every fourth step
-  WideInfo info[2];                              // of a unit and the next
+  uint64_t bars[2 * kPairRing + 3 * 2 * kPairRing + 3 + 8];      // K stored, V stored; S done, O done, P stored, of either tile; unit set up, unit seen, queries stored; scales
+  PairInfo info[2];                              // of a unit and the next
   int64_t where[2][kWideMostPart / kWideStep];   // first entry of each step; -1: none
-  uint32_t tmem_at, aborted, next_unit, any_absent;
+  uint32_t tmem_at, aborted;
 };
 constexpr uint32_t kPairSharedBytes = 2048;
 static_assert(sizeof(PairShared) <= kPairSharedBytes, "the operands follow");
-constexpr uint32_t kPairSmem = kPairSharedBytes + 2 * kWideOperand + 2 * kPairRing * kWideStage + 4 * uint32_t(sizeof(WideScales));
+constexpr uint32_t kPairSmem = kPairSharedBytes + 2 * kWideOperand + 2 * kPairRing * kWideStage + kPairScales * uint32_t(sizeof(WideScales));
 
 __global__ void __launch_bounds__(kPairThreads, 1)
 tree_pair_kernel(const TreeArgs a) {
@@ -38,7 +46,7 @@ tree_pair_kernel(const TreeArgs a) {
   WideScales* const scales = reinterpret_cast<WideScales*>(wide_smem + kPairSharedBytes + 2 * kWideOperand + 2 * kPairRing * kWideStage);
   constexpr uint32_t kRound = 8 * kPairRing;
   const uint32_t bar_k = smem_u32(&sm.bars[0]), bar_v = bar_k + kRound, bar_s = bar_v + kRound, bar_o = bar_s + 2 * kRound, bar_p = bar_o + 2 * kRound, bar_u = bar_p + 2 * kRound,
-                 bar_w = bar_u + 8, bar_t = bar_w + 8;
+                 bar_w = bar_u + 8, bar_q = bar_w + 8, bar_t = bar_q + 8;
   // (tensor memory is taken before the kernels behind this one may start: see tree_wide_kernel)
   if (tid == 0) {
     for (uint32_t b = 0; b < kRound; b += 8) {
@@ -50,13 +58,14 @@ tree_pair_kernel(const TreeArgs a) {
       mbar_init(bar_o + b, 1);
       mbar_init(bar_p + b, 4);
     }
-    mbar_init(bar_u, 4);
-    mbar_init(bar_w, 10);
-    for (uint32_t b = 0; b < 32; b += 8) mbar_init(bar_t + b, 4);
+    mbar_init(bar_u, 1);
+    mbar_init(bar_w, 18);
+    mbar_init(bar_q, 4);
+    for (uint32_t b = 0; b < 8 * kPairScales; b += 8) mbar_init(bar_t + b, 8);
     mbar_fence_init();
     sm.aborted = 0u;
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(smem_u32(&sm.tmem_at), kPairColumns);
     tmem_relinquish();
   }
@@ -66,7 +75,7 @@ tree_pair_kernel(const TreeArgs a) {
   step_kernel_entry();
   const uint32_t tiles = a.plan[2], units = a.plan[3], tile_rows = a.wide_rows / 2;
   if (blockIdx.x >= units) {
-    if (warp == 12) tmem_dealloc(sm.tmem_at, kPairColumns);
+    if (warp == 16) tmem_dealloc(sm.tmem_at, kPairColumns);
     return;
   }
   // A wait that runs out is everybody's: nobody waits again, every loop runs to its end, and the status says so.
@@ -79,74 +88,53 @@ tree_pair_kernel(const TreeArgs a) {
   };
   auto wait3 = [&](uint32_t bars, uint32_t step) { wait(bars + 8 * (step % kPairRing), step / kPairRing); };
   uint32_t step0 = 0;                                        // steps this CTA has taken before the unit
-  // registers, of the 128 that each thread of the launch has: 168 for the weights, 112 for loading, 40 for the products
-  if (warp >= 8 && warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    // ---- loading ------------------------------------------------------------------------------------------------
-    const uint32_t lt = tid - 256;
-    uint32_t tile = 0, n = 0;
-    for (uint32_t u = blockIdx.x; u < units; ++n) {
-      const uint32_t slot = n & 1u;
-      if (n) wait(bar_w, n - 1);                             // everybody has seen the unit before, and is through with the one whose tables are overwritten
-      for (;;) {
-        const uint32_t past = __ballot_sync(0xFFFFFFFFu, tile + 1 + lane < tiles && uint32_t(a.wide_tiles[tile + 1 + lane].z) <= u);
-        tile += __popc(past);
-        if (past != 0xFFFFFFFFu) break;
-      }
-      const int4 d = a.wide_tiles[tile];
-      const uint32_t local = u - uint32_t(d.z), part_positions = uint32_t(d.w), first = uint32_t(d.x), rows = uint32_t(d.y), kvh = local % a.nkv, part = local / a.nkv;
-      const int32_t seq = a.row_seq[first], start = int32_t(part * part_positions);
-      if (lt == 0) sm.next_unit = gridDim.x + atomicAdd(a.plan + 4, 1u);
-      if (warp == 8) {                                       // (a step's positions lie in one page)
-        int64_t place = 0;
-        if (lane < part_positions / kWideStep) {
-          place = kv_place(a.table, seq, start + int32_t(lane * kWideStep));
-          sm.where[slot][lane] = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, kvh));
-        }
-        const bool absent = __any_sync(0xFFFFFFFFu, place < 0);
-        if (lane == 0) sm.any_absent = absent;
-      }
-      int32_t extent = 0, all = 0x7FFFFFFF;
-      for (uint32_t i = lane; i < rows; i += 32) {
-        const int32_t e = a.extent[first + i];
-        extent = max(extent, e);
-        all = min(all, a.row_base ? min(max(a.row_base[first + i], 0), e) : e);
-      }
+  // registers, of the 96 that each thread of the launch has: 144 for the weights, 72 for loading, 40 for the others
+  if (warp >= 8 && warp < 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    // ---- loading: K and the queries, or V -------------------------------------------------------------------------
+    const bool of_k = warp < 12;
+    const uint32_t lt = tid & 127u, ring = of_k ? ks : vs, stored = of_k ? bar_k : bar_v, left = of_k ? bar_s : bar_o;      // left: a stage's last use
+    const uint8_t* const pool = static_cast<const uint8_t*>(of_k ? a.pages.k : a.pages.v);
+    // A thread's pieces of a step: the same group of 32 dimensions of every 32nd row; the lanes of the upper two groups take their words in another order, so
+    // that no two of eight lanes store to the same banks.  The first 64 threads also bring a position's exponent.
+    const uint32_t row0 = lt >> 2, swapped = lt & 2u;
+    uint32_t to_word[4];                                     // where a piece's words, eight dimensions each, go
 #pragma unroll
-      for (int off = 16; off; off >>= 1) {
-        extent = max(extent, __shfl_xor_sync(0xFFFFFFFFu, extent, off));
-        all = min(all, __shfl_xor_sync(0xFFFFFFFFu, all, off));
-      }
-      extent = min(extent, start + int32_t(part_positions));
-      const uint32_t steps = (uint32_t(extent - start) + kWideStep - 1) / kWideStep;       // (a unit has a position at least)
-      wide_loaders_meet();
-      u = sm.next_unit;
-      // (whole steps alone: the last one may reach past what the rows see, even where they all see as far)
-      const uint32_t plain = sm.any_absent ? 0u : uint32_t(max(min(all, extent) - start, 0)) / kWideStep;
-      // A thread's pieces of a step: the same group of 32 dimensions of every 32nd row; the lanes of the upper two groups take their words in another order, so
-      // that no two of eight lanes store to the same banks.  The first half of the threads also bring a position's exponent of K, the others one's of V.
-      const uint32_t row0 = lt >> 2, swapped = lt & 2u, at = lt & (kWideStep - 1);
-      struct Pieces {
-        uint4 x[2];
-        uint32_t scale;                                      // of the two, in bits 0-7 and 16-23
-      };
-      auto ask = [&](Pieces& p, const void* pool, uint32_t j) {
+    for (uint32_t q = 0; q < 4; ++q) to_word[q] = wide_offset<kWideStep>(row0, 4 * (lt & 3u) + (q ^ swapped));
+    struct Pieces {
+      uint4 x[2];
+      uint32_t scale;                                        // of the two, in bits 0-7 and 16-23
+      uint32_t exp;
+    };
+    for (uint32_t n = 0;; ++n) {
+      const uint32_t slot = n & 1u;
+      wait(bar_u, n);
+      const PairInfo unit = sm.info[slot];
+      if (!unit.valid || *reinterpret_cast<volatile uint32_t*>(&sm.aborted)) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_w);
+      const uint32_t steps = unit.steps;
+      auto ask = [&](Pieces& p, uint32_t j) {
         const int64_t entry = j < steps ? sm.where[slot][j] : -1;
-        const int32_t npos = entry < 0 ? 0 : extent - start - int32_t(j * kWideStep);
-        const uint8_t* const page = static_cast<const uint8_t*>(pool) + (entry < 0 ? 0 : q4_page_at(size_t(entry)));
-        const uint32_t place = uint32_t(entry) % kKvPage + row0;
+        const int32_t npos = entry < 0 ? 0 : unit.extent - unit.start - int32_t(j * kWideStep);
+        const uint8_t* const page = pool + (entry < 0 ? 0 : q4_page_at(size_t(entry)));
+        const uint32_t place = uint32_t(entry) % kKvPage;
         p.scale = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          const uint32_t at = place + row0 + 32 * i;
           const bool in = int32_t(row0 + 32 * i) < npos;
-          p.x[i] = in ? reinterpret_cast<const uint4*>(page)[(place + 32 * i) * (kQ4Codes / 16) + (lt & 3u)] : make_uint4(0u, 0u, 0u, 0u);
-          if (in) p.scale |= uint32_t(page[kQ4ScalesAt + (place + 32 * i) * 4 + (lt & 3u)]) << (16 * i);
+          p.x[i] = in ? reinterpret_cast<const uint4*>(page)[at * (kQ4Codes / 16) + (lt & 3u)] : make_uint4(0u, 0u, 0u, 0u);
+          if (in) p.scale |= uint32_t(page[kQ4ScalesAt + at * 4 + (lt & 3u)]) << (16 * i);
         }
+        p.exp = lt < kWideStep && entry >= 0 ? page[kQ4ExpsAt + place + lt] : 127u;
       };
-      uint32_t to_word[4];                                   // where a piece's words, eight dimensions each, go
-#pragma unroll
-      for (uint32_t q = 0; q < 4; ++q) to_word[q] = wide_offset<kWideStep>(row0, 4 * (lt & 3u) + (q ^ swapped));
-      auto store = [&](const Pieces& p, uint32_t dst) {
+      auto store = [&](const Pieces& p, uint32_t g) {
+        const uint32_t stage = g % kPairRing, dst = ring + stage * kWideStage;
+        if (g >= kPairRing) {
+          wait3(left, g - kPairRing);
+          wait3(left + kRound, g - kPairRing);
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const Q4Factors f = q4_factors((p.scale >> (16 * i) & 0xFFu) * 0x10001u);
@@ -158,89 +146,112 @@ tree_pair_kernel(const TreeArgs a) {
             sts128(dst + 4096 * i + to_word[q], make_uint4(y[0], y[1], y[2], y[3]));
           }
         }
-      };
-      auto ask_exp = [&](uint32_t j) -> uint32_t {
-        const int64_t entry = j < steps ? sm.where[slot][j] : -1;
-        return entry < 0 ? 127u : (static_cast<const uint8_t*>(lt < kWideStep ? a.pages.k : a.pages.v) + q4_page_at(size_t(entry)))[kQ4ExpsAt + uint32_t(entry) % kKvPage + at];
-      };
-      auto store_exp = [&](WideScales& s, uint32_t byte) {   // (a byte below what an entry has - 0, where nobody wrote - stands for zeros of the smallest size)
-        if (lt < kWideStep) {
-          s.k[at] = kv_scale(byte);
-        } else {
-          const uint32_t b = max(byte, kKvLeastByte);
-          s.v[at] = b == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(b) - 127);
-          s.v_inverse[at] = uint16_t(__float_as_uint(kv_inverse(b)) >> 16);
+        if (lt < kWideStep) {                                // (a byte below what an entry has - 0, where nobody wrote - stands for zeros of the smallest size)
+          WideScales& s = scales[g % kPairScales];
+          if (of_k) {
+            s.k[lt] = kv_scale(p.exp);
+          } else {
+            const uint32_t b = max(p.exp, kKvLeastByte);
+            s.v[lt] = b == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(b) - 127);
+            s.v_inverse[lt] = uint16_t(__float_as_uint(kv_inverse(b)) >> 16);
+          }
         }
-      };
-      Pieces k, v;
-      uint32_t byte = ask_exp(0);
-      ask(k, a.pages.k, 0);
-      ask(v, a.pages.v, 0);
-      wide_loaders_meet();                                   // (the unit after this one and its pages are known to all)
-      // the queries of both tiles, sixteen lanes a row, once the scores of the unit before are done
-      if (step0) {
-        wait3(bar_s, step0 - 1);
-        wait3(bar_s + kRound, step0 - 1);
-      }
-      const uint32_t used = rows * a.group, first_tile = tile_rows * a.group;
-      for (uint32_t i0 = 0; i0 < (rows > tile_rows ? 32u : 16u); i0 += 4) {
-        uint4 x[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const uint32_t m = (lt >> 4) + 8 * ((i0 + i) & 15u), col = i0 < 16 ? m : first_tile + m, r = col / a.group;
-          const bool in = col < used && m < first_tile;
-          x[i] = in ? reinterpret_cast<const uint4*>(a.q + (size_t(first + r) * a.nq + kvh * a.group + (col - r * a.group)) * kKvDim)[lt & 15u] : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) sts128(qs + (i0 < 16 ? 0u : kWideOperand) + wide_offset<kWideTile>((lt >> 4) + 8 * ((i0 + i) & 15u), lt & 15u), x[i]);
-      }
-      if (lt == 0) sm.info[slot] = WideInfo{1u, first, rows, kvh, part, steps, plain, start};
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_u);
-      for (uint32_t j = 0; j < steps; ++j) {
-        const uint32_t g = step0 + j, stage = g % kPairRing;
-        if (g >= kPairRing) {                                // both tiles' scores have been taken from the stage's K
-          wait3(bar_s, g - kPairRing);
-          wait3(bar_s + kRound, g - kPairRing);
-        }
-        store(k, ks + stage * kWideStage);
-        store_exp(scales[g & 3u], byte);                     // (the step four before has been weighed: its values' use was waited for a step ago)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(bar_t + 8 * (g & 3u));
-          mbar_arrive(bar_k + 8 * stage);
+          mbar_arrive(bar_t + 8 * (g % kPairScales));
+          mbar_arrive(stored + 8 * stage);
         }
-        byte = ask_exp(j + 1);
-        ask(k, a.pages.k, j + 1);
-        if (g >= kPairRing) {
-          wait3(bar_o, g - kPairRing);
-          wait3(bar_o + kRound, g - kPairRing);
+      };
+      Pieces p0, p1;
+      ask(p0, 0);
+      ask(p1, 1);
+      if (of_k) {                                            // the queries of both tiles, once the scores of the unit before are done
+        if (step0) {
+          wait3(bar_s, step0 - 1);
+          wait3(bar_s + kRound, step0 - 1);
         }
-        store(v, vs + stage * kWideStage);
+        const uint32_t used = unit.rows * a.group, first_tile = tile_rows * a.group;
+        for (uint32_t i = 0; i < (unit.rows > tile_rows ? 32u : 16u); ++i) {
+          const uint32_t m = (lt >> 4) + 8 * (i & 15u), col = i < 16 ? m : first_tile + m, r = col / a.group;
+          const bool in = col < used && m < first_tile;
+          const uint16_t* const src = in ? a.q + (size_t(unit.first + r) * a.nq + unit.kvh * a.group + (col - r * a.group)) * kKvDim + 8 * (lt & 15u) : a.q;
+          cp_async_16(qs + (i < 16 ? 0u : kWideOperand) + wide_offset<kWideTile>(m, lt & 15u), src, in ? 16u : 0u);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_v + 8 * stage);
-        ask(v, a.pages.v, j + 1);
+        if (lane == 0) mbar_arrive(bar_q);
+      }
+      for (uint32_t j = 0; j < steps; j += 2) {
+        store(p0, step0 + j);
+        ask(p0, j + 2);
+        if (j + 1 < steps) {
+          store(p1, step0 + j + 1);
+          ask(p1, j + 3);
+        }
       }
       step0 += steps;
     }
-    // no unit is left
-    if (n) wait(bar_w, n - 1);
-    if (lt == 0) sm.info[n & 1u].valid = 0u;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar_u);
-  } else if (warp >= 12) {
+  } else if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    // ---- products: warp 12 of tile 0, warp 13 of tile 1 -----------------------------------------------------------
-    const uint32_t x = warp - 12;
+    if (warp == 18) {
+      // ---- units: where the next one lies, while this one is at hand ------------------------------------------------
+      uint32_t tile = 0, n = 0;
+      for (uint32_t u = blockIdx.x; u < units; ++n) {
+        const uint32_t slot = n & 1u;
+        for (;;) {
+          const uint32_t past = __ballot_sync(0xFFFFFFFFu, tile + 1 + lane < tiles && uint32_t(a.wide_tiles[tile + 1 + lane].z) <= u);
+          tile += __popc(past);
+          if (past != 0xFFFFFFFFu) break;
+        }
+        const int4 d = a.wide_tiles[tile];
+        const uint32_t local = u - uint32_t(d.z), part_positions = uint32_t(d.w), first = uint32_t(d.x), rows = uint32_t(d.y), kvh = local % a.nkv, part = local / a.nkv;
+        const int32_t seq = a.row_seq[first], start = int32_t(part * part_positions);
+        int64_t place = 0, entry = 0;                        // (a step's positions lie in one page)
+        if (lane < part_positions / kWideStep) {
+          place = kv_place(a.table, seq, start + int32_t(lane * kWideStep));
+          entry = place < 0 ? -1 : int64_t(kv_entry(place, a.nkv, kvh));
+        }
+        const bool absent = __any_sync(0xFFFFFFFFu, place < 0);
+        int32_t extent = 0, all = 0x7FFFFFFF;
+        for (uint32_t i = lane; i < rows; i += 32) {
+          const int32_t e = a.extent[first + i];
+          extent = max(extent, e);
+          all = min(all, a.row_base ? min(max(a.row_base[first + i], 0), e) : e);
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) {
+          extent = max(extent, __shfl_xor_sync(0xFFFFFFFFu, extent, off));
+          all = min(all, __shfl_xor_sync(0xFFFFFFFFu, all, off));
+        }
+        extent = min(extent, start + int32_t(part_positions));
+        const uint32_t steps = (uint32_t(extent - start) + kWideStep - 1) / kWideStep;       // (a unit has a position at least)
+        // (whole steps alone: the last one may reach past what the rows see, even where they all see as far)
+        const uint32_t plain = absent ? 0u : uint32_t(max(min(all, extent) - start, 0)) / kWideStep;
+        if (n) wait(bar_w, n - 1);                           // everybody has seen the unit before, and is through with the one whose tables are overwritten
+        if (lane < part_positions / kWideStep) sm.where[slot][lane] = entry;
+        if (lane == 0) sm.info[slot] = PairInfo{1u, first, rows, kvh, part, steps, plain, start, extent};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_u);
+        if (lane == 0) u = gridDim.x + atomicAdd(a.plan + 4, 1u);
+        u = __shfl_sync(0xFFFFFFFFu, u, 0);
+      }
+      if (n) wait(bar_w, n - 1);                             // no unit is left
+      if (lane == 0) {
+        sm.info[n & 1u].valid = 0u;
+        mbar_arrive(bar_u);
+      }
+      __syncwarp();
+    }
+    // ---- products: warp 16 of tile 0, warp 17 of tile 1 -----------------------------------------------------------
+    const uint32_t x = warp - 16;
     constexpr uint32_t kFp16 = ~((1u << 7) | (1u << 10)), kIdesc = umma_idesc_bf16(128) & kFp16, kIdescS = umma_idesc_bf16(kWideStep) & kFp16;
     const uint32_t q = qs + x * kWideOperand, s_tmem = sm.tmem_at + x * 128, o_tmem = sm.tmem_at + 256 + x * 128, s_bars = bar_s + x * kRound, o_bars = bar_o + x * kRound, p_bars = bar_p + x * kRound;
     bool on = true;
-    uint32_t weighed = 0;                                    // steps whose weights this warp has waited for: those in which its tile does not stand still
     auto scores = [&](uint32_t g) {
-      if (on && g > 1) wait3(o_bars, g - 2);                 // the weights there have been used (issue order alone does not say so: the two products differ in shape)
+      if (g > 1) wait3(o_bars, g - 2);                // the weights there have been used (issue order alone does not say so: the two products differ in shape)
       wait3(bar_k, g);
       tc_fence_after();
       if (elect_one()) {
@@ -257,18 +268,19 @@ tree_pair_kernel(const TreeArgs a) {
     };
     for (uint32_t n = 0; x < 2; ++n) {
       wait(bar_u, n);
-      const WideInfo& unit = sm.info[n & 1u];
+      const PairInfo& unit = sm.info[n & 1u];
       if (!unit.valid || *reinterpret_cast<volatile uint32_t*>(&sm.aborted)) break;
       const uint32_t steps = unit.steps;
       on = x == 0 || unit.rows > tile_rows;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_w);
+      wait(bar_q, n);
       scores(step0);
       for (uint32_t j = 0; j < steps; ++j) {
         const uint32_t g = step0 + j;
         if (j + 1 < steps) scores(g + 1);
         wait3(bar_v, g);
-        if (on) wait3(p_bars, weighed++);
+        wait3(p_bars, g);
         tc_fence_after();
         if (elect_one()) {
           if (on) {
@@ -283,21 +295,26 @@ tree_pair_kernel(const TreeArgs a) {
       step0 += steps;
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // ---- weights: thread = row m of the tile, lane m of tensor memory ------------------------------------------------
     constexpr float kSlack = 8.f, kBias = 7.f;               // FP16: weights up to 2^(7 + 8)
     const uint32_t x = warp >> 2, m = tid & 127u, lanes = ((warp & 3u) * 32u) << 16;
     const uint32_t s_tmem = sm.tmem_at + lanes + x * 128, o_tmem = sm.tmem_at + lanes + 256 + x * 128, s_bars = bar_s + x * kRound, o_bars = bar_o + x * kRound, p_bars = bar_p + x * kRound;
-    uint32_t weighed = 0;                                    // steps in which this tile did not stand still
     for (uint32_t n = 0;; ++n) {
       const uint32_t slot = n & 1u;
       wait(bar_u, n);
-      const WideInfo unit = sm.info[slot];
+      const PairInfo unit = sm.info[slot];
       if (!unit.valid || *reinterpret_cast<volatile uint32_t*>(&sm.aborted)) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_w);
       const uint32_t steps = unit.steps, plain = unit.plain, rows = x ? (unit.rows > tile_rows ? unit.rows - tile_rows : 0u) : min(unit.rows, tile_rows);
-      if (!rows) {                                           // this tile stands still
+      if (!rows) {                                           // this tile stands still: the same waits and arrivals, nothing in between
+        for (uint32_t j = 0; j < steps; ++j) {
+          wait3(s_bars, step0 + j);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_bars + 8 * ((step0 + j) % kPairRing));
+        }
+        wait3(o_bars, step0 + steps - 1);
         step0 += steps;
         continue;
       }
@@ -344,8 +361,8 @@ tree_pair_kernel(const TreeArgs a) {
         }
         tmem_ld_wait();
         const float2 scale2 = make_float2(scale, scale);
-        const WideScales& of_step = scales[g & 3u];
-        wait(bar_t + 8 * (g & 3u), g >> 2);
+        const WideScales& of_step = scales[g % kPairScales];
+        wait(bar_t + 8 * (g % kPairScales), g / kPairScales);
 #pragma unroll
         for (int i = 0; i < 64; i += 4) {                    // S' (a NaN entry's is NaN)
           const float4 k4 = *reinterpret_cast<const float4*>(&of_step.k[i]), v4 = *reinterpret_cast<const float4*>(&of_step.v[i]);
@@ -412,8 +429,7 @@ tree_pair_kernel(const TreeArgs a) {
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_bars + 8 * (weighed % kPairRing));
-        ++weighed;
+        if (lane == 0) mbar_arrive(p_bars + 8 * (g % kPairRing));
       }
       // ---- the unit's partial result
       wait3(o_bars, step0 + steps - 1);
@@ -448,7 +464,7 @@ tree_pair_kernel(const TreeArgs a) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(sm.tmem_at, kPairColumns);
+  if (warp == 16) tmem_dealloc(sm.tmem_at, kPairColumns);
 }
 
 }  // namespace grb
