@@ -198,72 +198,6 @@ kv_rows_kernel(const KvRowsArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (in[i]) *(READ ? rows[i] : held(i)) = x[i];
-  } else if constexpr (FORMAT == kKvQ4) {
-    // a lane holds word l of the entry's codes, dimensions 8 l .. 8 l + 7; four lanes share a scale
-    auto page = [&](int i) { return static_cast<uint8_t*>(value[i] ? a.pages.v : a.pages.k) + q4_page_at(entry[i]); };
-    auto at = [&](int i) { return uint32_t(entry[i] % kKvPage); };
-    if constexpr (READ) {
-      uint32_t code[N], scale[N], exp[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (in[i]) {
-          code[i] = reinterpret_cast<const uint32_t*>(page(i))[at(i) * (kQ4Codes / 4) + l];
-          scale[i] = page(i)[kQ4ScalesAt + at(i) * 4 + (l >> 2)];
-          exp[i] = page(i)[kQ4ExpsAt + at(i)];
-        }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (!in[i]) continue;
-        const float step = __fmul_rn(q4_scale(scale[i]), q4_unit(exp[i]));      // (exact, as is its product with a code: eight bits)
-        auto one = [&](uint32_t nibble) { return __fmul_rn(float(int(code[i] >> (4 * nibble) & 15u) - 8), step); };
-        *rows[i] = make_uint4(pack_bf(one(0), one(4)), pack_bf(one(1), one(5)), pack_bf(one(2), one(6)), pack_bf(one(3), one(7)));
-      }
-    } else {
-      uint4 x[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = in[i] ? *rows[i] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        uint32_t m = 0;                               // (magnitudes of BF16 values compare as integers)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
-        m = max(m & 0xFFFFu, m >> 16);
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-        const float group = __uint_as_float(m << 16);
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
-        const bool finite = m < 0x7F80u;
-        const uint32_t exp = q4_exp_byte(__uint_as_float(m << 16), finite);
-        float step;
-        uint32_t scale = q4_scale_byte<true>(finite ? group : 0.f, finite ? exp : 127u, step);
-        if (exp == kQ4MostByte) {                     // (the only entries with values beyond 7 steps and a half; 7 steps are a BF16 number)
-          const __nv_bfloat162 most = __float2bfloat162_rn(__fmul_rn(step, 7.f)), least = __hneg2(most);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 v = __hmax2(__hmin2(*reinterpret_cast<__nv_bfloat162*>(&w[j]), most), least);
-            w[j] = *reinterpret_cast<const uint32_t*>(&v);
-          }
-        }
-        // The quotient of a value of eight bits and a step of five lies on a border between two codes, or 2^-11 or more from all of them.  A product with the
-        // reciprocal, 2^-19 of it off at most, rounded to 2^-13 - by adding 1536 - lands on the right side; added to 2^23 1.5 + 8, it is the code.
-        float inverse;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(step));
-        uint32_t code = 0;
-#pragma unroll
-        for (int j = 3; j >= 0; --j) {
-          auto nibble = [&](float v) { return __float_as_uint(__fadd_rn(__fmaf_rn(v, inverse, 1536.f), 12582920.f - 1536.f)); };     // code + 8 in the lowest byte, 0 in the next
-          code = code * 16 + __byte_perm(nibble(bf_lo(w[j])), nibble(bf_hi(w[j])), 0x5410);
-        }
-        if (!finite) { code = 0x88888888u; scale = 64u; }
-        if (in[i]) {
-          reinterpret_cast<uint32_t*>(page(i))[at(i) * (kQ4Codes / 4) + l] = code;
-          if ((l & 3u) == 0) page(i)[kQ4ScalesAt + at(i) * 4 + (l >> 2)] = uint8_t(scale);
-          if (l == 0) page(i)[kQ4ExpsAt + at(i)] = uint8_t(exp);
-        }
-      }
-    }
   } else {
     auto held = [&](int i) { return reinterpret_cast<uint2*>(static_cast<uint8_t*>(value[i] ? a.pages.v : a.pages.k) + entry[i] * kKvDim) + l; };
     auto exps = [&](int i) { return (value[i] ? a.pages.v_exp : a.pages.k_exp) + entry[i]; };
@@ -307,6 +241,108 @@ kv_rows_kernel(const KvRowsArgs a) {
           *held(i) = byte == kKvNanByte ? make_uint2(0u, 0u) : make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
           if (l == 0) *exps(i) = uint8_t(byte);
         }
+      }
+    }
+  }
+}
+
+// The same in 4 bits.  Eight lanes share an entry, sixteen neighbouring values each, two lanes a scale; a warp takes sixteen entries of a row, four at a time.
+// What is found once for a lane's values - the two maxima, the scale, its reciprocal - costs as much as eight of them do.  32768 rows of 8 heads: 37 us in, 37
+// out (sixteen lanes an entry, eight entries a warp: 57 and 40); out, the stores alone - 134 MB - take 35 at the 3.8 TB/s that a fill reaches here.
+constexpr uint32_t kQ4EntriesPerWarp = 16;
+template <bool READ>
+__global__ void __launch_bounds__(kKvWarps * 32)
+kv_rows_q4_kernel(const KvRowsArgs a) {
+  step_kernel_entry();
+  constexpr int N = kQ4EntriesPerWarp / 4;
+  const uint32_t lane = threadIdx.x & 31u, l = lane & 7u, heads = 2 * a.pages.nkv, per_row = (heads + kQ4EntriesPerWarp - 1) / kQ4EntriesPerWarp;
+  const uint32_t id = blockIdx.x * kKvWarps + (threadIdx.x >> 5), row = id / per_row, head0 = (id - row * per_row) * kQ4EntriesPerWarp + (lane >> 3);
+  if (row >= a.rows) return;
+  const int64_t place = kv_place(a.table, a.row_seq[row], a.row_pos[row]);
+  if (place < 0) return;
+  const uint32_t at = uint32_t(place % kKvPage);
+  const size_t first = size_t(place / kKvPage) * a.pages.nkv * kQ4Page;       // of the page's first head
+  uint4* const keys = reinterpret_cast<uint4*>(a.k + row * a.ldk);
+  uint4* const values = reinterpret_cast<uint4*>(a.v + row * a.ldv);
+  uint8_t* page[N];
+  uint4* rows[N];
+  bool in[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t head = head0 + 4 * i;
+    in[i] = head < heads;
+    const bool value = head >= a.pages.nkv;
+    const uint32_t h = in[i] ? value ? head - a.pages.nkv : head : 0u;
+    page[i] = static_cast<uint8_t*>(value ? a.pages.v : a.pages.k) + first + size_t(h) * kQ4Page;
+    rows[i] = (value ? values : keys) + h * (kKvDim / 8);
+  }
+  if constexpr (READ) {     // (a lane's words are 8 apart, so that eight lanes store 128 bytes in a row)
+    uint32_t code[N][2], scale[N][2], exp[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (in[i]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          code[i][j] = reinterpret_cast<const uint32_t*>(page[i] + at * kQ4Codes)[l + 8 * j];
+          scale[i][j] = page[i][kQ4ScalesAt + at * 4 + (l >> 2) + 2 * j];
+        }
+        exp[i] = page[i][kQ4ExpsAt + at];
+      }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!in[i]) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float step = __fmul_rn(q4_scale(scale[i][j]), q4_unit(exp[i]));   // (exact, as is its product with a code: eight bits)
+        // code + 8 in the lowest bits of 2^23; the sum with -(2^23 + 8) is the code
+        auto one = [&](uint32_t nibble) { return __fmul_rn(__fadd_rn(__uint_as_float(0x4B000000u | (code[i][j] >> (4 * nibble) & 15u)), -8388616.f), step); };
+        rows[i][int(l) + 8 * j] = make_uint4(pack_bf(one(0), one(4)), pack_bf(one(1), one(5)), pack_bf(one(2), one(6)), pack_bf(one(3), one(7)));
+      }
+    }
+  } else {
+    uint4 x[N][2];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x[i][j] = in[i] ? rows[i][2 * l + j] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t w[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w, x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
+      uint32_t m = 0;                                 // (magnitudes of BF16 values compare as integers)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+      m = max(m & 0xFFFFu, m >> 16);
+      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+      const float group = __uint_as_float(m << 16);
+      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
+      const bool finite = m < 0x7F80u;
+      const uint32_t exp = q4_exp_byte(__uint_as_float(m << 16), finite);
+      float step;
+      uint32_t scale = q4_scale_byte<true>(finite ? group : 0.f, finite ? exp : 127u, step);
+      if (exp == kQ4MostByte) {                       // (the only entries with values beyond 7 steps and a half; 7 steps are a BF16 number)
+        const __nv_bfloat162 most = __float2bfloat162_rn(__fmul_rn(step, 7.f)), least = __hneg2(most);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const __nv_bfloat162 v = __hmax2(__hmin2(*reinterpret_cast<__nv_bfloat162*>(&w[j]), most), least);
+          w[j] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+      // The quotient of a value of eight bits and a step of five lies on a border between two codes, or 2^-11 or more from all of them.  A product with the
+      // reciprocal, 2^-19 of it off at most, rounded to 2^-13 - by adding 1536 - lands on the right side; added to 2^23 1.5 + 8, it is the code.
+      float inverse;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(step));
+      uint32_t code[2] = {0, 0};
+#pragma unroll
+      for (int j = 7; j >= 0; --j) {
+        auto nibble = [&](float v) { return __float_as_uint(__fadd_rn(__fmaf_rn(v, inverse, 1536.f), 12582920.f - 1536.f)); };     // code + 8 in the lowest byte, 0 in the next
+        code[j >> 2] = code[j >> 2] * 16 + __byte_perm(nibble(bf_lo(w[j])), nibble(bf_hi(w[j])), 0x5410);
+      }
+      if (!finite) { code[0] = code[1] = 0x88888888u; scale = 64u; }
+      if (in[i]) {
+        reinterpret_cast<uint2*>(page[i] + at * kQ4Codes)[l] = make_uint2(code[0], code[1]);
+        if ((l & 1u) == 0) page[i][kQ4ScalesAt + at * 4 + (l >> 1)] = uint8_t(scale);
+        if (l == 0) page[i][kQ4ExpsAt + at] = uint8_t(exp);
       }
     }
   }

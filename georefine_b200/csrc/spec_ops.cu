@@ -35,9 +35,10 @@ int kv_rows(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t*
   a.ldk = ldk;
   a.ldv = ldv;
   a.rows = rows;
-  const uint64_t warps = uint64_t(rows) * ((2 * a.pages.nkv + kKvEntriesPerWarp - 1) / kKvEntriesPerWarp), ctas = (warps + kKvWarps - 1) / kKvWarps;
+  const uint32_t entries = pages->format == GRB_KV_Q4 ? kQ4EntriesPerWarp : kKvEntriesPerWarp;
+  const uint64_t warps = uint64_t(rows) * ((2 * a.pages.nkv + entries - 1) / entries), ctas = (warps + kKvWarps - 1) / kKvWarps;
   if (warps > 0xFFFFFF00ull) return GRB_ERR_UNSUPPORTED;   // (numbered in 32 bits)
-  const auto kernel = pages->format == GRB_KV_E4M3 ? kv_rows_kernel<READ, kKvE4m3> : pages->format == GRB_KV_Q4 ? kv_rows_kernel<READ, kKvQ4> : kv_rows_kernel<READ, kKvBf16>;
+  const auto kernel = pages->format == GRB_KV_E4M3 ? kv_rows_kernel<READ, kKvE4m3> : pages->format == GRB_KV_Q4 ? kv_rows_q4_kernel<READ> : kv_rows_kernel<READ, kKvBf16>;
   return launch_step(kernel, dim3(uint32_t(ctas)), dim3(kKvWarps * 32), 0, static_cast<cudaStream_t>(stream), a);
 }
 
