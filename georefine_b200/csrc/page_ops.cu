@@ -79,6 +79,8 @@ int grb_rotary(const grb_rotary_step* s, void* cuda_stream) {
     return (s->heads == 1 || head >= int64_t(s->dim)) && (s->rows <= 1 || row >= heads || (s->heads > 1 && row >= int64_t(s->dim) && head >= rows));
   };
   if (s->ldx < 0 || s->ldx_head < 0 || !apart(s->ldo, s->ldo_head)) return GRB_ERR_ARGUMENT;
+  // (in place: where it lies)
+  if (s->x == s->out && ((s->rows > 1 && s->ldx != s->ldo) || (s->rows && s->heads > 1 && s->ldx_head != s->ldo_head))) return GRB_ERR_ARGUMENT;
   if (!s->rows) return GRB_OK;
   RotaryArgs a{};
   a.x = s->x;

@@ -79,6 +79,8 @@ def test_rotary_arguments():
                         (dict(ldx=-1), ARGUMENT), (dict(ldx_head=-1), ARGUMENT), (dict(ldo=128, ldo_head=383), ARGUMENT)]):
         assert call(_rotary(**kw), None) == status, kw
     assert call(None, None) == ARGUMENT and call(_rotary(rows=0), None) == 0
+    for kw in (dict(ldx=2048), dict(ldx_head=256), dict(ldo=2048), dict(rows=1, ldo_head=256)):      # in place, and elsewhere
+        assert call(_rotary(**kw), None) == ARGUMENT
     assert call(_rotary(rows=0, ldo=128, ldo_head=384), None) == 0           # rows inside, heads outside
     assert _native.ROTARY_STEP.size == ctypes.sizeof(_native.RotaryStep)
     values = P, 7, 8, 2 * P, 9, 10, 3 * P, 4 * P, 1, 2, 3, 4, 1, 2, 1, 0, 0.5
