@@ -1090,10 +1090,10 @@ class MTPHead:
         z = lambda *shape, dtype=bf: torch.zeros(*shape, device=d.dev, dtype=dtype)
         self.kv, exps = kv_buffers((2, d.kv.shape[2], cfg.kv_heads), d.dev, getattr(d, "kv_format", "bf16"))
         paged = getattr(d, "kv_format", "bf16") != "bf16" or hasattr(d, "page_sets")
-        pages = ops.KVPages(self.kv[0], self.kv[1], *((None, None) if exps is None else exps)) if paged else None
-        self.pages = None if getattr(d, "kv_format", "bf16") == "bf16" else pages
+        self.cache = ops.KVPages(self.kv[0], self.kv[1], *((None, None) if exps is None else exps)) if paged else None
+        self.pages = None if getattr(d, "kv_format", "bf16") == "bf16" else self.cache
         if hasattr(d, "page_sets"):
-            d.page_sets.append(pages)
+            d.page_sets.append(self.cache)
         self.tok, self.hid = z(R, dtype=torch.int32), z(R, H)
         self.e, self.cat, self.z, self.x = z(R, H), z(R, 2 * H), z(R, H), z(R, H)
         self.qkv, self.ctx, self.o_out = z(R, cfg.qkv_rows), z(R, cfg.heads * cfg.head_dim), z(R, H)
@@ -1270,8 +1270,20 @@ class MTPSpeculator:
         return out
 
     def fork(self, slot: int, n: int = 1) -> list:
-        """``Batcher.fork`` with the head's pending draft and hidden state."""
+        """``Batcher.fork`` with the head's pending draft and hidden state, and its cache up to the pending token, which the trunk has not taken in yet."""
+        d, pos = self.b.d, self.b.active[slot]["pos"]
+        d.ensure_pages(slot, pos)
         children = self.b.fork(slot, n)
+        try:
+            for c in children:
+                d.ensure_pages(c, pos)
+        except RuntimeError:
+            for c in children:
+                self.b.retire(c)
+            raise
+        page, rest = divmod(pos, PAGE)
+        src, dst, counts = d._vectors([int(d._table_host[slot, page])] * n, [int(d._table_host[c, page]) for c in children], [rest + 1] * n)
+        ops.kv_copy(src, dst, self.head.cache, positions=counts)
         for c in children:
             self.first[c], self.hidden[c] = self.first[slot], self.hidden[slot].clone()
         return children

@@ -210,6 +210,37 @@ def test_a_draft_head_forks_with_its_trunk(dev, small):
         _consistent(d)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("length", [255, 256, 300])
+def test_a_forked_draft_head_has_seen_the_pending_token(dev, small, length, fmt):
+    """The head's entries are the parent's up to the pending token's, whose page the trunk may not have asked for; cycles go on alike."""
+    from georefine_b200 import ops, serve
+
+    d = _decoder(small, dev, kv_format=fmt)
+    # (pages that forks may get hold something else than zeros)
+    spec = serve.MTPSpeculator(serve.Batcher(d), serve.MTPHead.synthetic(d), k=3)
+    spec.retire(spec.admit(_prompt(small[0], 900, 8)))
+    slot = spec.admit(_prompt(small[0], length))
+    children = spec.fork(slot, 2)
+    _consistent(d)
+    n = length + 1
+
+    def entries(s):                               # (the head's first is that of position 1)
+        k, v = (torch.empty(n - 1, 2, 128, device=dev, dtype=torch.bfloat16) for _ in range(2))
+        i32 = lambda x: torch.tensor(list(x), dtype=torch.int32, device=dev)
+        ops.kv_read(i32([s] * (n - 1)), i32(range(1, n)), d.page_table, spec.head.cache, k, v)
+        return torch.stack([k, v])
+
+    want = entries(slot)
+    assert bool(want.abs().amax(dim=(0, 2, 3)).gt(0).all()) and all(torch.equal(entries(c), want) for c in children)
+    for _ in range(3):
+        spec.cycle()
+        for c in children:
+            assert spec.first[c] == spec.first[slot] and torch.equal(spec.hidden[c], spec.hidden[slot])
+    assert all(spec.b.active[c]["tokens"] == spec.b.active[slot]["tokens"] for c in children)
+    _consistent(d)
+
+
 ROPES = {"interleaved": dict(rope_layout="interleaved"), "part": dict(rope_dim=64), "both": dict(rope_layout="interleaved", rope_dim=32),
          "yarn": dict(rope_scaling={"kind": "yarn", "factor": 4.0, "original": 256}), "part, linear": dict(rope_dim=96, rope_scaling={"kind": "linear", "factor": 2.0})}
 
