@@ -196,41 +196,94 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, uint32_t part_posit
   if (tid == 0) a.plan[0] = uint32_t(done >> 32), a.plan[1] = uint32_t(done), a.plan[2] = uint32_t(wide_done >> 32), a.plan[3] = uint32_t(wide_done);
 }
 
-// An entry of a 4-bit page from a warp whose lanes hold dimensions 2 l, 2 l + 1, 64 + 2 l and 64 + 2 l + 1.
-__device__ __forceinline__ void tree_store_q4(uint8_t* page, uint32_t at, float (&x)[4], uint32_t lane) {
-  bool fine = true;
+// Entries of 4-bit pages from a warp whose lanes hold dimensions 2 l, 2 l + 1, 64 + 2 l and 64 + 2 l + 1 of each; no page: nothing is stored.  N entries side by
+// side, whose chains of exchanges and divisions would follow one another.
+template <int N>
+__device__ __forceinline__ void tree_store_q4(uint8_t* const (&page)[N], uint32_t at, float (&x)[N][4], uint32_t lane) {
+  float group[N][2];                                         // of dimensions 32 (l / 16) .. and 64 + 32 (l / 16) ..
+  bool fine[N];
+  uint32_t exp[N];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) fine = fine && fabsf(x[k]) <= 3.4028234e38f;
-  fine = __all_sync(0xFFFFFFFFu, fine);
-  float group[2];                                            // of dimensions 32 (l / 16) .. and 64 + 32 (l / 16) ..
+  for (int i = 0; i < N; ++i) {
+    fine[i] = true;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    group[h] = fine ? fmaxf(fabsf(x[2 * h]), fabsf(x[2 * h + 1])) : 0.f;
+    for (int k = 0; k < 4; ++k) fine[i] = fine[i] && fabsf(x[i][k]) <= 3.4028234e38f;
+    fine[i] = __all_sync(0xFFFFFFFFu, fine[i]);
 #pragma unroll
-    for (int off = 8; off; off >>= 1) group[h] = fmaxf(group[h], __shfl_xor_sync(0xFFFFFFFFu, group[h], off));
+    for (int h = 0; h < 2; ++h) group[i][h] = fine[i] ? fmaxf(fabsf(x[i][2 * h]), fabsf(x[i][2 * h + 1])) : 0.f;
   }
-  const float top = fmaxf(group[0], group[1]);
-  const uint32_t exp = q4_exp_byte(fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16)), true);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float step;
-    const uint32_t scale = q4_scale_byte<false>(group[h], exp, step);
-    // dimensions 2 l and 2 l + 1 are nibble l % 4 of either half of word l / 4
-    uint32_t code = 0x00080008u;
-    if (fine) code = q4_nibble(__fdiv_rn(x[2 * h], step)) | q4_nibble(__fdiv_rn(x[2 * h + 1], step)) << 16;
-    code <<= 4 * (lane & 3u);
-    code |= __shfl_xor_sync(0xFFFFFFFFu, code, 1);
-    code |= __shfl_xor_sync(0xFFFFFFFFu, code, 2);
-    if ((lane & 3u) == 0) reinterpret_cast<uint32_t*>(page)[at * (kQ4Codes / 4) + 8 * h + (lane >> 2)] = code;
-    if ((lane & 15u) == 0) page[kQ4ScalesAt + at * 4 + 2 * h + (lane >> 4)] = uint8_t(scale);
+  for (int off = 8; off; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) group[i][h] = fmaxf(group[i][h], __shfl_xor_sync(0xFFFFFFFFu, group[i][h], off));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float top = fmaxf(group[i][0], group[i][1]);
+    exp[i] = q4_exp_byte(fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16)), true);
   }
-  if (lane == 0) page[kQ4ExpsAt + at] = uint8_t(fine ? exp : kKvNanByte);
+  uint32_t code[N][2], scale[N][2];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float step;
+      scale[i][h] = q4_scale_byte<false>(group[i][h], exp[i], step);
+      // dimensions 2 l and 2 l + 1 are nibble l % 4 of either half of word l / 4
+      const uint32_t c = q4_nibble(__fdiv_rn(x[i][2 * h], step)) | q4_nibble(__fdiv_rn(x[i][2 * h + 1], step)) << 16;
+      code[i][h] = (fine[i] ? c : 0x00080008u) << 4 * (lane & 3u);
+    }
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) code[i][h] |= __shfl_xor_sync(0xFFFFFFFFu, code[i][h], off);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (!page[i]) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if ((lane & 3u) == 0) reinterpret_cast<uint32_t*>(page[i])[at * (kQ4Codes / 4) + 8 * h + (lane >> 2)] = code[i][h];
+      if ((lane & 15u) == 0) page[i][kQ4ScalesAt + at * 4 + 2 * h + (lane >> 4)] = uint8_t(scale[i][h]);
+    }
+    if (lane == 0) page[i][kQ4ExpsAt + at] = uint8_t(fine[i] ? exp[i] : kKvNanByte);
+  }
+}
+
+// Rotated queries of `count` neighbouring heads for caches that are decoded to FP16: times a power of two that brings the largest component to [2^14, 2^15): 11 bits
+// where BF16 has 8, and what falls below FP16's normal range is 2^-28 of the largest.  (Magnitudes compare as their bits do; those of numbers that are not finite
+// are the largest.)
+template <int N>
+__device__ __forceinline__ void tree_store_queries(const TreeArgs& a, uint32_t row, uint32_t head, uint32_t count, const float (&x)[N][4], float log2_scale, uint32_t lane) {
+  uint32_t most[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    auto size = [&](int k) { return __float_as_uint(x[i][k]) & 0x7FFFFFFFu; };
+    most[i] = __reduce_max_sync(0xFFFFFFFFu, max(max(size(0), size(1)), max(size(2), size(3))));
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (uint32_t(i) >= count) break;
+    const size_t pair = size_t(row) * a.nq + head + i;
+    uint32_t* const dst = reinterpret_cast<uint32_t*>(a.q + pair * kKvDim) + lane;
+    const bool fine = most[i] < 0x7F800000u;
+    const int e = max(int(most[i] >> 23) - 127 - 14, -100);  // (<= 113)
+    const float down = __uint_as_float(uint32_t(127 - e) << 23);
+    const __half2 h0 = fine ? __floats2half2_rn(x[i][0] * down, x[i][1] * down) : __floats2half2_rn(0.f, 0.f);
+    const __half2 h1 = fine ? __floats2half2_rn(x[i][2] * down, x[i][3] * down) : __floats2half2_rn(0.f, 0.f);
+    dst[0] = *reinterpret_cast<const uint32_t*>(&h0);
+    dst[32] = *reinterpret_cast<const uint32_t*>(&h1);
+    if (lane == 0) a.q_scale[pair] = fine ? __fmul_rn(log2_scale, __uint_as_float(uint32_t(127 + e) << 23)) : __uint_as_float(0x7FC00000u);
+  }
 }
 
 // The first CTA lays down the plan; in the others a warp takes up to eight neighbouring heads of a row, all their loads on their
 // way together.  A lane owns dimensions 2 l, 2 l + 1 and the two that the rotation pairs with them.  The products of BF16 values are
 // exact in FP32, so the rotation rounds once before the result is rounded to its type.  1024 rows of 56 heads: 15 us (one head a
-// warp 43; 256 rows of the plan at a time 27).  One row: 7 us, the plan's chain of dependent loads.
+// warp 43; 256 rows of the plan at a time 27).  One row: 7 us, the plan's chain of dependent loads.  4 bits: 21 us, of which
+// the entries of four heads side by side keep 2 (128 rows: 9.5 instead of 11.4).
 constexpr uint32_t kTreeHeadsPerWarp = 8;
 template <int FORMAT>
 __global__ void __launch_bounds__(kTreePrepMost)
@@ -255,6 +308,37 @@ tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
   const float c[4] = {bf_lo(cs[0]), bf_hi(cs[0]), bf_lo(cs[32]), bf_hi(cs[32])};
   const float s[4] = {bf_lo(sn[0]), bf_hi(sn[0]), bf_lo(sn[32]), bf_hi(sn[32])};
   const float log2_scale = __fmul_rn(a.scaling, 1.4426950408889634f);
+  if constexpr (FORMAT == kKvQ4) {                           // four at a time, the keys' and values' together
+    constexpr uint32_t kSide = 4;
+#pragma unroll
+    for (uint32_t i0 = 0; i0 < kTreeHeadsPerWarp; i0 += kSide) {
+      if (i0 >= n) break;
+      float x[kSide][4];
+#pragma unroll
+      for (uint32_t i = 0; i < kSide; ++i) {
+        const uint32_t l = i0 + i < n ? lo[i0 + i] : 0u, h = i0 + i < n ? hi[i0 + i] : 0u;
+        const float y[4] = {bf_lo(l), bf_hi(l), bf_lo(h), bf_hi(h)};
+        const bool value = head0 + i0 + i >= a.nq + a.nkv;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          x[i][k] = value ? y[k] : __fsub_rn(__fmul_rn(y[k], c[k]), __fmul_rn(y[k + 2], s[k]));
+          x[i][k + 2] = value ? y[k + 2] : __fadd_rn(__fmul_rn(y[k + 2], c[k + 2]), __fmul_rn(y[k], s[k + 2]));
+        }
+      }
+      if (head0 + i0 < a.nq) tree_store_queries<kSide>(a, row, head0 + i0, min(a.nq - head0 - i0, n - i0), x, log2_scale, lane);
+      if (head0 + min(n, i0 + kSide) > a.nq) {
+        uint8_t* page[kSide];
+#pragma unroll
+        for (uint32_t i = 0; i < kSide; ++i) {
+          const uint32_t head = head0 + i0 + i;
+          const bool value = head >= a.nq + a.nkv;
+          page[i] = i0 + i < n && head >= a.nq ? static_cast<uint8_t*>(value ? a.pages.v : a.pages.k) + q4_page_at(kv_entry(place, a.nkv, value ? head - a.nq - a.nkv : head - a.nq)) : nullptr;
+        }
+        tree_store_q4<kSide>(page, uint32_t(place % kKvPage), x, lane);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (uint32_t i = 0; i < kTreeHeadsPerWarp; ++i) {
     const uint32_t head = head0 + i;
@@ -280,24 +364,12 @@ tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
       for (int k = 0; k < 4; ++k) x[k] = y[k];
     }
     if (query) {
-      const size_t pair = size_t(row) * a.nq + head;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + pair * (F8 ? kKvDim : 2 * kKvDim)) + lane;
       if constexpr (F8) {
-        // FP16 times a power of two that brings the largest component to [2^14, 2^15): 11 bits where BF16 has 8, and what falls
-        // below FP16's normal range is 2^-28 of the largest.
-        const float m = warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
-        bool fine = true;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) fine = fine && fabsf(x[k]) <= 3.4028234e38f;
-        fine = __all_sync(0xFFFFFFFFu, fine);
-        const int e = max(int(__float_as_uint(m) >> 23) - 127 - 14, -100);        // (<= 113)
-        const float down = __uint_as_float(uint32_t(127 - e) << 23);
-        const __half2 h0 = fine ? __floats2half2_rn(x[0] * down, x[1] * down) : __floats2half2_rn(0.f, 0.f);
-        const __half2 h1 = fine ? __floats2half2_rn(x[2] * down, x[3] * down) : __floats2half2_rn(0.f, 0.f);
-        dst[0] = *reinterpret_cast<const uint32_t*>(&h0);
-        dst[32] = *reinterpret_cast<const uint32_t*>(&h1);
-        if (lane == 0) a.q_scale[pair] = fine ? __fmul_rn(log2_scale, __uint_as_float(uint32_t(127 + e) << 23)) : __uint_as_float(0x7FC00000u);
+        float one[1][4] = {{x[0], x[1], x[2], x[3]}};
+        tree_store_queries<1>(a, row, head, 1, one, log2_scale, lane);
       } else {
+        const size_t pair = size_t(row) * a.nq + head;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + pair * 2 * kKvDim) + lane;
         const uint32_t h0 = pack_bf(x[0], x[1]), h1 = pack_bf(x[2], x[3]);
         dst[0] = h0;
         dst[32] = h1;
@@ -309,9 +381,7 @@ tree_prep_kernel(const TreeArgs a, uint32_t part_positions) {
     }
     const size_t entry = kv_entry(place, a.nkv, value ? head - a.nq - a.nkv : head - a.nq);
     void* const pages = value ? a.pages.v : a.pages.k;
-    if constexpr (FORMAT == kKvQ4) {
-      tree_store_q4(static_cast<uint8_t*>(pages) + q4_page_at(entry), uint32_t(entry % kKvPage), x, lane);
-    } else if constexpr (F8) {
+    if constexpr (F8) {
       const uint32_t byte = kv_warp_byte(x);
       uint16_t* dst = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(pages) + entry * kKvDim) + lane;
       dst[0] = uint16_t(kv_codes(x[0], x[1], byte));
