@@ -282,8 +282,8 @@ __device__ __forceinline__ void tree_store_queries(const TreeArgs& a, uint32_t r
 // The first CTA lays down the plan; in the others a warp takes up to eight neighbouring heads of a row, all their loads on their
 // way together.  A lane owns dimensions 2 l, 2 l + 1 and the two that the rotation pairs with them.  The products of BF16 values are
 // exact in FP32, so the rotation rounds once before the result is rounded to its type.  1024 rows of 56 heads: 15 us (one head a
-// warp 43; 256 rows of the plan at a time 27).  One row: 7 us, the plan's chain of dependent loads.  4 bits: 21 us, of which
-// the entries of four heads side by side keep 2 (128 rows: 9.5 instead of 11.4).
+// warp 43; 256 rows of the plan at a time 27).  One row: 7 us, the plan's chain of dependent loads.  4 bits: 21 us (the
+// entries of a warp one after another: 23; 128 rows 9.5 and 11.4).
 constexpr uint32_t kTreeHeadsPerWarp = 8;
 template <int FORMAT>
 __global__ void __launch_bounds__(kTreePrepMost)
