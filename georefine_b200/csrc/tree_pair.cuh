@@ -95,7 +95,7 @@ tree_pair_kernel(const TreeArgs a) {
   };
   auto wait3 = [&](uint32_t bars, uint32_t step) { wait(bars + 8 * (step % kPairRing), step / kPairRing); };
   uint32_t step0 = 0;                                        // steps this CTA has taken before the unit
-  // registers, of the 96 that each thread of the launch has: 144 for the weights, 72 for loading, 40 for the others
+  // registers, of the 96 that each thread of the launch has: 144 for the weights, 72 for loading, 48 for the others
   if (warp >= 8 && warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ---- loading: K and the queries, or V -------------------------------------------------------------------------
@@ -105,6 +105,7 @@ tree_pair_kernel(const TreeArgs a) {
     // A thread's pieces of a step: the same group of 32 dimensions of every 32nd row; the lanes of the upper two groups take their words in another order, so
     // that no two of eight lanes store to the same banks.  The first 64 threads also bring a position's exponent.
     const uint32_t row0 = lt >> 2, swapped = lt & 2u;
+    const uint32_t per_group = 65536u / a.group + 1u;        // a column of 256 over the group, in units of 2^-16
     uint32_t to_word[4];                                     // where a piece's words, eight dimensions each, go
 #pragma unroll
     for (uint32_t q = 0; q < 4; ++q) to_word[q] = wide_offset<kWideStep>(row0, 4 * (lt & 3u) + (q ^ swapped));
@@ -178,12 +179,19 @@ tree_pair_kernel(const TreeArgs a) {
           wait3(bar_s, step0 - 1);
           wait3(bar_s + kRound, step0 - 1);
         }
+        // (piece lt % 16 of every eighth column; column c of the two tiles lies c + c / group (nq - group) heads behind the first)
         const uint32_t used = unit.rows * a.group, first_tile = tile_rows * a.group;
-        for (uint32_t i = 0; i < (unit.rows > tile_rows ? 32u : 16u); ++i) {
-          const uint32_t m = (lt >> 4) + 8 * (i & 15u), col = i < 16 ? m : first_tile + m, r = col / a.group;
-          const bool in = col < used && m < first_tile;
-          const uint16_t* const src = in ? a.q + (size_t(unit.first + r) * a.nq + unit.kvh * a.group + (col - r * a.group)) * kKvDim + 8 * (lt & 15u) : a.q;
-          cp_async_16(qs + (i < 16 ? 0u : kWideOperand) + wide_offset<kWideTile>(m, lt & 15u), src, in ? 16u : 0u);
+        const uint16_t* const src = a.q + (size_t(unit.first) * a.nq + unit.kvh * a.group) * kKvDim + 8 * (lt & 15u);
+        const uint32_t next_row = (a.nq - a.group) * kKvDim;
+#pragma unroll 1
+        for (uint32_t y = 0; y < (unit.rows > tile_rows ? 2u : 1u); ++y) {
+          const uint32_t dst = qs + y * kWideOperand + wide_offset<kWideTile>(lt >> 4, lt & 15u);
+#pragma unroll 4
+          for (uint32_t i = 0; i < kWideTile / 8; ++i) {
+            const uint32_t m = (lt >> 4) + 8 * i, column = y * first_tile + m;
+            const bool in = column < used && m < first_tile;
+            cp_async_16(dst + 1024 * i, in ? src + (column * kKvDim + (column * per_group >> 16) * next_row) : src, in ? 16u : 0u);
+          }
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -202,7 +210,7 @@ tree_pair_kernel(const TreeArgs a) {
       step0 += steps;
     }
   } else if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 18) {
       // ---- units: where the next one lies, while this one is at hand ------------------------------------------------
       uint32_t tile = 0, n = 0;
@@ -253,25 +261,44 @@ tree_pair_kernel(const TreeArgs a) {
       __syncwarp();
     }
     // ---- products: warp 16 of tile 0, warp 17 of tile 1 -----------------------------------------------------------
+    // (what these warps do between a wait and the next lies in the chain of every step, and they get an instruction in seven cycles at best: descriptors are one
+    // addition apart, stages and rounds are counted, not divided out)
     const uint32_t x = warp - 16;
-    constexpr uint32_t kFp16 = ~((1u << 7) | (1u << 10)), kIdesc = umma_idesc_bf16(128) & kFp16, kIdescS = umma_idesc_bf16(kWideStep) & kFp16;
-    const uint32_t q = qs + x * kWideOperand, s_tmem = sm.tmem_at + x * 128, o_tmem = sm.tmem_at + 256 + x * 128, s_bars = bar_s + x * kRound, o_bars = bar_o + x * kRound, p_bars = bar_p + x * kRound;
+    constexpr uint32_t kFp16 = ~((1u << 7) | (1u << 10)), kIdesc = umma_idesc_bf16(128) & kFp16 | (1u << 16), kIdescS = umma_idesc_bf16(kWideStep) & kFp16;
+    const uint32_t s_tmem = sm.tmem_at + x * 128, o_tmem = sm.tmem_at + 256 + x * 128, s_bars = bar_s + x * kRound, o_bars = bar_o + x * kRound, p_bars = bar_p + x * kRound;
+    const uint64_t q_desc = umma_desc_sw128(qs + x * kWideOperand), k_desc = umma_desc_sw128(ks), v_desc = wide_desc_v(vs);
+    struct Turn {                                            // a step's place in the ring, and the parity of its round
+      uint32_t stage, parity;
+      __device__ __forceinline__ void next() {
+        const bool last = stage == kPairRing - 1;
+        stage = last ? 0u : stage + 1u;
+        parity ^= uint32_t(last);
+      }
+    };
+    Turn s_turn{0, 0}, used{0, 0}, o_turn{0, 0};             // of the next scores, of the products two steps before them, of the next outputs
+    uint32_t s_at = s_tmem, p_at = s_tmem, behind = 0;       // (the two places of S and P take turns)
     bool on = true;
-    auto scores = [&](uint32_t g) {
-      if (g > 1) wait3(o_bars, g - 2);                // the weights there have been used (issue order alone does not say so: the two products differ in shape)
-      wait3(bar_k, g);
+    auto scores = [&] {
+      if (behind == 2) {                                     // the weights there have been used (issue order alone does not say so: the two products differ in shape)
+        wait(o_bars + 8 * used.stage, used.parity);
+        used.next();
+      } else {
+        ++behind;
+      }
+      wait(bar_k + 8 * s_turn.stage, s_turn.parity);
       tc_fence_after();
       if (elect_one()) {
         if (on) {
+          const uint64_t k = k_desc + s_turn.stage * (kWideStage >> 4);
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {                      // 16 dimensions each
-            const uint32_t half = (d >> 2) * (kWideOperand / 2), k16 = (d & 3) * 32;
-            umma_bf16(s_tmem + (g & 1u) * kWideStep, umma_desc_sw128(q + half + k16), umma_desc_sw128(ks + (g % kPairRing) * kWideStage + half / 2 + k16), kIdescS, d > 0);
-          }
+          for (int d = 0; d < 8; ++d)                        // 16 dimensions each
+            umma_bf16(s_at, q_desc + ((d >> 2) * (kWideOperand / 2) + (d & 3) * 32) / 16, k + ((d >> 2) * (kWideStage / 2) + (d & 3) * 32) / 16, kIdescS, d > 0);
         }
-        umma_commit(s_bars + 8 * (g % kPairRing));           // (of a tile that stands still: at once)
+        umma_commit(s_bars + 8 * s_turn.stage);              // (of a tile that stands still: at once)
       }
       __syncwarp();
+      s_turn.next();
+      s_at ^= kWideStep;
     };
     for (uint32_t n = 0; x < 2; ++n) {
       wait(bar_u, n);
@@ -282,22 +309,23 @@ tree_pair_kernel(const TreeArgs a) {
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_w);
       wait(bar_q, n);
-      scores(step0);
+      scores();
       for (uint32_t j = 0; j < steps; ++j) {
-        const uint32_t g = step0 + j;
-        if (j + 1 < steps) scores(g + 1);
-        wait3(bar_v, g);
-        wait3(p_bars, g);
+        if (j + 1 < steps) scores();
+        wait(bar_v + 8 * o_turn.stage, o_turn.parity);
+        wait(p_bars + 8 * o_turn.stage, o_turn.parity);
         tc_fence_after();
         if (elect_one()) {
           if (on) {
+            const uint64_t v = v_desc + o_turn.stage * (kWideStage >> 4);
 #pragma unroll
-            for (int d = 0; d < 4; ++d)                      // 16 positions each
-              umma_bf16_ts(o_tmem, s_tmem + (g & 1u) * kWideStep + 8 * d, wide_desc_v(vs + (g % kPairRing) * kWideStage + 2048 * d), kIdesc | (1u << 16), j > 0 || d > 0);
+            for (int d = 0; d < 4; ++d) umma_bf16_ts(o_tmem, p_at + 8 * d, v + 2048 / 16 * d, kIdesc, j > 0 || d > 0);        // 16 positions each
           }
-          umma_commit(o_bars + 8 * (g % kPairRing));
+          umma_commit(o_bars + 8 * o_turn.stage);
         }
         __syncwarp();
+        o_turn.next();
+        p_at ^= kWideStep;
       }
       step0 += steps;
     }
