@@ -34,6 +34,10 @@ struct PairInfo {
   uint32_t plain;                  // steps, from the first on, whose positions every row sees
   int32_t start, extent;           // positions start .. extent - 1: what some row sees, up to the last such
 };
+// What the exponents of a step's entries mean: 2^e of K; e and 2^-e of V.
+struct PairScales {
+  float k[kWideStep], v[kWideStep], v_inverse[kWideStep];
+};
 struct PairShared {
   uint64_t bars[2 * kPairRing + 3 * 2 * kPairRing + 3 + 8];      // K stored, V stored; S done, O done, P stored, of either tile; unit set up, unit seen, queries stored; scales
   PairInfo info[2];                              // of a unit and the next
@@ -42,7 +46,7 @@ struct PairShared {
 };
 constexpr uint32_t kPairSharedBytes = 2048;
 static_assert(sizeof(PairShared) <= kPairSharedBytes, "the operands follow");
-constexpr uint32_t kPairSmem = kPairSharedBytes + 2 * kWideOperand + 2 * kPairRing * kWideStage + kPairScales * uint32_t(sizeof(WideScales));
+constexpr uint32_t kPairSmem = kPairSharedBytes + 2 * kWideOperand + 2 * kPairRing * kWideStage + kPairScales * uint32_t(sizeof(PairScales));
 
 __global__ void __launch_bounds__(kPairThreads, 1)
 tree_pair_kernel(const TreeArgs a) {
@@ -50,7 +54,7 @@ tree_pair_kernel(const TreeArgs a) {
   PairShared& sm = *reinterpret_cast<PairShared*>(wide_smem);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t qs = smem_u32(wide_smem) + kPairSharedBytes, ks = qs + 2 * kWideOperand, vs = ks + kPairRing * kWideStage;
-  WideScales* const scales = reinterpret_cast<WideScales*>(wide_smem + kPairSharedBytes + 2 * kWideOperand + 2 * kPairRing * kWideStage);
+  PairScales* const scales = reinterpret_cast<PairScales*>(wide_smem + kPairSharedBytes + 2 * kWideOperand + 2 * kPairRing * kWideStage);
   constexpr uint32_t kRound = 8 * kPairRing;
   const uint32_t bar_k = smem_u32(&sm.bars[0]), bar_v = bar_k + kRound, bar_s = bar_v + kRound, bar_o = bar_s + 2 * kRound, bar_p = bar_o + 2 * kRound, bar_u = bar_p + 2 * kRound,
                  bar_w = bar_u + 8, bar_q = bar_w + 8, bar_t = bar_q + 8;
@@ -155,13 +159,13 @@ tree_pair_kernel(const TreeArgs a) {
           }
         }
         if (lt < kWideStep) {                                // (a byte below what an entry has - 0, where nobody wrote - stands for zeros of the smallest size)
-          WideScales& s = scales[g % kPairScales];
+          PairScales& s = scales[g % kPairScales];
           if (of_k) {
             s.k[lt] = kv_scale(p.exp);
           } else {
             const uint32_t b = max(p.exp, kKvLeastByte);
             s.v[lt] = b == kKvNanByte ? __uint_as_float(0x7FC00000u) : float(int(b) - 127);
-            s.v_inverse[lt] = uint16_t(__float_as_uint(kv_inverse(b)) >> 16);
+            s.v_inverse[lt] = kv_inverse(b);
           }
         }
         fence_proxy_async_smem();
@@ -396,7 +400,7 @@ tree_pair_kernel(const TreeArgs a) {
         }
         tmem_ld_wait();
         const float2 scale2 = make_float2(scale, scale);
-        const WideScales& of_step = scales[g % kPairScales];
+        const PairScales& of_step = scales[g % kPairScales];
         wait(bar_t + 8 * (g % kPairScales), g / kPairScales);
 #pragma unroll
         for (int i = 0; i < 64; i += 4) {                    // S' (a NaN entry's is NaN)
@@ -443,20 +447,19 @@ tree_pair_kernel(const TreeArgs a) {
         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          uint32_t p[16], inverse[16];
+          uint32_t p[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 q = *reinterpret_cast<const uint4*>(&of_step.v_inverse[32 * w + 8 * i]);
-            inverse[4 * i] = q.x; inverse[4 * i + 1] = q.y; inverse[4 * i + 2] = q.z; inverse[4 * i + 3] = q.w;
-          }
+          for (int i = 0; i < 16; i += 2) {
+            const float4 inverse = *reinterpret_cast<const float4*>(&of_step.v_inverse[32 * w + 2 * i]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = add2(make_float2(__uint_as_float(v[w][2 * i]), __uint_as_float(v[w][2 * i + 1])), low2);
-            e.x = exp2_approx(e.x);
-            e.y = exp2_approx(e.y);
-            sums[i & 1] = fma2(e, make_float2(bf_lo(inverse[i]), bf_hi(inverse[i])), sums[i & 1]);
-            const __half2 h = __floats2half2_rn(e.x, e.y);
-            p[i] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int n = 0; n < 2; ++n) {
+              float2 e = add2(make_float2(__uint_as_float(v[w][2 * (i + n)]), __uint_as_float(v[w][2 * (i + n) + 1])), low2);
+              e.x = exp2_approx(e.x);
+              e.y = exp2_approx(e.y);
+              sums[n] = fma2(e, n ? make_float2(inverse.z, inverse.w) : make_float2(inverse.x, inverse.y), sums[n]);
+              const __half2 h = __floats2half2_rn(e.x, e.y);
+              p[i + n] = *reinterpret_cast<const uint32_t*>(&h);
+            }
           }
           tmem_st16(s_at + 16 * w, p);                       // (over scores that have been read)
         }
