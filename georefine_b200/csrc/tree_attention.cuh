@@ -27,11 +27,20 @@ constexpr uint32_t kTreeRowAbsent = 0xFFFFFFFFu;             // row_parts of a r
 // Positions of a wide tile's unit: the most, for long contexts (a unit's result is as large as 256 positions of an 8-bit cache); fewer
 // for short ones and for runs of one or two tiles, whose few units would leave SMs idle.  1024 instead of 2048 behind 8192 positions,
 // 8 bits, 40 heads of 8: one run of 16 rows 35 us instead of 51, 16 runs 120 instead of 138; 16 runs of 64 rows (three tiles) 337
-// instead of 320, which keep 2048.  (4 bits: never fewer than a part of the narrow kernel has, for as many parts there is room.)
+// instead of 320, which keep 2048.  (4 bits: no more parts than the narrow kernel's, for as many there is room; parts of one size: 384 prompt rows behind 8000
+// positions 126 us instead of 134, the trees of three tiles 340 instead of 346, which would take 332 with 2048, and leave half of
+// the SMs idle where one of them is alone.)
 constexpr uint32_t kWideMostPart = 2048;
 template <int FORMAT>
 __device__ __forceinline__ uint32_t wide_part(uint32_t extent, bool many) {
-  return extent <= 1024 && FORMAT != kKvQ4 ? 256u : extent <= 4096 ? 512u : extent <= 16384 && !many ? 1024u : kWideMostPart;
+  const uint32_t part = extent <= 1024 && FORMAT != kKvQ4 ? 256u : extent <= 4096 ? 512u : extent <= 16384 && !many ? 1024u : kWideMostPart;
+  if constexpr (FORMAT == kKvQ4) {
+    // as many parts as come nearest to that (of the largest: as there have to be), all of them alike: a last part of one step costs a unit's beginning and end and
+    // a partial result like the others
+    const uint32_t parts = part == kWideMostPart ? (extent + part - 1) / part : (extent + part / 2) / part, each = (extent + max(parts, 1u) - 1) / max(parts, 1u);
+    return (max(each, 1u) + 63u) & ~63u;
+  }
+  return part;
 }
 
 struct TreeArgs {

@@ -259,6 +259,45 @@ def test_a_captured_step_replayed_on_new_inputs_and_two_streams(dev):
         s.check(inputs[r], [r], [int(pos[r])], outs[r], causal([int(pos[r])]))
 
 
+def test_runs_of_the_wide_kernel_without_anything_to_do(dev):
+    """Whole tiles of rows that are left out or see nothing, before, between and behind others."""
+    s = Setup(dev, 10, 2, [0, 300, 20, 40], 3)
+    seq = [-1] * 70 + [1] * 66 + [-1] * 130 + [2] * 3 + [0] * 64
+    pos = [5] * 70 + [300 + i for i in range(66)] + [700] * 130 + [20, 21, 22] + list(range(64))
+    rows = len(seq)
+    qkv, out = s.qkv(rows), torch.full((rows, 1280), 5.0, device=dev, dtype=BF)
+    attn = s.attention(rows)
+    attn(qkv, s.cos, s.sin, i32(seq, dev), i32(pos, dev), s.table, s.pages, out, longest_run=130)
+    keep = [r for r in range(rows) if seq[r] >= 0]
+    absent = [r for r in range(rows) if seq[r] < 0]
+    assert attn.check_status() == 0 and bool((out[absent] == 5.0).all())
+    s.check(qkv, seq, pos, out, causal(pos), rows=[keep[i] for i in (0, 1, 40, 65, 66, 68, 69, 100, 132)])
+    # nodes of trees that see nothing: 60 of one, all of another
+    seq, pos = [1] * 64 + [3] * 20, [300 + i for i in range(64)] + [40 + i for i in range(20)]
+    base, mask = [300] * 2 + [0] * 60 + [300] * 2 + [0] * 20, [[1], [3]] + [[0]] * 60 + [[1 << 62 | 1], [3 << 62 | 1]] + [[0]] * 20
+    rows = len(seq)
+    qkv, out = s.qkv(rows), torch.full((rows, 1280), 5.0, device=dev, dtype=BF)
+    attn = s.attention(rows)
+    attn(qkv, s.cos, s.sin, i32(seq, dev), i32(pos, dev), s.table, s.pages, out, tree=s.ops.TreeRows(i32(base, dev), i32(pos, dev), _masks([[m if m < 1 << 63 else m - (1 << 64) for m in x] for x in mask], dev)))
+    assert attn.check_status() == 0 and bool((out[2:62] == 0).all()) and bool((out[64:] == 0).all())
+    s.check(qkv, seq, pos, out, _seen(base, mask), pos, rows=[0, 1, 62, 63])
+
+
+@pytest.mark.parametrize("rows,before", [(66, 4031), (66, 4032), (70, 9000), (150, 4100), (66, 16400)])
+def test_prompt_rows_behind_long_contexts(dev, rows, before):
+    """Parts of every size, of which a tile's last may be short; a run by itself has the same bits."""
+    s = Setup(dev, 5, 1, [before, 100], -(-(before + rows) // 256), seed=rows)
+    seq, pos = [0] * rows + [1] * 64, list(range(before, before + rows)) + list(range(100, 164))
+    qkv, out = s.qkv(rows + 64), torch.full((rows + 64, 640), float("nan"), device=dev, dtype=BF)
+    attn = s.attention(rows + 64)
+    attn(qkv, s.cos, s.sin, i32(seq, dev), i32(pos, dev), s.table, s.pages, out, longest_run=rows)
+    assert attn.check_status() == 0
+    s.check(qkv, seq, pos, out, causal(pos), rows=[0, rows // 2, rows - 1, rows, rows + 63])
+    alone = torch.empty(rows, 640, device=dev, dtype=BF)
+    attn(qkv[:rows], s.cos, s.sin, i32(seq[:rows], dev), i32(pos[:rows], dev), s.table, s.pages, alone, longest_run=rows)
+    assert torch.equal(alone, out[:rows])
+
+
 def test_long_contexts_and_many_units_a_cta(dev):
     """Runs of units over several sequences, parts and heads, one and two blocks of columns."""
     lengths = [3000 + 37 * i for i in range(12)]
