@@ -11,12 +11,12 @@
 // no more, so nobody may be a round ahead of one who still waits, and nobody waits for a phase whose predecessor is open: everybody waits for every step in turn,
 // and the loaders for the products of the step whose place they take.  (Schedules of all roles in any order, run on the CPU, end and mistake no phase.)
 //
-// No single unit bounds it.  A step of two full tiles takes 3400 cycles: the products 1380 (two of S at 434 - the queries are read again for every 64 positions -
-// and two of O at 257), shared memory 2700 (the products 1024, the weights' reads of exponents 1030, the loaders' stores 290), the schedulers 1800 each, exp2 1024;
-// a unit's end and beginning - the partial results, the next queries - add 4000.  384 prompt rows behind 8000 positions, 40 heads of 8: 142 us, 455 TFLOP/s;
-// 16 trees of 64 nodes behind 8192: 383, of which 330 are this kernel.  (A CTA of 128 rows of its own, two an SM, each decoding K and V for itself: 153 and 356 -
-// better where half of a run's pairs have one tile, as these trees' do.  Two threads a row: the same; four threads for both tiles' rows at a time, whose
-// exponents they read once: 184 and 458; exponents in 16 bits, 40 % fewer reads: 147 and 396.)
+// No single unit bounds it.  A step of two full tiles takes 3100 cycles: the warps that turn scores into weights work 2400 of them, at an instruction in five cycles or
+// so each; the products 1380 (two of S at 434 - the queries are read again for every 64 positions - and two of O at 257), shared memory 2800 (the products 1024, the rest
+// mostly exponents that the weights' warps read), exp2 1024.  384 prompt rows behind 8000 positions, 40 heads of 8: 126 us, 510 TFLOP/s; 16 trees of 64 nodes
+// behind 8192: 340, of which 290 are this kernel.  What lies between units was dear: the queries' addresses with a division each kept a unit waiting for 4500 cycles (142
+// and 381).  (Two threads a row: 4 % slower; four threads for both tiles' rows at a time, whose exponents they read once: 40 %; weights by the reference as it is,
+// in one pass over the columns, done again where it moves: 17 %; K's exponents in the operands as far as they differ: 3 and 11 %.)
 #pragma once
 #include "tree_q4.cuh"
 #include "tree_wide.cuh"
