@@ -131,8 +131,9 @@ __device__ __forceinline__ T cta_scan(T v, T* scratch /* warps */, Op op) {
   return warp ? op(before, v) : v;
 }
 
-// Weight of a unit of so many positions in the 4-bit kernel: its steps of 128 positions, and a step's time for its beginning and end.
-__device__ __forceinline__ uint32_t tree_q4_weight(uint32_t positions) { return (positions + 127) / 128 + 1; }
+// Weight of a unit of so many positions in the 4-bit kernel: its steps of 128 positions, 2350 cycles each, and three more, for 6600 that its beginning and end take (with one:
+// 1 row behind 2048 17.8 us instead of 15.7, 128 rows 78.9 instead of 77.1).
+__device__ __forceinline__ uint32_t tree_q4_weight(uint32_t positions) { return (positions + 127) / 128 + 3; }
 
 // A tile is up to tile_rows (wide_rows) consecutive rows of one sequence; rows that are left out or see nothing may be among them.
 // What it needs of the rows is read once, side by side; the rest runs in shared memory.

@@ -11,8 +11,9 @@
 // A code becomes an FP16 operand with 1.1 instructions (q4_operands).  A group's scale goes into the operand, where it is exact; K's exponent
 // multiplies the score of its position, V's goes into the weight, as in 8 bits: S' = S 2^e_k scale + e_v, and the sum of the weights takes it out again.
 //
-// Instructions bound it: 740 for 32 positions of a head, of which 288 make operands of codes and 32 are the products, and the four warps of a scheduler issue in
-// 57 % of the cycles.  128 rows behind 2048 positions each, 40 heads of 8 (220 MB): 70 us, 3.1 TB/s, where the 8-bit cache takes 100 with 410 MB; 8 rows behind
+// Instructions bound it, and the chains between them: 560 for 32 positions of a head, of which 288 make operands of codes and 32 are the products; the four warps of a
+// scheduler issue in 57 % of the cycles.  A third of a warp's time goes to units' beginnings and ends - the next one found, its columns, the merge.  128 rows
+// behind 2048 positions each, 40 heads of 8 (220 MB): 69 us, 3.2 TB/s, where the 8-bit cache takes 100 with 410 MB; 8 rows behind
 // 32768: 70.  (Heads as rows of the products, as in 8 bits, would fill five rows of sixteen with twice the operands; a warp's four chunks written out one after
 // another no longer fit the instruction cache: 84.)
 #pragma once
