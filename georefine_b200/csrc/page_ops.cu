@@ -37,7 +37,13 @@ int own_table_of(const grb_kv_table* t) {
   if (!t || !t->table || !t->slots || !t->max_pages || t->ld < int64_t(t->max_pages)) return GRB_ERR_ARGUMENT;
   return t->max_pages > 0x7FFFFFu || t->slots > 0x7FFFFFFFu ? GRB_ERR_UNSUPPORTED : GRB_OK;
 }
-bool layers_fit(const KvPagesArgs& p) { return parts_of(p) <= 0x7FFFFFFFull; }
+// What whole pages are copied in: pieces of 16 bytes, numbered in 31 bits.  (What goes by entries moves exponents byte by byte, and takes layers of
+// them that lie any distance apart.)
+int copied_pages_of(const grb_kv_pages* pages, KvPagesArgs& a) {
+  if (int st = pages_of(pages, a)) return st;
+  if (pages->format == GRB_KV_E4M3 && pages->layers > 1 && (pages->exp_stride & 15)) return GRB_ERR_ARGUMENT;
+  return parts_of(a) <= 0x7FFFFFFFull ? GRB_OK : GRB_ERR_UNSUPPORTED;
+}
 
 template <class T, int V, bool HALF>
 int rotary_launch(RotaryArgs a, bool copy, cudaStream_t stream) {
@@ -107,9 +113,8 @@ int grb_rotary(const grb_rotary_step* s, void* cuda_stream) {
 
 int grb_kv_copy(const grb_kv_pages* pages, const int32_t* src, const int32_t* dst, const int32_t* positions, uint32_t n, void* cuda_stream) {
   KvCopyArgs a{};
-  if (int st = pages_of(pages, a.pages)) return st;
+  if (int st = copied_pages_of(pages, a.pages)) return st;
   if (!src || !dst) return GRB_ERR_ARGUMENT;
-  if (!layers_fit(a.pages)) return GRB_ERR_UNSUPPORTED;
   if (!n) return GRB_OK;
   a.src = src;
   a.dst = dst;
@@ -121,10 +126,9 @@ int grb_kv_copy(const grb_kv_pages* pages, const int32_t* src, const int32_t* ds
 int grb_kv_fork(const grb_kv_pages* pages, const grb_kv_table* table, const int32_t* parents, const int32_t* children, const int32_t* lengths, const int32_t* fresh,
                 int32_t* refs, int32_t empty, uint32_t n, void* cuda_stream) {
   KvForkArgs a{};
-  if (int st = pages_of(pages, a.pages)) return st;
+  if (int st = copied_pages_of(pages, a.pages)) return st;
   if (int st = own_table_of(table)) return st;
   if (!parents || !children || !lengths || !fresh || !refs) return GRB_ERR_ARGUMENT;
-  if (!layers_fit(a.pages)) return GRB_ERR_UNSUPPORTED;
   if (!n) return GRB_OK;
   a.table = const_cast<int32_t*>(table->table);
   a.ld = table->ld;
@@ -157,10 +161,9 @@ uint64_t grb_kv_compact_scratch_bytes(uint32_t pages) { return 16 + uint64_t(pag
 
 int grb_kv_compact(const grb_kv_pages* pages, const grb_kv_table* table, int32_t* refs, int32_t* where, int32_t* used, void* scratch, uint64_t scratch_bytes, void* cuda_stream) {
   KvCopyArgs moves{};
-  if (int st = pages_of(pages, moves.pages)) return st;
+  if (int st = copied_pages_of(pages, moves.pages)) return st;
   if (int st = own_table_of(table)) return st;
   if (!refs || !where || !used || !scratch || !aligned16(scratch)) return GRB_ERR_ARGUMENT;
-  if (!layers_fit(moves.pages)) return GRB_ERR_UNSUPPORTED;
   if (scratch_bytes < grb_kv_compact_scratch_bytes(pages->pages)) return GRB_ERR_WORKSPACE;
   KvCompactArgs a{const_cast<int32_t*>(table->table), table->ld, table->slots, table->max_pages, pages->pages, refs, where, used, static_cast<int32_t*>(scratch), nullptr, nullptr};
   a.src = a.moves + 4;

@@ -157,7 +157,8 @@ class KVPages:
     """Keys and values of one layer, [pages, kv heads, 256, 128], or of a stack of layers ([layers, pages, ...], layers may be
     strided): BF16, or ``float8_e4m3fn`` codes with an exponent byte per entry (128 values of one head at one position) in
     ``k_exp`` and ``v_exp``, [pages, kv heads, 256].  In 4 bits (``"q4"``: 69 bytes for an entry of 256) pages are ``uint8`` [pages, kv heads,
-    69, 256] and hold codes, scales and exponents together.  The formats are in ``csrc/kv_cache.cuh``.  An object holds no copies."""
+    69, 256] and hold codes, scales and exponents together.  Where whole pages are copied, layers of exponents lie a multiple of 16 bytes
+    apart.  The formats are in ``csrc/kv_cache.cuh``.  An object holds no copies."""
 
     def __init__(self, k, v, k_exp=None, v_exp=None):
         import torch
@@ -285,11 +286,18 @@ def _empty(empty):
     return int(empty)
 
 
+def _whole_pages(pages):
+    """Refuses exponents that cannot be moved in pieces of 16 bytes."""
+    if pages.k_exp is not None and pages.stacked and pages.k_exp.shape[0] > 1 and pages.k_exp.stride(0) % 16:
+        raise ValueError("exponents of keys and values: where whole pages are copied, layers lie a multiple of 16 bytes apart")
+
+
 def kv_copy(src, dst, pages, *, positions=None):
     """Entries of page ``src[i]`` to page ``dst[i]`` (int32 vectors), keys and values, in every layer of ``pages``: all 256, or the first
     ``positions[i]``.  A page of -1 is left out; no page is a destination twice, or a source and a destination."""
     n, device = src.shape[0], pages.device
     args = _vector(src, device, "src"), _vector(dst, device, "dst", n), 0 if positions is None else _vector(positions, device, "positions", n)
+    _whole_pages(pages)
     if n:
         _launch(device, "grb_kv_copy", pages._packed, *args, n)
 
@@ -303,6 +311,7 @@ def kv_fork(parents, children, lengths, fresh, page_table, refs, pages, *, empty
     n, device = parents.shape[0], pages.device
     args = _native.KV_TABLE.pack(*_table(page_table, device)), _vector(parents, device, "parents"), *(
         _vector(t, device, what, n) for t, what in ((children, "children"), (lengths, "lengths"), (fresh, "fresh"))), _refs(refs, pages), _empty(empty)
+    _whole_pages(pages)
     if n:
         _launch(device, "grb_kv_fork", pages._packed, *args, n)
 
@@ -333,6 +342,7 @@ def kv_compact(page_table, refs, pages, where, used, *, scratch=None):
     _on(scratch, device, torch.uint8, "scratch")
     if not scratch.is_contiguous():
         raise ValueError("scratch has to be contiguous")
+    _whole_pages(pages)
     _launch(device, "grb_kv_compact", pages._packed, *args, scratch.data_ptr(), scratch.numel())
 
 

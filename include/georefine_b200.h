@@ -517,6 +517,8 @@ typedef struct grb_rotary_step {
 } grb_rotary_step;
 int grb_rotary(const grb_rotary_step* step, void* cuda_stream);
 
+/* Whole pages (grb_kv_copy, grb_kv_fork, grb_kv_compact) move in pieces of 16 bytes: of more than one GRB_KV_E4M3 layer, exp_stride has to be a
+ * multiple of 16. */
 /* Entries of page src[i] to page dst[i], in all layers, keys and values: the first positions[i] of them (NULL: all 256).  A page outside the pool, or
  * one onto itself, is left out; no page may be a destination twice, or a source and a destination. */
 int grb_kv_copy(const grb_kv_pages* pages, const int32_t* src, const int32_t* dst, const int32_t* positions, uint32_t n, void* cuda_stream);
