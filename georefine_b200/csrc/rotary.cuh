@@ -4,9 +4,9 @@
 // paired (i, i + turned / 2) or (2 i, 2 i + 1); the rest is left as it is (copied, where the result goes elsewhere).  Backward: the same, turned the other
 // way.
 //
-// An angle is exact however far the position: a frequency is held as the 64-bit fraction of a turn that one position adds, the product with the
-// position wraps where whole turns do, and its upper 32 bits are the angle to 2^-32 of a turn.  (In FP32 a million times one radian is off by
-// 0.03.)  Values and sums are FP32, rounded once.
+// A frequency is held as the fraction of a turn that one position adds, to the nearest 2^-64; its product with the position is exact and wraps where
+// whole turns do, and the upper 32 bits are the angle: off by 2^-32 of a turn, and 2^-65 for every position - as much again at 2^33, 2^-25 at 2^40.
+// (In FP32 a million times one radian is off by 0.03.)  Values and sums are FP32, rounded once.
 //
 // Memory bounds it: a value is read and written once.  A thread takes a piece of four neighbouring heads of a row; their loads are on their way while
 // it works the piece's angles out, for itself: shared by the heads of a row through shared memory, they kept the row's loads and stores

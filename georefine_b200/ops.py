@@ -14,7 +14,9 @@ reference has no counterparts.
 from __future__ import annotations
 
 import ctypes
+import decimal
 import math
+from decimal import Decimal
 
 from . import _native
 
@@ -356,6 +358,8 @@ def kv_compact_scratch_bytes(pages) -> int:
 ROPE_LAYOUTS = ("half", "interleaved")
 _ROPE_KEYS = {"linear": ("factor",), "ntk": ("factor",), "yarn": ("factor", "original"), "bands": ("factor", "original", "low", "high")}
 _ROPE_MORE = {"yarn": {"fast": 32.0, "slow": 1.0, "attention": None}}
+_ROPE_DIGITS = decimal.Context(prec=60)
+_PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
 
 
 def rope_frequencies(dim: int, theta: float = 1e4, scaling=None):
@@ -367,6 +371,12 @@ def rope_frequencies(dim: int, theta: float = 1e4, scaling=None):
         trained context stay, those that turn ``slow`` times or fewer are slower by the factor, between the pairs' numbers it is a ramp; both
         components are multiplied by ``attention``, 0.1 ln(factor) + 1 where it is None (Peng et al., 2023);
       kind "bands", factor, original, low, high: the same with the ramp over the turns themselves, between ``low`` and ``high``, and no factor."""
+    frequencies, factor = _rope_frequencies(dim, theta, scaling)
+    return [float(f) for f in frequencies], factor
+
+
+def _rope_frequencies(dim, theta, scaling):
+    """``rope_frequencies`` to 60 digits: a position of millions multiplies what its frequency is off by."""
     if dim < 2 or dim % 2:
         raise ValueError("the turned dimensions are an even number of two or more")
     if not 0 < theta < float("inf"):
@@ -383,29 +393,33 @@ def rope_frequencies(dim: int, theta: float = 1e4, scaling=None):
             raise ValueError("the numbers of a scaling are positive")
     elif given:
         raise ValueError("a scaling has a kind")
-    if kind == "ntk" and dim > 2:
-        theta = theta * given["factor"] ** (dim / (dim - 2))
-    inv = [theta ** (-2 * i / dim) for i in range(dim // 2)]
-    if kind == "linear":
-        return [f / given["factor"] for f in inv], 1.0
-    if kind == "yarn":
-        if theta == 1 or given["fast"] <= given["slow"]:
-            raise ValueError("yarn needs a theta other than 1 and fast above slow")
-        number = lambda turns: dim / 2 * math.log(given["original"] / (2 * math.pi * turns)) / math.log(theta)
-        lo, hi = max(math.floor(number(given["fast"])), 0), min(math.ceil(number(given["slow"])), dim - 1)
-        slow = [min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0) for i in range(dim // 2)]
-        return [f / given["factor"] * s + f * (1 - s) for f, s in zip(inv, slow)], 0.1 * math.log(given["factor"]) + 1 if given["attention"] is None else float(given["attention"])
-    if kind == "bands":
-        if given["low"] >= given["high"]:
-            raise ValueError("low lies below high")
-        keep = [min(max((given["original"] * f / (2 * math.pi) - given["low"]) / (given["high"] - given["low"]), 0.0), 1.0) for f in inv]
-        return [f / given["factor"] * (1 - k) + f * k for f, k in zip(inv, keep)], 1.0
-    return inv, 1.0
+    if kind == "yarn" and (theta == 1 or given["fast"] <= given["slow"]):
+        raise ValueError("yarn needs a theta other than 1 and fast above slow")
+    if kind == "bands" and given["low"] >= given["high"]:
+        raise ValueError("low lies below high")
+    with decimal.localcontext(_ROPE_DIGITS):
+        number = {name: None if v is None else Decimal(float(v)) for name, v in given.items()}
+        base, factor, attention = Decimal(float(theta)).ln(), number.get("factor"), 1.0
+        if kind == "ntk" and dim > 2:
+            base += factor.ln() * dim / (dim - 2)
+        inv = [(base * (-2 * i) / dim).exp() for i in range(dim // 2)]
+        if kind == "linear":
+            inv = [f / factor for f in inv]
+        elif kind == "yarn":
+            pair = lambda turns: (number["original"] / (2 * _PI * turns)).ln() / base * dim / 2
+            lo, hi = max(math.floor(pair(number["fast"])), 0), min(math.ceil(pair(number["slow"])), dim - 1)
+            slow = [min(max((i - lo) / max(Decimal(hi - lo), Decimal("0.001")), Decimal(0)), Decimal(1)) for i in range(dim // 2)]
+            inv = [f / factor * s + f * (1 - s) for f, s in zip(inv, slow)]
+            attention = 0.1 * math.log(given["factor"]) + 1 if given["attention"] is None else float(given["attention"])
+        elif kind == "bands":
+            keep = [min(max((number["original"] * f / (2 * _PI) - number["low"]) / (number["high"] - number["low"]), Decimal(0)), Decimal(1)) for f in inv]
+            inv = [f / factor * (1 - k) + f * k for f, k in zip(inv, keep)]
+    return inv, attention
 
 
 class Rope:
     """Rotary positions of the first ``dim`` dimensions of a head: pairs (i, i + dim / 2) (``layout`` "half") or (2 i, 2 i + 1)
-    ("interleaved"), frequencies by ``theta`` and ``scaling`` (``rope_frequencies``), held on the device as 64-bit fractions of a turn."""
+    ("interleaved"), frequencies by ``theta`` and ``scaling`` (``rope_frequencies``), held on the device as the nearest 64-bit fractions of a turn."""
 
     def __init__(self, dim: int, theta: float = 1e4, *, layout="half", scaling=None, device="cuda:0"):
         import torch
@@ -413,8 +427,10 @@ class Rope:
         if layout not in ROPE_LAYOUTS:
             raise ValueError(f"the layout is one of {ROPE_LAYOUTS}")
         self.dim, self.layout = int(dim), layout
-        self.frequencies, self.factor = rope_frequencies(self.dim, theta, scaling)
-        turns = [round(f / (2 * math.pi) * 2.0 ** 64) % (1 << 64) for f in self.frequencies]
+        frequencies, self.factor = _rope_frequencies(self.dim, theta, scaling)
+        self.frequencies = [float(f) for f in frequencies]
+        with decimal.localcontext(_ROPE_DIGITS):
+            turns = [round(f / (2 * _PI) * (1 << 64)) % (1 << 64) for f in frequencies]
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64).to(device)
         self.device = self.turns.device
 
@@ -431,8 +447,8 @@ class Rope:
 
 def rotary(x, positions, rope, *, out=None, backward=False):
     """Turns the first ``rope.dim`` dimensions of every head of ``x`` ([rows, heads, head dim] BF16, FP16 or FP32; rows and heads may be any distance apart) by
-    ``positions`` (int32 or int64 [rows]), into ``out`` or, without it, in place.  Angles are exact for positions of any size; a value is rounded
-    once.  ``backward``: turned the other way - the gradient of the call, given that of its result, and where ``rope.factor`` is 1 its inverse."""
+    ``positions`` (int32 or int64 [rows]), into ``out`` or, without it, in place.  An angle is off by 2^-32 of a turn at most, and 2^-65 of one for
+    every position (2^-25 at 2^40); a value is rounded once.  ``backward``: turned the other way - the gradient of the call, given that of its result, and where ``rope.factor`` is 1 its inverse."""
     import torch
 
     device = rope.device
