@@ -369,7 +369,7 @@ def rope_frequencies(dim: int, theta: float = 1e4, scaling=None):
       kind "ntk", factor: theta factor^(dim / (dim - 2)), under which the slowest pair is slower by the factor and the fastest as it was;
       kind "yarn", factor, original (the trained context), fast=32, slow=1, attention=None: pairs that turn ``fast`` times or more within the
         trained context stay, those that turn ``slow`` times or fewer are slower by the factor, between the pairs' numbers it is a ramp; both
-        components are multiplied by ``attention``, 0.1 ln(factor) + 1 where it is None (Peng et al., 2023);
+        components are multiplied by ``attention``, where it is None 0.1 ln(factor) + 1, and 1 for a factor below one (Peng et al., 2023);
       kind "bands", factor, original, low, high: the same with the ramp over the turns themselves, between ``low`` and ``high``, and no factor."""
     frequencies, factor = _rope_frequencies(dim, theta, scaling)
     return [float(f) for f in frequencies], factor
@@ -410,7 +410,7 @@ def _rope_frequencies(dim, theta, scaling):
             lo, hi = max(math.floor(pair(number["fast"])), 0), min(math.ceil(pair(number["slow"])), dim - 1)
             slow = [min(max((i - lo) / max(Decimal(hi - lo), Decimal("0.001")), Decimal(0)), Decimal(1)) for i in range(dim // 2)]
             inv = [f / factor * s + f * (1 - s) for f, s in zip(inv, slow)]
-            attention = 0.1 * math.log(given["factor"]) + 1 if given["attention"] is None else float(given["attention"])
+            attention = 0.1 * math.log(max(given["factor"], 1.0)) + 1 if given["attention"] is None else float(given["attention"])
         elif kind == "bands":
             keep = [min(max((number["original"] * f / (2 * _PI) - number["low"]) / (number["high"] - number["low"]), Decimal(0)), Decimal(1)) for f in inv]
             inv = [f / factor * (1 - k) + f * k for f, k in zip(inv, keep)]

@@ -1,0 +1,17 @@
+"""Scalings of rotary positions at the edges of their rules.  No GPU."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from georefine_b200 import ops  # noqa: E402
+
+
+@pytest.mark.parametrize("factor,want", [(0.25, 1.0), (0.999, 1.0), (1.0, 1.0), (1.5, 0.1 * math.log(1.5) + 1), (32.0, 0.1 * math.log(32.0) + 1)])
+def test_yarn_leaves_components_as_they_are_where_a_context_is_not_extended(factor, want):
+    """The factor on both components grows with the extension, from 1 on: a shorter context takes none."""
+    scaling = {"kind": "yarn", "factor": factor, "original": 4096}
+    assert math.isclose(ops.rope_frequencies(64, 1e4, scaling)[1], want, rel_tol=1e-15)
+    assert math.isclose(ops.Rope(64, 1e4, scaling=scaling, device="cpu").factor, want, rel_tol=1e-15)
+    assert ops.rope_frequencies(64, 1e4, {**scaling, "attention": 0.75})[1] == 0.75
