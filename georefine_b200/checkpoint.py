@@ -62,7 +62,11 @@ def decoder_config(config, **overrides):
                       rope_theta=float(config.get("rope_theta", 10000.0)), eps=float(config.get("rms_norm_eps", 1e-6)))
     except (KeyError, TypeError, ValueError) as exc:
         raise ContextServingError(f"model config lacks a decoder field: {exc}") from exc
-    fields.update(_rotary_fields(config, fields["head_dim"]))
+    try:
+        fields.update(_rotary_fields(config, fields["head_dim"]))
+        DecoderConfig(**{name: value for name, value in fields.items() if name == "head_dim" or name.startswith("rope")})       # (refuses what no rotary positions can be)
+    except (TypeError, ValueError) as exc:
+        raise ContextServingError(f"unsupported rotary positions: {exc}") from exc
     for flag in ("attention_bias", "mlp_bias"):
         if config.get(flag):
             raise ContextServingError(f"unsupported decoder family: {flag} is set")
@@ -92,7 +96,8 @@ def _rotary_fields(config, head_dim):
             scaling = {"kind": "linear", "factor": float(given.pop("factor"))}
         elif kind == "yarn":
             scaling = {"kind": "yarn", "factor": float(given.pop("factor")), "original": float(original), "fast": float(given.pop("beta_fast", None) or 32.0),
-                       "slow": float(given.pop("beta_slow", None) or 1.0), "attention": given.pop("attention_factor", None)}
+                       "slow": float(given.pop("beta_slow", None) or 1.0), "attention": None if given.get("attention_factor") is None else float(given["attention_factor"])}
+            given.pop("attention_factor", None)
         elif kind == "default":
             scaling = None
         else:
