@@ -98,6 +98,8 @@ def _rotary_fields(config, head_dim):
             scaling = {"kind": "yarn", "factor": float(given.pop("factor")), "original": float(original), "fast": float(given.pop("beta_fast", None) or 32.0),
                        "slow": float(given.pop("beta_slow", None) or 1.0), "attention": None if given.get("attention_factor") is None else float(given["attention_factor"])}
             given.pop("attention_factor", None)
+            if given.get("truncate") is True:     # (the ramp's ends are whole numbers)
+                del given["truncate"]
         elif kind == "default":
             scaling = None
         else:

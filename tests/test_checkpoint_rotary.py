@@ -25,3 +25,17 @@ def test_numbers_that_mean_nothing_are_refused_as_the_checkpoint_s(given):
 def test_an_override_is_the_caller_s_mistake():
     with pytest.raises(ValueError):
         checkpoint.decoder_config(BASE, tp_world=3)
+
+
+@pytest.mark.parametrize("truncate", [True, None])
+def test_whole_numbers_at_the_ends_of_yarn_s_ramp_may_be_asked_for(truncate):
+    """They are what the ramp has anyway; a ramp between broken numbers is another one."""
+    plain = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 2048}
+    cfg = checkpoint.decoder_config({**BASE, "rope_scaling": {**plain, "truncate": truncate}})
+    assert cfg.rope_options == checkpoint.decoder_config({**BASE, "rope_scaling": plain}).rope_options
+
+
+@pytest.mark.parametrize("scaling", [{"rope_type": "yarn", "factor": 4.0, "truncate": False}, {"rope_type": "linear", "factor": 4.0, "truncate": True}])
+def test_other_ends_of_a_ramp_are_refused(scaling):
+    with pytest.raises(ContextServingError):
+        checkpoint.decoder_config({**BASE, "rope_scaling": scaling})
