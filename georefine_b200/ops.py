@@ -389,7 +389,7 @@ def _rope_frequencies(dim, theta, scaling):
         given = {**_ROPE_MORE.get(kind, {}), **given}
         if set(given) != {*_ROPE_KEYS[kind], *_ROPE_MORE.get(kind, {})}:
             raise ValueError(f"scaling {kind!r} takes {(*_ROPE_KEYS[kind], *_ROPE_MORE.get(kind, {}))}")
-        if any(not 0 < v < float("inf") for v in given.values() if v is not None):
+        if any(v is None or not 0 < v < float("inf") for name, v in given.items() if v is not None or name != "attention"):
             raise ValueError("the numbers of a scaling are positive")
     elif given:
         raise ValueError("a scaling has a kind")

@@ -15,3 +15,14 @@ def test_yarn_leaves_components_as_they_are_where_a_context_is_not_extended(fact
     assert math.isclose(ops.rope_frequencies(64, 1e4, scaling)[1], want, rel_tol=1e-15)
     assert math.isclose(ops.Rope(64, 1e4, scaling=scaling, device="cpu").factor, want, rel_tol=1e-15)
     assert ops.rope_frequencies(64, 1e4, {**scaling, "attention": 0.75})[1] == 0.75
+
+
+@pytest.mark.parametrize("scaling", [{"kind": "linear", "factor": None}, {"kind": "ntk", "factor": None}, {"kind": "yarn", "factor": 4.0, "original": None}, {"kind": "yarn", "factor": 4.0, "original": 64, "slow": None},
+                                     {"kind": "bands", "factor": 2.0, "original": 64, "low": None, "high": 4.0}])
+def test_only_yarn_s_factor_on_components_may_be_left_open(scaling):
+    from georefine_b200 import serve
+
+    with pytest.raises(ValueError, match="positive"):
+        ops.rope_frequencies(64, 1e4, scaling)
+    with pytest.raises(ValueError, match="positive"):
+        serve.DecoderConfig(rope_scaling=scaling)
