@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import inspect
 import math
+import weakref
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -296,7 +297,7 @@ class BatchDecoder:
         # how many slots' places name a page; the same on the device, brought up to date where pages are shared or moved
         self._refs = np.zeros(n_pages, dtype=np.int32)
         self._refs_dev = self._stack = None
-        self.page_sets = []          # caches beside the stack's under the same page table, of one layer each (a draft head's)
+        self.page_sets = weakref.WeakSet()       # caches beside the stack's under the same page table, of one layer each (a draft head's, while there is one)
         self._tree_attn = self._status_host = None
         self.attn = self._pages = None
         if kv_format == "bf16":
@@ -1093,7 +1094,7 @@ class MTPHead:
         self.cache = ops.KVPages(self.kv[0], self.kv[1], *((None, None) if exps is None else exps)) if paged else None
         self.pages = None if getattr(d, "kv_format", "bf16") == "bf16" else self.cache
         if hasattr(d, "page_sets"):
-            d.page_sets.append(self.cache)
+            d.page_sets.add(self.cache)
         self.tok, self.hid = z(R, dtype=torch.int32), z(R, H)
         self.e, self.cat, self.z, self.x = z(R, H), z(R, 2 * H), z(R, H), z(R, H)
         self.qkv, self.ctx, self.o_out = z(R, cfg.qkv_rows), z(R, cfg.heads * cfg.head_dim), z(R, H)
