@@ -405,6 +405,7 @@ class BatchDecoder:
                 self.page_table[slot, p] = page
 
     def _take_page(self) -> int:
+        """A page for one slot.  (There are as many as all slots' places, and one that several places name leaves others free: the pool has one.)"""
         if not self._free_pages:
             raise RuntimeError("KV page pool exhausted")
         page = self._free_pages.pop()
@@ -443,8 +444,6 @@ class BatchDecoder:
             raise ValueError(f"slot {slot} does not hold {length} positions")
         if len(self._free_slots) < n:
             raise RuntimeError("no free sequence slot")
-        if rest and len(self._free_pages) < n:
-            raise RuntimeError("KV page pool exhausted")
         pool, refs = self._pool()
         children = [self.open_slot() for _ in range(n)]
         fresh = [self._take_page() if rest else -1 for _ in children]
@@ -469,8 +468,6 @@ class BatchDecoder:
                 moves.append((p, page, max(first - p * PAGE, 0)))
         if not moves:
             return
-        if len(self._free_pages) < len(moves):
-            raise RuntimeError("KV page pool exhausted")
         pool, _ = self._pool()
         fresh = [self._take_page() for _ in moves]
         src, dst, counts = self._vectors([page for _, page, _ in moves], fresh, [n for _, _, n in moves])
@@ -1275,13 +1272,8 @@ class MTPSpeculator:
         d, pos = self.b.d, self.b.active[slot]["pos"]
         d.ensure_pages(slot, pos)
         children = self.b.fork(slot, n)
-        try:
-            for c in children:
-                d.ensure_pages(c, pos)
-        except RuntimeError:
-            for c in children:
-                self.b.retire(c)
-            raise
+        for c in children:
+            d.ensure_pages(c, pos)
         page, rest = divmod(pos, PAGE)
         src, dst, counts = d._vectors([int(d._table_host[slot, page])] * n, [int(d._table_host[c, page]) for c in children], [rest + 1] * n)
         ops.kv_copy(src, dst, self.head.cache, positions=counts)
