@@ -12,7 +12,9 @@
 // of the entry, e = clamp(floor(log2(a / 7)) + 9, -40, 22), kept as e + 127; a group's scale F is the number nearest to (its max |x|) / 7 2^(24 - e)
 // among (16 + m) 2^k, m 0 .. 15, k 0 .. 11, kept as the byte 64 + 16 k + m; code = x / (F 2^(e - 24)) to the nearest (ties to even) in -7 .. 7;
 // value = code F 2^(e - 24).  Uniform steps, because the largest of 32 values is about two standard deviations: a normal entry is held to
-// 20.2 dB (e2m1 codes under the same scales: 19.9).  A nibble holds code + 8: nibbles masked out of a word are FP16 subnormals, so that one
+// 20.2 dB (e2m1 codes under the same scales: 19.9).  A value is off by g / 14 (1 + 1/32) at most, g the largest magnitude of its group, or by a / 28672, half of
+// the smallest scale, where that is more, or by 2^-61 under the smallest exponent; beyond 111104, the largest value, it is held as that.
+// A nibble holds code + 8: nibbles masked out of a word are FP16 subnormals, so that one
 // fused multiply-add makes two FP16 operands of them - u 2^-24 F - 8 F 2^-24, exact, as F is a whole number of at most 16 bits, five of them
 // significant, which is also why the scales stay in twelve binades.  The exponent keeps the operands of an entry near the top of that range
 // whatever its size, as in 8 bits.  A scale byte below 16 reads as byte / 8, so that memory of zeros reads as zeros.

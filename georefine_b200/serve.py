@@ -261,7 +261,7 @@ class BatchDecoder:
 
     ``kv_format`` "e4m3" holds the KV cache in 8 bits (129 bytes for an entry of 256, each value off by at most 2^-4 of
     itself), "q4" in 4 (69 bytes, each value off by a fourteenth of the largest of its 32 neighbours, give or take a thirtieth of
-    that); the formats are in ``csrc/kv_cache.cuh``."""
+    that, or by 1 / 28672 of the largest of its 128 where that is more; beyond 111104 it is held as that); the formats are in ``csrc/kv_cache.cuh``."""
 
     def __init__(self, weights: DecoderWeights, *, max_rows=128, max_slots=128, max_context=2304, device="cuda:0", kv_format="bf16"):
         import torch
