@@ -9,7 +9,7 @@
 // A unit is a pair of tiles and a part of the positions.  Where a run's last tile has no partner, the products' and the weights' warps of the other half go through
 // all waits and arrivals without anything between them.  Barriers of a step are numbered by the step modulo three.  A wait tells a phase from the one before it and
 // no more, so nobody may be a round ahead of one who still waits, and nobody waits for a phase whose predecessor is open: everybody waits for every step in turn,
-// and the loaders for the products of the step whose place they take.  (Schedules of all roles in any order, run on the CPU, end and mistake no phase.)
+// and the loaders for the products of the step whose place they take.  (tests/test_pair_schedule.py runs these waits and arrivals in any order.)
 //
 // No single unit bounds it.  A step of two full tiles takes 3100 cycles: the warps that turn scores into weights work 2400 of them, at an instruction in five cycles or
 // so each; the products 1380 (two of S at 434 - the queries are read again for every 64 positions - and two of O at 257), shared memory 2800 (the products 1024, the rest
