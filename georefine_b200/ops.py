@@ -358,7 +358,7 @@ def kv_compact_scratch_bytes(pages) -> int:
 ROPE_LAYOUTS = ("half", "interleaved")
 _ROPE_KEYS = {"linear": ("factor",), "ntk": ("factor",), "yarn": ("factor", "original"), "bands": ("factor", "original", "low", "high")}
 _ROPE_MORE = {"yarn": {"fast": 32.0, "slow": 1.0, "attention": None}}
-_ROPE_DIGITS = decimal.Context(prec=60)
+_ROPE_DIGITS = decimal.Context(prec=40)
 _PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
 
 
@@ -376,7 +376,7 @@ def rope_frequencies(dim: int, theta: float = 1e4, scaling=None):
 
 
 def _rope_frequencies(dim, theta, scaling):
-    """``rope_frequencies`` to 60 digits: a position of millions multiplies what its frequency is off by."""
+    """``rope_frequencies`` to 36 digits or more: a position of millions multiplies what its frequency is off by."""
     if dim < 2 or dim % 2:
         raise ValueError("the turned dimensions are an even number of two or more")
     if not 0 < theta < float("inf"):
@@ -402,17 +402,21 @@ def _rope_frequencies(dim, theta, scaling):
         base, factor, attention = Decimal(float(theta)).ln(), number.get("factor"), 1.0
         if kind == "ntk" and dim > 2:
             base += factor.ln() * dim / (dim - 2)
-        inv = [(base * (-2 * i) / dim).exp() for i in range(dim // 2)]
+        ratio, inv = (base * -2 / dim).exp(), [Decimal(1)]
+        while 2 * len(inv) < dim:
+            inv.append(inv[-1] * ratio)           # (off by 10^-39 a pair)
         if kind == "linear":
             inv = [f / factor for f in inv]
         elif kind == "yarn":
             pair = lambda turns: (number["original"] / (2 * _PI * turns)).ln() / base * dim / 2
             lo, hi = max(math.floor(pair(number["fast"])), 0), min(math.ceil(pair(number["slow"])), dim - 1)
-            slow = [min(max((i - lo) / max(Decimal(hi - lo), Decimal("0.001")), Decimal(0)), Decimal(1)) for i in range(dim // 2)]
+            width = max(Decimal(hi - lo), Decimal("0.001"))
+            slow = [min(max((i - lo) / width, 0), 1) for i in range(dim // 2)]
             inv = [f / factor * s + f * (1 - s) for f, s in zip(inv, slow)]
             attention = 0.1 * math.log(max(given["factor"], 1.0)) + 1 if given["attention"] is None else float(given["attention"])
         elif kind == "bands":
-            keep = [min(max((number["original"] * f / (2 * _PI) - number["low"]) / (number["high"] - number["low"]), Decimal(0)), Decimal(1)) for f in inv]
+            turns, width = number["original"] / (2 * _PI), number["high"] - number["low"]
+            keep = [min(max((f * turns - number["low"]) / width, 0), 1) for f in inv]
             inv = [f / factor * (1 - k) + f * k for f, k in zip(inv, keep)]
     return inv, attention
 
@@ -430,7 +434,8 @@ class Rope:
         frequencies, self.factor = _rope_frequencies(self.dim, theta, scaling)
         self.frequencies = [float(f) for f in frequencies]
         with decimal.localcontext(_ROPE_DIGITS):
-            turns = [round(f / (2 * _PI) * (1 << 64)) % (1 << 64) for f in frequencies]
+            units = (1 << 64) / (2 * _PI)         # of a radian
+            turns = [round(f * units) % (1 << 64) for f in frequencies]
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64).to(device)
         self.device = self.turns.device
 
