@@ -1,4 +1,4 @@
-// Attention of a step's rows over a paged cache in BF16 or in 8 bits (kv_cache.cuh), for causal rows and for the nodes of
+// Attention of a step's rows over a paged cache in BF16, 8 or 4 bits (kv_cache.cuh), for causal rows and for the nodes of
 // draft trees: rotary embedding, the append of the rows' keys and values, soft-max attention in parts merged in part order.
 //
 //   out[r, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(q_rh . k_j / sqrt(128)),  j over the positions that row r sees:
@@ -6,8 +6,8 @@
 //
 // Three launches, four where many rows of a sequence may come together.  tree_prep: rotates the queries (once rounded, to the type
 // the matrix instruction takes), stores keys and values, and one CTA lays down the plan: tiles of rows of one sequence, and units =
-// (tile, part of the positions, kv head).  tree_part: persistent CTAs take runs of units.  tree_wide (tree_wide.cuh): the same for
-// runs of many rows.  tree_combine: merges a row's parts.  Which kernel takes a row and where its parts lie depends on its own
+// (tile, part of the positions, kv head).  tree_part (4 bits: tree_q4, tree_q4.cuh): persistent CTAs take runs of units.  tree_wide (tree_wide.cuh;
+// 4 bits: tree_pair, tree_pair.cuh): the same for runs of many rows.  tree_combine: merges a row's parts.  Which kernel takes a row and where its parts lie depends on its own
 // sequence's rows alone (and on whether the caller's longest_run lets tree_wide run at all), and every sum runs in a fixed order:
 // a row's bits do not depend on what else is in the batch.
 #pragma once
@@ -263,7 +263,8 @@ __device__ __forceinline__ void tree_store_q4(uint8_t* const (&page)[N], uint32_
 }
 
 // Rotated queries of `count` neighbouring heads for caches that are decoded to FP16: times a power of two that brings the largest component to [2^14, 2^15): 11 bits
-// where BF16 has 8, and what falls below FP16's normal range is 2^-28 of the largest.  (Magnitudes compare as their bits do; those of numbers that are not finite
+// where BF16 has 8 (one term: a component is off by 2^-11 of itself at most, outputs by 2.2 10^-4, an eighth of what their own rounding to BF16 makes), and
+// what falls below FP16's normal range is 2^-28 of the largest.  (Magnitudes compare as their bits do; those of numbers that are not finite
 // are the largest.)
 template <int N>
 __device__ __forceinline__ void tree_store_queries(const TreeArgs& a, uint32_t row, uint32_t head, uint32_t count, const float (&x)[N][4], float log2_scale, uint32_t lane) {

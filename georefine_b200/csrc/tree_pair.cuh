@@ -4,7 +4,8 @@
 // shared memory once for both tiles, their codes asked for two steps ahead; two warps issue the products, one for each tile; one looks up where the next unit lies:
 //   S = Q K^T (S in tensor memory, two steps of each tile);  weights P = exp2(S' - reference), written over S;  O += P V (P and O in tensor memory).
 // A step is 64 positions; K and V of three steps are held.  Arithmetic is that of tree_wide.cuh: K's exponent multiplies the score of its position, V's goes
-// into the weight, the sum of the weights takes it out again; the reference of a row moves when its maximum has passed it by 2^8.
+// into the weight, the sum of the weights takes it out again; the reference of a row moves when its maximum has passed it by 2^8.  Queries and weights are FP16, one term
+// each (what that costs: tree_q4.cuh); references, sums and O are FP32.
 //
 // A unit is a pair of tiles and a part of the positions.  Where a run's last tile has no partner, the products' and the weights' warps of the other half go through
 // all waits and arrivals without anything between them.  Barriers of a step are numbered by the step modulo three.  A wait tells a phase from the one before it and
@@ -14,7 +15,7 @@
 // No single unit bounds it.  A step of two full tiles takes 3100 cycles: the warps that turn scores into weights work 2400 of them, at an instruction in five cycles or
 // so each; the products 1380 (two of S at 434 - the queries are read again for every 64 positions - and two of O at 257), shared memory 2800 (the products 1024, the rest
 // mostly exponents that the weights' warps read), exp2 1024.  384 prompt rows behind 8000 positions, 40 heads of 8: 126 us, 510 TFLOP/s; 16 trees of 64 nodes
-// behind 8192: 340, of which 290 are this kernel.  What lies between units was dear: the queries' addresses with a division each kept a unit waiting for 4500 cycles (142
+// behind 4096 to 8192: 340, of which 290 are this kernel (over 8 bits 322: 64 nodes are 25 + 25 + 14 rows, so that half of the pairs have one tile).  What lies between units was dear: the queries' addresses with a division each kept a unit waiting for 4500 cycles (142
 // and 381).  (Two threads a row: 4 % slower; four threads for both tiles' rows at a time, whose exponents they read once: 40 %; weights by the reference as it is,
 // in one pass over the columns, done again where it moves: 17 %; K's exponents in the operands as far as they differ: 3 and 11 %.)
 #pragma once

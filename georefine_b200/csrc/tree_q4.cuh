@@ -11,10 +11,13 @@
 // A code becomes an FP16 operand with 1.1 instructions (q4_operands).  A group's scale goes into the operand, where it is exact; K's exponent
 // multiplies the score of its position, V's goes into the weight, as in 8 bits: S' = S 2^e_k scale + e_v, and the sum of the weights takes it out again.
 //
+// Queries and weights are FP16, one term each, as over 8 bits: rounded by 2^-11 of themselves at most, they put outputs behind 2048 normal entries 2.9 10^-4 off (relative),
+// which are then rounded to BF16, 1.63 10^-3: 1.66 in all.  A second term of either would double its products.  References, sums and O are FP32.
+//
 // Instructions bound it, and the chains between them: 560 for 32 positions of a head, of which 288 make operands of codes and 32 are the products; the four warps of a
-// scheduler issue in 57 % of the cycles.  A third of a warp's time goes to units' beginnings and ends - the next one found, its columns, the merge.  128 rows
-// behind 2048 positions each, 40 heads of 8 (220 MB): 69 us, 3.2 TB/s, where the 8-bit cache takes 100 with 410 MB; 8 rows behind
-// 32768: 70.  (Heads as rows of the products, as in 8 bits, would fill five rows of sixteen with twice the operands; a warp's four chunks written out one after
+// scheduler issue in 58 % of the cycles.  6600 of a unit's 15000 cycles (44 %) go to its beginning and end - the next one found, its columns, the merge.  128 rows
+// behind 1024 to 2048 positions, 40 heads of 8 (221 MB): 70 us, 3.2 TB/s; all launches 77, where the 8-bit cache takes 107 with 410 MB; 8 rows behind
+// 16384 to 32768 (230 MB): 69.  (Heads as rows of the products, as in 8 bits, would fill five rows of sixteen with twice the operands; a warp's four chunks written out one after
 // another no longer fit the instruction cache: 84.)
 #pragma once
 #include "tree_attention.cuh"

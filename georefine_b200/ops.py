@@ -452,7 +452,7 @@ class Rope:
 
 def rotary(x, positions, rope, *, out=None, backward=False):
     """Turns the first ``rope.dim`` dimensions of every head of ``x`` ([rows, heads, head dim] BF16, FP16 or FP32; rows and heads may be any distance apart) by
-    ``positions`` (int32 or int64 [rows]), into ``out`` or, without it, in place.  An angle is off by 2^-32 of a turn at most, and 2^-65 of one for
+    ``positions`` (int32 or int64 [rows]), into ``out`` - memory apart from that of ``x``, from its first to its last element - or, without it, in place.  An angle is off by 2^-32 of a turn at most, and 2^-65 of one for
     every position (2^-25 at 2^40); a value is rounded once.  ``backward``: turned the other way - the gradient of the call, given that of its result, and where ``rope.factor`` is 1 its inverse."""
     import torch
 

@@ -284,7 +284,8 @@ class BatchDecoder:
         self._table_host = np.full((self.max_slots + 1, self.pages_per_seq), -1, dtype=np.int64)
         self._free_pages = list(range(n_pages - 2, -1, -1))
         self._free_slots = list(range(self.max_slots - 1, -1, -1))
-        # The attention turns all of a head in halves, by tables; other rotary positions are applied to its rows before, and its tables are ones and zeros.
+        # The attention turns all of a head in halves, by tables; other rotary positions are applied to its rows before, and its tables are ones and zeros
+        # (queries and keys are then rounded to BF16 between the rotation and what the attention or the cache rounds them to).
         self.rope = None
         if cfg.rope_layout == "half" and cfg.rope_dim in (None, cfg.head_dim):
             if cfg.rope_scaling is None:
@@ -336,7 +337,7 @@ class BatchDecoder:
         self.graphs = {}
 
     def _tree_attention(self):
-        """The attention over an 8-bit cache, and of draft trees over either; made on first use (scratch of its own)."""
+        """The attention over an 8-bit or a 4-bit cache, and of draft trees over any; made on first use (scratch of its own)."""
         import torch
 
         if self._tree_attn is None:
@@ -372,7 +373,7 @@ class BatchDecoder:
             ops.rotary(qkv.unflatten(1, (heads + 2 * kv_heads, ops.HEAD_DIM))[:, :heads + kv_heads], positions, self.rope)
 
     def check_status(self) -> None:
-        """Raises when an attention over an 8-bit cache, or of draft trees, gave up a wait in the passes so far: their tokens and
+        """Raises when an attention over an 8-bit or a 4-bit cache, or of draft trees, gave up a wait in the passes so far: their tokens and
         the cache entries behind them are not to be used (retire the sequences).  Every such pass leaves its status in pinned memory, so
         a caller that has read a pass's tokens asks without waiting again."""
         if self._status_host is not None and self._status_host.item():
@@ -479,7 +480,8 @@ class BatchDecoder:
             self.page_table[slot, p] = own
 
     def compact_pages(self) -> int:
-        """Moves the pages in use to the front of the pool and returns how many there are (what lies behind them may be given to others)."""
+        """Moves the pages in use to the front of the pool and returns how many there are.  For callers who copy or save a cache by its
+        front: the engine itself never needs it, as any free page is as good as another."""
         import torch
 
         pool, refs = self._pool()
