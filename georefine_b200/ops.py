@@ -418,6 +418,8 @@ def _rope_frequencies(dim, theta, scaling):
             turns, width = number["original"] / (2 * _PI), number["high"] - number["low"]
             keep = [min(max((f * turns - number["low"]) / width, 0), 1) for f in inv]
             inv = [f / factor * (1 - k) + f * k for f, k in zip(inv, keep)]
+        if max(inv) >= 1 << 60:                   # (whose fraction of a turn would not be known to 2^-64)
+            raise ValueError("a position turns a pair by less than 2^60 radians")
     return inv, attention
 
 

@@ -26,3 +26,12 @@ def test_only_yarn_s_factor_on_components_may_be_left_open(scaling):
         ops.rope_frequencies(64, 1e4, scaling)
     with pytest.raises(ValueError, match="positive"):
         serve.DecoderConfig(rope_scaling=scaling)
+
+
+@pytest.mark.parametrize("kw", [dict(scaling={"kind": "linear", "factor": 5e-324}), dict(scaling={"kind": "linear", "factor": 2.0 ** -60}), dict(theta=1e-200), dict(scaling={"kind": "ntk", "factor": 1e-300})])
+def test_pairs_that_turn_too_far_a_position_are_refused(kw):
+    """Of 2^60 radians and more, 40 digits hold no fraction of a turn to 2^-64."""
+    for call in (lambda: ops.rope_frequencies(64, **kw), lambda: ops.Rope(64, device="cpu", **kw)):
+        with pytest.raises(ValueError, match="radians"):
+            call()
+    assert ops.rope_frequencies(2, 1e4, {"kind": "linear", "factor": 2.0 ** -59})[0] == [2.0 ** 59]
